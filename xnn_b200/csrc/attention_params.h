@@ -1,0 +1,25 @@
+// Launch parameters of the structure-attention kernels.
+#pragma once
+#include <stdint.h>
+
+namespace attn {
+
+// everything a launch needs; rows of q-like tensors are (N, H, D), of k-like ones (N, HK, D), any strides
+// but a contiguous last dimension
+template <typename T>
+struct Params {
+  const T *q, *k, *v, *o, *go;       // inputs, forward output, its cotangent
+  const T *ca, *cb, *cc;             // cotangents of dq, dk, dv (second derivative)
+  int64_t qs, ks, vs, os, gos, cas, cbs, ccs;      // row strides
+  int64_t qh, kh, vh, oh, goh, cah, cbh, cch;      // head strides
+  const int64_t* ptr;
+  const uint8_t* mask;               // 1 where an atom may be attended to, or null
+  T *out0, *out1, *out2, *out3;      // contiguous outputs
+  T *lse, *delta, *r, *c;            // (H, N) row statistics
+  T* work;                           // partial results of split passes
+  T scale;
+  int N, num, H, HK, D, splits;
+  int min_len, max_len;              // the lengths that this launch takes (others return at once)
+};
+
+}  // namespace attn

@@ -1,0 +1,204 @@
+// Shared pieces of the structure-attention kernels: which rows a block owns, tiles in shared memory
+// and the register-tiled products over them.
+//
+// The rows of a packed batch belong to structures given by a CSR pointer (num + 1 entries). With the
+// rows before the first and behind the last structure as two more parts that have no keys, the parts
+// are p = 0 .. num + 1 with the bounds 0, ptr[0], .., ptr[num], N. A part of x rows needs ceil(x / Q)
+// tiles of Q rows; numbering them from floor(start / Q) + p leaves room for all of them, since
+// floor((s + x) / Q) - floor(s / Q) + 1 >= ceil(x / Q). So a block finds its part from the pointer alone
+// (a warp-wide 32-ary search), the grid is floor(N / Q) + num + 2 whatever the lengths are, and no
+// host copy of the lengths is needed. Bounds are clamped to [0, N]: no pointer value leaves the arrays.
+#pragma once
+#include "attention_params.h"
+#include "common.cuh"
+
+namespace attn {
+
+struct Part { int lo, hi, row; bool keys; };   // the part's rows, the block's first row, whether it has keys
+
+__device__ __forceinline__ int part_bound(const int64_t* ptr, int num, int N, int p) {
+  if (p <= 0) return 0;
+  if (p >= num + 2) return N;
+  const int64_t v = ptr[p - 1];
+  return (int)(v < 0 ? 0 : (v > N ? N : v));
+}
+
+// the part and first row of tile `t` (tiles of Q rows); false where the tile number is one of the unused
+// ones. All lanes of a warp call it together.
+template <int Q>
+__device__ __forceinline__ bool find_part(const int64_t* ptr, int num, int N, int t, Part& out) {
+  const int lane = threadIdx.x & 31;
+  int at = 0, n = num + 2;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const bool ok = i < n && part_bound(ptr, num, N, at + i) / Q + at + i <= t;
+    const unsigned b = __ballot_sync(0xffffffffu, ok);
+    const int c = max(__popc(b) - 1, 0);
+    at += c * step;
+    n = min(step, n - c * step);
+  }
+  out.lo = part_bound(ptr, num, N, at);
+  out.hi = max(part_bound(ptr, num, N, at + 1), out.lo);
+  out.keys = at > 0 && at <= num;
+  const int64_t row = (int64_t)out.lo + (int64_t)(t - at - out.lo / Q) * Q;
+  out.row = (int)row;
+  return row >= out.lo && row < out.hi;
+}
+
+template <typename T> struct Vec { static constexpr int W = 16 / sizeof(T); };
+template <typename T> struct alignas(16) V16 { T x[16 / sizeof(T)]; };
+
+__device__ __forceinline__ float pow2(float x) { return exp2f(x); }
+__device__ __forceinline__ double pow2(double x) { return exp2(x); }
+__device__ __forceinline__ float lg2(float x) { return log2f(x); }
+__device__ __forceinline__ double lg2(double x) { return log2(x); }
+template <typename T> __device__ __forceinline__ T neg_inf();
+template <> __device__ __forceinline__ float neg_inf<float>() { return __int_as_float(0xff800000); }
+template <> __device__ __forceinline__ double neg_inf<double>() { return __longlong_as_double(0xfff0000000000000LL); }
+
+// whether 16-byte accesses are allowed for rows at p (+ any head) with these strides
+template <typename T>
+__host__ __device__ __forceinline__ bool vec_ok(const T* p, int64_t rs, int64_t hs, int D) {
+  constexpr int W = Vec<T>::W;
+  return (reinterpret_cast<uintptr_t>(p) % 16 == 0) && rs % W == 0 && hs % W == 0 && D % W == 0;
+}
+
+// rows row0 .. row0 + ROWS of g into s (row stride LD), zero behind `end`, behind column D and where the
+// mask is 0: what is masked or belongs to another structure never enters a product, NaN included
+template <typename T, int ROWS, int DP, int LD, int NT>
+__device__ __forceinline__ void load_tile(T* s, const T* g, int64_t stride, int row0, int end, int D, bool vec,
+                                          const uint8_t* mask = nullptr) {
+  constexpr int W = Vec<T>::W, CH = DP / W;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < ROWS * CH; i += NT) {
+    const int r = i / CH, c = (i % CH) * W, row = row0 + r;
+    V16<T> v;
+#pragma unroll
+    for (int e = 0; e < W; ++e) v.x[e] = T(0);
+    if (row < end && c < D && (mask == nullptr || mask[row])) {
+      const T* p = g + (int64_t)row * stride + c;
+      if (vec) {
+        v = *reinterpret_cast<const V16<T>*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          if (c + e < D) v.x[e] = p[e];
+      }
+    }
+    *reinterpret_cast<V16<T>*>(s + r * LD + c) = v;
+  }
+}
+
+// acc[r][c] += sum_d A[i0 + r][d] B[j0 + TX c][d]: row-major tiles, rows of A contiguous per thread and
+// columns strided by TX so that a warp's 16-byte reads of B fall into different banks (LD = DP + 16 bytes)
+template <typename T, int RI, int RJ, int TX, int DP, int LD>
+__device__ __forceinline__ void tile_nt(T (&acc)[RI][RJ], const T* A, int i0, const T* B, int j0) {
+  constexpr int W = Vec<T>::W;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += W) {
+    V16<T> a[RI], b[RJ];
+#pragma unroll
+    for (int r = 0; r < RI; ++r) a[r] = *reinterpret_cast<const V16<T>*>(A + (i0 + r) * LD + d);
+#pragma unroll
+    for (int c = 0; c < RJ; ++c) b[c] = *reinterpret_cast<const V16<T>*>(B + (j0 + TX * c) * LD + d);
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+#pragma unroll
+      for (int r = 0; r < RI; ++r)
+#pragma unroll
+        for (int c = 0; c < RJ; ++c) acc[r][c] += a[r].x[e] * b[c].x[e];
+  }
+}
+
+// how a thread's DP / TX output columns are laid out: NC groups of VW neighbours, TX * VW apart
+template <typename T, int DP, int TX>
+struct Cols {
+  static constexpr int PER = DP / TX;
+  static constexpr int VW = PER < Vec<T>::W ? PER : Vec<T>::W;
+  static constexpr int NC = PER / VW;
+};
+
+// acc[r][.] += sum_{j < J} P[i0 + r][j] V[j][columns of tx]
+template <typename T, int RI, int J, int TX, int DP, int LDP, int LD>
+__device__ __forceinline__ void tile_nn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx) {
+  using C = Cols<T, DP, TX>;
+  constexpr int W = Vec<T>::W;
+#pragma unroll 2
+  for (int j = 0; j < J; j += W) {
+    V16<T> p[RI];
+#pragma unroll
+    for (int r = 0; r < RI; ++r) p[r] = *reinterpret_cast<const V16<T>*>(P + (i0 + r) * LDP + j);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const T* row = V + (j + e) * LD + tx * C::VW;
+#pragma unroll
+      for (int n = 0; n < C::NC; ++n) {
+        T v[C::VW];
+        if constexpr (C::VW == W) {
+          *reinterpret_cast<V16<T>*>(v) = *reinterpret_cast<const V16<T>*>(row + n * TX * C::VW);
+        } else {
+#pragma unroll
+          for (int w = 0; w < C::VW; ++w) v[w] = row[n * TX * C::VW + w];
+        }
+#pragma unroll
+        for (int r = 0; r < RI; ++r)
+#pragma unroll
+          for (int w = 0; w < C::VW; ++w) acc[r][n * C::VW + w] += p[r].x[e] * v[w];
+      }
+    }
+  }
+}
+
+// acc[r][.] += sum_{j < J} P[j][i0 + r] V[j][columns of tx] (P read transposed; RI neighbouring columns)
+template <typename T, int RI, int J, int TX, int DP, int LDP, int LD>
+__device__ __forceinline__ void tile_tn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx) {
+  using C = Cols<T, DP, TX>;
+  constexpr int W = Vec<T>::W;
+#pragma unroll 4
+  for (int j = 0; j < J; ++j) {
+    T p[RI];
+#pragma unroll
+    for (int r = 0; r < RI; r += W) *reinterpret_cast<V16<T>*>(p + r) = *reinterpret_cast<const V16<T>*>(P + j * LDP + i0 + r);
+    const T* row = V + j * LD + tx * C::VW;
+#pragma unroll
+    for (int n = 0; n < C::NC; ++n) {
+      T v[C::VW];
+#pragma unroll
+      for (int w = 0; w < C::VW; ++w) v[w] = row[n * TX * C::VW + w];
+#pragma unroll
+      for (int r = 0; r < RI; ++r)
+#pragma unroll
+        for (int w = 0; w < C::VW; ++w) acc[r][n * C::VW + w] += p[r] * v[w];
+    }
+  }
+}
+
+// columns of tx of one row: out[column] = f * acc, guarded by D
+template <typename T, int DP, int TX>
+__device__ __forceinline__ void store_row(T* out, const T (&acc)[DP / TX], T f, int D, int tx) {
+  using C = Cols<T, DP, TX>;
+#pragma unroll
+  for (int n = 0; n < C::NC; ++n)
+#pragma unroll
+    for (int w = 0; w < C::VW; ++w) {
+      const int d = n * TX * C::VW + tx * C::VW + w;
+      if (d < D) out[d] = f * acc[n * C::VW + w];
+    }
+}
+
+// sum / maximum over the TX lanes that share a row
+template <int TX, typename T>
+__device__ __forceinline__ T row_sum(T v) {
+#pragma unroll
+  for (int o = TX / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int TX, typename T>
+__device__ __forceinline__ T row_max(T v) {
+#pragma unroll
+  for (int o = TX / 2; o; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, v, o); v = v > u ? v : u; }
+  return v;
+}
+
+}  // namespace attn

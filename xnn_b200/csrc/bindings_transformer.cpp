@@ -1,0 +1,305 @@
+// Python bindings of the transformer operators (attention.cu, dropout.cu, embedding.cu), launched on
+// the current stream of the operands' device; workspaces come from the caching allocator on that stream.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <limits>
+
+#include "attention.h"
+#include "attention_params.h"
+
+template <typename T>
+cudaError_t counter_dropout(int64_t outer, int64_t shared, int64_t inner, double p, const int64_t* rng, const T* x, T* y,
+                            cudaStream_t s);
+template <typename T, typename I>
+cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const I* ids, double scale, T* out, cudaStream_t s);
+template <typename T, typename I>
+cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g, double scale, int* ints, T* partials,
+                           T* table, cudaStream_t s);
+int64_t embedding_grad_ints(int64_t N, int64_t V);
+int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C);
+
+namespace {
+
+#define XNN_OK(call)                                                                          \
+  do {                                                                                        \
+    const cudaError_t err_ = (call);                                                          \
+    TORCH_CHECK(err_ == cudaSuccess, #call, " failed: ", cudaGetErrorString(err_));           \
+  } while (0)
+
+constexpr int ANY_LENGTH = std::numeric_limits<int>::max();
+constexpr int SHORT = 32;            // rows of the square tiles that hold a short structure whole
+constexpr int SMS = 148;
+
+void check_rows(const torch::Tensor& t, const torch::Tensor& like, int64_t N, int64_t heads, int64_t D, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type(), "structure attention: ",
+              name, " must be on ", like.device(), " with the dtype of q");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == N && t.size(1) == heads && t.size(2) == D && (D == 1 || N == 0 || t.stride(2) == 1),
+              "structure attention: ", name, " must be (", N, ", ", heads, ", ", D, ") with contiguous rows");
+}
+
+// the parameters that every pass shares; strides of a size-one dimension do not matter
+template <typename T>
+attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ptr,
+                            const c10::optional<torch::Tensor>& mask, double scale) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, "structure attention: q (atoms, heads, width) on a CUDA device");
+  const int64_t N = q.size(0), H = q.size(1), D = q.size(2), HK = k.dim() == 3 ? k.size(1) : 0;
+  TORCH_CHECK(HK > 0 && H > 0 && H % HK == 0 && H <= 65535, "structure attention: ", H, " heads over ", HK, " key heads");
+  TORCH_CHECK(D > 0 && D <= 128 && N < (1 << 30), "structure attention: width 1 .. 128, fewer than 2^30 atoms");
+  check_rows(q, q, N, H, D, "q");
+  check_rows(k, q, N, HK, D, "k");
+  check_rows(v, q, N, HK, D, "v");
+  TORCH_CHECK(ptr.device() == q.device() && ptr.scalar_type() == torch::kInt64 && ptr.dim() == 1 && ptr.is_contiguous() &&
+                  ptr.numel() >= 1 && ptr.numel() < (1 << 30), "structure attention: ptr must be int64 (structures + 1) on ", q.device());
+  attn::Params<T> p{};
+  p.q = q.data_ptr<T>(); p.qs = q.stride(0); p.qh = q.stride(1);
+  p.k = k.data_ptr<T>(); p.ks = k.stride(0); p.kh = k.stride(1);
+  p.v = v.data_ptr<T>(); p.vs = v.stride(0); p.vh = v.stride(1);
+  p.ptr = ptr.data_ptr<int64_t>();
+  if (mask.has_value()) {
+    TORCH_CHECK(mask->device() == q.device() && mask->scalar_type() == torch::kBool && mask->dim() == 1 &&
+                    mask->size(0) == N && mask->is_contiguous(), "structure attention: key_mask must be bool (atoms) on ", q.device());
+    p.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
+  }
+  p.scale = (T)scale;
+  p.N = (int)N; p.num = (int)ptr.numel() - 1; p.H = (int)H; p.HK = (int)HK; p.D = (int)D;
+  p.splits = 1;
+  p.min_len = 0;
+  p.max_len = ANY_LENGTH;
+  return p;
+}
+
+// Few row blocks and long structures: the walk over the other axis is shared out among up to 16 blocks
+// and their results added in order, until there are two blocks a multiprocessor; a share has four tiles
+// at least, or the second pass over the partial results costs what it saves.
+int choose_splits(int64_t row_tiles, int64_t max_len, int tile) {
+  const int64_t walk = (max_len + tile - 1) / tile;
+  int64_t s = 2 * SMS / std::max<int64_t>(row_tiles, 1);
+  s = std::min({s, walk / 4, (int64_t)16});
+  return (int)std::max<int64_t>(s, 1);
+}
+
+// mostly short structures: tiles of 32 rows leave less of each tile empty than those of 64
+template <typename T>
+bool mostly_short(const attn::Params<T>& p, int64_t max_len) { return max_len <= SHORT || (int64_t)p.N < 48 * (int64_t)p.num; }
+
+template <typename T>
+std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                         const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, int64_t max_len,
+                                         double scale, bool want_stats) {
+  auto p = make_params<T>(q, k, v, ptr, mask, scale);
+  torch::Tensor out = torch::empty({p.N, p.H, p.D}, q.options());
+  torch::Tensor lse;
+  if (want_stats) lse = torch::empty({p.H, p.N}, q.options());
+  if (p.N == 0) return {out, want_stats ? lse : out};
+  const auto s = at::cuda::getCurrentCUDAStream();
+  p.out0 = out.data_ptr<T>();
+  p.lse = want_stats ? lse.data_ptr<T>() : nullptr;
+  const bool small = mostly_short(p, max_len);
+  const int tile = small || sizeof(T) == 8 ? 32 : 64;
+  p.splits = choose_splits((int64_t)(p.N / tile + 1) * p.H, max_len, tile);
+  torch::Tensor work;
+  if (p.splits > 1) {
+    work = torch::empty({(int64_t)p.splits * p.H * p.N * (p.D + 2)}, q.options());
+    p.work = work.data_ptr<T>();
+  }
+  XNN_OK(attn::forward<T>(p, small, s));
+  if (p.splits > 1) XNN_OK(attn::forward_join<T>(p, s));
+  return {out, want_stats ? lse : out};
+}
+
+template <typename T>
+void set_outputs(attn::Params<T>& p, const torch::Tensor& go, const torch::Tensor& o, const torch::Tensor& lse,
+                 const torch::Tensor& q) {
+  check_rows(go, q, p.N, p.H, p.D, "the output's gradient");
+  check_rows(o, q, p.N, p.H, p.D, "the output");
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == q.scalar_type() && lse.is_contiguous() &&
+                  lse.numel() == (int64_t)p.H * p.N, "structure attention: row statistics of another call");
+  p.go = go.data_ptr<T>(); p.gos = go.stride(0); p.goh = go.stride(1);
+  p.o = o.data_ptr<T>(); p.os = o.stride(0); p.oh = o.stride(1);
+  p.lse = lse.data_ptr<T>();
+}
+
+template <typename T>
+std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::Tensor& q, const torch::Tensor& k,
+                                          const torch::Tensor& v, const torch::Tensor& o, const torch::Tensor& lse,
+                                          const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, int64_t max_len,
+                                          double scale) {
+  auto p = make_params<T>(q, k, v, ptr, mask, scale);
+  set_outputs(p, go, o, lse, q);
+  torch::Tensor dq = torch::empty({p.N, p.H, p.D}, q.options()), dk = torch::empty({p.N, p.HK, p.D}, q.options()),
+       dv = torch::empty({p.N, p.HK, p.D}, q.options());
+  if (p.N == 0) return {dq, dk, dv};
+  const auto s = at::cuda::getCurrentCUDAStream();
+  p.out0 = dq.data_ptr<T>(); p.out1 = dk.data_ptr<T>(); p.out2 = dv.data_ptr<T>();
+  const bool short_first = mostly_short(p, max_len);
+  if (short_first) {
+    auto ps = p;
+    if (max_len > SHORT) ps.max_len = SHORT;
+    XNN_OK(attn::backward_short<T>(ps, s));
+    if (max_len <= SHORT) return {dq, dk, dv};
+    p.min_len = SHORT + 1;
+  }
+  torch::Tensor delta = torch::empty({p.H, p.N}, q.options());
+  p.delta = delta.data_ptr<T>();
+  XNN_OK(attn::row_delta<T>(p, s));
+  const int tile = sizeof(T) == 8 ? 32 : 64;
+  const int64_t tiles = p.N / tile + 1;
+  torch::Tensor work;
+  const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
+  const int sq = short_first ? 1 : choose_splits(tiles * p.H, max_len, tile);
+  const int sk = short_first ? 1 : choose_splits(tiles * p.HK, max_len, tile);
+  if (sq > 1 || sk > 1) {
+    work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+    p.work = work.data_ptr<T>();
+  }
+  p.splits = sq;
+  XNN_OK(attn::backward_dq<T>(p, false, s));
+  if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, p.work, p.out0, s));
+  p.splits = sk;
+  XNN_OK(attn::backward_dkv<T>(p, false, s));
+  if (sk > 1) {
+    XNN_OK(attn::sum_splits<T>(nk, sk, p.work, p.out1, s));
+    XNN_OK(attn::sum_splits<T>(nk, sk, p.work + (int64_t)sk * nk, p.out2, s));
+  }
+  return {dq, dk, dv};
+}
+
+template <typename T>
+std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& c,
+                                        const torch::Tensor& go, const torch::Tensor& q, const torch::Tensor& k,
+                                        const torch::Tensor& v, const torch::Tensor& o, const torch::Tensor& lse,
+                                        const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, double scale) {
+  auto p = make_params<T>(q, k, v, ptr, mask, scale);
+  set_outputs(p, go, o, lse, q);
+  check_rows(a, q, p.N, p.H, p.D, "the cotangent of dq");
+  check_rows(b, q, p.N, p.HK, p.D, "the cotangent of dk");
+  check_rows(c, q, p.N, p.HK, p.D, "the cotangent of dv");
+  p.ca = a.data_ptr<T>(); p.cas = a.stride(0); p.cah = a.stride(1);
+  p.cb = b.data_ptr<T>(); p.cbs = b.stride(0); p.cbh = b.stride(1);
+  p.cc = c.data_ptr<T>(); p.ccs = c.stride(0); p.cch = c.stride(1);
+  torch::Tensor q2 = torch::empty({p.N, p.H, p.D}, q.options()), k2 = torch::empty({p.N, p.HK, p.D}, q.options()),
+       v2 = torch::empty({p.N, p.HK, p.D}, q.options()), do2 = torch::empty({p.N, p.H, p.D}, q.options());
+  if (p.N == 0) return {q2, k2, v2, do2};
+  const auto s = at::cuda::getCurrentCUDAStream();
+  torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
+  p.delta = stats.data_ptr<T>();
+  p.r = p.delta + (int64_t)p.H * p.N;
+  p.c = p.r + (int64_t)p.H * p.N;
+  p.out0 = q2.data_ptr<T>(); p.out1 = k2.data_ptr<T>(); p.out2 = v2.data_ptr<T>(); p.out3 = do2.data_ptr<T>();
+  XNN_OK(attn::row_delta<T>(p, s));
+  XNN_OK(attn::second_rows<T>(p, s));
+  XNN_OK(attn::second_keys<T>(p, s));
+  return {q2, k2, v2, do2};
+}
+
+using Tensors = std::vector<torch::Tensor>;
+
+Tensors attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor ptr,
+                          c10::optional<torch::Tensor> mask, int64_t max_len, double scale, bool want_stats) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensors r;
+  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention",
+                             [&] { r = forward_typed<scalar_t>(q, k, v, ptr, mask, max_len, scale, want_stats); });
+  return r;
+}
+
+Tensors attention_backward(torch::Tensor go, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
+                           torch::Tensor lse, torch::Tensor ptr, c10::optional<torch::Tensor> mask, int64_t max_len, double scale) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensors r;
+  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward",
+                             [&] { r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale); });
+  return r;
+}
+
+Tensors attention_second(torch::Tensor a, torch::Tensor b, torch::Tensor c, torch::Tensor go, torch::Tensor q, torch::Tensor k,
+                         torch::Tensor v, torch::Tensor o, torch::Tensor lse, torch::Tensor ptr,
+                         c10::optional<torch::Tensor> mask, double scale) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensors r;
+  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention second derivative",
+                             [&] { r = second_typed<scalar_t>(a, b, c, go, q, k, v, o, lse, ptr, mask, scale); });
+  return r;
+}
+
+// x (outer, shared, inner) contiguous; rng int64 (seed, offset) on x's device
+torch::Tensor dropout_op(torch::Tensor x, int64_t outer, int64_t shared, int64_t inner, double p, torch::Tensor rng) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.numel() == outer * shared * inner, "counter_dropout: contiguous CUDA tensor");
+  TORCH_CHECK(rng.device() == x.device() && rng.scalar_type() == torch::kInt64 && rng.numel() == 2 && rng.is_contiguous(),
+              "counter_dropout: rng must be two int64 numbers on ", x.device());
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, "counter_dropout: p in [0, 1]");
+  TORCH_CHECK(shared < (1 << 30), "counter_dropout: too many shared copies");
+  auto y = torch::empty_like(x);
+  if (x.numel() == 0) return y;
+  const auto s = at::cuda::getCurrentCUDAStream();
+  AT_DISPATCH_FLOATING_TYPES(x.scalar_type(), "counter_dropout", [&] {
+    XNN_OK(counter_dropout<scalar_t>(outer, shared, inner, p, rng.data_ptr<int64_t>(), x.data_ptr<scalar_t>(),
+                                     y.data_ptr<scalar_t>(), s));
+  });
+  return y;
+}
+
+void check_ids(const torch::Tensor& ids, const torch::Tensor& like) {
+  TORCH_CHECK(ids.device() == like.device() && ids.is_contiguous() &&
+                  (ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32),
+              "embedding_lookup: ids must be contiguous int64 or int32 on ", like.device());
+  TORCH_CHECK(ids.numel() < (1 << 30), "embedding_lookup: fewer than 2^30 ids");
+}
+
+torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
+  const c10::cuda::CUDAGuard guard(table.device());
+  TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.is_contiguous() && table.size(0) < (1 << 30) &&
+                  table.size(1) < (1 << 20), "embedding_lookup: table (rows, width), contiguous on a CUDA device");
+  check_ids(ids, table);
+  auto shape = ids.sizes().vec();
+  shape.push_back(table.size(1));
+  auto out = torch::empty(shape, table.options());
+  if (out.numel() == 0) return out;
+  const auto s = at::cuda::getCurrentCUDAStream();
+  AT_DISPATCH_FLOATING_TYPES(table.scalar_type(), "embedding_lookup", [&] {
+    if (ids.scalar_type() == torch::kInt64)
+      XNN_OK((embedding_lookup<scalar_t, int64_t>(ids.numel(), table.size(0), (int)table.size(1), table.data_ptr<scalar_t>(),
+                                                  ids.data_ptr<int64_t>(), scale, out.data_ptr<scalar_t>(), s)));
+    else
+      XNN_OK((embedding_lookup<scalar_t, int>(ids.numel(), table.size(0), (int)table.size(1), table.data_ptr<scalar_t>(),
+                                              ids.data_ptr<int>(), scale, out.data_ptr<scalar_t>(), s)));
+  });
+  return out;
+}
+
+torch::Tensor lookup_grad_op(torch::Tensor ids, torch::Tensor g, int64_t rows, double scale) {
+  const c10::cuda::CUDAGuard guard(g.device());
+  const int64_t N = ids.numel(), C = g.size(-1);
+  TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.numel() == N * C && rows < (1 << 30) && C < (1 << 20),
+              "embedding_lookup: gradient (ids, width), contiguous on a CUDA device");
+  check_ids(ids, g);
+  auto out = torch::empty({rows, C}, g.options());
+  if (out.numel() == 0) return out;
+  if (N == 0) return out.zero_();
+  const auto s = at::cuda::getCurrentCUDAStream();
+  auto ints = torch::empty({embedding_grad_ints(N, rows)}, g.options().dtype(torch::kInt32));
+  auto parts = torch::empty({embedding_grad_partials(N, rows, C)}, g.options());
+  AT_DISPATCH_FLOATING_TYPES(g.scalar_type(), "embedding_lookup gradient", [&] {
+    if (ids.scalar_type() == torch::kInt64)
+      XNN_OK((embedding_grad<scalar_t, int64_t>(N, rows, (int)C, ids.data_ptr<int64_t>(), g.data_ptr<scalar_t>(), scale,
+                                                ints.data_ptr<int>(), parts.data_ptr<scalar_t>(), out.data_ptr<scalar_t>(), s)));
+    else
+      XNN_OK((embedding_grad<scalar_t, int>(N, rows, (int)C, ids.data_ptr<int>(), g.data_ptr<scalar_t>(), scale,
+                                            ints.data_ptr<int>(), parts.data_ptr<scalar_t>(), out.data_ptr<scalar_t>(), s)));
+  });
+  return out;
+}
+
+}  // namespace
+
+void register_transformer(pybind11::module& m) {
+  m.def("attention_forward", &attention_forward);
+  m.def("attention_backward", &attention_backward);
+  m.def("attention_second", &attention_second);
+  m.def("counter_dropout", &dropout_op);
+  m.def("embedding_lookup", &lookup_op);
+  m.def("embedding_lookup_grad", &lookup_grad_op);
+}

@@ -1,0 +1,364 @@
+// Lookup of table rows by id with a scale, and its gradient by sorted ids.
+//
+//   out[n] = scale table[id_n]        (zero where id_n is outside the table: a padded entry)
+//   gtable[v] = scale sum_{n: id_n = v} g[n]
+//
+// The gradient sorts the ids (stable radix sort, eight bits a pass, (key, row) pairs), then walks the sorted
+// order in chunks: a warp sums the rows of each run of equal ids inside its chunk. A run inside one chunk
+// goes to the table; the part of a run that began before the chunk, and the one that goes on behind it, are
+// written to one of the chunk's two partial rows. A block per table row then adds the partials of its run in their order
+// and writes zeros where no id came. Every sum has a fixed order; there are no atomics on values.
+// Small inputs (rule at `embedding_grad`) skip the sort: a block per table row collects its ids itself.
+#include "common.cuh"
+
+namespace {
+
+template <typename T> struct alignas(16) Pack { T x[16 / sizeof(T)]; };
+
+template <typename I>
+__device__ __forceinline__ int64_t row_of(const I* ids, int64_t n, int64_t V) {
+  const int64_t v = (int64_t)ids[n];
+  return v >= 0 && v < V ? v : -1;
+}
+
+template <typename T, typename I, int W>
+__global__ void __launch_bounds__(256) lookup_kernel(int64_t N, int64_t V, int C, const T* __restrict__ table,
+                                                     const I* __restrict__ ids, T scale, T* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = C / W;
+  const int64_t n = i / per;
+  if (n >= N) return;
+  const int c = (int)(i - n * per) * W;
+  const int64_t v = row_of(ids, n, V);
+  if constexpr (W == 1) {
+    out[n * C + c] = v < 0 ? T(0) : scale * table[v * C + c];
+  } else {
+    Pack<T> a;
+#pragma unroll
+    for (int e = 0; e < W; ++e) a.x[e] = T(0);
+    if (v >= 0) {
+      a = *reinterpret_cast<const Pack<T>*>(table + v * C + c);
+#pragma unroll
+      for (int e = 0; e < W; ++e) a.x[e] *= scale;
+    }
+    *reinterpret_cast<Pack<T>*>(out + n * C + c) = a;
+  }
+}
+
+// ---- sort: each block takes `tile` pairs, each of its 8 warps a contiguous eighth, in strips of 32 ----
+constexpr int SORT_WARPS = 8;
+
+template <typename I>
+__device__ __forceinline__ int key_at(const I* ids, const int* keys, int64_t i, int64_t V) {
+  if (keys) return keys[i];
+  const int64_t v = row_of(ids, i, V);
+  return v < 0 ? (int)V : (int)v;                       // padded entries sort behind the table
+}
+
+template <typename I>
+__global__ void __launch_bounds__(256) count_kernel(int N, int64_t V, int tile, int shift, const I* __restrict__ ids,
+                                                    const int* __restrict__ keys, int* __restrict__ counts) {
+  __shared__ int c[256];
+  c[threadIdx.x] = 0;
+  __syncthreads();
+  const int end = min(N, (int)(blockIdx.x + 1) * tile);
+  for (int i = blockIdx.x * tile + threadIdx.x; i < end; i += 256) atomicAdd(&c[(key_at(ids, keys, i, V) >> shift) & 255], 1);
+  __syncthreads();
+  counts[blockIdx.x * 256 + threadIdx.x] = c[threadIdx.x];
+}
+
+template <typename I>
+__global__ void __launch_bounds__(256) place_kernel(int N, int64_t V, int tile, int shift, const I* __restrict__ ids,
+                                                    const int* __restrict__ keys, const int* __restrict__ rows,
+                                                    const int* __restrict__ counts, int* __restrict__ keys_out,
+                                                    int* __restrict__ rows_out) {
+  __shared__ int base[SORT_WARPS][256];
+  __shared__ int scan[SORT_WARPS];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  // where this block's entries of digit t start: entries of smaller digits, then those of earlier blocks
+  int before = 0, total = 0;
+  for (int b = 0; b < (int)gridDim.x; ++b) {
+    const int v = counts[b * 256 + t];
+    before += b < (int)blockIdx.x ? v : 0;
+    total += v;
+  }
+  int incl = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
+  if (lane == 31) scan[warp] = incl;
+#pragma unroll
+  for (int w = 0; w < SORT_WARPS; ++w) base[w][t] = 0;
+  __syncthreads();
+  int start = incl - total + before;
+  for (int w = 0; w < warp; ++w) start += scan[w];
+  const int per = ((tile + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
+  const int end = min(N, (int)(blockIdx.x + 1) * tile);
+  const int first = blockIdx.x * tile + warp * per, last = min(end, first + per);
+  for (int i = first + lane; i < last; i += 32) atomicAdd(&base[warp][(key_at(ids, keys, i, V) >> shift) & 255], 1);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SORT_WARPS; ++w) { const int c = base[w][t]; base[w][t] = start; start += c; }
+  __syncthreads();
+  for (int i0 = first; i0 < last; i0 += 32) {
+    const int i = i0 + lane;
+    const bool in = i < last;
+    const int key = in ? key_at(ids, keys, i, V) : 0, digit = in ? (key >> shift) & 255 : 256;
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    int at = 0;
+    if (in) at = base[warp][digit] + rank;
+    __syncwarp();
+    if (in && rank == 0) base[warp][digit] += __popc(same);
+    __syncwarp();
+    if (in) {
+      keys_out[at] = key;
+      rows_out[at] = rows ? rows[i] : i;
+    }
+  }
+}
+
+// ---- sums over the sorted order: a warp per (chunk of R entries, 32 W columns) ----
+template <typename T, int W>
+__device__ __forceinline__ void put(T* row, const T (&a)[W], T f, int c, int C) {
+#pragma unroll
+  for (int e = 0; e < W; ++e)
+    if (c + e < C) row[c + e] = f * a[e];
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void get(const T* row, T (&a)[W], int c, int C) {
+  if constexpr (W == 1) {
+    a[0] = c < C ? row[c] : T(0);
+  } else {
+    Pack<T> v;
+    if (c < C) v = *reinterpret_cast<const Pack<T>*>(row + c);
+#pragma unroll
+    for (int e = 0; e < W; ++e) a[e] = c < C ? v.x[e] : T(0);
+  }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(128) runs_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
+                                                   const int* __restrict__ rows, const T* __restrict__ g, T scale,
+                                                   T* __restrict__ table, T* __restrict__ part) {
+  const int chunk = blockIdx.x * 4 + threadIdx.x / 32;
+  const int64_t first = (int64_t)chunk * R;
+  if (first >= N) return;
+  const int last = (int)(first + R < N ? first + R : N), i0 = (int)first;
+  const int c = (blockIdx.y * 32 + (threadIdx.x & 31)) * W;
+  T acc[W] = {};
+  int key = keys[i0];
+  bool open = i0 > 0 && keys[i0 - 1] == key;            // the run began in an earlier chunk
+  constexpr int U = 8;
+  for (int i = i0; i < last; i += U) {
+    int k[U];
+    T v[U][W];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = i + u < last ? keys[i + u] : V;
+      if (k[u] < V) get<T, W>(g + (int64_t)rows[i + u] * C, v[u], c, C);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= last) break;
+      if (k[u] != key) {
+        if (key < V) {
+          if (open) put<T, W>(part + (int64_t)(2 * chunk) * C, acc, T(1), c, C);
+          else put<T, W>(table + (int64_t)key * C, acc, scale, c, C);
+        }
+        open = false;
+        key = k[u];
+#pragma unroll
+        for (int e = 0; e < W; ++e) acc[e] = T(0);
+      }
+      if (key < V) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) acc[e] += v[u][e];
+      }
+    }
+  }
+  if (key < V) {
+    const bool goes_on = last < N && keys[last] == key;
+    if (open) put<T, W>(part + (int64_t)(2 * chunk) * C, acc, T(1), c, C);
+    else if (goes_on) put<T, W>(part + (int64_t)(2 * chunk + 1) * C, acc, T(1), c, C);
+    else put<T, W>(table + (int64_t)key * C, acc, scale, c, C);
+  }
+}
+
+// first sorted position with a key >= v (all lanes of a warp together)
+__device__ __forceinline__ int lower_bound(const int* keys, int N, int v) {
+  const int lane = threadIdx.x & 31;
+  int at = 0, n = N;                                    // the answer is in [at, at + n]
+  while (n > 0) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step + step - 1;
+    const bool less = i < n && keys[at + i] < v;
+    const int c = __popc(__ballot_sync(0xffffffffu, less));
+    at += c * step;
+    n = min(step - 1, n - c * step);
+    if (n < 0) n = 0;
+  }
+  return at;
+}
+
+// a block per table row: zeros where no id came, the partials of runs over several chunks otherwise
+template <typename T>
+__global__ void __launch_bounds__(256) rows_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
+                                                   const T* __restrict__ part, T scale, T* __restrict__ table) {
+  __shared__ T sums[256];
+  const int v = blockIdx.x, t = threadIdx.x;
+  const int a = lower_bound(keys, N, v), b = lower_bound(keys, N, v + 1);
+  T* out = table + (int64_t)v * C;
+  if (a == b) {
+    for (int c = t; c < C; c += 256) out[c] = T(0);
+    return;
+  }
+  const int c0 = a / R, c1 = (b - 1) / R;
+  if (c0 == c1) return;                                 // one chunk had the whole run
+  const int lanes = C < 256 ? (C <= 32 ? 32 : (C <= 64 ? 64 : (C <= 128 ? 128 : 256))) : 256, groups = 256 / lanes;
+  const int group = t / lanes;
+  // the first chunk's share is in its second partial row unless the run began before (it did not: c0 holds a)
+  const int n = c1 - c0 + 1, per = (n + groups - 1) / groups;
+  for (int cb = 0; cb < C; cb += lanes) {
+    const int c = cb + t % lanes;
+    T s = T(0);
+    if (c < C) {
+      const int j1 = min(n, (group + 1) * per);
+#pragma unroll 8
+      for (int j = group * per; j < j1; ++j) s += part[(int64_t)(2 * (c0 + j) + (j == 0 ? 1 : 0)) * C + c];
+    }
+    __syncthreads();
+    sums[t] = s;
+    __syncthreads();
+    if (group == 0 && c < C) {
+      for (int k = 1; k < groups; ++k) s += sums[k * lanes + t];
+      out[c] = scale * s;
+    }
+  }
+}
+
+// ---- small inputs: a block per table row lists its entries in order, then sums them ----
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) collect_kernel(int N, int64_t V, int C, const I* __restrict__ ids,
+                                                      const T* __restrict__ g, T scale, T* __restrict__ table) {
+  extern __shared__ __align__(16) char raw[];
+  T* sums = reinterpret_cast<T*>(raw);
+  int* list = reinterpret_cast<int*>(sums + 256);
+  __shared__ int warp_n[8];
+  const int v = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int n = 0;
+  for (int i0 = 0; i0 < N; i0 += 256) {
+    const int i = i0 + t;
+    const bool hit = i < N && (int64_t)ids[i] == v;
+    const unsigned b = __ballot_sync(0xffffffffu, hit);
+    if (lane == 0) warp_n[warp] = __popc(b);
+    __syncthreads();
+    int at = n;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      at += w < warp ? warp_n[w] : 0;
+      n += warp_n[w];
+    }
+    if (hit) list[at + __popc(b & ((1u << lane) - 1))] = i;
+    __syncthreads();
+  }
+  T* out = table + (int64_t)v * C;
+  const int lanes = C <= 32 ? 32 : (C <= 64 ? 64 : (C <= 128 ? 128 : 256)), groups = 256 / lanes, group = t / lanes;
+  const int per = (n + groups - 1) / groups;
+  for (int cb = 0; cb < C; cb += lanes) {
+    const int c = cb + t % lanes;
+    T s = T(0);
+    if (c < C) {
+      const int j1 = min(n, (group + 1) * per);
+#pragma unroll 8
+      for (int j = group * per; j < j1; ++j) s += g[(int64_t)list[j] * C + c];
+    }
+    __syncthreads();
+    sums[t] = s;
+    __syncthreads();
+    if (group == 0 && c < C) {
+      for (int k = 1; k < groups; ++k) s += sums[k * lanes + t];
+      out[c] = scale * s;
+    }
+  }
+}
+
+constexpr int SMALL_ROWS = 4096;
+
+// pairs a sort block takes: at most 148 blocks (each reads every block's counts), 1024 pairs at least
+int sort_tile(int64_t N) {
+  const int64_t t = (N + 147) / 148;
+  return (int)(t < 1024 ? 1024 : (t + 255) / 256 * 256);
+}
+// entries a summing warp takes: 64, more when that would pass 64 warps a multiprocessor
+int run_chunk(int64_t N) {
+  const int64_t r = (N + 148 * 64 - 1) / (148 * 64);
+  return (int)(r < 64 ? 64 : (r + 7) / 8 * 8);
+}
+bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 22; }
+
+}  // namespace
+
+template <typename T, typename I>
+cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const I* ids, double scale, T* out, cudaStream_t s) {
+  constexpr int W = 16 / sizeof(T);
+  const bool vec = C % W == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const int64_t items = N * (vec ? C / W : C);
+  const unsigned grid = (unsigned)((items + 255) / 256);
+  if (vec) lookup_kernel<T, I, W><<<grid, 256, 0, s>>>(N, V, C, table, ids, (T)scale, out);
+  else lookup_kernel<T, I, 1><<<grid, 256, 0, s>>>(N, V, C, table, ids, (T)scale, out);
+  return cudaGetLastError();
+}
+
+// int32 words of workspace for the sort, and elements of T for the partial rows
+int64_t embedding_grad_ints(int64_t N, int64_t V) {
+  if (collects(N, V)) return 0;
+  const int64_t tile = sort_tile(N);
+  return 4 * N + (N + tile - 1) / tile * 256;
+}
+int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C) {
+  if (collects(N, V)) return 0;
+  const int64_t R = run_chunk(N);
+  return (N + R - 1) / R * 2 * C;
+}
+
+template <typename T, typename I>
+cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g, double scale, int* ints, T* partials,
+                           T* table, cudaStream_t s) {
+  // collecting costs N V id reads in all and sums a row's entries in one block; the sort costs four to ten
+  // launches: below some thousand entries the former is one short launch
+  if (collects(N, V)) {
+    collect_kernel<T, I><<<(unsigned)V, 256, 256 * sizeof(T) + sizeof(int) * (size_t)N, s>>>((int)N, V, C, ids, g, (T)scale, table);
+    return cudaGetLastError();
+  }
+  const int tile = sort_tile(N), blocks = (int)((N + tile - 1) / tile);
+  int *keys[2] = {ints, ints + N}, *rows[2] = {ints + 2 * N, ints + 3 * N}, *counts = ints + 4 * N;
+  int bits = 1;
+  while (((int64_t)1 << bits) <= V) ++bits;             // keys 0 .. V
+  int at = 0;
+  for (int shift = 0; shift < bits; shift += 8) {
+    const int* kin = shift ? keys[at ^ 1] : nullptr;
+    const int* rin = shift ? rows[at ^ 1] : nullptr;
+    count_kernel<I><<<blocks, 256, 0, s>>>((int)N, V, tile, shift, ids, kin, counts);
+    place_kernel<I><<<blocks, 256, 0, s>>>((int)N, V, tile, shift, ids, kin, rin, counts, keys[at], rows[at]);
+    at ^= 1;
+  }
+  const int *k = keys[at ^ 1], *r = rows[at ^ 1];
+  const int R = run_chunk(N), chunks = (int)((N + R - 1) / R);
+  constexpr int W = 16 / sizeof(T);
+  const bool vec = C % W == 0 && reinterpret_cast<uintptr_t>(g) % 16 == 0;
+  const int cols = 32 * (vec ? W : 1);
+  const dim3 grid((chunks + 3) / 4, (C + cols - 1) / cols);
+  if (vec) runs_kernel<T, W><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
+  else runs_kernel<T, 1><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
+  rows_kernel<T><<<(unsigned)V, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
+  return cudaGetLastError();
+}
+
+#define XNN_EMB_INST(T, I)                                                                                          \
+  template cudaError_t embedding_lookup<T, I>(int64_t, int64_t, int, const T*, const I*, double, T*, cudaStream_t); \
+  template cudaError_t embedding_grad<T, I>(int64_t, int64_t, int, const I*, const T*, double, int*, T*, T*, cudaStream_t);
+XNN_EMB_INST(float, int64_t)
+XNN_EMB_INST(float, int)
+XNN_EMB_INST(double, int64_t)
+XNN_EMB_INST(double, int)
