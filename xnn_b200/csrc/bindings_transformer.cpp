@@ -1,5 +1,5 @@
-// Python bindings of the transformer operators (attention.cu, dropout.cu, embedding.cu), launched on
-// the current stream of the operands' device; workspaces come from the caching allocator on that stream.
+// Python bindings and autograd nodes of the transformer operators (attention.cu, dropout.cu, embedding.cu),
+// launched on the current stream of the operands' device; workspaces come from the caching allocator on that stream.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -195,9 +195,12 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
 }
 
 using Tensors = std::vector<torch::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
 
-Tensors attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor ptr,
-                          c10::optional<torch::Tensor> mask, int64_t max_len, double scale, bool want_stats) {
+Tensors attention_forward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ptr,
+                          const c10::optional<torch::Tensor>& mask, int64_t max_len, double scale, bool want_stats) {
   const c10::cuda::CUDAGuard guard(q.device());
   Tensors r;
   AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention",
@@ -205,27 +208,89 @@ Tensors attention_forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, tor
   return r;
 }
 
-Tensors attention_backward(torch::Tensor go, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
-                           torch::Tensor lse, torch::Tensor ptr, c10::optional<torch::Tensor> mask, int64_t max_len, double scale) {
-  const c10::cuda::CUDAGuard guard(q.device());
-  Tensors r;
-  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward",
-                             [&] { r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale); });
-  return r;
+torch::Tensor rows(const torch::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+c10::optional<torch::Tensor> maybe(const torch::Tensor& t) {
+  return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt;
 }
 
-Tensors attention_second(torch::Tensor a, torch::Tensor b, torch::Tensor c, torch::Tensor go, torch::Tensor q, torch::Tensor k,
-                         torch::Tensor v, torch::Tensor o, torch::Tensor lse, torch::Tensor ptr,
-                         c10::optional<torch::Tensor> mask, double scale) {
-  const c10::cuda::CUDAGuard guard(q.device());
-  Tensors r;
-  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention second derivative",
-                             [&] { r = second_typed<scalar_t>(a, b, c, go, q, k, v, o, lse, ptr, mask, scale); });
-  return r;
+// The autograd nodes are C++: a backward pass runs on the engine's thread without the interpreter, which
+// for the smallest calls costs more than the kernels. What the passes share beyond the saved tensors:
+struct Setting { int64_t max_len; double scale; };
+void keep(AutogradContext* ctx, const Setting& s) {
+  ctx->saved_data["max_len"] = s.max_len;
+  ctx->saved_data["scale"] = s.scale;
+}
+Setting kept(AutogradContext* ctx) { return {ctx->saved_data["max_len"].toInt(), ctx->saved_data["scale"].toDouble()}; }
+
+// the gradients of <a, dq> + <b, dk> + <c, dv> in do, q, k, v; a node of its own, so that a third derivative
+// meets it on every path to the inputs and is refused
+struct AttentionSecond : torch::autograd::Function<AttentionSecond> {
+  static variable_list forward(AutogradContext*, Variable a, Variable b, Variable c, Variable go, Variable q, Variable k,
+                               Variable v, Variable o, Variable lse, Variable ptr, c10::optional<Variable> mask, double scale) {
+    const c10::cuda::CUDAGuard guard(q.device());
+    Tensors r;
+    AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention second derivative", [&] {
+      r = second_typed<scalar_t>(rows(a), rows(b), rows(c), go, q, k, v, o, lse, ptr, mask, scale);
+    });
+    return {r[3], r[0], r[1], r[2]};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "structure_attention on CUDA differentiates twice, not three times");
+  }
+};
+
+// (dq, dk, dv); its own derivative is the total one, through o and the row statistics too
+struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
+  static variable_list forward(AutogradContext* ctx, Variable go, Variable q, Variable k, Variable v, Variable o, Variable lse,
+                               Variable ptr, c10::optional<Variable> mask, int64_t max_len, double scale) {
+    go = rows(go);
+    ctx->save_for_backward({go, q, k, v, o, lse, ptr, mask.value_or(Variable())});
+    keep(ctx, {max_len, scale});
+    const c10::cuda::CUDAGuard guard(q.device());
+    Tensors r;
+    AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward", [&] {
+      r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale);
+    });
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    auto r = AttentionSecond::apply(g[0], g[1], g[2], s[0], s[1], s[2], s[3], s[4], s[5], s[6], maybe(s[7]), kept(ctx).scale);
+    r.resize(10);
+    return r;
+  }
+};
+
+struct Attention : torch::autograd::Function<Attention> {
+  static Variable forward(AutogradContext* ctx, Variable q, Variable k, Variable v, Variable ptr, c10::optional<Variable> mask,
+                          int64_t max_len, double scale) {
+    auto r = attention_forward(q, k, v, ptr, mask, max_len, scale, true);
+    ctx->save_for_backward({q, k, v, r[0], r[1], ptr, mask.value_or(Variable())});
+    keep(ctx, {max_len, scale});
+    return r[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const auto set = kept(ctx);
+    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), set.max_len, set.scale);
+    r.resize(7);
+    return r;
+  }
+};
+
+torch::Tensor structure_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor ptr,
+                                  c10::optional<torch::Tensor> mask, int64_t max_len, double scale) {
+  q = rows(q); k = rows(k); v = rows(v);
+  ptr = ptr.contiguous();
+  if (mask.has_value()) mask = mask->contiguous();
+  if (torch::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return Attention::apply(q, k, v, ptr, mask, max_len, scale);
+  return attention_forward(q, k, v, ptr, mask, max_len, scale, false)[0];
 }
 
 // x (outer, shared, inner) contiguous; rng int64 (seed, offset) on x's device
-torch::Tensor dropout_op(torch::Tensor x, int64_t outer, int64_t shared, int64_t inner, double p, torch::Tensor rng) {
+torch::Tensor dropout_raw(const torch::Tensor& x, int64_t outer, int64_t shared, int64_t inner, double p, const torch::Tensor& rng) {
   const c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.numel() == outer * shared * inner, "counter_dropout: contiguous CUDA tensor");
   TORCH_CHECK(rng.device() == x.device() && rng.scalar_type() == torch::kInt64 && rng.numel() == 2 && rng.is_contiguous(),
@@ -242,6 +307,27 @@ torch::Tensor dropout_op(torch::Tensor x, int64_t outer, int64_t shared, int64_t
   return y;
 }
 
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Variable forward(AutogradContext* ctx, Variable x, Variable rng, int64_t outer, int64_t shared, int64_t inner, double p) {
+    ctx->save_for_backward({rng});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{outer, shared, inner};
+    ctx->saved_data["p"] = p;
+    return dropout_raw(x, outer, shared, inner, p, rng);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto n = ctx->saved_data["sizes"].toIntVector();
+    return {Dropout::apply(g[0].contiguous(), ctx->get_saved_variables()[0], n[0], n[1], n[2], ctx->saved_data["p"].toDouble()),
+            Variable(), Variable(), Variable(), Variable(), Variable()};
+  }
+};
+
+torch::Tensor dropout_op(torch::Tensor x, int64_t outer, int64_t shared, int64_t inner, double p, torch::Tensor rng) {
+  x = x.contiguous();
+  rng = rng.contiguous();
+  if (torch::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, rng, outer, shared, inner, p);
+  return dropout_raw(x, outer, shared, inner, p, rng);
+}
+
 void check_ids(const torch::Tensor& ids, const torch::Tensor& like) {
   TORCH_CHECK(ids.device() == like.device() && ids.is_contiguous() &&
                   (ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32),
@@ -249,7 +335,7 @@ void check_ids(const torch::Tensor& ids, const torch::Tensor& like) {
   TORCH_CHECK(ids.numel() < (1 << 30), "embedding_lookup: fewer than 2^30 ids");
 }
 
-torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
+torch::Tensor lookup_raw(const torch::Tensor& table, const torch::Tensor& ids, double scale) {
   const c10::cuda::CUDAGuard guard(table.device());
   TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.is_contiguous() && table.size(0) < (1 << 30) &&
                   table.size(1) < (1 << 20), "embedding_lookup: table (rows, width), contiguous on a CUDA device");
@@ -270,7 +356,7 @@ torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
   return out;
 }
 
-torch::Tensor lookup_grad_op(torch::Tensor ids, torch::Tensor g, int64_t rows, double scale) {
+torch::Tensor lookup_grad_raw(const torch::Tensor& ids, const torch::Tensor& g, int64_t rows, double scale) {
   const c10::cuda::CUDAGuard guard(g.device());
   const int64_t N = ids.numel(), C = g.size(-1);
   TORCH_CHECK(g.is_cuda() && g.is_contiguous() && g.numel() == N * C && rows < (1 << 30) && C < (1 << 20),
@@ -293,13 +379,44 @@ torch::Tensor lookup_grad_op(torch::Tensor ids, torch::Tensor g, int64_t rows, d
   return out;
 }
 
+// the lookup and its adjoint: each is the other's backward pass
+struct LookupGrad : torch::autograd::Function<LookupGrad> {
+  static Variable forward(AutogradContext* ctx, Variable g, Variable ids, int64_t rows, double scale);
+  static variable_list backward(AutogradContext* ctx, variable_list t);
+};
+struct Lookup : torch::autograd::Function<Lookup> {
+  static Variable forward(AutogradContext* ctx, Variable table, Variable ids, double scale) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    return lookup_raw(table, ids, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    return {LookupGrad::apply(g[0].contiguous(), ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
+                              ctx->saved_data["scale"].toDouble()), Variable(), Variable()};
+  }
+};
+Variable LookupGrad::forward(AutogradContext* ctx, Variable g, Variable ids, int64_t rows, double scale) {
+  ctx->save_for_backward({ids});
+  ctx->saved_data["scale"] = scale;
+  return lookup_grad_raw(ids, g, rows, scale);
+}
+variable_list LookupGrad::backward(AutogradContext* ctx, variable_list t) {
+  return {Lookup::apply(t[0].contiguous(), ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble()),
+          Variable(), Variable(), Variable()};
+}
+
+torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
+  table = table.contiguous();
+  ids = ids.contiguous();
+  if (torch::GradMode::is_enabled() && table.requires_grad()) return Lookup::apply(table, ids, scale);
+  return lookup_raw(table, ids, scale);
+}
+
 }  // namespace
 
 void register_transformer(pybind11::module& m) {
-  m.def("attention_forward", &attention_forward);
-  m.def("attention_backward", &attention_backward);
-  m.def("attention_second", &attention_second);
+  m.def("structure_attention", &structure_attention);
   m.def("counter_dropout", &dropout_op);
   m.def("embedding_lookup", &lookup_op);
-  m.def("embedding_lookup_grad", &lookup_grad_op);
 }

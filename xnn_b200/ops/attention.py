@@ -23,7 +23,6 @@ from typing import Optional
 
 import torch
 from torch import Tensor
-from torch.autograd import Function
 
 from .. import _ext
 
@@ -33,57 +32,9 @@ _TYPES = (torch.float32, torch.float64)
 
 def _kernels():
     mod = _ext.ops()
-    if not hasattr(mod, "attention_forward"):
+    if not hasattr(mod, "structure_attention"):
         raise RuntimeError("xnn_b200 extension without the attention kernels: rebuild it (xnn_b200.build)")
     return mod
-
-
-def _rows(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-class _Attention(Function):
-    @staticmethod
-    def forward(ctx, q, k, v, ptr, mask, max_len, scale):
-        o, lse = _kernels().attention_forward(q, k, v, ptr, mask, max_len, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, ptr, mask)
-        ctx.max_len, ctx.scale = max_len, scale
-        return o
-
-    @staticmethod
-    def backward(ctx, go):
-        q, k, v, o, lse, ptr, mask = ctx.saved_tensors
-        return _AttentionGrad.apply(go, q, k, v, o, lse, ptr, mask, ctx.max_len, ctx.scale) + (None,) * 4
-
-
-class _AttentionGrad(Function):
-    """``(dq, dk, dv)``; its own derivative is the total one through ``o`` and the row statistics."""
-
-    @staticmethod
-    def forward(ctx, go, q, k, v, o, lse, ptr, mask, max_len, scale):
-        go = _rows(go)
-        ctx.save_for_backward(go, q, k, v, o, lse, ptr, mask)
-        ctx.max_len, ctx.scale = max_len, scale
-        return tuple(_kernels().attention_backward(go, q, k, v, o.detach(), lse, ptr, mask, max_len, scale))
-
-    @staticmethod
-    def backward(ctx, a, b, c):
-        return _AttentionSecond.apply(a, b, c, *ctx.saved_tensors, ctx.scale) + (None,) * 6
-
-
-class _AttentionSecond(Function):
-    """The gradients of ``<a, dq> + <b, dk> + <c, dv>`` in ``do, q, k, v``. A function of its own, so that a third
-    derivative finds it on every path to the inputs and is refused."""
-
-    @staticmethod
-    def forward(ctx, a, b, c, go, q, k, v, o, lse, ptr, mask, scale):
-        q2, k2, v2, go2 = _kernels().attention_second(_rows(a), _rows(b), _rows(c), go, q, k, v, o.detach(), lse, ptr,
-                                                      mask, scale)
-        return go2, q2, k2, v2
-
-    @staticmethod
-    def backward(ctx, *_):
-        raise RuntimeError("structure_attention on CUDA differentiates twice, not three times")
 
 
 def _formula(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, mask: Optional[Tensor], scale: float) -> Tensor:
@@ -150,9 +101,4 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, max_len: O
         return _formula(q, k, v, ptr, key_mask, scale)
     if d > MAX_WIDTH:
         raise ValueError(f"head width {d}: the kernels take up to {MAX_WIDTH}")
-    q, k, v, ptr = _rows(q), _rows(k), _rows(v), ptr.contiguous()
-    if key_mask is not None:
-        key_mask = key_mask.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _Attention.apply(q, k, v, ptr, key_mask, max_len, scale)
-    return _kernels().attention_forward(q, k, v, ptr, key_mask, max_len, scale, False)[0]
+    return _kernels().structure_attention(q, k, v, ptr, key_mask, max_len, scale)

@@ -60,31 +60,34 @@ def _split(shape: torch.Size, shared: Tuple[int, ...]) -> Tuple[int, int, int]:
     return (1, 1, outer) if common == 1 else (outer, common, inner)
 
 
-def _apply(x: Tensor, p: float, rng: Tensor, sizes: Tuple[int, int, int]) -> Tensor:
-    x = x.contiguous()
-    if x.is_cuda:
-        mod = _ext.ops()
-        if not hasattr(mod, "counter_dropout"):
-            raise RuntimeError("xnn_b200 extension without the dropout kernel: rebuild it (xnn_b200.build)")
-        return mod.counter_dropout(x, *sizes, p, rng)
+def _formula(x: Tensor, p: float, rng: Tensor, sizes: Tuple[int, int, int]) -> Tensor:
     outer, common, inner = sizes
     n = outer * inner
     words = philox(torch.arange((n + 3) // 4, device=x.device), rng).reshape(-1)[:n]
     keep = (words >= int(p * 2.0 ** 32)).view(outer, 1, inner)
     factor = 1.0 / (1.0 - p) if p < 1.0 else 0.0
-    return torch.where(keep, x.view(outer, common, inner) * factor, 0.0).view(x.shape)
+    return torch.where(keep, x.reshape(outer, common, inner) * factor, 0.0).view(x.shape)
 
 
 class _Dropout(Function):
+    """The formula with the mask formed again in the backward pass."""
+
     @staticmethod
     def forward(ctx, x, p, rng, sizes):
         ctx.save_for_backward(rng)
         ctx.p, ctx.sizes = p, sizes
-        return _apply(x, p, rng, sizes)
+        return _formula(x, p, rng, sizes)
 
     @staticmethod
     def backward(ctx, g):
         return _Dropout.apply(g, ctx.p, ctx.saved_tensors[0], ctx.sizes), None, None, None
+
+
+def _kernels():
+    mod = _ext.ops()
+    if not hasattr(mod, "counter_dropout"):
+        raise RuntimeError("xnn_b200 extension without the dropout kernel: rebuild it (xnn_b200.build)")
+    return mod
 
 
 def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -> Tensor:
@@ -106,10 +109,9 @@ def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -
     sizes = _split(x.shape, tuple(int(d) % x.dim() for d in shared))
     if 0 in x.shape:
         return x.clone()
-    rng = rng.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, p, rng, sizes)
-    return _apply(x, p, rng, sizes)
+    if x.is_cuda:
+        return _kernels().counter_dropout(x, *sizes, p, rng)
+    return _Dropout.apply(x, p, rng, sizes)
 
 
 class CounterDropout(nn.Module):

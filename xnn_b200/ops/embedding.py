@@ -22,32 +22,19 @@ def _kernels():
     return mod
 
 
-def _lookup(table: Tensor, ids: Tensor, scale: float) -> Tensor:
-    if table.is_cuda:
-        return _kernels().embedding_lookup(table, ids, scale)
-    on = (ids >= 0) & (ids < table.shape[0])
-    if table.shape[0] == 0:
-        return table.new_zeros(tuple(ids.shape) + (table.shape[1],))
-    return torch.where(on[..., None], scale * table[torch.where(on, ids, 0)], 0.0)
-
-
-def _gradient(ids: Tensor, g: Tensor, rows: int, scale: float) -> Tensor:
-    if g.is_cuda:
-        return _kernels().embedding_lookup_grad(ids, g, rows, scale)
-    on = (ids >= 0) & (ids < rows)
-    return scale * g.new_zeros(rows, g.shape[-1]).index_add_(0, ids[on].long(), g[on])
-
-
 class _Lookup(Function):
     @staticmethod
     def forward(ctx, table, ids, scale):
         ctx.save_for_backward(ids)
         ctx.rows, ctx.scale = table.shape[0], scale
-        return _lookup(table, ids, scale)
+        if table.shape[0] == 0:
+            return table.new_zeros(tuple(ids.shape) + (table.shape[1],))
+        on = (ids >= 0) & (ids < table.shape[0])
+        return torch.where(on[..., None], scale * table[torch.where(on, ids, 0)], 0.0)
 
     @staticmethod
     def backward(ctx, g):
-        return _LookupGrad.apply(g.contiguous(), ctx.saved_tensors[0], ctx.rows, ctx.scale), None, None
+        return _LookupGrad.apply(g, ctx.saved_tensors[0], ctx.rows, ctx.scale), None, None
 
 
 class _LookupGrad(Function):
@@ -55,11 +42,12 @@ class _LookupGrad(Function):
     def forward(ctx, g, ids, rows, scale):
         ctx.save_for_backward(ids)
         ctx.scale = scale
-        return _gradient(ids, g, rows, scale)
+        on = (ids >= 0) & (ids < rows)
+        return scale * g.new_zeros(rows, g.shape[-1]).index_add_(0, ids[on].long(), g[on])
 
     @staticmethod
     def backward(ctx, t):
-        return _Lookup.apply(t.contiguous(), ctx.saved_tensors[0], ctx.scale), None, None, None
+        return _Lookup.apply(t, ctx.saved_tensors[0], ctx.scale), None, None, None
 
 
 def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
@@ -70,10 +58,9 @@ def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
         raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
     if ids.device != table.device:
         raise ValueError(f"table on {table.device}, ids on {ids.device}")
-    ids, scale = ids.contiguous(), float(scale)
-    if torch.is_grad_enabled() and table.requires_grad:
-        return _Lookup.apply(table.contiguous(), ids, scale)
-    return _lookup(table.contiguous(), ids, scale)
+    if table.is_cuda:
+        return _kernels().embedding_lookup(table, ids, float(scale))
+    return _Lookup.apply(table, ids, float(scale))
 
 
 class ScaledEmbedding(nn.Embedding):
