@@ -12,15 +12,11 @@
 //             do' = P (T - r) V + P C.
 // Row-owning blocks write dq, q', do' and key-owning ones dk, dv, k', v': every sum has a fixed order
 // and there are no atomics. Statistics and accumulators have the operands' type (32 or 64 bits).
-#include <limits>
-
 #include "attention.h"
 #include "attention_tile.cuh"
 
 namespace attn {
 namespace {
-
-template <typename T> __device__ __forceinline__ T log2e() { return T(1.4426950408889634074); }
 
 template <typename T, int BQ_, int BK_, int DP_, int RI_, int TX_>
 struct Cfg {
@@ -31,22 +27,6 @@ struct Cfg {
 
 __device__ __forceinline__ bool allowed(int j, int hi, const uint8_t* mask) {
   return j < hi && (mask == nullptr || mask[j]);
-}
-
-template <typename T>
-__device__ __forceinline__ bool takes(const Params<T>& p, const Part& part) {
-  const int len = part.hi - part.lo;
-  // the parts without keys go with the longest lengths
-  return part.keys ? (len >= p.min_len && len <= p.max_len) : p.max_len == std::numeric_limits<int>::max();
-}
-
-// the share of split z of the tiles of `B` rows in [lo, hi)
-template <int B>
-__device__ __forceinline__ void split_range(int& lo, int& hi, int z, int splits) {
-  const int tiles = (hi - lo + B - 1) / B, per = (tiles + splits - 1) / splits;
-  const int end = hi;
-  hi = min(end, lo + min(tiles, (z + 1) * per) * B);
-  lo = min(end, lo + min(tiles, z * per) * B);
 }
 
 // ------------------------------------------------------------------------------------------ forward
@@ -126,7 +106,7 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
         stats[p.splits * rows + at] = l[r];
       }
     } else {
-      const bool none = m[r] == neg_inf<T>();
+      const bool none = m[r] == neg_inf<T>() && l[r] == T(0);   // NaN scores are not an empty row
       store_row<T, C::DP, C::TX>(p.out0 + ((int64_t)row * p.H + h) * p.D, acc[r], none ? T(0) : T(1) / l[r], p.D, tx);
       if (tx == 0 && p.lse) p.lse[(int64_t)h * p.N + row] = none ? -neg_inf<T>() : m[r] + lg2(l[r]);
     }
@@ -144,14 +124,13 @@ __global__ void __launch_bounds__(128) join_kernel(const Params<T> p) {
   const int64_t at = (int64_t)h * p.N + row;
   T m = neg_inf<T>();
   for (int z = 0; z < p.splits; ++z) { const T v = stats[z * rows + at]; m = v > m ? v : m; }
-  const bool none = m == neg_inf<T>();
+  const T base = m == neg_inf<T>() ? T(0) : m;
   T l = T(0);
-  for (int z = 0; z < p.splits; ++z)
-    l += none ? T(0) : pow2(stats[z * rows + at] - m) * stats[(p.splits + z) * rows + at];
+  for (int z = 0; z < p.splits; ++z) l += pow2(stats[z * rows + at] - base) * stats[(p.splits + z) * rows + at];
+  const bool none = m == neg_inf<T>() && l == T(0);
   for (int d = lane; d < p.D; d += 32) {
     T a = T(0);
-    for (int z = 0; z < p.splits; ++z)
-      if (!none) a += pow2(stats[z * rows + at] - m) * p.work[(z * rows + at) * p.D + d];
+    for (int z = 0; z < p.splits; ++z) a += pow2(stats[z * rows + at] - base) * p.work[(z * rows + at) * p.D + d];
     p.out0[((int64_t)row * p.H + h) * p.D + d] = none ? T(0) : a / l;
   }
   if (lane == 0 && p.lse) p.lse[at] = none ? -neg_inf<T>() : m + lg2(l);

@@ -1,4 +1,4 @@
-// Host entry points of the structure-attention kernels (attention.cu).
+// Host entry points of the structure-attention kernels (attention.cu, attention_tc.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -16,5 +16,14 @@ template <typename T> cudaError_t backward_dkv(const Params<T>&, bool small, cud
 template <typename T> cudaError_t backward_short(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t second_rows(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t second_keys(const Params<T>&, cudaStream_t);
+
+// tensor-core forms for float32; `work` holds the operands' images (the byte counts say how much), `status` is set
+// where a bounded wait ran out
+int64_t tc_forward_bytes(const Params<float>&);
+int64_t tc_backward_bytes(const Params<float>&);
+cudaError_t tc_forward(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_backward_prepare(const Params<float>&, char* work, cudaStream_t);
+cudaError_t tc_backward_dq(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_backward_dkv(const Params<float>&, char* work, int* status, cudaStream_t);
 
 }  // namespace attn

@@ -1,0 +1,711 @@
+// Structure attention of float32 operands on the tensor cores (tcgen05), for structures of some hundred atoms on.
+//
+// The streamed operands are first written as images of bf16 parts (attention_tc.cuh), once per call: 10 bytes
+// moved an element against the hundred times that every image is read again from L2. A block then owns 128
+// rows (the lanes of tensor memory), keeps their parts in tensor memory and lets bulk copies bring the
+// images through shared memory; products run with the left operand in tensor memory, since with both in
+// shared memory a 128 x 64 x 16 step would read 6 KB in the 32 cycles that it takes.
+#include <limits>
+
+#include "attention.h"
+#include "attention_tc.cuh"
+
+namespace attn {
+namespace {
+
+struct Source { const float* at; int64_t row, head; int heads; const uint8_t* mask; char* out; };
+struct Sources { Source s[4]; };
+
+// writes the images of up to four tensors: a block per (slot, head, tensor); zeros behind the structure's last
+// row, behind column D and where the mask is 0
+template <int DP>
+__global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const Sources src, int slots) {
+  const Source s = src.s[blockIdx.z];
+  if ((int)blockIdx.y >= s.heads) return;
+  Part part;
+  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
+  const float* g = s.at + blockIdx.y * s.head;
+  const bool vec = vec_ok(s.at, s.row, s.head, p.D);
+  uint4* out = reinterpret_cast<uint4*>(s.out + ((int64_t)blockIdx.y * slots + blockIdx.x) * Image<DP>::BYTES);
+#pragma unroll 2
+  for (int i = threadIdx.x; i < SLOT * DP / 8; i += 256) {
+    const int r = i / DP * 8 + i % 8, c = i / 8 % (DP / 8) * 8, row = part.row + r;
+    alignas(16) float v[8] = {};
+    if (row < part.hi && (s.mask == nullptr || s.mask[row])) {
+      const float* x = g + row * s.row + c;
+      if (vec && c + 8 <= p.D) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(x);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(x + 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < p.D) v[e] = x[e];
+      }
+    }
+    uint32_t w[3][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_pair(v[2 * e], v[2 * e + 1], w[0][e], w[1][e], w[2][e]);
+#pragma unroll
+    for (int x = 0; x < 3; ++x) out[x * (Image<DP>::PLANE / 16) + i] = make_uint4(w[x][0], w[x][1], w[x][2], w[x][3]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ forward
+// Warps 0-3 own a row each thread; a lane of warp 4 copies and issues. Tensor memory: the rows' parts, one
+// region that holds S and then the parts of P in its place, and the product P V of one tile, which the rows'
+// threads add to their accumulators in registers (rounded to nearest, which a sum over thousands of keys
+// inside the tensor core is not). At 64 columns that is 256 of 512 columns and 96 KB, so two blocks share an SM
+// and one's softmax runs under the other's products.
+template <int DP>
+struct Fwd {
+  static constexpr int Q = 0, S = 3 * DP / 2, O = S + 96, COLUMNS = O + DP <= 256 ? 256 : 512;
+  static constexpr int SMEM = 4 * Image<DP>::BYTES + 128;
+  static constexpr int BLOCKS = COLUMNS == 256 ? 2 : 1;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Params<float> p, const Images ik, const Images iv,
+                                                                      int* status) {
+  using F = Fwd<DP>;
+  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  extern __shared__ __align__(128) char smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 4 * BYTES);
+  uint64_t *full_k = bars, *full_v = bars + 2, *s_done = bars + 4, *p_ready = bars + 5;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 6);
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 7);
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int h = blockIdx.y, hk = h / (p.H / p.HK);
+  int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
+  split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
+  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
+  if (warp == 4) tmem_alloc(tmem_slot, F::COLUMNS);
+  if (tid == 0) {
+    for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
+    tc::mbar_init(p_ready, 4);
+    *dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int row = part.row + tid;
+  const bool on = tid < 128 && row < part.hi;
+  if (warp < 4 && n > 0) {
+    stage_row<DP>(tmem + ((uint32_t)warp << 21) + F::Q, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D,
+                  p.scale * log2e<float>());
+    tmem_st_wait();
+    tc::tc_fence_before();
+  }
+  __syncthreads();
+  tc::tc_fence_after();
+
+  if (warp == 4) {
+    if (lane == 0 && n > 0) {
+      const auto load = [&](uint64_t* bar, int at, const Images& im, int i) {
+        tc::mbar_arrive_expect_tx(bar, BYTES);
+        tc::bulk_g2s(smem + at * BYTES, image<DP>(im, hk, slot0 + i), BYTES, bar);
+      };
+      const uint32_t sk = tc::smem_u32(smem), sv = sk + 2 * BYTES;
+      const uint32_t is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
+      const auto scores = [&](int i) {
+        mma_parts<DP / 16>(tmem + F::S, tmem + F::Q, DP / 2, sk + (i & 1) * BYTES, PLANE, 256, 128, DP * 16, is);
+        tc::commit_to(s_done);
+      };
+      int loaded_k = min(n, 2), loaded_v = min(n, 2);
+      for (int i = 0; i < loaded_k; ++i) {
+        load(full_k + i, i, ik, i);
+        load(full_v + i, 2 + i, iv, i);
+      }
+      bool ok = wait(full_k, 0, dead, status);
+      if (ok) scores(0);
+      for (int i = 0; ok && i < n; ++i) {
+        // the probabilities of tile i are there, so S(i) and P V(i - 1) are done and their images free
+        if (!(ok = wait(p_ready, i & 1, dead, status))) break;
+        tc::tc_fence_after();
+        if (i + 2 < n) { load(full_k + (i & 1), i & 1, ik, i + 2); loaded_k = i + 3; }
+        if (i > 0 && i + 1 < n) { load(full_v + ((i + 1) & 1), 2 + ((i + 1) & 1), iv, i + 1); loaded_v = i + 2; }
+        if (!(ok = wait(full_v + (i & 1), (i >> 1) & 1, dead, status))) break;
+        mma_parts<SLOT / 16>(tmem + F::O, tmem + F::S, SLOT / 2, sv + (i & 1) * BYTES, PLANE, DP * 32, DP * 16, 128, io);
+        if (i + 1 < n) {
+          if (!(ok = wait(full_k + ((i + 1) & 1), ((i + 1) >> 1) & 1, dead, status))) break;
+          scores(i + 1);
+        } else {
+          tc::commit_to(s_done);
+        }
+      }
+      if (!ok) {                                        // copies in flight must land before the block ends
+        for (int i = max(0, loaded_k - 2); i < loaded_k; ++i) tc::mbar_wait(full_k + (i & 1), (i >> 1) & 1, SPINS);
+        for (int i = max(0, loaded_v - 2); i < loaded_v; ++i) tc::mbar_wait(full_v + (i & 1), (i >> 1) & 1, SPINS);
+      }
+    }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = tmem + ((uint32_t)warp << 21);
+    float m = neg_inf<float>(), l = 0.f, f = 1.f, acc[DP];
+#pragma unroll
+    for (int d = 0; d < DP; ++d) acc[d] = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const uint64_t bits = allowed_bits(k_lo + i * SLOT, k_hi, p.mask);
+      if (!(ok = wait_all(s_done, i & 1, dead, status))) break;
+      tc::tc_fence_after();
+      float s[SLOT];
+      tmem_ld32(lanes + F::S, s);
+      tmem_ld32(lanes + F::S + 32, s + 32);
+      tmem_ld_wait();
+      if (bits != ~0ull) {
+#pragma unroll
+        for (int j = 0; j < SLOT; ++j)
+          if (!((bits >> j) & 1)) s[j] = neg_inf<float>();
+      }
+      float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
+#pragma unroll
+      for (int j = 4; j < SLOT; j += 4) {
+        t0 = fmaxf(t0, s[j]); t1 = fmaxf(t1, s[j + 1]); t2 = fmaxf(t2, s[j + 2]); t3 = fmaxf(t3, s[j + 3]);
+      }
+      const float mn = fmaxf(m, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
+      const float base = mn == neg_inf<float>() ? 0.f : mn;
+      const float fn = ex2(m - base);
+      m = mn;
+      float u0 = 0.f, u1 = 0.f;
+#pragma unroll
+      for (int c = 0; c < SLOT; c += 16) {
+#pragma unroll
+        for (int j = c; j < c + 16; j += 2) {
+          s[j] = ex2(s[j] - base);
+          s[j + 1] = ex2(s[j + 1] - base);
+          u0 += s[j];
+          u1 += s[j + 1];
+        }
+        store_parts16(lanes + F::S + c / 2, SLOT / 2, s + c);
+      }
+      l = fmaf(l, fn, u0 + u1);
+      if (i > 0) {                                      // P V of the tile before, relative to its maximum
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          tmem_ld32(lanes + F::O + c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
+        }
+      }
+      f = fn;
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(p_ready);
+    }
+    if (ok && n > 0 && (ok = wait_all(s_done, n & 1, dead, status))) {
+      tc::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        tmem_ld32(lanes + F::O + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
+      }
+    }
+    if (on) {
+      const bool none = m == neg_inf<float>() && l == 0.f;
+      const bool split = p.splits > 1;
+      const int64_t rows = (int64_t)p.H * p.N, at = blockIdx.z * rows + (int64_t)h * p.N + row;
+      const float g = !ok ? __int_as_float(0x7fc00000) : split ? 1.f : none ? 0.f : 1.f / l;
+      float* out = split ? p.work + at * p.D : p.out0 + ((int64_t)row * p.H + h) * p.D;
+#pragma unroll
+      for (int d = 0; d < DP; d += 4) {
+        if (p.D % 4 == 0) {
+          if (d < p.D) *reinterpret_cast<float4*>(out + d) = make_float4(g * acc[d], g * acc[d + 1], g * acc[d + 2], g * acc[d + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < p.D) out[d + e] = g * acc[d + e];
+        }
+      }
+      if (split) {
+        float* stats = p.work + p.splits * rows * p.D;
+        stats[at] = m;
+        stats[p.splits * rows + at] = l;
+      } else if (p.lse) {
+        p.lse[(int64_t)h * p.N + row] = none ? -neg_inf<float>() : m + log2f(l);
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc::tc_fence_after();
+    tmem_free(tmem, F::COLUMNS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward
+// L and D of the rows of a slot, D = do.o: 64 + 64 numbers a (head, slot), L = +inf behind the last row, so that P is zero there
+__global__ void __launch_bounds__(256) stats_kernel(const Params<float> p, float* __restrict__ out, int slots) {
+  Part part;
+  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
+  const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float* at = out + ((int64_t)h * slots + blockIdx.x) * 2 * SLOT;
+  for (int r = warp; r < SLOT; r += 8) {
+    const int row = part.row + r;
+    float s = 0.f, L = -neg_inf<float>();
+    if (row < part.hi) {
+      const float *a = p.go + row * p.gos + h * p.goh, *b = p.o + row * p.os + h * p.oh;
+      for (int d = lane; d < p.D; d += 32) s = fmaf(a[d], b[d], s);
+      L = p.lse[(int64_t)h * p.N + row];
+    }
+    s = row_sum<32>(s);
+    if (lane == 0) {
+      at[r] = L;
+      at[SLOT + r] = s;
+    }
+  }
+}
+
+// Eight warps of rows: warp w reaches the lanes 32 (w % 4) .. of tensor memory and takes half w / 4 of the columns;
+// a ninth copies and issues. A ring of three stages holds the streamed images.
+constexpr int BWD_THREADS = 288, STAGES = 3;
+
+template <int DP>
+struct Bwd {
+  static constexpr int PARTS = 3 * DP / 2;
+  static constexpr int STAGE = 2 * Image<DP>::BYTES + 2 * SLOT * 4;
+  static constexpr int SMEM = STAGES * STAGE + 128;
+  // dq: parts of q and do, S, dP, the parts of dS, the product of one tile
+  static constexpr int Q_S = 2 * PARTS, Q_DP = Q_S + SLOT, Q_DS = Q_DP + SLOT, Q_OUT = Q_DS + 96;
+  // dk, dv: parts of k and v, S^T then P^T, dP^T then dS^T, the products of one tile
+  static constexpr int K_S = 2 * PARTS, K_DP = K_S + 96, K_DV = K_DP + 96, K_DK = K_DV + DP;
+  static_assert(Q_OUT + DP <= 512 && K_DK + DP <= 512, "tensor memory");
+};
+
+struct Block {                                          // what the two kernels set up alike
+  uint64_t *full, *bars;
+  volatile int* dead;
+  uint32_t tmem;
+  int warp, lane;
+};
+
+// barriers, tensor memory and the parts of the two resident operands
+template <int DP>
+__device__ __forceinline__ Block set_up(char* smem, const Part& part, const float* a, int64_t as, bool av, float af,
+                                        const float* b, int64_t bs, bool bv, int D, const uint8_t* mask, int n) {
+  using B = Bwd<DP>;
+  Block k;
+  k.full = reinterpret_cast<uint64_t*>(smem + STAGES * B::STAGE);
+  k.bars = k.full + STAGES;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(k.bars + 8);
+  k.dead = reinterpret_cast<volatile int*>(k.bars + 9);
+  k.warp = threadIdx.x / 32;
+  k.lane = threadIdx.x % 32;
+  if (k.warp == 8) tmem_alloc(slot, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) tc::mbar_init(k.full + i, 1);
+    tc::mbar_init(k.bars, 1);
+    tc::mbar_init(k.bars + 1, 1);
+    tc::mbar_init(k.bars + 2, 8);
+    tc::mbar_init(k.bars + 3, 8);
+    for (int i = 4; i < 8; ++i) tc::mbar_init(k.bars + i, 2);
+    *k.dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  k.tmem = *slot;
+  if (k.warp < 8 && n > 0) {
+    const int row = part.row + (threadIdx.x & 127);
+    const bool on = row < part.hi && (mask == nullptr || mask[row]);
+    const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
+    if (k.warp < 4) stage_row<DP>(lanes, a + row * as, on, av, D, af);
+    else stage_row<DP>(lanes + B::PARTS, b + row * bs, on, bv, D, 1.f);
+    tmem_st_wait();
+    tc::tc_fence_before();
+  }
+  __syncthreads();
+  tc::tc_fence_after();
+  return k;
+}
+
+__device__ __forceinline__ void tear_down(const Block& k) {
+  tc::tc_fence_before();
+  __syncthreads();
+  if (k.warp == 8) {
+    tc::tc_fence_after();
+    tmem_free(k.tmem, 512);
+  }
+}
+
+// dq of 128 queries. S and dP of the next tile run while the rows' threads form dS of this one.
+template <int DP>
+__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<float> p, const Images ik, const Images iv,
+                                                               const float* __restrict__ stats, int* status) {
+  using B = Bwd<DP>;
+  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  extern __shared__ __align__(128) char smem[];
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  const int h = blockIdx.y, hk = h / (p.H / p.HK);
+  int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
+  split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
+  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
+  const Block k = set_up<DP>(smem, part, p.q + h * p.qh, p.qs, vec_ok(p.q, p.qs, p.qh, p.D), p.scale * log2e<float>(),
+                             p.go + h * p.goh, p.gos, vec_ok(p.go, p.gos, p.goh, p.D), p.D, nullptr, n);
+  uint64_t *sd_done = k.bars, *dq_done = k.bars + 1, *taken = k.bars + 2, *ds_ready = k.bars + 3;
+  if (k.warp == 8) {
+    if (k.lane == 0 && n > 0) {
+      const auto load = [&](int i) {
+        char* at = smem + (i % STAGES) * B::STAGE;
+        tc::mbar_arrive_expect_tx(k.full + i % STAGES, 2 * BYTES);
+        tc::bulk_g2s(at, image<DP>(ik, hk, slot0 + i), BYTES, k.full + i % STAGES);
+        tc::bulk_g2s(at + BYTES, image<DP>(iv, hk, slot0 + i), BYTES, k.full + i % STAGES);
+      };
+      const uint32_t base = tc::smem_u32(smem), is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
+      const auto scores = [&](int i) {
+        const uint32_t at = base + (i % STAGES) * B::STAGE;
+        mma_parts<DP / 16>(k.tmem + B::Q_S, k.tmem, DP / 2, at, PLANE, 256, 128, DP * 16, is);
+        mma_parts<DP / 16>(k.tmem + B::Q_DP, k.tmem + B::PARTS, DP / 2, at + BYTES, PLANE, 256, 128, DP * 16, is);
+        tc::commit_to(sd_done);
+      };
+      int loaded = min(n, STAGES);
+      for (int i = 0; i < loaded; ++i) load(i);
+      bool ok = wait(k.full, 0, k.dead, status);
+      if (ok) scores(0);
+      for (int i = 0; ok && i < n; ++i) {
+        if (!(ok = wait(taken, i & 1, k.dead, status))) break;
+        tc::tc_fence_after();
+        if (i + 1 < n) {
+          if (!(ok = wait(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
+          scores(i + 1);
+        }
+        if (!(ok = wait(ds_ready, i & 1, k.dead, status))) break;
+        tc::tc_fence_after();
+        // dq of tile i - 1 is done: its stage is free
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
+        mma_parts<SLOT / 16>(k.tmem + B::Q_OUT, k.tmem + B::Q_DS, SLOT / 2, base + (i % STAGES) * B::STAGE, PLANE, DP * 32,
+                             DP * 16, 128, io);
+        tc::commit_to(dq_done);
+      }
+      if (!ok)
+        for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
+    const int half = k.warp / 4, r = threadIdx.x & 127, row = part.row + r;
+    const bool on = row < part.hi;
+    float L = -neg_inf<float>(), D = 0.f, acc[DP / 2];
+    if (on && n > 0) {
+      const float* at = stats + ((int64_t)h * ik.slots + first_slot(part) + (row - part.lo) / SLOT) * 2 * SLOT;
+      L = at[(row - part.lo) % SLOT];
+      D = at[SLOT + (row - part.lo) % SLOT];
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 2; ++d) acc[d] = 0.f;
+    bool ok = true;
+    const auto add = [&] {
+#pragma unroll
+      for (int c = 0; c < DP / 2; c += 16) {
+        float o[16];
+        tc::tmem_ld16(lanes + B::Q_OUT + half * (DP / 2) + c, o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
+      }
+    };
+    for (int i = 0; i < n; ++i) {
+      const uint32_t bits = (uint32_t)(allowed_bits(k_lo + i * SLOT, k_hi, p.mask) >> (32 * half));
+      if (!(ok = wait_all(sd_done, i & 1, k.dead, status))) break;
+      tc::tc_fence_after();
+      float s[32], dp[32];
+      tmem_ld32(lanes + B::Q_S + 32 * half, s);
+      tmem_ld32(lanes + B::Q_DP + 32 * half, dp);
+      tmem_ld_wait();
+      tc::tc_fence_before();
+      arrive(taken);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s[j] = ex2(s[j] - L) * (dp[j] - D);
+      if (bits != ~0u) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (!((bits >> j) & 1)) s[j] = 0.f;
+      }
+      if (i > 0) {
+        if (!(ok = wait_all(dq_done, (i - 1) & 1, k.dead, status))) break;
+        tc::tc_fence_after();
+        add();
+      }
+      store_parts16(lanes + B::Q_DS + 16 * half, SLOT / 2, s);
+      store_parts16(lanes + B::Q_DS + 16 * half + 8, SLOT / 2, s + 16);
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(ds_ready);
+    }
+    if (ok && n > 0 && (ok = wait_all(dq_done, (n - 1) & 1, k.dead, status))) {
+      tc::tc_fence_after();
+      add();
+    }
+    if (on) {
+      const float g = ok ? p.scale : __int_as_float(0x7fc00000);
+      float* out = (p.splits > 1 ? p.work + (int64_t)blockIdx.z * p.N * p.H * p.D : p.out0) + ((int64_t)row * p.H + h) * p.D;
+#pragma unroll
+      for (int d = 0; d < DP / 2; d += 4) {
+        const int c = half * (DP / 2) + d;
+        if (p.D % 4 == 0) {
+          if (c < p.D) *reinterpret_cast<float4*>(out + c) = make_float4(g * acc[d], g * acc[d + 1], g * acc[d + 2], g * acc[d + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < p.D) out[c + e] = g * acc[d + e];
+        }
+      }
+    }
+  }
+  tear_down(k);
+}
+
+// dk and dv of 128 keys of one key head, over the queries of every head that shares it. Two chains share the
+// tensor cores: while the threads form P^T of a tile, dK of the tile before and dP^T of this one run; while they form
+// dS^T, dV of this tile and S^T of the next.
+template <int DP>
+__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<float> p, const Images iq, const Images io_,
+                                                                const float* __restrict__ stats, int* status) {
+  using B = Bwd<DP>;
+  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  extern __shared__ __align__(128) char smem[];
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  const int hk = blockIdx.y, group = p.H / p.HK;
+  int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
+  split_range<SLOT>(q_lo, q_hi, blockIdx.z, p.splits);
+  const int tiles = (q_hi - q_lo + SLOT - 1) / SLOT, n = tiles * group, slot0 = first_slot(part) + (q_lo - part.lo) / SLOT;
+  const Block k = set_up<DP>(smem, part, p.k + hk * p.kh, p.ks, vec_ok(p.k, p.ks, p.kh, p.D), p.scale * log2e<float>(),
+                             p.v + hk * p.vh, p.vs, vec_ok(p.v, p.vs, p.vh, p.D), p.D, p.mask, n);
+  uint64_t *s_done = k.bars, *dp_done = k.bars + 1, *p_ready = k.bars + 2, *ds_ready = k.bars + 3;
+  if (k.warp == 8) {
+    if (k.lane == 0 && n > 0) {
+      const auto load = [&](int i) {
+        char* at = smem + (i % STAGES) * B::STAGE;
+        uint64_t* bar = k.full + i % STAGES;
+        const int h = hk * group + i / tiles, slot = slot0 + i % tiles;
+        tc::mbar_arrive_expect_tx(bar, B::STAGE);
+        tc::bulk_g2s(at, image<DP>(iq, h, slot), BYTES, bar);
+        tc::bulk_g2s(at + BYTES, image<DP>(io_, h, slot), BYTES, bar);
+        tc::bulk_g2s(at + 2 * BYTES, stats + ((int64_t)h * iq.slots + slot) * 2 * SLOT, 2 * SLOT * 4, bar);
+      };
+      const uint32_t base = tc::smem_u32(smem), is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
+      const auto stage = [&](int i) { return base + (i % STAGES) * B::STAGE; };
+      const auto scores = [&](int i) {
+        mma_parts<DP / 16>(k.tmem + B::K_S, k.tmem, DP / 2, stage(i), PLANE, 256, 128, DP * 16, is);
+        tc::commit_to(s_done);
+      };
+      const auto dots = [&](int i) {
+        mma_parts<DP / 16>(k.tmem + B::K_DP, k.tmem + B::PARTS, DP / 2, stage(i) + BYTES, PLANE, 256, 128, DP * 16, is);
+        tc::commit_to(dp_done);
+      };
+      int loaded = min(n, STAGES);
+      for (int i = 0; i < loaded; ++i) load(i);
+      bool ok = wait(k.full, 0, k.dead, status);
+      if (ok) {
+        scores(0);
+        dots(0);
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        if (!(ok = wait(p_ready, i & 1, k.dead, status))) break;
+        tc::tc_fence_after();
+        mma_parts<SLOT / 16>(k.tmem + B::K_DV, k.tmem + B::K_S, SLOT / 2, stage(i) + BYTES, PLANE, DP * 32, DP * 16, 128, io);
+        if (i + 1 < n) {
+          if (!(ok = wait(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
+          scores(i + 1);
+        } else {
+          tc::commit_to(s_done);
+        }
+        if (!(ok = wait(ds_ready, i & 1, k.dead, status))) break;
+        tc::tc_fence_after();
+        // dK of tile i - 1, the last to read its stage, is done
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
+        mma_parts<SLOT / 16>(k.tmem + B::K_DK, k.tmem + B::K_DP, SLOT / 2, stage(i), PLANE, DP * 32, DP * 16, 128, io);
+        if (i + 1 < n) dots(i + 1);
+        else tc::commit_to(dp_done);
+      }
+      if (!ok)
+        for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
+    const int half = k.warp / 4, row = part.row + (threadIdx.x & 127);
+    uint64_t* both = k.bars + 4 + (k.warp & 3);
+    // the first half of the warps adds up dV, the second dK
+    float acc[DP];
+#pragma unroll
+    for (int d = 0; d < DP; ++d) acc[d] = 0.f;
+    const auto add = [&](int column) {
+#pragma unroll
+      for (int c = 0; c < DP; c += 16) {
+        float o[16];
+        tc::tmem_ld16(lanes + column + c, o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
+      }
+    };
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const float* st = reinterpret_cast<const float*>(smem + (i % STAGES) * B::STAGE + 2 * BYTES) + 32 * half;
+      float s[32], dp[32];
+      if (!(ok = wait_all(s_done, i & 1, k.dead, status))) break;
+      // the statistics came with the tile's images: its barrier is passed (the issuing lane waited for it),
+      // this thread's own wait makes them visible to it
+      if (!(ok = wait_all(k.full + i % STAGES, (i / STAGES) & 1, k.dead, status))) break;
+      tc::tc_fence_after();
+      tmem_ld32(lanes + B::K_S + 32 * half, s);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 L = *reinterpret_cast<const float4*>(st + j);
+        s[j] = ex2(s[j] - L.x); s[j + 1] = ex2(s[j + 1] - L.y); s[j + 2] = ex2(s[j + 2] - L.z); s[j + 3] = ex2(s[j + 3] - L.w);
+      }
+      // the other half's warp of these lanes has read its S too before either writes P over it
+      arrive(both);
+      if (!(ok = wait_all(both, 0, k.dead, status))) break;
+      if (half == 0 && i > 0) add(B::K_DV);
+      store_parts16(lanes + B::K_S + 16 * half, SLOT / 2, s);
+      store_parts16(lanes + B::K_S + 16 * half + 8, SLOT / 2, s + 16);
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(p_ready);
+      if (!(ok = wait_all(dp_done, i & 1, k.dead, status))) break;
+      tc::tc_fence_after();
+      tmem_ld32(lanes + B::K_DP + 32 * half, dp);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 D = *reinterpret_cast<const float4*>(st + SLOT + j);
+        s[j] *= dp[j] - D.x; s[j + 1] *= dp[j + 1] - D.y; s[j + 2] *= dp[j + 2] - D.z; s[j + 3] *= dp[j + 3] - D.w;
+      }
+      arrive(both);
+      if (!(ok = wait_all(both, 1, k.dead, status))) break;
+      if (half == 1 && i > 0) add(B::K_DK);
+      store_parts16(lanes + B::K_DP + 16 * half, SLOT / 2, s);
+      store_parts16(lanes + B::K_DP + 16 * half + 8, SLOT / 2, s + 16);
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(ds_ready);
+    }
+    if (ok && n > 0 && (ok = wait_all(s_done, n & 1, k.dead, status)) && (ok = wait_all(dp_done, n & 1, k.dead, status))) {
+      tc::tc_fence_after();
+      add(half ? B::K_DK : B::K_DV);
+    }
+    if (row < part.hi) {
+      const bool hidden = p.mask != nullptr && !p.mask[row];
+      const float g = !ok ? __int_as_float(0x7fc00000) : half ? p.scale : 1.f;
+      const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)row * p.HK + hk) * p.D;
+      float* out = p.splits > 1 ? p.work + ((half ? 0 : p.splits) + (int64_t)blockIdx.z) * all + at : (half ? p.out1 : p.out2) + at;
+#pragma unroll
+      for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : g * acc[d];
+#pragma unroll
+      for (int d = 0; d < DP; d += 4) {
+        if (p.D % 4 == 0) {
+          if (d < p.D) *reinterpret_cast<float4*>(out + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < p.D) out[d + e] = acc[d + e];
+        }
+      }
+    }
+  }
+  tear_down(k);
+}
+
+template <typename K>
+cudaError_t raise_smem(K kernel, size_t bytes) {
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int DP>
+cudaError_t write_images(const Params<float>& p, const Sources& src, int count, int slots, cudaStream_t s) {
+  image_kernel<DP><<<dim3(slots, p.H, count), 256, 0, s>>>(p, src, slots);
+  return cudaGetLastError();
+}
+
+int image_slots(const Params<float>& p) { return p.N / SLOT + p.num + 2; }
+
+template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { return (int64_t)heads * image_slots(p) * Image<DP>::BYTES; }
+
+template <int DP>
+cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  const int slots = image_slots(p);
+  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK);
+  Sources src{};
+  src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, ik};
+  src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
+  cudaError_t e = write_images<DP>(p, src, 2, slots, s);
+  if (e != cudaSuccess) return e;
+  if ((e = raise_smem(tc_fwd_kernel<DP>, Fwd<DP>::SMEM)) != cudaSuccess) return e;
+  tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), 160, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t prepare_dp(const Params<float>& p, char* work, cudaStream_t s) {
+  const int slots = image_slots(p);
+  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
+  float* stats = reinterpret_cast<float*>(io + image_bytes<DP>(p, p.H));
+  Sources src{};
+  src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, ik};
+  src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
+  src.s[2] = {p.q, p.qs, p.qh, p.H, nullptr, iq};
+  src.s[3] = {p.go, p.gos, p.goh, p.H, nullptr, io};
+  const cudaError_t e = write_images<DP>(p, src, 4, slots, s);
+  if (e != cudaSuccess) return e;
+  stats_kernel<<<dim3(slots, p.H), 256, 0, s>>>(p, stats, slots);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t dq_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  const int slots = image_slots(p);
+  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK);
+  const float* stats = reinterpret_cast<const float*>(iv + image_bytes<DP>(p, p.HK) + 2 * image_bytes<DP>(p, p.H));
+  const cudaError_t e = raise_smem(tc_dq_kernel<DP>, Bwd<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  tc_dq_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, stats, status);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  const int slots = image_slots(p);
+  char *iq = work + 2 * image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
+  const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
+  const cudaError_t e = raise_smem(tc_dkv_kernel<DP>, Bwd<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  tc_dkv_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{iq, slots}, Images{io, slots}, stats, status);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int64_t tc_forward_bytes(const Params<float>& p) {
+  return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK) : p.D <= 64 ? image_bytes<64>(p, p.HK) : image_bytes<128>(p, p.HK));
+}
+int64_t tc_backward_bytes(const Params<float>& p) {
+  return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK + p.H) : image_bytes<64>(p, p.HK + p.H)) +
+         (int64_t)p.H * image_slots(p) * 2 * SLOT * 4;
+}
+cudaError_t tc_forward(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  return p.D <= 32 ? forward_dp<32>(p, work, status, s) : p.D <= 64 ? forward_dp<64>(p, work, status, s) : forward_dp<128>(p, work, status, s);
+}
+cudaError_t tc_backward_prepare(const Params<float>& p, char* work, cudaStream_t s) {
+  return p.D <= 32 ? prepare_dp<32>(p, work, s) : prepare_dp<64>(p, work, s);
+}
+cudaError_t tc_backward_dq(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  return p.D <= 32 ? dq_dp<32>(p, work, status, s) : dq_dp<64>(p, work, status, s);
+}
+cudaError_t tc_backward_dkv(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  return p.D <= 32 ? dkv_dp<32>(p, work, status, s) : dkv_dp<64>(p, work, status, s);
+}
+
+}  // namespace attn

@@ -1,0 +1,187 @@
+// Pieces of the tensor-core attention kernels: float32 operands as three bf16 parts, their images in memory, tcgen05 issue
+// with the left operand in tensor memory, and bounded waits.
+//
+// A float32 number is exactly x1 + x2 + x3 with bf16 parts (8 significant bits each, rounded to nearest, the
+// remainders exact), so a product of two is six products of parts up to terms below 2^-24 of it:
+//   x3 y1 + x1 y3 + x2 y2 + x2 y1 + x1 y2 + x1 y1,
+// added by the tensor cores in 32 bits from the smallest to the largest. Six bf16 products cost what three
+// TF32 products would and keep 24 bits instead of 22, in six bytes an element instead of eight.
+#pragma once
+#include "attention_tile.cuh"
+#include "tc_common.cuh"
+
+namespace attn {
+
+constexpr int PLANES = 3, SLOT = 64;                   // bf16 parts of a number, rows of an image
+
+// An image holds SLOT rows of one head as PLANES planes of bf16 core matrices (8 rows x 16 bytes, 128 bytes
+// each): element (r, d) of a plane at (r / 8) DP 16 + (d / 8) 128 + (r % 8) 16 + (d % 8) 2 bytes. As a K-major operand
+// (rows x d) its strides are 128 between columns of 16 bytes and DP 16 between groups of 8 rows; as an MN-major one
+// (d x rows) the two change places. One bulk copy brings an image to shared memory.
+template <int DP> struct Image {
+  static constexpr int PLANE = SLOT * DP * 2, BYTES = PLANES * PLANE;
+};
+
+struct Images {                                        // of a tensor: head h, slot t at ((h slots) + t) BYTES
+  const char* at;
+  int slots;
+};
+
+template <int DP>
+__device__ __forceinline__ const char* image(const Images& im, int head, int slot) {
+  return im.at + ((int64_t)head * im.slots + slot) * Image<DP>::BYTES;
+}
+
+// the slot of a part's first rows (parts start at slots as they do at tiles of SLOT rows)
+__device__ __forceinline__ int first_slot(const Part& part) { return part.lo / SLOT + part.index; }
+
+// two numbers as three packed pairs of bf16, the first number in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  p0 = pack_bf16(a, b);
+  a -= __uint_as_float(p0 << 16);
+  b -= __uint_as_float(p0 & 0xffff0000u);
+  p1 = pack_bf16(a, b);
+  a -= __uint_as_float(p1 << 16);
+  b -= __uint_as_float(p1 & 0xffff0000u);
+  p2 = pack_bf16(a, b);
+}
+
+__device__ __forceinline__ uint32_t idesc_bf16(int n, int b_mn_major) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+
+// D (128 x N, tensor memory) (+)= A (tensor memory) B (shared memory)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y b_plane bytes,
+// K = 16 k steps of 8 columns of A and b_step bytes of B
+template <int KSTEPS>
+__device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_plane, uint32_t b, uint32_t b_plane,
+                                          uint32_t b_step, uint32_t lbo, uint32_t sbo, uint32_t idesc) {
+  constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k)
+      mma_ts(d, a + X[i] * a_plane + 8 * k, tc::make_desc2(b + Y[i] * b_plane + k * b_step, lbo, sbo), idesc, i + k > 0);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// sixteen neighbouring numbers of a row as three planes of eight columns
+__device__ __forceinline__ void store_parts16(uint32_t addr, uint32_t plane, const float* v) {
+  uint32_t a[8], b[8], c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) split_pair(v[2 * j], v[2 * j + 1], a[j], b[j], c[j]);
+  tmem_st8(addr, a);
+  tmem_st8(addr + plane, b);
+  tmem_st8(addr + 2 * plane, c);
+}
+
+// a row of D numbers times f (zero where `on` is false) as three planes of DP / 2 columns
+template <int DP>
+__device__ __forceinline__ void stage_row(uint32_t addr, const float* row, bool on, bool vec, int D, float f) {
+#pragma unroll
+  for (int c = 0; c < DP; c += 16) {
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on && c + e < D) {
+        if (vec) {
+          x = *reinterpret_cast<const float4*>(row + c + e);
+        } else {
+          x.x = row[c + e];
+          if (c + e + 1 < D) x.y = row[c + e + 1];
+          if (c + e + 2 < D) x.z = row[c + e + 2];
+          if (c + e + 3 < D) x.w = row[c + e + 3];
+        }
+      }
+      v[e] = f * x.x; v[e + 1] = f * x.y; v[e + 2] = f * x.z; v[e + 3] = f * x.w;
+    }
+    store_parts16(addr + c / 2, DP / 2, v);
+  }
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(tc::smem_u32(slot)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+}
+// one arrival a warp
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(tc::smem_u32(bar)) : "memory");
+}
+
+// one phase of a barrier; false after SPINS polls or once another role of the block gave up. Whoever gives
+// up first records it; the block then writes NaN instead of results.
+constexpr int SPINS = 1 << 20;
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* dead, int* status) {
+  for (int n = 0; n < SPINS; ++n) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((n & 63) == 63 && *dead) return false;
+  }
+  *dead = 1;
+  atomicExch(status, 7);
+  return false;
+}
+
+// the same for a whole warp, with one answer for its lanes: they leave a loop together or not at all
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* dead, int* status) {
+  return __all_sync(0xffffffffu, wait(bar, parity, dead, status));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// which of the SLOT keys from k0 on may be attended to (all lanes of a warp together)
+__device__ __forceinline__ uint64_t allowed_bits(int k0, int hi, const uint8_t* mask) {
+  const int left = hi - k0;
+  uint64_t bits = left >= SLOT ? ~0ull : (1ull << (left > 0 ? left : 0)) - 1;
+  if (mask) {
+    const int lane = threadIdx.x & 31;
+    const uint64_t a = __ballot_sync(0xffffffffu, k0 + lane < hi && mask[k0 + lane]);
+    const uint64_t b = __ballot_sync(0xffffffffu, k0 + 32 + lane < hi && mask[k0 + 32 + lane]);
+    bits &= a | (b << 32);
+  }
+  return bits;
+}
+
+}  // namespace attn

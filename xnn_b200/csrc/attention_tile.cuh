@@ -9,12 +9,14 @@
 // (a warp-wide 32-ary search), the grid is floor(N / Q) + num + 2 whatever the lengths are, and no
 // host copy of the lengths is needed. Bounds are clamped to [0, N]: no pointer value leaves the arrays.
 #pragma once
+#include <limits>
+
 #include "attention_params.h"
 #include "common.cuh"
 
 namespace attn {
 
-struct Part { int lo, hi, row; bool keys; };   // the part's rows, the block's first row, whether it has keys
+struct Part { int lo, hi, row, index; bool keys; };   // the part's rows, the block's first row, the part, whether it has keys
 
 __device__ __forceinline__ int part_bound(const int64_t* ptr, int num, int N, int p) {
   if (p <= 0) return 0;
@@ -40,10 +42,29 @@ __device__ __forceinline__ bool find_part(const int64_t* ptr, int num, int N, in
   }
   out.lo = part_bound(ptr, num, N, at);
   out.hi = max(part_bound(ptr, num, N, at + 1), out.lo);
+  out.index = at;
   out.keys = at > 0 && at <= num;
   const int64_t row = (int64_t)out.lo + (int64_t)(t - at - out.lo / Q) * Q;
   out.row = (int)row;
   return row >= out.lo && row < out.hi;
+}
+
+template <typename T> __device__ __forceinline__ T log2e() { return T(1.4426950408889634074); }
+
+template <typename T>
+__device__ __forceinline__ bool takes(const Params<T>& p, const Part& part) {
+  const int len = part.hi - part.lo;
+  // the parts without keys go with the longest lengths
+  return part.keys ? (len >= p.min_len && len <= p.max_len) : p.max_len == std::numeric_limits<int>::max();
+}
+
+// the share of split z of the tiles of `B` rows in [lo, hi)
+template <int B>
+__device__ __forceinline__ void split_range(int& lo, int& hi, int z, int splits) {
+  const int tiles = (hi - lo + B - 1) / B, per = (tiles + splits - 1) / splits;
+  const int end = hi;
+  hi = min(end, lo + min(tiles, (z + 1) * per) * B);
+  lo = min(end, lo + min(tiles, z * per) * B);
 }
 
 template <typename T> struct Vec { static constexpr int W = 16 / sizeof(T); };

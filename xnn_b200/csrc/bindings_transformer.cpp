@@ -84,10 +84,26 @@ int choose_splits(int64_t row_tiles, int64_t max_len, int tile) {
 template <typename T>
 bool mostly_short(const attn::Params<T>& p, int64_t max_len) { return max_len <= SHORT || (int64_t)p.N < 48 * (int64_t)p.num; }
 
+// Long structures of float32 take the tensor cores.
+constexpr int64_t TC_LENGTH = 96;
+template <typename T>
+bool tensor_cores(const attn::Params<T>& p, int width) {
+  return sizeof(T) == 4 && p.D <= width && (int64_t)p.N >= TC_LENGTH * std::max(p.num, 1);
+}
+constexpr int TC_FORWARD_WIDTH = 128, TC_BACKWARD_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
+
+torch::Tensor bytes(int64_t n, const torch::Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kUInt8)); }
+
+int* status_of(const torch::Tensor& status, const torch::Tensor& q) {
+  TORCH_CHECK(status.device() == q.device() && status.scalar_type() == torch::kInt32 && status.numel() >= 1,
+              "structure attention: an int32 status word on ", q.device());
+  return status.data_ptr<int>();
+}
+
 template <typename T>
 std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                                          const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, int64_t max_len,
-                                         double scale, bool want_stats) {
+                                         double scale, bool want_stats, const torch::Tensor& status) {
   auto p = make_params<T>(q, k, v, ptr, mask, scale);
   torch::Tensor out = torch::empty({p.N, p.H, p.D}, q.options());
   torch::Tensor lse;
@@ -96,15 +112,21 @@ std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Te
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = out.data_ptr<T>();
   p.lse = want_stats ? lse.data_ptr<T>() : nullptr;
-  const bool small = mostly_short(p, max_len);
-  const int tile = small || sizeof(T) == 8 ? 32 : 64;
-  p.splits = choose_splits((int64_t)(p.N / tile + 1) * p.H, max_len, tile);
+  const bool tc = tensor_cores(p, TC_FORWARD_WIDTH), small = !tc && mostly_short(p, max_len);
+  const int rows = tc ? TC_ROWS : small || sizeof(T) == 8 ? 32 : 64;
+  p.splits = choose_splits((int64_t)(p.N / rows + 1) * p.H, max_len, tc ? TC_TILE : rows);
   torch::Tensor work;
   if (p.splits > 1) {
     work = torch::empty({(int64_t)p.splits * p.H * p.N * (p.D + 2)}, q.options());
     p.work = work.data_ptr<T>();
   }
-  XNN_OK(attn::forward<T>(p, small, s));
+  if constexpr (sizeof(T) == 4) {
+    if (tc) {
+      auto images = bytes(attn::tc_forward_bytes(p), q);
+      XNN_OK(attn::tc_forward(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+    }
+  }
+  if (!tc) XNN_OK(attn::forward<T>(p, small, s));
   if (p.splits > 1) XNN_OK(attn::forward_join<T>(p, s));
   return {out, want_stats ? lse : out};
 }
@@ -125,7 +147,7 @@ template <typename T>
 std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::Tensor& q, const torch::Tensor& k,
                                           const torch::Tensor& v, const torch::Tensor& o, const torch::Tensor& lse,
                                           const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, int64_t max_len,
-                                          double scale) {
+                                          double scale, const torch::Tensor& status) {
   auto p = make_params<T>(q, k, v, ptr, mask, scale);
   set_outputs(p, go, o, lse, q);
   torch::Tensor dq = torch::empty({p.N, p.H, p.D}, q.options()), dk = torch::empty({p.N, p.HK, p.D}, q.options()),
@@ -133,7 +155,7 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
   if (p.N == 0) return {dq, dk, dv};
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = dq.data_ptr<T>(); p.out1 = dk.data_ptr<T>(); p.out2 = dv.data_ptr<T>();
-  const bool short_first = mostly_short(p, max_len);
+  const bool tc = tensor_cores(p, TC_BACKWARD_WIDTH), short_first = !tc && mostly_short(p, max_len);
   if (short_first) {
     auto ps = p;
     if (max_len > SHORT) ps.max_len = SHORT;
@@ -141,11 +163,20 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
     if (max_len <= SHORT) return {dq, dk, dv};
     p.min_len = SHORT + 1;
   }
-  torch::Tensor delta = torch::empty({p.H, p.N}, q.options());
-  p.delta = delta.data_ptr<T>();
-  XNN_OK(attn::row_delta<T>(p, s));
-  const int tile = sizeof(T) == 8 ? 32 : 64;
-  const int64_t tiles = p.N / tile + 1;
+  torch::Tensor delta, images;
+  if constexpr (sizeof(T) == 4) {
+    if (tc) {
+      images = bytes(attn::tc_backward_bytes(p), q);
+      XNN_OK(attn::tc_backward_prepare(p, static_cast<char*>(images.data_ptr()), s));
+    }
+  }
+  if (!tc) {
+    delta = torch::empty({p.H, p.N}, q.options());
+    p.delta = delta.data_ptr<T>();
+    XNN_OK(attn::row_delta<T>(p, s));
+  }
+  const int tile = tc ? TC_TILE : sizeof(T) == 8 ? 32 : 64;
+  const int64_t tiles = p.N / (tc ? TC_ROWS : tile) + 1;
   torch::Tensor work;
   const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
   const int sq = short_first ? 1 : choose_splits(tiles * p.H, max_len, tile);
@@ -155,10 +186,16 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
     p.work = work.data_ptr<T>();
   }
   p.splits = sq;
-  XNN_OK(attn::backward_dq<T>(p, false, s));
+  if constexpr (sizeof(T) == 4) {
+    if (tc) XNN_OK(attn::tc_backward_dq(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+  }
+  if (!tc) XNN_OK(attn::backward_dq<T>(p, false, s));
   if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, p.work, p.out0, s));
   p.splits = sk;
-  XNN_OK(attn::backward_dkv<T>(p, false, s));
+  if constexpr (sizeof(T) == 4) {
+    if (tc) XNN_OK(attn::tc_backward_dkv(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+  }
+  if (!tc) XNN_OK(attn::backward_dkv<T>(p, false, s));
   if (sk > 1) {
     XNN_OK(attn::sum_splits<T>(nk, sk, p.work, p.out1, s));
     XNN_OK(attn::sum_splits<T>(nk, sk, p.work + (int64_t)sk * nk, p.out2, s));
@@ -200,11 +237,11 @@ using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
 Tensors attention_forward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ptr,
-                          const c10::optional<torch::Tensor>& mask, int64_t max_len, double scale, bool want_stats) {
+                          const c10::optional<torch::Tensor>& mask, int64_t max_len, double scale, bool want_stats, const torch::Tensor& status) {
   const c10::cuda::CUDAGuard guard(q.device());
   Tensors r;
   AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention",
-                             [&] { r = forward_typed<scalar_t>(q, k, v, ptr, mask, max_len, scale, want_stats); });
+                             [&] { r = forward_typed<scalar_t>(q, k, v, ptr, mask, max_len, scale, want_stats, status); });
   return r;
 }
 
@@ -243,50 +280,52 @@ struct AttentionSecond : torch::autograd::Function<AttentionSecond> {
 // (dq, dk, dv); its own derivative is the total one, through o and the row statistics too
 struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
   static variable_list forward(AutogradContext* ctx, Variable go, Variable q, Variable k, Variable v, Variable o, Variable lse,
-                               Variable ptr, c10::optional<Variable> mask, int64_t max_len, double scale) {
+                               Variable ptr, c10::optional<Variable> mask, Variable status, int64_t max_len, double scale) {
     go = rows(go);
     ctx->save_for_backward({go, q, k, v, o, lse, ptr, mask.value_or(Variable())});
     keep(ctx, {max_len, scale});
     const c10::cuda::CUDAGuard guard(q.device());
     Tensors r;
     AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward", [&] {
-      r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale);
+      r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale, status);
     });
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     auto r = AttentionSecond::apply(g[0], g[1], g[2], s[0], s[1], s[2], s[3], s[4], s[5], s[6], maybe(s[7]), kept(ctx).scale);
-    r.resize(10);
+    r.resize(11);
     return r;
   }
 };
 
 struct Attention : torch::autograd::Function<Attention> {
   static Variable forward(AutogradContext* ctx, Variable q, Variable k, Variable v, Variable ptr, c10::optional<Variable> mask,
-                          int64_t max_len, double scale) {
-    auto r = attention_forward(q, k, v, ptr, mask, max_len, scale, true);
+                          Variable status, int64_t max_len, double scale) {
+    auto r = attention_forward(q, k, v, ptr, mask, max_len, scale, true, status);
     ctx->save_for_backward({q, k, v, r[0], r[1], ptr, mask.value_or(Variable())});
+    ctx->saved_data["status"] = status;
     keep(ctx, {max_len, scale});
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const auto set = kept(ctx);
-    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), set.max_len, set.scale);
-    r.resize(7);
+    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]),
+                                  ctx->saved_data["status"].toTensor(), set.max_len, set.scale);
+    r.resize(8);
     return r;
   }
 };
 
 torch::Tensor structure_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor ptr,
-                                  c10::optional<torch::Tensor> mask, int64_t max_len, double scale) {
+                                  c10::optional<torch::Tensor> mask, int64_t max_len, double scale, torch::Tensor status) {
   q = rows(q); k = rows(k); v = rows(v);
   ptr = ptr.contiguous();
   if (mask.has_value()) mask = mask->contiguous();
   if (torch::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
-    return Attention::apply(q, k, v, ptr, mask, max_len, scale);
-  return attention_forward(q, k, v, ptr, mask, max_len, scale, false)[0];
+    return Attention::apply(q, k, v, ptr, mask, status, max_len, scale);
+  return attention_forward(q, k, v, ptr, mask, max_len, scale, false, status)[0];
 }
 
 // x (outer, shared, inner) contiguous; rng int64 (seed, offset) on x's device

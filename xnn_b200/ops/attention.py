@@ -25,6 +25,7 @@ import torch
 from torch import Tensor
 
 from .. import _ext
+from .gemm import _status
 
 MAX_WIDTH = 128
 _TYPES = (torch.float32, torch.float64)
@@ -101,4 +102,4 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, max_len: O
         return _formula(q, k, v, ptr, key_mask, scale)
     if d > MAX_WIDTH:
         raise ValueError(f"head width {d}: the kernels take up to {MAX_WIDTH}")
-    return _kernels().structure_attention(q, k, v, ptr, key_mask, max_len, scale)
+    return _kernels().structure_attention(q, k, v, ptr, key_mask, max_len, scale, _status(q.device))
