@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 7);
   Part part;
   if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = tid / 32;
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
@@ -103,36 +103,39 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
   tc::tc_fence_after();
 
   if (warp == 4) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
       const auto load = [&](uint64_t* bar, int at, const Images& im, int i) {
-        tc::mbar_arrive_expect_tx(bar, BYTES);
-        tc::bulk_g2s(smem + at * BYTES, image<DP>(im, hk, slot0 + i), BYTES, bar);
+        if (elect()) {
+          tc::mbar_arrive_expect_tx(bar, BYTES);
+          tc::bulk_g2s(smem + at * BYTES, image<DP>(im, hk, slot0 + i), BYTES, bar);
+        }
       };
       const uint32_t sk = tc::smem_u32(smem), sv = sk + 2 * BYTES;
-      const uint32_t is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
       const auto scores = [&](int i) {
-        mma_parts<DP / 16>(tmem + F::S, tmem + F::Q, DP / 2, sk + (i & 1) * BYTES, PLANE, 256, 128, DP * 16, is);
-        tc::commit_to(s_done);
+        if (elect()) {
+          mma_scores<DP>(tmem + F::S, tmem + F::Q, sk + (i & 1) * BYTES);
+          tc::commit_to(s_done);
+        }
       };
       int loaded_k = min(n, 2), loaded_v = min(n, 2);
       for (int i = 0; i < loaded_k; ++i) {
         load(full_k + i, i, ik, i);
         load(full_v + i, 2 + i, iv, i);
       }
-      bool ok = wait(full_k, 0, dead, status);
+      bool ok = wait_all(full_k, 0, dead, status);
       if (ok) scores(0);
       for (int i = 0; ok && i < n; ++i) {
         // the probabilities of tile i are there, so S(i) and P V(i - 1) are done and their images free
-        if (!(ok = wait(p_ready, i & 1, dead, status))) break;
+        if (!(ok = wait_all(p_ready, i & 1, dead, status))) break;
         tc::tc_fence_after();
         if (i + 2 < n) { load(full_k + (i & 1), i & 1, ik, i + 2); loaded_k = i + 3; }
         if (i > 0 && i + 1 < n) { load(full_v + ((i + 1) & 1), 2 + ((i + 1) & 1), iv, i + 1); loaded_v = i + 2; }
-        if (!(ok = wait(full_v + (i & 1), (i >> 1) & 1, dead, status))) break;
-        mma_parts<SLOT / 16>(tmem + F::O, tmem + F::S, SLOT / 2, sv + (i & 1) * BYTES, PLANE, DP * 32, DP * 16, 128, io);
+        if (!(ok = wait_all(full_v + (i & 1), (i >> 1) & 1, dead, status))) break;
+        if (elect()) mma_sums<DP>(tmem + F::O, tmem + F::S, sv + (i & 1) * BYTES);
         if (i + 1 < n) {
-          if (!(ok = wait(full_k + ((i + 1) & 1), ((i + 1) >> 1) & 1, dead, status))) break;
+          if (!(ok = wait_all(full_k + ((i + 1) & 1), ((i + 1) >> 1) & 1, dead, status))) break;
           scores(i + 1);
-        } else {
+        } else if (elect()) {
           tc::commit_to(s_done);
         }
       }
@@ -285,7 +288,7 @@ struct Block {                                          // what the two kernels 
   uint64_t *full, *bars;
   volatile int* dead;
   uint32_t tmem;
-  int warp, lane;
+  int warp;
 };
 
 // barriers, tensor memory and the parts of the two resident operands
@@ -299,7 +302,6 @@ __device__ __forceinline__ Block set_up(char* smem, const Part& part, const floa
   uint32_t* slot = reinterpret_cast<uint32_t*>(k.bars + 8);
   k.dead = reinterpret_cast<volatile int*>(k.bars + 9);
   k.warp = threadIdx.x / 32;
-  k.lane = threadIdx.x % 32;
   if (k.warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(k.full + i, 1);
@@ -355,38 +357,43 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
                              p.go + h * p.goh, p.gos, vec_ok(p.go, p.gos, p.goh, p.D), p.D, nullptr, n);
   uint64_t *sd_done = k.bars, *dq_done = k.bars + 1, *taken = k.bars + 2, *ds_ready = k.bars + 3;
   if (k.warp == 8) {
-    if (k.lane == 0 && n > 0) {
+    if (n > 0) {
       const auto load = [&](int i) {
-        char* at = smem + (i % STAGES) * B::STAGE;
-        tc::mbar_arrive_expect_tx(k.full + i % STAGES, 2 * BYTES);
-        tc::bulk_g2s(at, image<DP>(ik, hk, slot0 + i), BYTES, k.full + i % STAGES);
-        tc::bulk_g2s(at + BYTES, image<DP>(iv, hk, slot0 + i), BYTES, k.full + i % STAGES);
+        if (elect()) {
+          char* at = smem + (i % STAGES) * B::STAGE;
+          tc::mbar_arrive_expect_tx(k.full + i % STAGES, 2 * BYTES);
+          tc::bulk_g2s(at, image<DP>(ik, hk, slot0 + i), BYTES, k.full + i % STAGES);
+          tc::bulk_g2s(at + BYTES, image<DP>(iv, hk, slot0 + i), BYTES, k.full + i % STAGES);
+        }
       };
-      const uint32_t base = tc::smem_u32(smem), is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
+      const uint32_t base = tc::smem_u32(smem);
       const auto scores = [&](int i) {
-        const uint32_t at = base + (i % STAGES) * B::STAGE;
-        mma_parts<DP / 16>(k.tmem + B::Q_S, k.tmem, DP / 2, at, PLANE, 256, 128, DP * 16, is);
-        mma_parts<DP / 16>(k.tmem + B::Q_DP, k.tmem + B::PARTS, DP / 2, at + BYTES, PLANE, 256, 128, DP * 16, is);
-        tc::commit_to(sd_done);
+        if (elect()) {
+          const uint32_t at = base + (i % STAGES) * B::STAGE;
+          mma_scores<DP>(k.tmem + B::Q_S, k.tmem, at);
+          mma_scores<DP>(k.tmem + B::Q_DP, k.tmem + B::PARTS, at + BYTES);
+          tc::commit_to(sd_done);
+        }
       };
       int loaded = min(n, STAGES);
       for (int i = 0; i < loaded; ++i) load(i);
-      bool ok = wait(k.full, 0, k.dead, status);
+      bool ok = wait_all(k.full, 0, k.dead, status);
       if (ok) scores(0);
       for (int i = 0; ok && i < n; ++i) {
-        if (!(ok = wait(taken, i & 1, k.dead, status))) break;
+        if (!(ok = wait_all(taken, i & 1, k.dead, status))) break;
         tc::tc_fence_after();
         if (i + 1 < n) {
-          if (!(ok = wait(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
+          if (!(ok = wait_all(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
           scores(i + 1);
         }
-        if (!(ok = wait(ds_ready, i & 1, k.dead, status))) break;
+        if (!(ok = wait_all(ds_ready, i & 1, k.dead, status))) break;
         tc::tc_fence_after();
         // dq of tile i - 1 is done: its stage is free
         if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
-        mma_parts<SLOT / 16>(k.tmem + B::Q_OUT, k.tmem + B::Q_DS, SLOT / 2, base + (i % STAGES) * B::STAGE, PLANE, DP * 32,
-                             DP * 16, 128, io);
-        tc::commit_to(dq_done);
+        if (elect()) {
+          mma_sums<DP>(k.tmem + B::Q_OUT, k.tmem + B::Q_DS, base + (i % STAGES) * B::STAGE);
+          tc::commit_to(dq_done);
+        }
       }
       if (!ok)
         for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);
@@ -469,7 +476,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
 // tensor cores: while the threads form P^T of a tile, dK of the tile before and dP^T of this one run; while they form
 // dS^T, dV of this tile and S^T of the next.
 template <int DP>
-__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<float> p, const Images iq, const Images io_,
+__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<float> p, const Images iq, const Images io,
                                                                 const float* __restrict__ stats, int* status) {
   using B = Bwd<DP>;
   constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
@@ -484,50 +491,49 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
                              p.v + hk * p.vh, p.vs, vec_ok(p.v, p.vs, p.vh, p.D), p.D, p.mask, n);
   uint64_t *s_done = k.bars, *dp_done = k.bars + 1, *p_ready = k.bars + 2, *ds_ready = k.bars + 3;
   if (k.warp == 8) {
-    if (k.lane == 0 && n > 0) {
+    if (n > 0) {
       const auto load = [&](int i) {
-        char* at = smem + (i % STAGES) * B::STAGE;
-        uint64_t* bar = k.full + i % STAGES;
-        const int h = hk * group + i / tiles, slot = slot0 + i % tiles;
-        tc::mbar_arrive_expect_tx(bar, B::STAGE);
-        tc::bulk_g2s(at, image<DP>(iq, h, slot), BYTES, bar);
-        tc::bulk_g2s(at + BYTES, image<DP>(io_, h, slot), BYTES, bar);
-        tc::bulk_g2s(at + 2 * BYTES, stats + ((int64_t)h * iq.slots + slot) * 2 * SLOT, 2 * SLOT * 4, bar);
+        if (elect()) {
+          char* at = smem + (i % STAGES) * B::STAGE;
+          uint64_t* bar = k.full + i % STAGES;
+          const int h = hk * group + i / tiles, slot = slot0 + i % tiles;
+          tc::mbar_arrive_expect_tx(bar, B::STAGE);
+          tc::bulk_g2s(at, image<DP>(iq, h, slot), BYTES, bar);
+          tc::bulk_g2s(at + BYTES, image<DP>(io, h, slot), BYTES, bar);
+          tc::bulk_g2s(at + 2 * BYTES, stats + ((int64_t)h * iq.slots + slot) * 2 * SLOT, 2 * SLOT * 4, bar);
+        }
       };
-      const uint32_t base = tc::smem_u32(smem), is = idesc_bf16(SLOT, 0), io = idesc_bf16(DP, 1);
+      const uint32_t base = tc::smem_u32(smem);
       const auto stage = [&](int i) { return base + (i % STAGES) * B::STAGE; };
-      const auto scores = [&](int i) {
-        mma_parts<DP / 16>(k.tmem + B::K_S, k.tmem, DP / 2, stage(i), PLANE, 256, 128, DP * 16, is);
-        tc::commit_to(s_done);
+      // a product of tile i and the score product of the next tile (or of none) behind it
+      const auto step = [&](uint32_t sum, uint32_t a, uint32_t rows, uint32_t d, uint32_t parts, uint32_t image, bool next, uint64_t* bar) {
+        if (elect()) {
+          mma_sums<DP>(sum, a, rows);
+          if (next) mma_scores<DP>(d, parts, image);
+          tc::commit_to(bar);
+        }
       };
-      const auto dots = [&](int i) {
-        mma_parts<DP / 16>(k.tmem + B::K_DP, k.tmem + B::PARTS, DP / 2, stage(i) + BYTES, PLANE, 256, 128, DP * 16, is);
-        tc::commit_to(dp_done);
-      };
+      const uint32_t s = k.tmem + B::K_S, dp = k.tmem + B::K_DP, kp = k.tmem, vp = k.tmem + B::PARTS;
       int loaded = min(n, STAGES);
       for (int i = 0; i < loaded; ++i) load(i);
-      bool ok = wait(k.full, 0, k.dead, status);
-      if (ok) {
-        scores(0);
-        dots(0);
+      bool ok = wait_all(k.full, 0, k.dead, status);
+      if (ok && elect()) {
+        mma_scores<DP>(s, kp, stage(0));
+        tc::commit_to(s_done);
+        mma_scores<DP>(dp, vp, stage(0) + BYTES);
+        tc::commit_to(dp_done);
       }
       for (int i = 0; ok && i < n; ++i) {
-        if (!(ok = wait(p_ready, i & 1, k.dead, status))) break;
+        const bool next = i + 1 < n;
+        if (!(ok = wait_all(p_ready, i & 1, k.dead, status))) break;
         tc::tc_fence_after();
-        mma_parts<SLOT / 16>(k.tmem + B::K_DV, k.tmem + B::K_S, SLOT / 2, stage(i) + BYTES, PLANE, DP * 32, DP * 16, 128, io);
-        if (i + 1 < n) {
-          if (!(ok = wait(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
-          scores(i + 1);
-        } else {
-          tc::commit_to(s_done);
-        }
-        if (!(ok = wait(ds_ready, i & 1, k.dead, status))) break;
+        if (next && !(ok = wait_all(k.full + (i + 1) % STAGES, ((i + 1) / STAGES) & 1, k.dead, status))) break;
+        step(k.tmem + B::K_DV, s, stage(i) + BYTES, s, kp, stage(i + 1), next, s_done);
+        if (!(ok = wait_all(ds_ready, i & 1, k.dead, status))) break;
         tc::tc_fence_after();
         // dK of tile i - 1, the last to read its stage, is done
         if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
-        mma_parts<SLOT / 16>(k.tmem + B::K_DK, k.tmem + B::K_DP, SLOT / 2, stage(i), PLANE, DP * 32, DP * 16, 128, io);
-        if (i + 1 < n) dots(i + 1);
-        else tc::commit_to(dp_done);
+        step(k.tmem + B::K_DK, dp, stage(i), dp, vp, stage(i + 1) + BYTES, next, dp_done);
       }
       if (!ok)
         for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);

@@ -55,26 +55,49 @@ __device__ __forceinline__ uint32_t idesc_bf16(int n, int b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
-// D (128 x N, tensor memory) (+)= A (tensor memory) B (shared memory)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-      :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// One lane of a converged warp. Issued under this predicate a run of 128 x 64 x 16 products takes 34 cycles each, under
+// `lane == 0` 48: the compiler then keeps the operands in uniform registers.
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
-// the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y b_plane bytes,
-// K = 16 k steps of 8 columns of A and b_step bytes of B
-template <int KSTEPS>
-__device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_plane, uint32_t b, uint32_t b_plane,
-                                          uint32_t b_step, uint32_t lbo, uint32_t sbo, uint32_t idesc) {
+// D (128 x N, tensor memory) (+)= A (tensor memory) B (shared memory, descriptor in two words)
+template <int ACCUMULATE>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}\n"
+      :: "r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACCUMULATE) : "memory");
+}
+
+// the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y B_PLANE bytes,
+// 16 K elements a step of 8 columns of A and B_STEP bytes of B
+template <int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO>
+__device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_plane, uint32_t b, uint32_t idesc) {
   constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
+  const uint32_t lo = (b >> 4) | ((LBO >> 4) << 16);
+  constexpr uint32_t hi = (SBO >> 4) | (1u << 14);      // bit 46: descriptor version
 #pragma unroll
   for (int i = 0; i < 6; ++i)
 #pragma unroll
-    for (int k = 0; k < KSTEPS; ++k)
-      mma_ts(d, a + X[i] * a_plane + 8 * k, tc::make_desc2(b + Y[i] * b_plane + k * b_step, lbo, sbo), idesc, i + k > 0);
+    for (int k = 0; k < KSTEPS; ++k) {
+      const uint32_t at = lo + (Y[i] * B_PLANE + k * B_STEP) / 16;
+      if (i + k) mma_ts<1>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
+      else mma_ts<0>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
+    }
+}
+// the operand image as rows x d (scores) and as d x rows (sums over the rows)
+template <int DP>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
+  mma_parts<DP / 16, Image<DP>::PLANE, 256, 128, DP * 16>(d, a, DP / 2, b, idesc_bf16(SLOT, 0));
+}
+template <int DP>
+__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b) {
+  mma_parts<SLOT / 16, Image<DP>::PLANE, DP * 32, DP * 16, 128>(d, a, SLOT / 2, b, idesc_bf16(DP, 1));
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {

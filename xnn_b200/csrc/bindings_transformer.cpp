@@ -311,7 +311,8 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const auto set = kept(ctx);
-    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]),
+    // o without its graph: the second derivative holds what goes through it
+    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3].detach(), s[4], s[5], maybe(s[6]),
                                   ctx->saved_data["status"].toTensor(), set.max_len, set.scale);
     r.resize(8);
     return r;
