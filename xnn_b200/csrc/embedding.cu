@@ -6,7 +6,7 @@
 // The gradient sorts the ids (stable radix sort, eight bits a pass, (key, row) pairs), then walks the sorted
 // order in chunks: a warp sums the rows of each run of equal ids inside its chunk. A run inside one chunk
 // goes to the table; the part of a run that began before the chunk, and the one that goes on behind it, are
-// written to one of the chunk's two partial rows. A block per table row then adds the partials of its run in their order
+// written to one of the chunk's two partial rows. A warp (or, for long runs, a block) per table row then adds the partials of its run in their order
 // and writes zeros where no id came. Every sum has a fixed order; there are no atomics on values.
 // Small inputs (rule at `embedding_grad`) skip the sort: a block per table row collects its ids itself.
 #include "common.cuh"
@@ -21,32 +21,46 @@ __device__ __forceinline__ int64_t row_of(const I* ids, int64_t n, int64_t V) {
   return v >= 0 && v < V ? v : -1;
 }
 
+// A thread takes LOOKUPS pieces of 16 bytes, a block apart, so that its id and row loads overlap; what is
+// written is not read again here, so it goes past the caches. 400000 rows of 128 floats: 34 us, 6.1 TB/s written.
+constexpr int LOOKUPS = 4;
+
 template <typename T, typename I, int W>
-__global__ void __launch_bounds__(256) lookup_kernel(int64_t N, int64_t V, int C, const T* __restrict__ table,
+__global__ void __launch_bounds__(256) lookup_kernel(uint32_t items, uint32_t per, int64_t V, int C, const T* __restrict__ table,
                                                      const I* __restrict__ ids, T scale, T* __restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = C / W;
-  const int64_t n = i / per;
-  if (n >= N) return;
-  const int c = (int)(i - n * per) * W;
-  const int64_t v = row_of(ids, n, V);
+  const uint32_t first = blockIdx.x * (256u * LOOKUPS) + threadIdx.x;
+  int64_t v[LOOKUPS];
+  uint32_t n[LOOKUPS], c[LOOKUPS];
+#pragma unroll
+  for (int u = 0; u < LOOKUPS; ++u) {
+    const uint32_t i = first + u * 256u;
+    n[u] = i / per;
+    c[u] = (i - n[u] * per) * W;
+    v[u] = i < items ? row_of(ids, n[u], V) : -1;
+  }
   if constexpr (W == 1) {
-    out[n * C + c] = v < 0 ? T(0) : scale * table[v * C + c];
+#pragma unroll
+    for (int u = 0; u < LOOKUPS; ++u)
+      if (first + u * 256u < items) out[(int64_t)n[u] * C + c[u]] = v[u] < 0 ? T(0) : scale * table[v[u] * C + c[u]];
   } else {
-    Pack<T> a;
+    Pack<T> a[LOOKUPS];
 #pragma unroll
-    for (int e = 0; e < W; ++e) a.x[e] = T(0);
-    if (v >= 0) {
-      a = *reinterpret_cast<const Pack<T>*>(table + v * C + c);
+    for (int u = 0; u < LOOKUPS; ++u) {
 #pragma unroll
-      for (int e = 0; e < W; ++e) a.x[e] *= scale;
+      for (int e = 0; e < W; ++e) a[u].x[e] = T(0);
+      if (v[u] >= 0) a[u] = *reinterpret_cast<const Pack<T>*>(table + v[u] * C + c[u]);
     }
-    *reinterpret_cast<Pack<T>*>(out + n * C + c) = a;
+#pragma unroll
+    for (int u = 0; u < LOOKUPS; ++u) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) a[u].x[e] *= scale;
+      if (first + u * 256u < items) __stcs(reinterpret_cast<float4*>(out + (int64_t)n[u] * C + c[u]), *reinterpret_cast<float4*>(&a[u]));
+    }
   }
 }
 
-// ---- sort: each block takes `tile` pairs, each of its 8 warps a contiguous eighth, in strips of 32 ----
-constexpr int SORT_WARPS = 8;
+// ---- sort: each block takes `tile` pairs, each of its 32 warps a contiguous share, in strips of 32 ----
+constexpr int SORT_WARPS = 32;
 
 template <typename I>
 __device__ __forceinline__ int key_at(const I* ids, const int* keys, int64_t i, int64_t V) {
@@ -68,47 +82,62 @@ __global__ void __launch_bounds__(256) count_kernel(int N, int64_t V, int tile, 
 }
 
 template <typename I>
-__global__ void __launch_bounds__(256) place_kernel(int N, int64_t V, int tile, int shift, const I* __restrict__ ids,
-                                                    const int* __restrict__ keys, const int* __restrict__ rows,
-                                                    const int* __restrict__ counts, int* __restrict__ keys_out,
-                                                    int* __restrict__ rows_out) {
+__global__ void __launch_bounds__(1024) place_kernel(int N, int64_t V, int tile, int shift, const I* __restrict__ ids,
+                                                     const int* __restrict__ keys, const int* __restrict__ rows,
+                                                     const int* __restrict__ counts, int* __restrict__ keys_out,
+                                                     int* __restrict__ rows_out) {
   __shared__ int base[SORT_WARPS][256];
-  __shared__ int scan[SORT_WARPS];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  // where this block's entries of digit t start: entries of smaller digits, then those of earlier blocks
+  __shared__ int scan[8];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, digit = t & 255, quarter = t >> 8;
+  // where this block's entries of a digit start: entries of smaller digits, then those of earlier blocks; each
+  // quarter of the block adds up a quarter of the blocks' counts
   int before = 0, total = 0;
-  for (int b = 0; b < (int)gridDim.x; ++b) {
-    const int v = counts[b * 256 + t];
+  const int share = ((int)gridDim.x + 3) / 4, b1 = min((int)gridDim.x, (quarter + 1) * share);
+#pragma unroll 16
+  for (int b = quarter * share; b < b1; ++b) {
+    const int v = counts[b * 256 + digit];
     before += b < (int)blockIdx.x ? v : 0;
     total += v;
   }
-  int incl = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
-  if (lane == 31) scan[warp] = incl;
-#pragma unroll
-  for (int w = 0; w < SORT_WARPS; ++w) base[w][t] = 0;
+  base[quarter][digit] = before;
+  base[4 + quarter][digit] = total;
   __syncthreads();
-  int start = incl - total + before;
-  for (int w = 0; w < warp; ++w) start += scan[w];
-  const int per = ((tile + SORT_WARPS - 1) / SORT_WARPS + 31) / 32 * 32;
+  int start = 0, incl = 0;
+  if (t < 256) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) { start += base[x][t]; incl += base[4 + x][t]; }
+    start -= incl;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += u; }
+    start += incl;
+    if (lane == 31) scan[warp] = incl;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < SORT_WARPS / 4; ++x) base[quarter + 4 * x][digit] = 0;
+  if (t < 256)
+    for (int w = 0; w < warp; ++w) start += scan[w];
+  __syncthreads();
+  const int per = tile / SORT_WARPS;
   const int end = min(N, (int)(blockIdx.x + 1) * tile);
   const int first = blockIdx.x * tile + warp * per, last = min(end, first + per);
   for (int i = first + lane; i < last; i += 32) atomicAdd(&base[warp][(key_at(ids, keys, i, V) >> shift) & 255], 1);
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < SORT_WARPS; ++w) { const int c = base[w][t]; base[w][t] = start; start += c; }
+  if (t < 256) {
+#pragma unroll 8
+    for (int w = 0; w < SORT_WARPS; ++w) { const int c = base[w][t]; base[w][t] = start; start += c; }
+  }
   __syncthreads();
   for (int i0 = first; i0 < last; i0 += 32) {
     const int i = i0 + lane;
     const bool in = i < last;
-    const int key = in ? key_at(ids, keys, i, V) : 0, digit = in ? (key >> shift) & 255 : 256;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const int key = in ? key_at(ids, keys, i, V) : 0, d = in ? (key >> shift) & 255 : 256;
+    const unsigned same = __match_any_sync(0xffffffffu, d);
     const int rank = __popc(same & ((1u << lane) - 1));
     int at = 0;
-    if (in) at = base[warp][digit] + rank;
+    if (in) at = base[warp][d] + rank;
     __syncwarp();
-    if (in && rank == 0) base[warp][digit] += __popc(same);
+    if (in && rank == 0) base[warp][d] += __popc(same);
     __syncwarp();
     if (in) {
       keys_out[at] = key;
@@ -137,43 +166,54 @@ __device__ __forceinline__ void get(const T* row, T (&a)[W], int c, int C) {
   }
 }
 
+// The lanes fetch the keys and rows of 32 entries at once (one dependent load for 32 entries) and pass them round;
+// eight gradient rows are then in flight a warp.
 template <typename T, int W>
 __global__ void __launch_bounds__(128) runs_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
                                                    const int* __restrict__ rows, const T* __restrict__ g, T scale,
                                                    T* __restrict__ table, T* __restrict__ part) {
-  const int chunk = blockIdx.x * 4 + threadIdx.x / 32;
+  const int chunk = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x & 31;
   const int64_t first = (int64_t)chunk * R;
   if (first >= N) return;
   const int last = (int)(first + R < N ? first + R : N), i0 = (int)first;
-  const int c = (blockIdx.y * 32 + (threadIdx.x & 31)) * W;
+  const int c = (blockIdx.y * 32 + lane) * W;
   T acc[W] = {};
   int key = keys[i0];
   bool open = i0 > 0 && keys[i0 - 1] == key;            // the run began in an earlier chunk
   constexpr int U = 8;
-  for (int i = i0; i < last; i += U) {
-    int k[U];
-    T v[U][W];
+  int next_key = i0 + lane < last ? keys[i0 + lane] : V, next_row = i0 + lane < last ? rows[i0 + lane] : 0;
+  for (int i = i0; i < last; i += 32) {
+    const int my_key = next_key, my_row = next_row;
+    const int j = i + 32 + lane;
+    next_key = j < last ? keys[j] : V;
+    next_row = j < last ? rows[j] : 0;
+    const int count = min(32, last - i);
+    for (int s = 0; s < count; s += U) {
+      int k[U];
+      T v[U][W];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      k[u] = i + u < last ? keys[i + u] : V;
-      if (k[u] < V) get<T, W>(g + (int64_t)rows[i + u] * C, v[u], c, C);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= last) break;
-      if (k[u] != key) {
-        if (key < V) {
-          if (open) put<T, W>(part + (int64_t)(2 * chunk) * C, acc, T(1), c, C);
-          else put<T, W>(table + (int64_t)key * C, acc, scale, c, C);
-        }
-        open = false;
-        key = k[u];
-#pragma unroll
-        for (int e = 0; e < W; ++e) acc[e] = T(0);
+      for (int u = 0; u < U; ++u) {
+        k[u] = __shfl_sync(0xffffffffu, my_key, s + u);
+        const int row = __shfl_sync(0xffffffffu, my_row, s + u);
+        if (k[u] < V) get<T, W>(g + (int64_t)row * C, v[u], c, C);
       }
-      if (key < V) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) acc[e] += v[u][e];
+      for (int u = 0; u < U; ++u) {
+        if (s + u >= count) break;
+        if (k[u] != key) {
+          if (key < V) {
+            if (open) put<T, W>(part + (int64_t)(2 * chunk) * C, acc, T(1), c, C);
+            else put<T, W>(table + (int64_t)key * C, acc, scale, c, C);
+          }
+          open = false;
+          key = k[u];
+#pragma unroll
+          for (int e = 0; e < W; ++e) acc[e] = T(0);
+        }
+        if (key < V) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) acc[e] += v[u][e];
+        }
       }
     }
   }
@@ -201,38 +241,70 @@ __device__ __forceinline__ int lower_bound(const int* keys, int N, int v) {
   return at;
 }
 
-// a block per table row: zeros where no id came, the partials of runs over several chunks otherwise
-template <typename T>
+// sum of the partials j0 .. j1 - 1 of a run that begins in chunk c0; the first chunk's share is in its second partial row
+template <typename T, int W>
+__device__ __forceinline__ void run_part(const T* part, int c0, int j0, int j1, int C, int c, T (&s)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) s[e] = T(0);
+#pragma unroll 8
+  for (int j = j0; j < j1; ++j) {
+    T v[W];
+    get<T, W>(part + (int64_t)(2 * (c0 + j) + (j == 0 ? 1 : 0)) * C, v, c, C);
+#pragma unroll
+    for (int e = 0; e < W; ++e) s[e] += v[e];
+  }
+}
+
+// A warp per table row: zeros where no id came, the partials of a run over several chunks added up. Rows of more
+// than MANY partials (the few elements that most atoms are) are left to the whole block. A block's eight rows lie
+// gridDim apart, so that the popular ids, which are neighbours, meet in different blocks.
+constexpr int MANY = 32;
+
+template <typename T, int W>
 __global__ void __launch_bounds__(256) rows_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
                                                    const T* __restrict__ part, T scale, T* __restrict__ table) {
-  __shared__ T sums[256];
-  const int v = blockIdx.x, t = threadIdx.x;
-  const int a = lower_bound(keys, N, v), b = lower_bound(keys, N, v + 1);
-  T* out = table + (int64_t)v * C;
-  if (a == b) {
-    for (int c = t; c < C; c += 256) out[c] = T(0);
-    return;
-  }
-  const int c0 = a / R, c1 = (b - 1) / R;
-  if (c0 == c1) return;                                 // one chunk had the whole run
-  const int lanes = C < 256 ? (C <= 32 ? 32 : (C <= 64 ? 64 : (C <= 128 ? 128 : 256))) : 256, groups = 256 / lanes;
-  const int group = t / lanes;
-  // the first chunk's share is in its second partial row unless the run began before (it did not: c0 holds a)
-  const int n = c1 - c0 + 1, per = (n + groups - 1) / groups;
-  for (int cb = 0; cb < C; cb += lanes) {
-    const int c = cb + t % lanes;
-    T s = T(0);
-    if (c < C) {
-      const int j1 = min(n, (group + 1) * per);
-#pragma unroll 8
-      for (int j = group * per; j < j1; ++j) s += part[(int64_t)(2 * (c0 + j) + (j == 0 ? 1 : 0)) * C + c];
+  __shared__ T sums[8][32 * W];
+  __shared__ int heavy_first[8], heavy_count[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v = blockIdx.x + warp * gridDim.x;
+  int n = 0, c0 = 0;
+  T s[W];
+  if (v < V) {
+    const int a = lower_bound(keys, N, v), b = lower_bound(keys, N, v + 1);
+    T* out = table + (int64_t)v * C;
+    if (a == b) {
+      for (int c = lane; c < C; c += 32) out[c] = T(0);
+    } else {
+      c0 = a / R;
+      n = (b - 1) / R - c0 + 1;                         // 1: one chunk had the whole run and has written it
+      if (n > 1 && n <= MANY)
+        for (int c = lane * W; c < C; c += 32 * W) {
+          run_part<T, W>(part, c0, 0, n, C, c, s);
+          put<T, W>(out, s, scale, c, C);
+        }
     }
-    __syncthreads();
-    sums[t] = s;
-    __syncthreads();
-    if (group == 0 && c < C) {
-      for (int k = 1; k < groups; ++k) s += sums[k * lanes + t];
-      out[c] = scale * s;
+  }
+  if (lane == 0) {
+    heavy_first[warp] = c0;
+    heavy_count[warp] = n > MANY ? n : 0;
+  }
+  __syncthreads();
+  for (int w = 0; w < 8; ++w) {
+    const int m = heavy_count[w];
+    if (m == 0) continue;
+    const int per = (m + 7) / 8;
+    for (int cb = 0; cb < C; cb += 32 * W) {
+      const int c = cb + lane * W;
+      run_part<T, W>(part, heavy_first[w], warp * per, min(m, (warp + 1) * per), C, c, s);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < W; ++e) sums[warp][lane * W + e] = s[e];
+      __syncthreads();
+      if (warp == 0) {
+        for (int k = 1; k < 8; ++k)
+#pragma unroll
+          for (int e = 0; e < W; ++e) s[e] += sums[k][lane * W + e];
+        put<T, W>(table + (int64_t)(blockIdx.x + w * gridDim.x) * C, s, scale, c, C);
+      }
     }
   }
 }
@@ -288,12 +360,13 @@ constexpr int SMALL_ROWS = 4096;
 // pairs a sort block takes: at most 148 blocks (each reads every block's counts), 1024 pairs at least
 int sort_tile(int64_t N) {
   const int64_t t = (N + 147) / 148;
-  return (int)(t < 1024 ? 1024 : (t + 255) / 256 * 256);
+  return (int)((t + 1023) / 1024 * 1024);
 }
-// entries a summing warp takes: 64, more when that would pass 64 warps a multiprocessor
+// entries a summing warp takes: 32, more when that would pass 24 warps a multiprocessor (eight rows in flight in each
+// of them are enough for the memory's latency, and longer chunks leave fewer partial rows)
 int run_chunk(int64_t N) {
-  const int64_t r = (N + 148 * 64 - 1) / (148 * 64);
-  return (int)(r < 64 ? 64 : (r + 7) / 8 * 8);
+  const int64_t r = (N + 148 * 24 - 1) / (148 * 24);
+  return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
 bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 22; }
 
@@ -303,10 +376,16 @@ template <typename T, typename I>
 cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const I* ids, double scale, T* out, cudaStream_t s) {
   constexpr int W = 16 / sizeof(T);
   const bool vec = C % W == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const int64_t items = N * (vec ? C / W : C);
-  const unsigned grid = (unsigned)((items + 255) / 256);
-  if (vec) lookup_kernel<T, I, W><<<grid, 256, 0, s>>>(N, V, C, table, ids, (T)scale, out);
-  else lookup_kernel<T, I, 1><<<grid, 256, 0, s>>>(N, V, C, table, ids, (T)scale, out);
+  const int64_t per = vec ? C / W : C;
+  // pieces are counted in 32 bits: rows in groups that fit
+  const int64_t group = ((int64_t)1 << 31) / per;
+  for (int64_t n0 = 0; n0 < N; n0 += group) {
+    const int64_t n = N - n0 < group ? N - n0 : group;
+    const uint32_t items = (uint32_t)(n * per);
+    const unsigned grid = (unsigned)(((int64_t)items + 256 * LOOKUPS - 1) / (256 * LOOKUPS));
+    if (vec) lookup_kernel<T, I, W><<<grid, 256, 0, s>>>(items, (uint32_t)per, V, C, table, ids + n0, (T)scale, out + n0 * C);
+    else lookup_kernel<T, I, 1><<<grid, 256, 0, s>>>(items, (uint32_t)per, V, C, table, ids + n0, (T)scale, out + n0 * C);
+  }
   return cudaGetLastError();
 }
 
@@ -340,7 +419,7 @@ cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g
     const int* kin = shift ? keys[at ^ 1] : nullptr;
     const int* rin = shift ? rows[at ^ 1] : nullptr;
     count_kernel<I><<<blocks, 256, 0, s>>>((int)N, V, tile, shift, ids, kin, counts);
-    place_kernel<I><<<blocks, 256, 0, s>>>((int)N, V, tile, shift, ids, kin, rin, counts, keys[at], rows[at]);
+    place_kernel<I><<<blocks, 1024, 0, s>>>((int)N, V, tile, shift, ids, kin, rin, counts, keys[at], rows[at]);
     at ^= 1;
   }
   const int *k = keys[at ^ 1], *r = rows[at ^ 1];
@@ -351,7 +430,10 @@ cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g
   const dim3 grid((chunks + 3) / 4, (C + cols - 1) / cols);
   if (vec) runs_kernel<T, W><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
   else runs_kernel<T, 1><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
-  rows_kernel<T><<<(unsigned)V, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
+  const unsigned row_blocks = (unsigned)((V + 7) / 8);
+  // partial rows start on 16-byte boundaries where a whole number of vectors makes a row
+  if (C % W == 0) rows_kernel<T, W><<<row_blocks, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
+  else rows_kernel<T, 1><<<row_blocks, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
   return cudaGetLastError();
 }
 
