@@ -1,4 +1,4 @@
-// Host entry points of the structure-attention kernels (attention.cu, attention_tc.cu).
+// Host entry points of the structure-attention kernels (attention.cu, attention_tc*.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -25,5 +25,12 @@ cudaError_t tc_forward(const Params<float>&, char* work, int* status, cudaStream
 cudaError_t tc_backward_prepare(const Params<float>&, char* work, cudaStream_t);
 cudaError_t tc_backward_dq(const Params<float>&, char* work, int* status, cudaStream_t);
 cudaError_t tc_backward_dkv(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_wide_dq(const Params<float>&, char* work, int* status, cudaStream_t);      // 65 .. 128 columns
+cudaError_t tc_wide_dkv(const Params<float>&, char* work, int* status, cudaStream_t);
+int64_t tc_second_bytes(const Params<float>&);
+cudaError_t tc_second_prepare(const Params<float>&, char* work, cudaStream_t);
+cudaError_t tc_second_rows(const Params<float>&, char* work, int walk, int* status, cudaStream_t);
+cudaError_t tc_second_join(const Params<float>&, char* work, cudaStream_t);
+cudaError_t tc_second_keys(const Params<float>&, char* work, int* status, cudaStream_t);
 
 }  // namespace attn

@@ -13,10 +13,7 @@
 namespace attn {
 namespace {
 
-struct Source { const float* at; int64_t row, head; int heads; const uint8_t* mask; char* out; };
-struct Sources { Source s[4]; };
-
-// writes the images of up to four tensors: a block per (slot, head, tensor); zeros behind the structure's last
+// writes the images of up to seven tensors: a block per (slot, head, tensor); zeros behind the structure's last
 // row, behind column D and where the mask is 0
 template <int DP>
 __global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const Sources src, int slots) {
@@ -247,11 +244,11 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
 
 // ------------------------------------------------------------------------------------------ backward
 // L and D of the rows of a slot, D = do.o: 64 + 64 numbers a (head, slot), L = +inf behind the last row, so that P is zero there
-__global__ void __launch_bounds__(256) stats_kernel(const Params<float> p, float* __restrict__ out, int slots) {
+__global__ void __launch_bounds__(256) stats_kernel(const Params<float> p, float* __restrict__ out, int slots, int kinds) {
   Part part;
   if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
   const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float* at = out + ((int64_t)h * slots + blockIdx.x) * 2 * SLOT;
+  float* at = out + ((int64_t)h * slots + blockIdx.x) * kinds * SLOT;
   for (int r = warp; r < SLOT; r += 8) {
     const int row = part.row + r;
     float s = 0.f, L = -neg_inf<float>();
@@ -625,21 +622,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
   tear_down(k);
 }
 
-template <typename K>
-cudaError_t raise_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
-template <int DP>
-cudaError_t write_images(const Params<float>& p, const Sources& src, int count, int slots, cudaStream_t s) {
-  image_kernel<DP><<<dim3(slots, p.H, count), 256, 0, s>>>(p, src, slots);
-  return cudaGetLastError();
-}
-
-int image_slots(const Params<float>& p) { return p.N / SLOT + p.num + 2; }
-
-template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { return (int64_t)heads * image_slots(p) * Image<DP>::BYTES; }
-
 template <int DP>
 cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   const int slots = image_slots(p);
@@ -647,16 +629,15 @@ cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStre
   Sources src{};
   src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, ik};
   src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
-  cudaError_t e = write_images<DP>(p, src, 2, slots, s);
+  cudaError_t e = write_images<DP>(p, src, 2, s);
   if (e != cudaSuccess) return e;
-  if ((e = raise_smem(tc_fwd_kernel<DP>, Fwd<DP>::SMEM)) != cudaSuccess) return e;
+  if ((e = raise_smem_limit(tc_fwd_kernel<DP>, Fwd<DP>::SMEM)) != cudaSuccess) return e;
   tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), 160, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
   return cudaGetLastError();
 }
 
 template <int DP>
 cudaError_t prepare_dp(const Params<float>& p, char* work, cudaStream_t s) {
-  const int slots = image_slots(p);
   char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
   float* stats = reinterpret_cast<float*>(io + image_bytes<DP>(p, p.H));
   Sources src{};
@@ -664,10 +645,8 @@ cudaError_t prepare_dp(const Params<float>& p, char* work, cudaStream_t s) {
   src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
   src.s[2] = {p.q, p.qs, p.qh, p.H, nullptr, iq};
   src.s[3] = {p.go, p.gos, p.goh, p.H, nullptr, io};
-  const cudaError_t e = write_images<DP>(p, src, 4, slots, s);
-  if (e != cudaSuccess) return e;
-  stats_kernel<<<dim3(slots, p.H), 256, 0, s>>>(p, stats, slots);
-  return cudaGetLastError();
+  const cudaError_t e = write_images<DP>(p, src, 4, s);
+  return e != cudaSuccess ? e : write_stats(p, stats, 2, s);
 }
 
 template <int DP>
@@ -675,7 +654,7 @@ cudaError_t dq_dp(const Params<float>& p, char* work, int* status, cudaStream_t 
   const int slots = image_slots(p);
   char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK);
   const float* stats = reinterpret_cast<const float*>(iv + image_bytes<DP>(p, p.HK) + 2 * image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem(tc_dq_kernel<DP>, Bwd<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit(tc_dq_kernel<DP>, Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
   tc_dq_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, stats, status);
   return cudaGetLastError();
@@ -686,7 +665,7 @@ cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t
   const int slots = image_slots(p);
   char *iq = work + 2 * image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem(tc_dkv_kernel<DP>, Bwd<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit(tc_dkv_kernel<DP>, Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
   tc_dkv_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{iq, slots}, Images{io, slots}, stats, status);
   return cudaGetLastError();
@@ -694,24 +673,38 @@ cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t
 
 }  // namespace
 
+template <int DP>
+cudaError_t write_images(const Params<float>& p, const Sources& src, int count, cudaStream_t s) {
+  image_kernel<DP><<<dim3(p.N / SLOT + p.num + 2, p.H, count), 256, 0, s>>>(p, src, image_slots(p));
+  return cudaGetLastError();
+}
+template cudaError_t write_images<32>(const Params<float>&, const Sources&, int, cudaStream_t);
+template cudaError_t write_images<64>(const Params<float>&, const Sources&, int, cudaStream_t);
+template cudaError_t write_images<128>(const Params<float>&, const Sources&, int, cudaStream_t);
+
+cudaError_t write_stats(const Params<float>& p, float* out, int kinds, cudaStream_t s) {
+  stats_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H), 256, 0, s>>>(p, out, image_slots(p), kinds);
+  return cudaGetLastError();
+}
+
 int64_t tc_forward_bytes(const Params<float>& p) {
   return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK) : p.D <= 64 ? image_bytes<64>(p, p.HK) : image_bytes<128>(p, p.HK));
 }
 int64_t tc_backward_bytes(const Params<float>& p) {
-  return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK + p.H) : image_bytes<64>(p, p.HK + p.H)) +
+  return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK + p.H) : p.D <= 64 ? image_bytes<64>(p, p.HK + p.H) : image_bytes<128>(p, p.HK + p.H)) +
          (int64_t)p.H * image_slots(p) * 2 * SLOT * 4;
 }
 cudaError_t tc_forward(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   return p.D <= 32 ? forward_dp<32>(p, work, status, s) : p.D <= 64 ? forward_dp<64>(p, work, status, s) : forward_dp<128>(p, work, status, s);
 }
 cudaError_t tc_backward_prepare(const Params<float>& p, char* work, cudaStream_t s) {
-  return p.D <= 32 ? prepare_dp<32>(p, work, s) : prepare_dp<64>(p, work, s);
+  return p.D <= 32 ? prepare_dp<32>(p, work, s) : p.D <= 64 ? prepare_dp<64>(p, work, s) : prepare_dp<128>(p, work, s);
 }
 cudaError_t tc_backward_dq(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  return p.D <= 32 ? dq_dp<32>(p, work, status, s) : dq_dp<64>(p, work, status, s);
+  return p.D <= 32 ? dq_dp<32>(p, work, status, s) : p.D <= 64 ? dq_dp<64>(p, work, status, s) : tc_wide_dq(p, work, status, s);
 }
 cudaError_t tc_backward_dkv(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  return p.D <= 32 ? dkv_dp<32>(p, work, status, s) : dkv_dp<64>(p, work, status, s);
+  return p.D <= 32 ? dkv_dp<32>(p, work, status, s) : p.D <= 64 ? dkv_dp<64>(p, work, status, s) : tc_wide_dkv(p, work, status, s);
 }
 
 }  // namespace attn

@@ -75,8 +75,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
 }
 
 // the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y B_PLANE bytes,
-// 16 K elements a step of 8 columns of A and B_STEP bytes of B
-template <int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO>
+// 16 K elements a step of 8 columns of A and B_STEP bytes of B; MORE: added to what D holds
+template <int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO, bool MORE>
 __device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_plane, uint32_t b, uint32_t idesc) {
   constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
   const uint32_t lo = (b >> 4) | ((LBO >> 4) << 16);
@@ -86,18 +86,44 @@ __device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_pla
 #pragma unroll
     for (int k = 0; k < KSTEPS; ++k) {
       const uint32_t at = lo + (Y[i] * B_PLANE + k * B_STEP) / 16;
-      if (i + k) mma_ts<1>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
+      if (i + k || MORE) mma_ts<1>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
       else mma_ts<0>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
     }
 }
-// the operand image as rows x d (scores) and as d x rows (sums over the rows)
-template <int DP>
+// an operand image of ROWS rows as rows x d (scores) and as d x rows (sums over the rows)
+template <int DP, int ROWS = SLOT, bool MORE = false>
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<DP / 16, Image<DP>::PLANE, 256, 128, DP * 16>(d, a, DP / 2, b, idesc_bf16(SLOT, 0));
+  mma_parts<DP / 16, ROWS * DP * 2, 256, 128, DP * 16, MORE>(d, a, DP / 2, b, idesc_bf16(ROWS, 0));
 }
-template <int DP>
+template <int DP, int ROWS = SLOT, bool MORE = false>
 __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<SLOT / 16, Image<DP>::PLANE, DP * 32, DP * 16, 128>(d, a, SLOT / 2, b, idesc_bf16(DP, 1));
+  mma_parts<ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128, MORE>(d, a, ROWS / 2, b, idesc_bf16(DP, 1));
+}
+
+// the scores with the left operand's parts in shared memory too: 128 rows, planes of 128 DP 2 bytes
+template <int ACCUMULATE>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}\n"
+      :: "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACCUMULATE) : "memory");
+}
+template <int DP, int ROWS>
+__device__ __forceinline__ void mma_scores_ss(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
+  const uint32_t lo_a = (a >> 4) | (8u << 16), lo_b = (b >> 4) | (8u << 16);
+  constexpr uint32_t hi = (uint32_t)DP | (1u << 14);    // DP 16 bytes between groups of 8 rows
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      const uint32_t x = lo_a + X[i] * (DP * 16) + k * 16, y = lo_b + Y[i] * (ROWS * DP / 8) + k * 16;
+      if (i + k) mma_ss<1>(d, x, y, hi, idesc_bf16(ROWS, 0));
+      else mma_ss<0>(d, x, y, hi, idesc_bf16(ROWS, 0));
+    }
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
@@ -113,6 +139,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
       : "r"(addr));
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
@@ -205,6 +242,77 @@ __device__ __forceinline__ uint64_t allowed_bits(int k0, int hi, const uint8_t* 
     bits &= a | (b << 32);
   }
   return bits;
+}
+
+// ---- kernels that stream halves of images: eight warps of rows, a ninth that copies and issues ----
+constexpr int HALF = SLOT / 2, ROW_THREADS = 288;
+template <int DP> constexpr int half_bytes() { return PLANES * HALF * DP * 2; }
+
+// half `half` of an image: its planes one behind the other
+template <int DP>
+__device__ __forceinline__ void load_half(char* to, const char* im, int half, uint64_t* bar) {
+  constexpr int PLANE = HALF * DP * 2;
+#pragma unroll
+  for (int x = 0; x < PLANES; ++x) tc::bulk_g2s(to + x * PLANE, im + x * Image<DP>::PLANE + half * PLANE, PLANE, bar);
+}
+// two neighbouring images as one operand of 128 rows (what the second holds of other structures ends in rows that are not stored)
+template <int DP>
+__device__ __forceinline__ void load_block(char* to, const char* im, uint64_t* bar) {
+#pragma unroll
+  for (int x = 0; x < PLANES; ++x)
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      tc::bulk_g2s(to + (2 * x + s) * Image<DP>::PLANE, im + s * Image<DP>::BYTES + x * Image<DP>::PLANE, Image<DP>::PLANE, bar);
+}
+
+// which of the HALF keys from k0 on may be attended to (all lanes of a warp together)
+__device__ __forceinline__ uint32_t allowed_half(int k0, int hi, const uint8_t* mask) {
+  const int k = k0 + (threadIdx.x & 31);
+  return __ballot_sync(0xffffffffu, k < hi && (mask == nullptr || mask[k]));
+}
+
+// N neighbouring columns of a row, guarded by D
+template <int N>
+__device__ __forceinline__ void store_columns(float* out, const float* v, int c0, int D) {
+#pragma unroll
+  for (int d = 0; d < N; d += 4) {
+    if (D % 4 == 0) {
+      if (c0 + d < D) *reinterpret_cast<float4*>(out + c0 + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c0 + d + e < D) out[c0 + d + e] = v[d + e];
+    }
+  }
+}
+
+// acc += N columns of tensor memory
+template <int N>
+__device__ __forceinline__ void add_columns(uint32_t addr, float* acc) {
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    float o[16];
+    tmem_ld16(addr + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
+  }
+}
+
+// ---- images on the host side ----
+struct Source { const float* at; int64_t row, head; int heads; const uint8_t* mask; char* out; };
+constexpr int MAX_SOURCES = 7;
+struct Sources { Source s[MAX_SOURCES]; };
+
+inline int image_slots(const Params<float>& p) { return p.N / SLOT + p.num + 3; }   // the last: read behind the end by load_block
+template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { return (int64_t)heads * image_slots(p) * Image<DP>::BYTES; }
+template <int DP> cudaError_t write_images(const Params<float>& p, const Sources& src, int count, cudaStream_t s);
+// L, D (and room for two more) of the rows of each slot: `kinds` x SLOT numbers a (head, slot)
+cudaError_t write_stats(const Params<float>& p, float* out, int kinds, cudaStream_t s);
+
+template <typename K>
+cudaError_t raise_smem_limit(K kernel, size_t bytes) {
+  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 }  // namespace attn

@@ -1,0 +1,482 @@
+// The second derivative of structure attention on the tensor cores, up to 64 columns a head (formulas: attention.cu).
+//
+// rows   a block owns 128 queries with the parts of q, A and do in tensor memory and streams halves of the images of
+//        k, v, B, C. Walk 0 forms r = sum P T, sum P (T dP + E) and sum_j (P T) V + P C; walk 1 the products of q'.
+//        Between them a small kernel joins the splits: r, c and do' = sum - r O.
+// keys   a block owns 128 keys with the parts of k and B in tensor memory, those of v and C in shared memory, and streams
+//        q, do and A: k' and v'.
+// The score products of a tile follow the sums of the tile before in one stretch (the weights' parts take the
+// scores' place in tensor memory, which at 64 columns is full), so the threads' work is not hidden under them.
+#include "attention.h"
+#include "attention_tc.cuh"
+
+namespace attn {
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;              // the staged rows carry log2 e: T times it comes out of the products
+constexpr int KINDS = 4;                                // L, D, r, c of a slot's rows
+
+struct Streams { Images a, b, c, d; };
+
+template <int DP>
+struct Rows {
+  static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = 3 * STAGE, SUMS = BARS + 128, SMEM = SUMS + 2 * 128 * 4;
+  static constexpr int P = 3 * DP / 2, S = 3 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W0 = S, W1 = DPO, OUT = E + HALF;
+  static_assert(OUT + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
+};
+
+template <int DP, int WALK>
+__global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Params<float> p, const Streams im,
+                                                                     const float* __restrict__ stats, float* __restrict__ parts,
+                                                                     int* status) {
+  using B = Rows<DP>;
+  constexpr int HB = B::HB;
+  extern __shared__ __align__(128) char smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
+  uint64_t *full = bars, *done = bars + 3, *ready = bars + 4, *pair = bars + 5;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 9);
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 10);
+  float* sums = reinterpret_cast<float*>(smem + B::SUMS);
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  const int warp = threadIdx.x / 32, h = blockIdx.y, hk = h / (p.H / p.HK);
+  int lo = part.lo, hi = part.keys ? part.hi : part.lo;
+  split_range<SLOT>(lo, hi, blockIdx.z, p.splits);
+  const int n = (hi - lo + HALF - 1) / HALF, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
+  if (warp == 8) tmem_alloc(slot, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) tc::mbar_init(bars + i, 1);
+    tc::mbar_init(ready, 8);
+    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
+    *dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *slot, lanes = tmem + ((uint32_t)(warp & 3) << 21);
+  const int row = part.row + (threadIdx.x & 127), half = warp / 4;
+  const bool on = warp < 8 && row < part.hi;
+  if (warp < 8 && n > 0) {
+    const float c2 = p.scale * log2e<float>();
+    if (half == 0) {
+      stage_row<DP>(lanes, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D, c2);
+    } else {
+      stage_row<DP>(lanes + B::P, p.ca + row * p.cas + h * p.cah, on, vec_ok(p.ca, p.cas, p.cah, p.D), p.D, c2);
+      stage_row<DP>(lanes + 2 * B::P, p.go + row * p.gos + h * p.goh, on, vec_ok(p.go, p.gos, p.goh, p.D), p.D, 1.f);
+    }
+    tmem_st_wait();
+    tc::tc_fence_before();
+  }
+  __syncthreads();
+  tc::tc_fence_after();
+  bool ok = true;
+  float acc[DP / 2], R = 0.f, U = 0.f;
+#pragma unroll
+  for (int d = 0; d < DP / 2; ++d) acc[d] = 0.f;
+
+  if (warp == 8) {
+    if (n > 0) {
+      const auto load = [&](int i) {
+        if (elect()) {
+          char* to = smem + i % 3 * B::STAGE;
+          uint64_t* bar = full + i % 3;
+          tc::mbar_arrive_expect_tx(bar, B::STAGE);
+          load_half<DP>(to, image<DP>(im.a, hk, slot0 + i / 2), i % 2, bar);
+          load_half<DP>(to + HB, image<DP>(im.b, hk, slot0 + i / 2), i % 2, bar);
+          load_half<DP>(to + 2 * HB, image<DP>(im.c, hk, slot0 + i / 2), i % 2, bar);
+          load_half<DP>(to + 3 * HB, image<DP>(im.d, hk, slot0 + i / 2), i % 2, bar);
+        }
+      };
+      const uint32_t base = tc::smem_u32(smem);
+      // the sums of tile i - 1 and the scores of tile i, whichever of them there are
+      const auto step = [&](int i, bool sum, bool score) {
+        if (elect()) {
+          if (sum) {
+            const uint32_t at = base + (i + 2) % 3 * B::STAGE;
+            mma_sums<DP, HALF>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0));
+            mma_sums<DP, HALF, true>(tmem + B::OUT, tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
+          }
+          if (score) {
+            const uint32_t at = base + i % 3 * B::STAGE;
+            mma_scores<DP, HALF>(tmem + B::S, tmem, at);
+            mma_scores<DP, HALF>(tmem + B::T, tmem + B::P, at);
+            mma_scores<DP, HALF, true>(tmem + B::T, tmem, at + 2 * HB);
+            mma_scores<DP, HALF>(tmem + B::DPO, tmem + 2 * B::P, at + HB);
+            mma_scores<DP, HALF>(tmem + B::E, tmem + 2 * B::P, at + 3 * HB);
+          }
+          tc::commit_to(done);
+        }
+      };
+      int loaded = min(n, 3);
+      for (int i = 0; i < loaded; ++i) load(i);
+      ok = wait_all(full, 0, dead, status);
+      if (ok) step(0, false, true);
+      for (int i = 0; ok && i < n; ++i) {
+        if (!(ok = wait_all(ready, i & 1, dead, status))) break;
+        tc::tc_fence_after();
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }     // the sums of tile i - 1 are done
+        if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
+        step(i + 1, true, i + 1 < n);
+      }
+      if (!ok)
+        for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
+    }
+    __syncwarp();
+  } else {
+    float L = -neg_inf<float>(), D = 0.f, r = 0.f, c = 0.f;
+    if (on && n > 0) {
+      const float* at = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
+      L = at[0];
+      D = at[SLOT];
+      if (WALK == 1) { r = at[2 * SLOT]; c = at[3 * SLOT]; }
+    }
+    for (int i = 0; i < n; ++i) {
+      const uint32_t bits = allowed_half(lo + i * HALF, hi, p.mask) >> (16 * half);
+      if (!(ok = wait_all(done, i & 1, dead, status))) break;
+      tc::tc_fence_after();
+      float s[16], t[16], dp[16], e[16];
+      tmem_ld16(lanes + B::S + 16 * half, s);
+      tmem_ld16(lanes + B::T + 16 * half, t);
+      tmem_ld16(lanes + B::DPO + 16 * half, dp);
+      tmem_ld16(lanes + B::E + 16 * half, e);
+      tmem_ld_wait();
+      tc::tc_fence_before();
+      arrive(pair + (warp & 3));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const bool in = (bits >> j) & 1;
+        const float pr = in ? ex2(s[j] - L) : 0.f, tt = t[j] * LN2;
+        if (WALK == 0) {
+          s[j] = in ? pr * tt : 0.f;
+          t[j] = pr;
+          R += s[j];
+          U += in ? pr * fmaf(tt, dp[j], e[j]) : 0.f;
+        } else {
+          s[j] = in ? pr * (fmaf(tt - r, dp[j] - D, e[j]) - c) : 0.f;
+          t[j] = in ? pr * (dp[j] - D) : 0.f;
+        }
+      }
+      if (i > 0) add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
+      // the other half's warp of these lanes has read its scores before either writes over them
+      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
+      tc::tc_fence_after();
+      store_parts16(lanes + B::W0 + 8 * half, HALF / 2, s);
+      store_parts16(lanes + B::W1 + 8 * half, HALF / 2, t);
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(ready);
+    }
+    if (ok && n > 0 && (ok = wait_all(done, n & 1, dead, status))) {
+      tc::tc_fence_after();
+      add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
+    }
+    if (WALK == 0 && half == 1) {
+      sums[threadIdx.x & 127] = ok ? R : __int_as_float(0x7fc00000);
+      sums[128 + (threadIdx.x & 127)] = U;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (on) {
+    const int64_t rows = (int64_t)p.H * p.N, at = (int64_t)h * p.N + row;
+    const float g = !ok ? __int_as_float(0x7fc00000) : WALK == 0 ? 1.f : p.scale;
+#pragma unroll
+    for (int d = 0; d < DP / 2; ++d) acc[d] *= g;
+    float* out = WALK == 1 && p.splits == 1 ? p.out0 : p.work + (int64_t)blockIdx.z * rows * p.D;
+    store_columns<DP / 2>(out + ((int64_t)row * p.H + h) * p.D, acc, half * (DP / 2), p.D);
+    if (WALK == 0 && half == 0) {
+      parts[(2 * (int64_t)blockIdx.z) * rows + at] = R + sums[threadIdx.x];
+      parts[(2 * (int64_t)blockIdx.z + 1) * rows + at] = U + sums[128 + threadIdx.x];
+    }
+  }
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// a warp per row of a (slot, head): r, c and do' from the splits; rows without keys give zero
+__global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p, float* __restrict__ stats,
+                                                          const float* __restrict__ parts, int slots) {
+  Part part;
+  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part)) return;
+  const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t rows = (int64_t)p.H * p.N;
+  float* st = stats + ((int64_t)h * slots + blockIdx.x) * KINDS * SLOT;
+  for (int i = warp; i < SLOT; i += 8) {
+    const int row = part.row + i;
+    float r = 0.f, c = 0.f;
+    if (row < part.hi) {
+      if (part.keys) {
+        for (int z = 0; z < p.splits; ++z) {
+          r += parts[(2 * (int64_t)z) * rows + (int64_t)h * p.N + row];
+          c += parts[(2 * (int64_t)z + 1) * rows + (int64_t)h * p.N + row];
+        }
+        c -= st[SLOT + i] * r;
+      }
+      for (int d = lane; d < p.D; d += 32) {
+        float v = 0.f;
+        if (part.keys) {
+          for (int z = 0; z < p.splits; ++z) v += p.work[(z * rows + (int64_t)row * p.H + h) * p.D + d];
+          v -= r * p.o[row * p.os + h * p.oh + d];
+        }
+        p.out3[((int64_t)row * p.H + h) * p.D + d] = v;
+      }
+    }
+    if (lane == 0 && part.keys) {
+      st[2 * SLOT + i] = r;
+      st[3 * SLOT + i] = c;
+    }
+  }
+}
+
+template <int DP>
+struct Keys {
+  static constexpr int HB = half_bytes<DP>(), BLOCK = PLANES * 128 * DP * 2, ST = 2 * BLOCK, STAGE = 3 * HB + KINDS * HALF * 4,
+                       BARS = ST + 3 * STAGE, SMEM = BARS + 128;
+  static constexpr int P = 3 * DP / 2, S = 2 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W = 3 * HALF / 2, M = S, DS = M + W,
+                       PT = DS + W, K2 = PT + W, V2 = K2 + DP;
+  static_assert(V2 + DP <= 512 && K2 >= E + HALF && SMEM <= 232448, "tensor and shared memory");
+};
+
+template <int DP>
+__global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Params<float> p, const Images iv, const Images ic,
+                                                                     const Streams im, const float* __restrict__ stats, int* status) {
+  using B = Keys<DP>;
+  constexpr int HB = B::HB;
+  extern __shared__ __align__(128) char smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
+  uint64_t *full = bars, *full_2 = bars + 3, *done = bars + 4, *ready = bars + 5, *pair = bars + 6;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 10);
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 11);
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  const int warp = threadIdx.x / 32, hk = blockIdx.y, group = p.H / p.HK;
+  int lo = part.lo, hi = part.keys ? part.hi : part.lo;
+  split_range<SLOT>(lo, hi, blockIdx.z, p.splits);
+  const int tiles = (hi - lo + HALF - 1) / HALF, n = tiles * group, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
+  if (warp == 8) tmem_alloc(slot, 512);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
+    tc::mbar_init(ready, 8);
+    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
+    *dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *slot, lanes = tmem + ((uint32_t)(warp & 3) << 21);
+  const int row = part.row + (threadIdx.x & 127), half = warp / 4;
+  if (warp < 8 && n > 0) {
+    const bool on = row < part.hi && (p.mask == nullptr || p.mask[row]);
+    const float c2 = p.scale * log2e<float>();
+    if (half == 0) stage_row<DP>(lanes, p.k + row * p.ks + hk * p.kh, on, vec_ok(p.k, p.ks, p.kh, p.D), p.D, c2);
+    else stage_row<DP>(lanes + B::P, p.cb + row * p.cbs + hk * p.cbh, on, vec_ok(p.cb, p.cbs, p.cbh, p.D), p.D, c2);
+    tmem_st_wait();
+    tc::tc_fence_before();
+  }
+  __syncthreads();
+  tc::tc_fence_after();
+
+  if (warp == 8) {
+    if (n > 0) {
+      const auto load = [&](int i) {                    // q, do, A and the statistics of tile i
+        if (elect()) {
+          char* to = smem + B::ST + i % 3 * B::STAGE;
+          uint64_t* bar = full + i % 3;
+          const int head = hk * group + i / tiles, t = i % tiles;
+          tc::mbar_arrive_expect_tx(bar, B::STAGE);
+          load_half<DP>(to, image<DP>(im.a, head, slot0 + t / 2), t % 2, bar);
+          load_half<DP>(to + HB, image<DP>(im.b, head, slot0 + t / 2), t % 2, bar);
+          load_half<DP>(to + 2 * HB, image<DP>(im.c, head, slot0 + t / 2), t % 2, bar);
+          const float* st = stats + ((int64_t)head * im.a.slots + slot0 + t / 2) * KINDS * SLOT + t % 2 * HALF;
+#pragma unroll
+          for (int x = 0; x < KINDS; ++x) tc::bulk_g2s(to + 3 * HB + x * HALF * 4, st + x * SLOT, HALF * 4, bar);
+        }
+      };
+      const uint32_t base = tc::smem_u32(smem), ring = base + B::ST;
+      const auto step = [&](int i, bool sum, bool score) {
+        if (elect()) {
+          if (sum) {
+            const uint32_t at = ring + (i + 2) % 3 * B::STAGE;
+            mma_sums<DP, HALF>(tmem + B::K2, tmem + B::M, at);
+            mma_sums<DP, HALF, true>(tmem + B::K2, tmem + B::DS, at + 2 * HB);
+            mma_sums<DP, HALF>(tmem + B::V2, tmem + B::PT, at + HB);
+          }
+          if (score) {
+            const uint32_t at = ring + i % 3 * B::STAGE;
+            mma_scores<DP, HALF>(tmem + B::S, tmem, at);
+            mma_scores<DP, HALF>(tmem + B::T, tmem, at + 2 * HB);
+            mma_scores<DP, HALF, true>(tmem + B::T, tmem + B::P, at);
+            mma_scores_ss<DP, HALF>(tmem + B::DPO, base, at + HB);
+            mma_scores_ss<DP, HALF>(tmem + B::E, base + B::BLOCK, at + HB);
+          }
+          tc::commit_to(done);
+        }
+      };
+      if (elect()) {
+        const int s = first_slot(part) + (part.row - part.lo) / SLOT;
+        tc::mbar_arrive_expect_tx(full_2, 2 * B::BLOCK);
+        load_block<DP>(smem, image<DP>(iv, hk, s), full_2);
+        load_block<DP>(smem + B::BLOCK, image<DP>(ic, hk, s), full_2);
+      }
+      __syncwarp();
+      int loaded = min(n, 3);
+      for (int i = 0; i < loaded; ++i) load(i);
+      bool ok = wait_all(full_2, 0, dead, status) && wait_all(full, 0, dead, status);
+      if (ok) step(0, false, true);
+      for (int i = 0; ok && i < n; ++i) {
+        if (!(ok = wait_all(ready, i & 1, dead, status))) break;
+        tc::tc_fence_after();
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
+        if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
+        step(i + 1, true, i + 1 < n);
+      }
+      if (!ok) {
+        tc::mbar_wait(full_2, 0, SPINS);
+        for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
+      }
+    }
+    __syncwarp();
+  } else {
+    float acc[DP];                                      // the first half of the warps adds up k', the second v'
+#pragma unroll
+    for (int d = 0; d < DP; ++d) acc[d] = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      if (!(ok = wait_all(done, i & 1, dead, status))) break;
+      if (!(ok = wait_all(full + i % 3, (i / 3) & 1, dead, status))) break;
+      tc::tc_fence_after();
+      const float* st = reinterpret_cast<const float*>(smem + B::ST + i % 3 * B::STAGE + 3 * HB) + 16 * half;
+      float s[16], t[16], dp[16], e[16];
+      tmem_ld16(lanes + B::S + 16 * half, s);
+      tmem_ld16(lanes + B::T + 16 * half, t);
+      tmem_ld16(lanes + B::DPO + 16 * half, dp);
+      tmem_ld16(lanes + B::E + 16 * half, e);
+      tmem_ld_wait();
+      tc::tc_fence_before();
+      arrive(pair + (warp & 3));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float pr = ex2(s[j] - st[j]), x = t[j] * LN2 - st[2 * HALF + j], y = dp[j] - st[HALF + j];
+        s[j] = pr * (fmaf(x, y, e[j]) - st[3 * HALF + j]);
+        t[j] = pr * y;
+        dp[j] = pr * x;
+      }
+      if (i > 0) add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
+      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
+      tc::tc_fence_after();
+      store_parts16(lanes + B::M + 8 * half, HALF / 2, s);
+      store_parts16(lanes + B::DS + 8 * half, HALF / 2, t);
+      store_parts16(lanes + B::PT + 8 * half, HALF / 2, dp);
+      tmem_st_wait();
+      tc::tc_fence_before();
+      arrive(ready);
+    }
+    if (ok && n > 0 && (ok = wait_all(done, n & 1, dead, status))) {
+      tc::tc_fence_after();
+      add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
+    }
+    if (row < part.hi) {
+      const bool hidden = p.mask != nullptr && !p.mask[row];
+      const float g = !ok ? __int_as_float(0x7fc00000) : half ? 1.f : p.scale;
+#pragma unroll
+      for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : g * acc[d];
+      const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)row * p.HK + hk) * p.D;
+      float* out = p.splits > 1 ? p.work + ((half ? p.splits : 0) + (int64_t)blockIdx.z) * all + at : (half ? p.out2 : p.out1) + at;
+      store_columns<DP>(out, acc, 0, p.D);
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+// where things lie in the workspace: images of k, v, B, C, then q, do, A, the statistics, the splits' r and c
+template <int DP>
+struct Layout {
+  char* at[7];
+  float *stats, *parts;
+  int slots;
+  Layout(const Params<float>& p, char* work) : slots(image_slots(p)) {
+    for (int i = 0; i < 7; ++i) {
+      at[i] = work;
+      work += image_bytes<DP>(p, i < 4 ? p.HK : p.H);
+    }
+    stats = reinterpret_cast<float*>(work);
+    parts = stats + (int64_t)p.H * slots * KINDS * SLOT;
+  }
+  Images operator[](int i) const { return Images{at[i], slots}; }
+};
+
+template <int DP>
+cudaError_t prepare(const Params<float>& p, char* work, cudaStream_t s) {
+  const Layout<DP> w(p, work);
+  Sources src{};
+  src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, w.at[0]};
+  src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, w.at[1]};
+  src.s[2] = {p.cb, p.cbs, p.cbh, p.HK, p.mask, w.at[2]};
+  src.s[3] = {p.cc, p.ccs, p.cch, p.HK, p.mask, w.at[3]};
+  src.s[4] = {p.q, p.qs, p.qh, p.H, nullptr, w.at[4]};
+  src.s[5] = {p.go, p.gos, p.goh, p.H, nullptr, w.at[5]};
+  src.s[6] = {p.ca, p.cas, p.cah, p.H, nullptr, w.at[6]};
+  const cudaError_t e = write_images<DP>(p, src, 7, s);
+  return e != cudaSuccess ? e : write_stats(p, w.stats, KINDS, s);
+}
+
+template <int DP, int WALK>
+cudaError_t rows(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  const Layout<DP> w(p, work);
+  const cudaError_t e = raise_smem_limit(second_rows_kernel<DP, WALK>, Rows<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  second_rows_kernel<DP, WALK><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Rows<DP>::SMEM, s>>>(
+      p, Streams{w[0], w[1], w[2], w[3]}, w.stats, w.parts, status);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t join(const Params<float>& p, char* work, cudaStream_t s) {
+  const Layout<DP> w(p, work);
+  second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
+  return cudaGetLastError();
+}
+
+template <int DP>
+cudaError_t keys(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  const Layout<DP> w(p, work);
+  const cudaError_t e = raise_smem_limit(second_keys_kernel<DP>, Keys<DP>::SMEM);
+  if (e != cudaSuccess) return e;
+  second_keys_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), ROW_THREADS, Keys<DP>::SMEM, s>>>(
+      p, w[1], w[3], Streams{w[4], w[5], w[6], w[6]}, w.stats, status);
+  return cudaGetLastError();
+}
+
+template <int DP>
+int64_t bytes(const Params<float>& p) {
+  return image_bytes<DP>(p, 4 * p.HK + 3 * p.H) + (int64_t)p.H * image_slots(p) * KINDS * SLOT * 4;
+}
+
+}  // namespace
+
+// without the splits' r and c, two numbers a row, head and split, which follow
+int64_t tc_second_bytes(const Params<float>& p) { return p.D <= 32 ? bytes<32>(p) : bytes<64>(p); }
+cudaError_t tc_second_prepare(const Params<float>& p, char* work, cudaStream_t s) {
+  return p.D <= 32 ? prepare<32>(p, work, s) : prepare<64>(p, work, s);
+}
+cudaError_t tc_second_rows(const Params<float>& p, char* work, int walk, int* status, cudaStream_t s) {
+  if (p.D <= 32) return walk == 0 ? rows<32, 0>(p, work, status, s) : rows<32, 1>(p, work, status, s);
+  return walk == 0 ? rows<64, 0>(p, work, status, s) : rows<64, 1>(p, work, status, s);
+}
+cudaError_t tc_second_join(const Params<float>& p, char* work, cudaStream_t s) {
+  return p.D <= 32 ? join<32>(p, work, s) : join<64>(p, work, s);
+}
+cudaError_t tc_second_keys(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  return p.D <= 32 ? keys<32>(p, work, status, s) : keys<64>(p, work, status, s);
+}
+
+}  // namespace attn

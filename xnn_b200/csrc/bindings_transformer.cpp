@@ -90,7 +90,7 @@ template <typename T>
 bool tensor_cores(const attn::Params<T>& p, int width) {
   return sizeof(T) == 4 && p.D <= width && (int64_t)p.N >= TC_LENGTH * std::max(p.num, 1);
 }
-constexpr int TC_FORWARD_WIDTH = 128, TC_BACKWARD_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
+constexpr int TC_FORWARD_WIDTH = 128, TC_BACKWARD_WIDTH = 128, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
 
 torch::Tensor bytes(int64_t n, const torch::Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kUInt8)); }
 
@@ -207,7 +207,8 @@ template <typename T>
 std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& c,
                                         const torch::Tensor& go, const torch::Tensor& q, const torch::Tensor& k,
                                         const torch::Tensor& v, const torch::Tensor& o, const torch::Tensor& lse,
-                                        const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, double scale) {
+                                        const torch::Tensor& ptr, const c10::optional<torch::Tensor>& mask, int64_t max_len, double scale,
+                                        const torch::Tensor& status) {
   auto p = make_params<T>(q, k, v, ptr, mask, scale);
   set_outputs(p, go, o, lse, q);
   check_rows(a, q, p.N, p.H, p.D, "the cotangent of dq");
@@ -220,11 +221,35 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
        v2 = torch::empty({p.N, p.HK, p.D}, q.options()), do2 = torch::empty({p.N, p.H, p.D}, q.options());
   if (p.N == 0) return {q2, k2, v2, do2};
   const auto s = at::cuda::getCurrentCUDAStream();
+  p.out0 = q2.data_ptr<T>(); p.out1 = k2.data_ptr<T>(); p.out2 = v2.data_ptr<T>(); p.out3 = do2.data_ptr<T>();
+  if constexpr (sizeof(T) == 4) {
+    if (tensor_cores(p, TC_SECOND_WIDTH)) {
+      const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D, tiles = p.N / TC_ROWS + 1;
+      const int sq = choose_splits(tiles * p.H, max_len, TC_TILE), sk = choose_splits(tiles * p.HK, max_len, TC_TILE);
+      auto images = bytes(attn::tc_second_bytes(p) + (int64_t)sq * 2 * p.H * p.N * 4, q);
+      auto work = torch::empty({std::max(sq * nq, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+      char* im = static_cast<char*>(images.data_ptr());
+      int* flag = status_of(status, q);
+      p.work = work.template data_ptr<T>();
+      p.splits = sq;
+      XNN_OK(attn::tc_second_prepare(p, im, s));
+      XNN_OK(attn::tc_second_rows(p, im, 0, flag, s));
+      XNN_OK(attn::tc_second_join(p, im, s));
+      XNN_OK(attn::tc_second_rows(p, im, 1, flag, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, p.work, p.out0, s));
+      p.splits = sk;
+      XNN_OK(attn::tc_second_keys(p, im, flag, s));
+      if (sk > 1) {
+        XNN_OK(attn::sum_splits<T>(nk, sk, p.work, p.out1, s));
+        XNN_OK(attn::sum_splits<T>(nk, sk, p.work + (int64_t)sk * nk, p.out2, s));
+      }
+      return {q2, k2, v2, do2};
+    }
+  }
   torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
   p.delta = stats.data_ptr<T>();
   p.r = p.delta + (int64_t)p.H * p.N;
   p.c = p.r + (int64_t)p.H * p.N;
-  p.out0 = q2.data_ptr<T>(); p.out1 = k2.data_ptr<T>(); p.out2 = v2.data_ptr<T>(); p.out3 = do2.data_ptr<T>();
   XNN_OK(attn::row_delta<T>(p, s));
   XNN_OK(attn::second_rows<T>(p, s));
   XNN_OK(attn::second_keys<T>(p, s));
@@ -264,11 +289,12 @@ Setting kept(AutogradContext* ctx) { return {ctx->saved_data["max_len"].toInt(),
 // meets it on every path to the inputs and is refused
 struct AttentionSecond : torch::autograd::Function<AttentionSecond> {
   static variable_list forward(AutogradContext*, Variable a, Variable b, Variable c, Variable go, Variable q, Variable k,
-                               Variable v, Variable o, Variable lse, Variable ptr, c10::optional<Variable> mask, double scale) {
+                               Variable v, Variable o, Variable lse, Variable ptr, c10::optional<Variable> mask, Variable status,
+                               int64_t max_len, double scale) {
     const c10::cuda::CUDAGuard guard(q.device());
     Tensors r;
     AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention second derivative", [&] {
-      r = second_typed<scalar_t>(rows(a), rows(b), rows(c), go, q, k, v, o, lse, ptr, mask, scale);
+      r = second_typed<scalar_t>(rows(a), rows(b), rows(c), go, q, k, v, o, lse, ptr, mask, max_len, scale, status);
     });
     return {r[3], r[0], r[1], r[2]};
   }
@@ -283,6 +309,7 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
                                Variable ptr, c10::optional<Variable> mask, Variable status, int64_t max_len, double scale) {
     go = rows(go);
     ctx->save_for_backward({go, q, k, v, o, lse, ptr, mask.value_or(Variable())});
+    ctx->saved_data["status"] = status;
     keep(ctx, {max_len, scale});
     const c10::cuda::CUDAGuard guard(q.device());
     Tensors r;
@@ -293,7 +320,8 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
-    auto r = AttentionSecond::apply(g[0], g[1], g[2], s[0], s[1], s[2], s[3], s[4], s[5], s[6], maybe(s[7]), kept(ctx).scale);
+    auto r = AttentionSecond::apply(g[0], g[1], g[2], s[0], s[1], s[2], s[3], s[4], s[5], s[6], maybe(s[7]),
+                                    ctx->saved_data["status"].toTensor(), kept(ctx).max_len, kept(ctx).scale);
     r.resize(11);
     return r;
   }
