@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
   }
 }
 
-// joins the splits of a row: a warp per (row, head)
+// Joins the splits of a row, a warp per (row, head): the lanes fetch the splits' statistics at once (at most 32
+// splits), then the partial rows, whose loads do not depend on one another.
 template <typename T>
 __global__ void __launch_bounds__(128) join_kernel(const Params<T> p) {
   const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 32, rows = (int64_t)p.H * p.N;
@@ -122,16 +123,19 @@ __global__ void __launch_bounds__(128) join_kernel(const Params<T> p) {
   const int h = (int)(i % p.H), row = (int)(i / p.H);
   const T* stats = p.work + p.splits * rows * p.D;
   const int64_t at = (int64_t)h * p.N + row;
-  T m = neg_inf<T>();
-  for (int z = 0; z < p.splits; ++z) { const T v = stats[z * rows + at]; m = v > m ? v : m; }
-  const T base = m == neg_inf<T>() ? T(0) : m;
-  T l = T(0);
-  for (int z = 0; z < p.splits; ++z) l += pow2(stats[z * rows + at] - base) * stats[(p.splits + z) * rows + at];
+  const bool in = lane < p.splits;
+  const T mz = in ? stats[lane * rows + at] : neg_inf<T>(), lz = in ? stats[(p.splits + lane) * rows + at] : T(0);
+  const T m = row_max<32>(mz), base = m == neg_inf<T>() ? T(0) : m;
+  const T f = pow2(mz - base), l = row_sum<32>(in ? f * lz : T(0));
   const bool none = m == neg_inf<T>() && l == T(0);
-  for (int d = lane; d < p.D; d += 32) {
+  for (int d = lane; d - lane < p.D; d += 32) {
     T a = T(0);
-    for (int z = 0; z < p.splits; ++z) a += pow2(stats[z * rows + at] - base) * p.work[(z * rows + at) * p.D + d];
-    p.out0[((int64_t)row * p.H + h) * p.D + d] = none ? T(0) : a / l;
+#pragma unroll 4
+    for (int z = 0; z < p.splits; ++z) {
+      const T g = __shfl_sync(0xffffffffu, f, z);
+      if (d < p.D) a += g * p.work[(z * rows + at) * p.D + d];
+    }
+    if (d < p.D) p.out0[((int64_t)row * p.H + h) * p.D + d] = none ? T(0) : a / l;
   }
   if (lane == 0 && p.lse) p.lse[at] = none ? -neg_inf<T>() : m + lg2(l);
 }
@@ -560,19 +564,14 @@ __global__ void __launch_bounds__(C::NT) second_key_kernel(const Params<T> p) {
 }
 
 // ------------------------------------------------------------------------------------------ launches
-template <typename K>
-cudaError_t raise_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
-template <typename T, typename C, typename K>
-cudaError_t launch(K kernel, const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s) {
+template <typename T, typename C, auto KERNEL>
+cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s) {
   const size_t bytes = sizeof(T) * ((size_t)row_tiles * C::BQ * C::LD + (size_t)key_tiles * C::BK * C::LD +
                                     (size_t)squares * C::BQ * C::LDP);
-  const cudaError_t e = raise_smem(kernel, bytes);
+  const cudaError_t e = raise_smem_limit<KERNEL>(bytes);
   if (e != cudaSuccess) return e;
   const dim3 grid(p.N / C::BQ + p.num + 2, heads, p.splits);
-  kernel<<<grid, C::NT, bytes, s>>>(p);
+  KERNEL<<<grid, C::NT, bytes, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -589,19 +588,20 @@ template <int DP> struct Large<double, DP> { using C = typename Small<double, DP
 
 // the second derivative holds seven tiles: 128 double columns leave room for 16 streamed rows
 template <typename T, int DP> struct Second { using C = typename Small<T, DP>::C; };
+template <int DP> struct Second<float, DP> { using C = Cfg<float, 32, 64, DP, 2, 16>; };
 template <> struct Second<double, 128> { using C = Cfg<double, 32, 16, 128, 2, 16>; };
 
 template <typename T, typename C>
 cudaError_t forward_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C>(fwd_kernel<T, C>, p, p.H, 1, 2, 1, s);
+  return launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s);
 }
 template <typename T, typename C>
 cudaError_t dq_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C>(dq_kernel<T, C>, p, p.H, 2, 2, 1, s);
+  return launch<T, C, dq_kernel<T, C>>(p, p.H, 2, 2, 1, s);
 }
 template <typename T, typename C>
 cudaError_t dkv_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C>(dkv_kernel<T, C>, p, p.HK, 2, 2, 2, s);
+  return launch<T, C, dkv_kernel<T, C>>(p, p.HK, 2, 2, 2, s);
 }
 
 #define XNN_ATTN_DIM(D_, ...)                            \
@@ -642,15 +642,15 @@ cudaError_t backward_dkv(const Params<T>& p, bool small, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C>(bwd_short_kernel<T, C>, p, p.HK, 2, 2, 2, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, bwd_short_kernel<T, C>>(p, p.HK, 2, 2, 2, s)))
 }
 template <typename T>
 cudaError_t second_rows(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C>(second_row_kernel<T, C>, p, p.H, 3, 4, 2, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C, second_row_kernel<T, C>>(p, p.H, 3, 4, 2, s)))
 }
 template <typename T>
 cudaError_t second_keys(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C>(second_key_kernel<T, C>, p, p.HK, 4, 3, 3, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C, second_key_kernel<T, C>>(p, p.HK, 4, 3, 3, s)))
 }
 
 #define XNN_ATTN_INST(T)                                                                  \

@@ -90,7 +90,19 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
   const uint32_t tmem = *tmem_slot;
   const int row = part.row + tid;
   const bool on = tid < 128 && row < part.hi;
-  if (warp < 4 && n > 0) {
+  const auto load = [&](uint64_t* bar, int at, const Images& im, int i) {
+    if (elect()) {
+      tc::mbar_arrive_expect_tx(bar, BYTES);
+      tc::bulk_g2s(smem + at * BYTES, image<DP>(im, hk, slot0 + i), BYTES, bar);
+    }
+  };
+  int loaded_k = min(n, 2), loaded_v = min(n, 2);
+  if (warp == 4) {                                      // the copies run while the other warps stage their rows
+    for (int i = 0; i < loaded_k; ++i) {
+      load(full_k + i, i, ik, i);
+      load(full_v + i, 2 + i, iv, i);
+    }
+  } else if (n > 0) {
     stage_row<DP>(tmem + ((uint32_t)warp << 21) + F::Q, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D,
                   p.scale * log2e<float>());
     tmem_st_wait();
@@ -101,12 +113,6 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
 
   if (warp == 4) {
     if (n > 0) {
-      const auto load = [&](uint64_t* bar, int at, const Images& im, int i) {
-        if (elect()) {
-          tc::mbar_arrive_expect_tx(bar, BYTES);
-          tc::bulk_g2s(smem + at * BYTES, image<DP>(im, hk, slot0 + i), BYTES, bar);
-        }
-      };
       const uint32_t sk = tc::smem_u32(smem), sv = sk + 2 * BYTES;
       const auto scores = [&](int i) {
         if (elect()) {
@@ -114,11 +120,6 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
           tc::commit_to(s_done);
         }
       };
-      int loaded_k = min(n, 2), loaded_v = min(n, 2);
-      for (int i = 0; i < loaded_k; ++i) {
-        load(full_k + i, i, ik, i);
-        load(full_v + i, 2 + i, iv, i);
-      }
       bool ok = wait_all(full_k, 0, dead, status);
       if (ok) scores(0);
       for (int i = 0; ok && i < n; ++i) {
@@ -249,18 +250,31 @@ __global__ void __launch_bounds__(256) stats_kernel(const Params<float> p, float
   if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
   const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   float* at = out + ((int64_t)h * slots + blockIdx.x) * kinds * SLOT;
-  for (int r = warp; r < SLOT; r += 8) {
-    const int row = part.row + r;
-    float s = 0.f, L = -neg_inf<float>();
-    if (row < part.hi) {
-      const float *a = p.go + row * p.gos + h * p.goh, *b = p.o + row * p.os + h * p.oh;
-      for (int d = lane; d < p.D; d += 32) s = fmaf(a[d], b[d], s);
-      L = p.lse[(int64_t)h * p.N + row];
+  // a warp's eight rows at once: their loads overlap
+  const bool vec = vec_ok(p.go, p.gos, p.goh, p.D) && vec_ok(p.o, p.os, p.oh, p.D);
+  float s[SLOT / 8], L[SLOT / 8];
+#pragma unroll
+  for (int i = 0; i < SLOT / 8; ++i) {
+    const int row = part.row + warp + 8 * i;
+    s[i] = 0.f;
+    L[i] = row < part.hi ? p.lse[(int64_t)h * p.N + row] : -neg_inf<float>();
+    if (row >= part.hi) continue;
+    const float *a = p.go + row * p.gos + h * p.goh, *b = p.o + row * p.os + h * p.oh;
+    if (vec) {
+      if (4 * lane < p.D) {
+        const float4 x = *reinterpret_cast<const float4*>(a + 4 * lane), y = *reinterpret_cast<const float4*>(b + 4 * lane);
+        s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, x.w * y.w)));
+      }
+    } else {
+      for (int d = lane; d < p.D; d += 32) s[i] = fmaf(a[d], b[d], s[i]);
     }
-    s = row_sum<32>(s);
+  }
+#pragma unroll
+  for (int i = 0; i < SLOT / 8; ++i) {
+    const float v = row_sum<32>(s[i]);
     if (lane == 0) {
-      at[r] = L;
-      at[SLOT + r] = s;
+      at[warp + 8 * i] = L[i];
+      at[SLOT + warp + 8 * i] = v;
     }
   }
 }
@@ -288,13 +302,11 @@ struct Block {                                          // what the two kernels 
   int warp;
 };
 
-// barriers, tensor memory and the parts of the two resident operands
+// barriers and tensor memory
 template <int DP>
-__device__ __forceinline__ Block set_up(char* smem, const Part& part, const float* a, int64_t as, bool av, float af,
-                                        const float* b, int64_t bs, bool bv, int D, const uint8_t* mask, int n) {
-  using B = Bwd<DP>;
+__device__ __forceinline__ Block set_up(char* smem) {
   Block k;
-  k.full = reinterpret_cast<uint64_t*>(smem + STAGES * B::STAGE);
+  k.full = reinterpret_cast<uint64_t*>(smem + STAGES * Bwd<DP>::STAGE);
   k.bars = k.full + STAGES;
   uint32_t* slot = reinterpret_cast<uint32_t*>(k.bars + 8);
   k.dead = reinterpret_cast<volatile int*>(k.bars + 9);
@@ -314,18 +326,20 @@ __device__ __forceinline__ Block set_up(char* smem, const Part& part, const floa
   __syncthreads();
   tc::tc_fence_after();
   k.tmem = *slot;
-  if (k.warp < 8 && n > 0) {
-    const int row = part.row + (threadIdx.x & 127);
-    const bool on = row < part.hi && (mask == nullptr || mask[row]);
-    const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
-    if (k.warp < 4) stage_row<DP>(lanes, a + row * as, on, av, D, af);
-    else stage_row<DP>(lanes + B::PARTS, b + row * bs, on, bv, D, 1.f);
-    tmem_st_wait();
-    tc::tc_fence_before();
-  }
-  __syncthreads();
-  tc::tc_fence_after();
   return k;
+}
+
+// the parts of the two resident operands: a (times af) by the first four warps, b by the others
+template <int DP>
+__device__ __forceinline__ void stage_rows(const Block& k, const Part& part, const float* a, int64_t as, bool av, float af,
+                                           const float* b, int64_t bs, bool bv, int D, const uint8_t* mask) {
+  const int row = part.row + (threadIdx.x & 127);
+  const bool on = row < part.hi && (mask == nullptr || mask[row]);
+  const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
+  if (k.warp < 4) stage_row<DP>(lanes, a + row * as, on, av, D, af);
+  else stage_row<DP>(lanes + Bwd<DP>::PARTS, b + row * bs, on, bv, D, 1.f);
+  tmem_st_wait();
+  tc::tc_fence_before();
 }
 
 __device__ __forceinline__ void tear_down(const Block& k) {
@@ -350,19 +364,27 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
   const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
-  const Block k = set_up<DP>(smem, part, p.q + h * p.qh, p.qs, vec_ok(p.q, p.qs, p.qh, p.D), p.scale * log2e<float>(),
-                             p.go + h * p.goh, p.gos, vec_ok(p.go, p.gos, p.goh, p.D), p.D, nullptr, n);
+  const Block k = set_up<DP>(smem);
+  const auto load = [&](int i) {
+    if (elect()) {
+      char* at = smem + (i % STAGES) * B::STAGE;
+      tc::mbar_arrive_expect_tx(k.full + i % STAGES, 2 * BYTES);
+      tc::bulk_g2s(at, image<DP>(ik, hk, slot0 + i), BYTES, k.full + i % STAGES);
+      tc::bulk_g2s(at + BYTES, image<DP>(iv, hk, slot0 + i), BYTES, k.full + i % STAGES);
+    }
+  };
+  int loaded = min(n, STAGES);
+  if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
+    for (int i = 0; i < loaded; ++i) load(i);
+  } else if (n > 0) {
+    stage_rows<DP>(k, part, p.q + h * p.qh, p.qs, vec_ok(p.q, p.qs, p.qh, p.D), p.scale * log2e<float>(),
+                             p.go + h * p.goh, p.gos, vec_ok(p.go, p.gos, p.goh, p.D), p.D, nullptr);
+  }
+  __syncthreads();
+  tc::tc_fence_after();
   uint64_t *sd_done = k.bars, *dq_done = k.bars + 1, *taken = k.bars + 2, *ds_ready = k.bars + 3;
   if (k.warp == 8) {
     if (n > 0) {
-      const auto load = [&](int i) {
-        if (elect()) {
-          char* at = smem + (i % STAGES) * B::STAGE;
-          tc::mbar_arrive_expect_tx(k.full + i % STAGES, 2 * BYTES);
-          tc::bulk_g2s(at, image<DP>(ik, hk, slot0 + i), BYTES, k.full + i % STAGES);
-          tc::bulk_g2s(at + BYTES, image<DP>(iv, hk, slot0 + i), BYTES, k.full + i % STAGES);
-        }
-      };
       const uint32_t base = tc::smem_u32(smem);
       const auto scores = [&](int i) {
         if (elect()) {
@@ -372,8 +394,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
           tc::commit_to(sd_done);
         }
       };
-      int loaded = min(n, STAGES);
-      for (int i = 0; i < loaded; ++i) load(i);
       bool ok = wait_all(k.full, 0, k.dead, status);
       if (ok) scores(0);
       for (int i = 0; ok && i < n; ++i) {
@@ -484,22 +504,30 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
   int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(q_lo, q_hi, blockIdx.z, p.splits);
   const int tiles = (q_hi - q_lo + SLOT - 1) / SLOT, n = tiles * group, slot0 = first_slot(part) + (q_lo - part.lo) / SLOT;
-  const Block k = set_up<DP>(smem, part, p.k + hk * p.kh, p.ks, vec_ok(p.k, p.ks, p.kh, p.D), p.scale * log2e<float>(),
-                             p.v + hk * p.vh, p.vs, vec_ok(p.v, p.vs, p.vh, p.D), p.D, p.mask, n);
+  const Block k = set_up<DP>(smem);
+  const auto load = [&](int i) {
+    if (elect()) {
+      char* at = smem + (i % STAGES) * B::STAGE;
+      uint64_t* bar = k.full + i % STAGES;
+      const int h = hk * group + i / tiles, slot = slot0 + i % tiles;
+      tc::mbar_arrive_expect_tx(bar, B::STAGE);
+      tc::bulk_g2s(at, image<DP>(iq, h, slot), BYTES, bar);
+      tc::bulk_g2s(at + BYTES, image<DP>(io, h, slot), BYTES, bar);
+      tc::bulk_g2s(at + 2 * BYTES, stats + ((int64_t)h * iq.slots + slot) * 2 * SLOT, 2 * SLOT * 4, bar);
+    }
+  };
+  int loaded = min(n, STAGES);
+  if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
+    for (int i = 0; i < loaded; ++i) load(i);
+  } else if (n > 0) {
+    stage_rows<DP>(k, part, p.k + hk * p.kh, p.ks, vec_ok(p.k, p.ks, p.kh, p.D), p.scale * log2e<float>(),
+                             p.v + hk * p.vh, p.vs, vec_ok(p.v, p.vs, p.vh, p.D), p.D, p.mask);
+  }
+  __syncthreads();
+  tc::tc_fence_after();
   uint64_t *s_done = k.bars, *dp_done = k.bars + 1, *p_ready = k.bars + 2, *ds_ready = k.bars + 3;
   if (k.warp == 8) {
     if (n > 0) {
-      const auto load = [&](int i) {
-        if (elect()) {
-          char* at = smem + (i % STAGES) * B::STAGE;
-          uint64_t* bar = k.full + i % STAGES;
-          const int h = hk * group + i / tiles, slot = slot0 + i % tiles;
-          tc::mbar_arrive_expect_tx(bar, B::STAGE);
-          tc::bulk_g2s(at, image<DP>(iq, h, slot), BYTES, bar);
-          tc::bulk_g2s(at + BYTES, image<DP>(io, h, slot), BYTES, bar);
-          tc::bulk_g2s(at + 2 * BYTES, stats + ((int64_t)h * iq.slots + slot) * 2 * SLOT, 2 * SLOT * 4, bar);
-        }
-      };
       const uint32_t base = tc::smem_u32(smem);
       const auto stage = [&](int i) { return base + (i % STAGES) * B::STAGE; };
       // a product of tile i and the score product of the next tile (or of none) behind it
@@ -511,8 +539,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
         }
       };
       const uint32_t s = k.tmem + B::K_S, dp = k.tmem + B::K_DP, kp = k.tmem, vp = k.tmem + B::PARTS;
-      int loaded = min(n, STAGES);
-      for (int i = 0; i < loaded; ++i) load(i);
       bool ok = wait_all(k.full, 0, k.dead, status);
       if (ok && elect()) {
         mma_scores<DP>(s, kp, stage(0));
@@ -631,7 +657,7 @@ cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStre
   src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
   cudaError_t e = write_images<DP>(p, src, 2, s);
   if (e != cudaSuccess) return e;
-  if ((e = raise_smem_limit(tc_fwd_kernel<DP>, Fwd<DP>::SMEM)) != cudaSuccess) return e;
+  if ((e = raise_smem_limit<tc_fwd_kernel<DP>>(Fwd<DP>::SMEM)) != cudaSuccess) return e;
   tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), 160, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
   return cudaGetLastError();
 }
@@ -654,7 +680,7 @@ cudaError_t dq_dp(const Params<float>& p, char* work, int* status, cudaStream_t 
   const int slots = image_slots(p);
   char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK);
   const float* stats = reinterpret_cast<const float*>(iv + image_bytes<DP>(p, p.HK) + 2 * image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit(tc_dq_kernel<DP>, Bwd<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit<tc_dq_kernel<DP>>(Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
   tc_dq_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, stats, status);
   return cudaGetLastError();
@@ -665,7 +691,7 @@ cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t
   const int slots = image_slots(p);
   char *iq = work + 2 * image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit(tc_dkv_kernel<DP>, Bwd<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit<tc_dkv_kernel<DP>>(Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
   tc_dkv_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{iq, slots}, Images{io, slots}, stats, status);
   return cudaGetLastError();

@@ -169,28 +169,32 @@ __device__ __forceinline__ void store_parts16(uint32_t addr, uint32_t plane, con
   tmem_st8(addr + 2 * plane, c);
 }
 
-// a row of D numbers times f (zero where `on` is false) as three planes of DP / 2 columns
-template <int DP>
-__device__ __forceinline__ void stage_row(uint32_t addr, const float* row, bool on, bool vec, int D, float f) {
+// N columns from c0 on of a row of D numbers times f (zero where `on` is false) as three planes of DP / 2 columns. The
+// loads come first, all of them in flight.
+template <int DP, int N = DP>
+__device__ __forceinline__ void stage_row(uint32_t addr, const float* row, bool on, bool vec, int D, float f, int c0 = 0) {
+  constexpr int STEP = N < 64 ? N : 64;
 #pragma unroll
-  for (int c = 0; c < DP; c += 16) {
-    float v[16];
+  for (int b = 0; b < N; b += STEP) {
+    float v[STEP];
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
+    for (int e = 0; e < STEP; e += 4) {
+      const int c = c0 + b + e;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (on && c + e < D) {
+      if (on && c < D) {
         if (vec) {
-          x = *reinterpret_cast<const float4*>(row + c + e);
+          x = *reinterpret_cast<const float4*>(row + c);
         } else {
-          x.x = row[c + e];
-          if (c + e + 1 < D) x.y = row[c + e + 1];
-          if (c + e + 2 < D) x.z = row[c + e + 2];
-          if (c + e + 3 < D) x.w = row[c + e + 3];
+          x.x = row[c];
+          if (c + 1 < D) x.y = row[c + 1];
+          if (c + 2 < D) x.z = row[c + 2];
+          if (c + 3 < D) x.w = row[c + 3];
         }
       }
       v[e] = f * x.x; v[e + 1] = f * x.y; v[e + 2] = f * x.z; v[e + 3] = f * x.w;
     }
-    store_parts16(addr + c / 2, DP / 2, v);
+#pragma unroll
+    for (int e = 0; e < STEP; e += 16) store_parts16(addr + (c0 + b + e) / 2, DP / 2, v + e);
   }
 }
 
@@ -309,10 +313,5 @@ template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { retur
 template <int DP> cudaError_t write_images(const Params<float>& p, const Sources& src, int count, cudaStream_t s);
 // L, D (and room for two more) of the rows of each slot: `kinds` x SLOT numbers a (head, slot)
 cudaError_t write_stats(const Params<float>& p, float* out, int kinds, cudaStream_t s);
-
-template <typename K>
-cudaError_t raise_smem_limit(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
 
 }  // namespace attn

@@ -57,7 +57,21 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   const uint32_t tmem = *slot, lanes = tmem + ((uint32_t)(warp & 3) << 21);
   const int row = part.row + (threadIdx.x & 127), half = warp / 4;
   const bool on = warp < 8 && row < part.hi;
-  if (warp < 8 && n > 0) {
+  const auto load = [&](int i) {
+    if (elect()) {
+      char* to = smem + i % 3 * B::STAGE;
+      uint64_t* bar = full + i % 3;
+      tc::mbar_arrive_expect_tx(bar, B::STAGE);
+      load_half<DP>(to, image<DP>(im.a, hk, slot0 + i / 2), i % 2, bar);
+      load_half<DP>(to + HB, image<DP>(im.b, hk, slot0 + i / 2), i % 2, bar);
+      load_half<DP>(to + 2 * HB, image<DP>(im.c, hk, slot0 + i / 2), i % 2, bar);
+      load_half<DP>(to + 3 * HB, image<DP>(im.d, hk, slot0 + i / 2), i % 2, bar);
+    }
+  };
+  int loaded = min(n, 3);
+  if (warp == 8) {                                      // the copies run while the other warps stage their rows
+    for (int i = 0; i < loaded; ++i) load(i);
+  } else if (n > 0) {
     const float c2 = p.scale * log2e<float>();
     if (half == 0) {
       stage_row<DP>(lanes, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D, c2);
@@ -77,17 +91,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
 
   if (warp == 8) {
     if (n > 0) {
-      const auto load = [&](int i) {
-        if (elect()) {
-          char* to = smem + i % 3 * B::STAGE;
-          uint64_t* bar = full + i % 3;
-          tc::mbar_arrive_expect_tx(bar, B::STAGE);
-          load_half<DP>(to, image<DP>(im.a, hk, slot0 + i / 2), i % 2, bar);
-          load_half<DP>(to + HB, image<DP>(im.b, hk, slot0 + i / 2), i % 2, bar);
-          load_half<DP>(to + 2 * HB, image<DP>(im.c, hk, slot0 + i / 2), i % 2, bar);
-          load_half<DP>(to + 3 * HB, image<DP>(im.d, hk, slot0 + i / 2), i % 2, bar);
-        }
-      };
       const uint32_t base = tc::smem_u32(smem);
       // the sums of tile i - 1 and the scores of tile i, whichever of them there are
       const auto step = [&](int i, bool sum, bool score) {
@@ -108,8 +111,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
           tc::commit_to(done);
         }
       };
-      int loaded = min(n, 3);
-      for (int i = 0; i < loaded; ++i) load(i);
       ok = wait_all(full, 0, dead, status);
       if (ok) step(0, false, true);
       for (int i = 0; ok && i < n; ++i) {
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   }
 }
 
-// a warp per row of a (slot, head): r, c and do' from the splits; rows without keys give zero
+// A warp per eight rows of a (slot, head), two rows at a time: r, c and do' from the splits; rows without keys give zero.
 __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p, float* __restrict__ stats,
                                                           const float* __restrict__ parts, int slots) {
   Part part;
@@ -204,29 +205,26 @@ __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p,
   const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t rows = (int64_t)p.H * p.N;
   float* st = stats + ((int64_t)h * slots + blockIdx.x) * KINDS * SLOT;
+#pragma unroll 2
   for (int i = warp; i < SLOT; i += 8) {
     const int row = part.row + i;
-    float r = 0.f, c = 0.f;
-    if (row < part.hi) {
-      if (part.keys) {
-        for (int z = 0; z < p.splits; ++z) {
-          r += parts[(2 * (int64_t)z) * rows + (int64_t)h * p.N + row];
-          c += parts[(2 * (int64_t)z + 1) * rows + (int64_t)h * p.N + row];
-        }
-        c -= st[SLOT + i] * r;
+    const bool in = row < part.hi, live = in && part.keys;
+    const int64_t at = (int64_t)h * p.N + (live ? row : 0);
+    const bool mine = live && lane < p.splits;           // a lane per split (at most 32)
+    const float r = row_sum<32>(mine ? parts[(2 * (int64_t)lane) * rows + at] : 0.f);
+    const float u = row_sum<32>(mine ? parts[(2 * (int64_t)lane + 1) * rows + at] : 0.f);
+    for (int d = lane; d < p.D; d += 32) {
+      float v = 0.f;
+      if (live) {
+#pragma unroll 4
+        for (int z = 0; z < p.splits; ++z) v += p.work[(z * rows + (int64_t)row * p.H + h) * p.D + d];
+        v -= r * p.o[row * p.os + h * p.oh + d];
       }
-      for (int d = lane; d < p.D; d += 32) {
-        float v = 0.f;
-        if (part.keys) {
-          for (int z = 0; z < p.splits; ++z) v += p.work[(z * rows + (int64_t)row * p.H + h) * p.D + d];
-          v -= r * p.o[row * p.os + h * p.oh + d];
-        }
-        p.out3[((int64_t)row * p.H + h) * p.D + d] = v;
-      }
+      if (in) p.out3[((int64_t)row * p.H + h) * p.D + d] = v;
     }
     if (lane == 0 && part.keys) {
       st[2 * SLOT + i] = r;
-      st[3 * SLOT + i] = c;
+      st[3 * SLOT + i] = live ? u - st[SLOT + i] * r : 0.f;
     }
   }
 }
@@ -269,7 +267,31 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   tc::tc_fence_after();
   const uint32_t tmem = *slot, lanes = tmem + ((uint32_t)(warp & 3) << 21);
   const int row = part.row + (threadIdx.x & 127), half = warp / 4;
-  if (warp < 8 && n > 0) {
+  const auto load = [&](int i) {                    // q, do, A and the statistics of tile i
+    if (elect()) {
+      char* to = smem + B::ST + i % 3 * B::STAGE;
+      uint64_t* bar = full + i % 3;
+      const int head = hk * group + i / tiles, t = i % tiles;
+      tc::mbar_arrive_expect_tx(bar, B::STAGE);
+      load_half<DP>(to, image<DP>(im.a, head, slot0 + t / 2), t % 2, bar);
+      load_half<DP>(to + HB, image<DP>(im.b, head, slot0 + t / 2), t % 2, bar);
+      load_half<DP>(to + 2 * HB, image<DP>(im.c, head, slot0 + t / 2), t % 2, bar);
+      const float* st = stats + ((int64_t)head * im.a.slots + slot0 + t / 2) * KINDS * SLOT + t % 2 * HALF;
+#pragma unroll
+      for (int x = 0; x < KINDS; ++x) tc::bulk_g2s(to + 3 * HB + x * HALF * 4, st + x * SLOT, HALF * 4, bar);
+    }
+  };
+  int loaded = min(n, 3);
+  if (warp == 8 && n > 0) {
+    if (elect()) {
+      const int s = first_slot(part) + (part.row - part.lo) / SLOT;
+      tc::mbar_arrive_expect_tx(full_2, 2 * B::BLOCK);
+      load_block<DP>(smem, image<DP>(iv, hk, s), full_2);
+      load_block<DP>(smem + B::BLOCK, image<DP>(ic, hk, s), full_2);
+    }
+    __syncwarp();
+    for (int i = 0; i < loaded; ++i) load(i);
+  } else if (n > 0) {
     const bool on = row < part.hi && (p.mask == nullptr || p.mask[row]);
     const float c2 = p.scale * log2e<float>();
     if (half == 0) stage_row<DP>(lanes, p.k + row * p.ks + hk * p.kh, on, vec_ok(p.k, p.ks, p.kh, p.D), p.D, c2);
@@ -282,20 +304,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
 
   if (warp == 8) {
     if (n > 0) {
-      const auto load = [&](int i) {                    // q, do, A and the statistics of tile i
-        if (elect()) {
-          char* to = smem + B::ST + i % 3 * B::STAGE;
-          uint64_t* bar = full + i % 3;
-          const int head = hk * group + i / tiles, t = i % tiles;
-          tc::mbar_arrive_expect_tx(bar, B::STAGE);
-          load_half<DP>(to, image<DP>(im.a, head, slot0 + t / 2), t % 2, bar);
-          load_half<DP>(to + HB, image<DP>(im.b, head, slot0 + t / 2), t % 2, bar);
-          load_half<DP>(to + 2 * HB, image<DP>(im.c, head, slot0 + t / 2), t % 2, bar);
-          const float* st = stats + ((int64_t)head * im.a.slots + slot0 + t / 2) * KINDS * SLOT + t % 2 * HALF;
-#pragma unroll
-          for (int x = 0; x < KINDS; ++x) tc::bulk_g2s(to + 3 * HB + x * HALF * 4, st + x * SLOT, HALF * 4, bar);
-        }
-      };
       const uint32_t base = tc::smem_u32(smem), ring = base + B::ST;
       const auto step = [&](int i, bool sum, bool score) {
         if (elect()) {
@@ -316,15 +324,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
           tc::commit_to(done);
         }
       };
-      if (elect()) {
-        const int s = first_slot(part) + (part.row - part.lo) / SLOT;
-        tc::mbar_arrive_expect_tx(full_2, 2 * B::BLOCK);
-        load_block<DP>(smem, image<DP>(iv, hk, s), full_2);
-        load_block<DP>(smem + B::BLOCK, image<DP>(ic, hk, s), full_2);
-      }
-      __syncwarp();
-      int loaded = min(n, 3);
-      for (int i = 0; i < loaded; ++i) load(i);
       bool ok = wait_all(full_2, 0, dead, status) && wait_all(full, 0, dead, status);
       if (ok) step(0, false, true);
       for (int i = 0; ok && i < n; ++i) {
@@ -432,7 +431,7 @@ cudaError_t prepare(const Params<float>& p, char* work, cudaStream_t s) {
 template <int DP, int WALK>
 cudaError_t rows(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   const Layout<DP> w(p, work);
-  const cudaError_t e = raise_smem_limit(second_rows_kernel<DP, WALK>, Rows<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit<second_rows_kernel<DP, WALK>>(Rows<DP>::SMEM);
   if (e != cudaSuccess) return e;
   second_rows_kernel<DP, WALK><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Rows<DP>::SMEM, s>>>(
       p, Streams{w[0], w[1], w[2], w[3]}, w.stats, w.parts, status);
@@ -449,7 +448,7 @@ cudaError_t join(const Params<float>& p, char* work, cudaStream_t s) {
 template <int DP>
 cudaError_t keys(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   const Layout<DP> w(p, work);
-  const cudaError_t e = raise_smem_limit(second_keys_kernel<DP>, Keys<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit<second_keys_kernel<DP>>(Keys<DP>::SMEM);
   if (e != cudaSuccess) return e;
   second_keys_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), ROW_THREADS, Keys<DP>::SMEM, s>>>(
       p, w[1], w[3], Streams{w[4], w[5], w[6], w[6]}, w.stats, status);

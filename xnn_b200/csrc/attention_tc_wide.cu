@@ -56,12 +56,38 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *slot;
-  if (warp < 4 && n > 0) {
-    const int row = part.row + threadIdx.x;
+  // the images of tile i: the sums read b (do) for dv, a otherwise
+  const auto load = [&](int i, bool y) {
+    if (elect()) {
+      const int head = MODE == DQ ? own / group : own * group + i / tiles, t = MODE == DQ ? i : i % tiles;
+      uint64_t* bar = y ? full_y + i % 3 : full_x + i % 2;
+      char* to = smem + (y ? B::Y + i % 3 * B::HB : B::X + i % 2 * B::HB);
+      const bool with_stats = y && MODE != DQ;
+      tc::mbar_arrive_expect_tx(bar, B::HB + (with_stats ? 2 * HALF * 4 : 0));
+      load_half<DP>(to, image<DP>(y == (MODE == DV) ? b : a, head, slot0 + t / 2), t % 2, bar);
+      if (with_stats) {
+        const float* st = stats + ((int64_t)head * a.slots + slot0 + t / 2) * 2 * SLOT + t % 2 * HALF;
+        char* at = smem + B::ST + i % 3 * (2 * HALF * 4);
+        tc::bulk_g2s(at, st, HALF * 4, bar);
+        tc::bulk_g2s(at + HALF * 4, st + SLOT, HALF * 4, bar);
+      }
+    }
+  };
+  int loaded_x = min(n, 2), loaded_y = min(n, 3);
+  if (warp == 8 && n > 0) {                             // the copies run while the other warps stage their rows
+    if (MODE != DV && elect()) {
+      tc::mbar_arrive_expect_tx(full_2, B::SECOND);
+      load_block<DP>(smem, image<DP>(second, own, first_slot(part) + (part.row - part.lo) / SLOT), full_2);
+    }
+    __syncwarp();
+    for (int i = 0; i < loaded_x; ++i) load(i, false);
+    for (int i = 0; i < loaded_y; ++i) load(i, true);
+  } else if (n > 0) {
+    const int row = part.row + (threadIdx.x & 127);
     const bool on = row < part.hi && (MODE == DQ || p.mask == nullptr || p.mask[row]);
     const float* x = MODE == DQ ? p.q + row * p.qs + own * p.qh : p.k + row * p.ks + own * p.kh;
     const bool vec = MODE == DQ ? vec_ok(p.q, p.qs, p.qh, p.D) : vec_ok(p.k, p.ks, p.kh, p.D);
-    stage_row<DP>(tmem + ((uint32_t)warp << 21), x, on, vec, p.D, p.scale * log2e<float>());
+    stage_row<DP, DP / 2>(tmem + ((uint32_t)(warp & 3) << 21), x, on, vec, p.D, p.scale * log2e<float>(), warp / 4 * (DP / 2));
     tmem_st_wait();
     tc::tc_fence_before();
   }
@@ -70,23 +96,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
 
   if (warp == 8) {
     if (n > 0) {
-      // the images of tile i: the sums read b (do) for dv, a otherwise
-      const auto load = [&](int i, bool y) {
-        if (elect()) {
-          const int head = MODE == DQ ? own / group : own * group + i / tiles, t = MODE == DQ ? i : i % tiles;
-          uint64_t* bar = y ? full_y + i % 3 : full_x + i % 2;
-          char* to = smem + (y ? B::Y + i % 3 * B::HB : B::X + i % 2 * B::HB);
-          const bool with_stats = y && MODE != DQ;
-          tc::mbar_arrive_expect_tx(bar, B::HB + (with_stats ? 2 * HALF * 4 : 0));
-          load_half<DP>(to, image<DP>(y == (MODE == DV) ? b : a, head, slot0 + t / 2), t % 2, bar);
-          if (with_stats) {
-            const float* st = stats + ((int64_t)head * a.slots + slot0 + t / 2) * 2 * SLOT + t % 2 * HALF;
-            char* at = smem + B::ST + i % 3 * (2 * HALF * 4);
-            tc::bulk_g2s(at, st, HALF * 4, bar);
-            tc::bulk_g2s(at + HALF * 4, st + SLOT, HALF * 4, bar);
-          }
-        }
-      };
       const uint32_t base = tc::smem_u32(smem);
       const auto scores = [&](int i) {
         if (elect()) {
@@ -96,15 +105,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
           tc::commit_to(scored);
         }
       };
-      const bool block = MODE != DV && elect();
-      if (block) {
-        tc::mbar_arrive_expect_tx(full_2, B::SECOND);
-        load_block<DP>(smem, image<DP>(second, own, first_slot(part) + (part.row - part.lo) / SLOT), full_2);
-      }
-      __syncwarp();
-      int loaded_x = min(n, 2), loaded_y = min(n, 3);
-      for (int i = 0; i < loaded_x; ++i) load(i, false);
-      for (int i = 0; i < loaded_y; ++i) load(i, true);
       bool ok = (MODE == DV || wait_all(full_2, 0, dead, status)) && wait_all(full_x, 0, dead, status) &&
                 (MODE == DV || wait_all(full_y, 0, dead, status));
       if (ok) scores(0);
@@ -208,7 +208,7 @@ cudaError_t launch_wide(const Params<float>& p, char* work, int* status, cudaStr
   const int slots = image_slots(p);
   char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit(wide_kernel<DP, MODE>, Wide<DP, MODE>::SMEM);
+  const cudaError_t e = raise_smem_limit<wide_kernel<DP, MODE>>(Wide<DP, MODE>::SMEM);
   if (e != cudaSuccess) return e;
   const Images q{iq, slots}, k{ik, slots}, v{iv, slots}, o{io, slots};
   const dim3 grid(p.N / 128 + p.num + 2, MODE == DQ ? p.H : p.HK, p.splits);

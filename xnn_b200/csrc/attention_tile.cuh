@@ -9,6 +9,7 @@
 // (a warp-wide 32-ary search), the grid is floor(N / Q) + num + 2 whatever the lengths are, and no
 // host copy of the lengths is needed. Bounds are clamped to [0, N]: no pointer value leaves the arrays.
 #pragma once
+#include <atomic>
 #include <limits>
 
 #include "attention_params.h"
@@ -220,6 +221,20 @@ __device__ __forceinline__ T row_max(T v) {
 #pragma unroll
   for (int o = TX / 2; o; o >>= 1) { const T u = __shfl_xor_sync(0xffffffffu, v, o); v = v > u ? v : u; }
   return v;
+}
+
+// Shared memory beyond the default 48 KB is asked for once a kernel and device, not at every launch.
+template <auto KERNEL>
+cudaError_t raise_smem_limit(size_t bytes) {
+  static std::atomic<uint64_t> done{0};                  // a bit per device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || bytes <= 48 * 1024) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 }  // namespace attn
