@@ -575,34 +575,15 @@ cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, 
   return cudaGetLastError();
 }
 
-// the square tiles of 32 rows that short structures and the second derivative take; double: two rows and
-// columns a thread (four would need 128 registers for the accumulators alone at 128 columns)
+// The square tiles of 32 rows; double: two rows and columns a thread (four would need 128 registers for the
+// accumulators alone at 128 columns).
 template <typename T, int DP> struct Small;
 template <int DP> struct Small<float, DP> { using C = Cfg<float, 32, 32, DP, 4, 8>; };
 template <int DP> struct Small<double, DP> { using C = Cfg<double, 32, 32, DP, 2, 16>; };
-// the tiles of longer structures; 128 columns take half the streamed rows, so that two blocks fit an SM
-template <typename T, int DP> struct Large;
-template <int DP> struct Large<float, DP> { using C = Cfg<float, 64, 64, DP, 4, 16>; };
-template <> struct Large<float, 128> { using C = Cfg<float, 64, 32, 128, 4, 8>; };
-template <int DP> struct Large<double, DP> { using C = typename Small<double, DP>::C; };
-
 // the second derivative holds seven tiles: 128 double columns leave room for 16 streamed rows
 template <typename T, int DP> struct Second { using C = typename Small<T, DP>::C; };
 template <int DP> struct Second<float, DP> { using C = Cfg<float, 32, 64, DP, 2, 16>; };
 template <> struct Second<double, 128> { using C = Cfg<double, 32, 16, 128, 2, 16>; };
-
-template <typename T, typename C>
-cudaError_t forward_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s);
-}
-template <typename T, typename C>
-cudaError_t dq_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C, dq_kernel<T, C>>(p, p.H, 2, 2, 1, s);
-}
-template <typename T, typename C>
-cudaError_t dkv_with(const Params<T>& p, cudaStream_t s) {
-  return launch<T, C, dkv_kernel<T, C>>(p, p.HK, 2, 2, 2, s);
-}
 
 #define XNN_ATTN_DIM(D_, ...)                            \
   if ((D_) <= 32) { constexpr int DP = 32; __VA_ARGS__; } \
@@ -612,8 +593,8 @@ cudaError_t dkv_with(const Params<T>& p, cudaStream_t s) {
 }  // namespace
 
 template <typename T>
-cudaError_t forward(const Params<T>& p, bool small, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, return small ? (forward_with<T, typename Small<T, DP>::C>(p, s)) : (forward_with<T, typename Large<T, DP>::C>(p, s)))
+cudaError_t forward(const Params<T>& p, cudaStream_t s) {
+  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s)))
 }
 template <typename T>
 cudaError_t forward_join(const Params<T>& p, cudaStream_t s) {
@@ -632,13 +613,11 @@ cudaError_t row_delta(const Params<T>& p, cudaStream_t s) {
   delta_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
   return cudaGetLastError();
 }
-template <typename T>
-cudaError_t backward_dq(const Params<T>& p, bool small, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, return small ? (dq_with<T, typename Small<T, DP>::C>(p, s)) : (dq_with<T, typename Large<T, DP>::C>(p, s)))
+cudaError_t backward_dq(const Params<double>& p, cudaStream_t s) {
+  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dq_kernel<double, C>>(p, p.H, 2, 2, 1, s)))
 }
-template <typename T>
-cudaError_t backward_dkv(const Params<T>& p, bool small, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, return small ? (dkv_with<T, typename Small<T, DP>::C>(p, s)) : (dkv_with<T, typename Large<T, DP>::C>(p, s)))
+cudaError_t backward_dkv(const Params<double>& p, cudaStream_t s) {
+  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dkv_kernel<double, C>>(p, p.HK, 2, 2, 2, s)))
 }
 template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {
@@ -654,12 +633,10 @@ cudaError_t second_keys(const Params<T>& p, cudaStream_t s) {
 }
 
 #define XNN_ATTN_INST(T)                                                                  \
-  template cudaError_t forward<T>(const Params<T>&, bool, cudaStream_t);                  \
+  template cudaError_t forward<T>(const Params<T>&, cudaStream_t);                        \
   template cudaError_t forward_join<T>(const Params<T>&, cudaStream_t);                   \
   template cudaError_t sum_splits<T>(int64_t, int, const T*, T*, cudaStream_t);           \
   template cudaError_t row_delta<T>(const Params<T>&, cudaStream_t);                      \
-  template cudaError_t backward_dq<T>(const Params<T>&, bool, cudaStream_t);              \
-  template cudaError_t backward_dkv<T>(const Params<T>&, bool, cudaStream_t);             \
   template cudaError_t backward_short<T>(const Params<T>&, cudaStream_t);                 \
   template cudaError_t second_rows<T>(const Params<T>&, cudaStream_t);                    \
   template cudaError_t second_keys<T>(const Params<T>&, cudaStream_t);

@@ -70,27 +70,52 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
   return p;
 }
 
+// Which kernels take a call. Structures of at most SHORT atoms fill a square tile of the FP32 pipes; the tensor cores
+// own 128 rows at a time, most of them empty for such a structure, but cost little more for the first 128. float32:
+//   all within SHORT            the short kernels
+//   TC_AVERAGE atoms on average the tensor cores for all; 64 structures of 24-40 atoms at 64 columns, forward /
+//                               backward / second: 11 / 26 / 61 us, short and 64-row FP32 tiles 14 / 44 / 50; of 48-80
+//                               atoms 14 / 33 / 79 and 16 / 48 / 146; 400 x 2 heads of 24-40: 38 / 131 / 274 and 32 / 102 / 298
+//   otherwise                   tensor cores for the structures above SHORT, then the short kernels for the rest
+// float64 has no tensor-core form: 32-row tiles, for short structures with the whole backward pass in one kernel.
+constexpr int TC_AVERAGE = 32, TC_WIDTH = 128, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
+
+struct Plan { bool long_ones, short_ones; };
+
+template <typename T>
+Plan choose(const attn::Params<T>& p, int64_t max_len, bool covered) {
+  if (max_len <= SHORT) return {false, true};
+  if (sizeof(T) == 8 || !covered) return {true, (int64_t)p.N < 48 * (int64_t)p.num};
+  return {true, (int64_t)p.N < TC_AVERAGE * (int64_t)p.num};
+}
+
+// the parameters of the two launches: the long structures (with the rows of none), the short ones
+template <typename T>
+attn::Params<T> long_part(attn::Params<T> p, const Plan& plan) {
+  p.min_len = plan.short_ones ? SHORT + 1 : 0;
+  return p;
+}
+template <typename T>
+attn::Params<T> short_part(attn::Params<T> p, const Plan& plan) {
+  if (plan.long_ones) p.max_len = SHORT;
+  p.splits = 1;
+  return p;
+}
+
 // Few row blocks and long structures: the walk over the other axis is shared out among up to 16 blocks
 // and their results added in order, until there are two blocks a multiprocessor; a share has four tiles
 // at least, or the second pass over the partial results costs what it saves.
-int choose_splits(int64_t row_tiles, int64_t max_len, int tile) {
+int choose_splits(int64_t row_blocks, int64_t max_len, int tile) {
   const int64_t walk = (max_len + tile - 1) / tile;
-  int64_t s = 2 * SMS / std::max<int64_t>(row_tiles, 1);
+  int64_t s = 2 * SMS / std::max<int64_t>(row_blocks, 1);
   s = std::min({s, walk / 4, (int64_t)16});
   return (int)std::max<int64_t>(s, 1);
 }
-
-// mostly short structures: tiles of 32 rows leave less of each tile empty than those of 64
 template <typename T>
-bool mostly_short(const attn::Params<T>& p, int64_t max_len) { return max_len <= SHORT || (int64_t)p.N < 48 * (int64_t)p.num; }
-
-// Long structures of float32 take the tensor cores.
-constexpr int64_t TC_LENGTH = 96;
-template <typename T>
-bool tensor_cores(const attn::Params<T>& p, int width) {
-  return sizeof(T) == 4 && p.D <= width && (int64_t)p.N >= TC_LENGTH * std::max(p.num, 1);
+int splits_of(const attn::Params<T>& p, int heads, int64_t max_len) {
+  const int rows = sizeof(T) == 4 ? TC_ROWS : SHORT;
+  return choose_splits(((int64_t)p.N / rows + std::max(p.num, 1)) * heads, max_len, sizeof(T) == 4 ? TC_TILE : SHORT);
 }
-constexpr int TC_FORWARD_WIDTH = 128, TC_BACKWARD_WIDTH = 128, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
 
 torch::Tensor bytes(int64_t n, const torch::Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kUInt8)); }
 
@@ -112,22 +137,25 @@ std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Te
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = out.data_ptr<T>();
   p.lse = want_stats ? lse.data_ptr<T>() : nullptr;
-  const bool tc = tensor_cores(p, TC_FORWARD_WIDTH), small = !tc && mostly_short(p, max_len);
-  const int rows = tc ? TC_ROWS : small || sizeof(T) == 8 ? 32 : 64;
-  p.splits = choose_splits((int64_t)(p.N / rows + 1) * p.H, max_len, tc ? TC_TILE : rows);
-  torch::Tensor work;
-  if (p.splits > 1) {
-    work = torch::empty({(int64_t)p.splits * p.H * p.N * (p.D + 2)}, q.options());
-    p.work = work.data_ptr<T>();
-  }
-  if constexpr (sizeof(T) == 4) {
-    if (tc) {
-      auto images = bytes(attn::tc_forward_bytes(p), q);
-      XNN_OK(attn::tc_forward(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+  auto plan = choose(p, max_len, true);
+  if (sizeof(T) == 8 && plan.long_ones) plan.short_ones = false;         // one tile for every length
+  if (plan.long_ones) {
+    auto pl = long_part(p, plan);
+    pl.splits = splits_of(p, p.H, max_len);
+    torch::Tensor work, images;
+    if (pl.splits > 1) {
+      work = torch::empty({(int64_t)pl.splits * p.H * p.N * (p.D + 2)}, q.options());
+      pl.work = work.data_ptr<T>();
     }
+    if constexpr (sizeof(T) == 4) {
+      images = bytes(attn::tc_forward_bytes(pl), q);
+      XNN_OK(attn::tc_forward(pl, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+    } else {
+      XNN_OK(attn::forward<T>(pl, s));
+    }
+    if (pl.splits > 1) XNN_OK(attn::forward_join<T>(pl, s));             // short structures' rows hold nothing yet
   }
-  if (!tc) XNN_OK(attn::forward<T>(p, small, s));
-  if (p.splits > 1) XNN_OK(attn::forward_join<T>(p, s));
+  if (plan.short_ones) XNN_OK(attn::forward<T>(short_part(p, plan), s));
   return {out, want_stats ? lse : out};
 }
 
@@ -155,51 +183,41 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
   if (p.N == 0) return {dq, dk, dv};
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = dq.data_ptr<T>(); p.out1 = dk.data_ptr<T>(); p.out2 = dv.data_ptr<T>();
-  const bool tc = tensor_cores(p, TC_BACKWARD_WIDTH), short_first = !tc && mostly_short(p, max_len);
-  if (short_first) {
-    auto ps = p;
-    if (max_len > SHORT) ps.max_len = SHORT;
-    XNN_OK(attn::backward_short<T>(ps, s));
-    if (max_len <= SHORT) return {dq, dk, dv};
-    p.min_len = SHORT + 1;
-  }
-  torch::Tensor delta, images;
-  if constexpr (sizeof(T) == 4) {
-    if (tc) {
-      images = bytes(attn::tc_backward_bytes(p), q);
-      XNN_OK(attn::tc_backward_prepare(p, static_cast<char*>(images.data_ptr()), s));
+  const auto plan = choose(p, max_len, true);
+  if (plan.long_ones) {
+    auto pl = long_part(p, plan);
+    const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
+    const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
+    torch::Tensor work, scratch;
+    if (sq > 1 || sk > 1) {
+      work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+      pl.work = work.data_ptr<T>();
+    }
+    if constexpr (sizeof(T) == 4) {
+      scratch = bytes(attn::tc_backward_bytes(pl), q);
+      char* images = static_cast<char*>(scratch.data_ptr());
+      XNN_OK(attn::tc_backward_prepare(pl, images, s));
+      pl.splits = sq;
+      XNN_OK(attn::tc_backward_dq(pl, images, status_of(status, q), s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      pl.splits = sk;
+      XNN_OK(attn::tc_backward_dkv(pl, images, status_of(status, q), s));
+    } else {
+      scratch = torch::empty({p.H, p.N}, q.options());
+      pl.delta = scratch.data_ptr<T>();
+      XNN_OK(attn::row_delta<T>(pl, s));
+      pl.splits = sq;
+      XNN_OK(attn::backward_dq(pl, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      pl.splits = sk;
+      XNN_OK(attn::backward_dkv(pl, s));
+    }
+    if (sk > 1) {
+      XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, s));
+      XNN_OK(attn::sum_splits<T>(nk, sk, pl.work + (int64_t)sk * nk, p.out2, s));
     }
   }
-  if (!tc) {
-    delta = torch::empty({p.H, p.N}, q.options());
-    p.delta = delta.data_ptr<T>();
-    XNN_OK(attn::row_delta<T>(p, s));
-  }
-  const int tile = tc ? TC_TILE : sizeof(T) == 8 ? 32 : 64;
-  const int64_t tiles = p.N / (tc ? TC_ROWS : tile) + 1;
-  torch::Tensor work;
-  const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
-  const int sq = short_first ? 1 : choose_splits(tiles * p.H, max_len, tile);
-  const int sk = short_first ? 1 : choose_splits(tiles * p.HK, max_len, tile);
-  if (sq > 1 || sk > 1) {
-    work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
-    p.work = work.data_ptr<T>();
-  }
-  p.splits = sq;
-  if constexpr (sizeof(T) == 4) {
-    if (tc) XNN_OK(attn::tc_backward_dq(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
-  }
-  if (!tc) XNN_OK(attn::backward_dq<T>(p, false, s));
-  if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, p.work, p.out0, s));
-  p.splits = sk;
-  if constexpr (sizeof(T) == 4) {
-    if (tc) XNN_OK(attn::tc_backward_dkv(p, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
-  }
-  if (!tc) XNN_OK(attn::backward_dkv<T>(p, false, s));
-  if (sk > 1) {
-    XNN_OK(attn::sum_splits<T>(nk, sk, p.work, p.out1, s));
-    XNN_OK(attn::sum_splits<T>(nk, sk, p.work + (int64_t)sk * nk, p.out2, s));
-  }
+  if (plan.short_ones) XNN_OK(attn::backward_short<T>(short_part(p, plan), s));
   return {dq, dk, dv};
 }
 
@@ -222,37 +240,44 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
   if (p.N == 0) return {q2, k2, v2, do2};
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = q2.data_ptr<T>(); p.out1 = k2.data_ptr<T>(); p.out2 = v2.data_ptr<T>(); p.out3 = do2.data_ptr<T>();
+  bool rest = true;                                    // what the FP32 / FP64 pipes take
+  auto pr = p;
   if constexpr (sizeof(T) == 4) {
-    if (tensor_cores(p, TC_SECOND_WIDTH)) {
-      const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D, tiles = p.N / TC_ROWS + 1;
-      const int sq = choose_splits(tiles * p.H, max_len, TC_TILE), sk = choose_splits(tiles * p.HK, max_len, TC_TILE);
-      auto images = bytes(attn::tc_second_bytes(p) + (int64_t)sq * 2 * p.H * p.N * 4, q);
-      auto work = torch::empty({std::max(sq * nq, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+    const auto plan = choose(p, max_len, p.D <= TC_SECOND_WIDTH);
+    if (plan.long_ones && p.D <= TC_SECOND_WIDTH) {
+      auto pl = long_part(p, plan);
+      const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
+      const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
+      auto images = bytes(attn::tc_second_bytes(pl) + (int64_t)sq * 2 * p.H * p.N * 4, q);
+      torch::Tensor work = torch::empty({std::max(sq * nq, sk > 1 ? 2 * sk * nk : 0)}, q.options());
       char* im = static_cast<char*>(images.data_ptr());
       int* flag = status_of(status, q);
-      p.work = work.template data_ptr<T>();
-      p.splits = sq;
-      XNN_OK(attn::tc_second_prepare(p, im, s));
-      XNN_OK(attn::tc_second_rows(p, im, 0, flag, s));
-      XNN_OK(attn::tc_second_join(p, im, s));
-      XNN_OK(attn::tc_second_rows(p, im, 1, flag, s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, p.work, p.out0, s));
-      p.splits = sk;
-      XNN_OK(attn::tc_second_keys(p, im, flag, s));
+      pl.work = work.data_ptr<T>();
+      pl.splits = sq;
+      XNN_OK(attn::tc_second_prepare(pl, im, s));
+      XNN_OK(attn::tc_second_rows(pl, im, 0, flag, s));
+      XNN_OK(attn::tc_second_join(pl, im, s));
+      XNN_OK(attn::tc_second_rows(pl, im, 1, flag, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      pl.splits = sk;
+      XNN_OK(attn::tc_second_keys(pl, im, flag, s));
       if (sk > 1) {
-        XNN_OK(attn::sum_splits<T>(nk, sk, p.work, p.out1, s));
-        XNN_OK(attn::sum_splits<T>(nk, sk, p.work + (int64_t)sk * nk, p.out2, s));
+        XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, s));
+        XNN_OK(attn::sum_splits<T>(nk, sk, pl.work + (int64_t)sk * nk, p.out2, s));
       }
-      return {q2, k2, v2, do2};
+      rest = plan.short_ones;
+      pr = short_part(p, plan);
     }
   }
-  torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
-  p.delta = stats.data_ptr<T>();
-  p.r = p.delta + (int64_t)p.H * p.N;
-  p.c = p.r + (int64_t)p.H * p.N;
-  XNN_OK(attn::row_delta<T>(p, s));
-  XNN_OK(attn::second_rows<T>(p, s));
-  XNN_OK(attn::second_keys<T>(p, s));
+  if (rest) {
+    torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
+    pr.delta = stats.data_ptr<T>();
+    pr.r = pr.delta + (int64_t)p.H * p.N;
+    pr.c = pr.r + (int64_t)p.H * p.N;
+    XNN_OK(attn::row_delta<T>(pr, s));
+    XNN_OK(attn::second_rows<T>(pr, s));
+    XNN_OK(attn::second_keys<T>(pr, s));
+  }
   return {q2, k2, v2, do2};
 }
 
