@@ -75,29 +75,42 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
 }
 
 // the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y B_PLANE bytes,
-// 16 K elements a step of 8 columns of A and B_STEP bytes of B; MORE: added to what D holds
-template <int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO, bool MORE>
-__device__ __forceinline__ void mma_parts(uint32_t d, uint32_t a, uint32_t a_plane, uint32_t b, uint32_t idesc) {
+// 16 K elements a step of 8 columns of A and B_STEP bytes of B. With PAIRS = 2 the sum of two such products, part by
+// part: the tensor cores cut what a sum does not hold, so nothing small should come after something large.
+template <int PAIRS, int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO>
+__device__ __forceinline__ void mma_parts(uint32_t d, const uint32_t (&a)[PAIRS], uint32_t a_plane, const uint32_t (&b)[PAIRS],
+                                          uint32_t idesc) {
   constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
-  const uint32_t lo = (b >> 4) | ((LBO >> 4) << 16);
   constexpr uint32_t hi = (SBO >> 4) | (1u << 14);      // bit 46: descriptor version
 #pragma unroll
   for (int i = 0; i < 6; ++i)
 #pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
-      const uint32_t at = lo + (Y[i] * B_PLANE + k * B_STEP) / 16;
-      if (i + k || MORE) mma_ts<1>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
-      else mma_ts<0>(d, a + X[i] * a_plane + 8 * k, at, hi, idesc);
+    for (int j = 0; j < PAIRS; ++j) {
+      const uint32_t lo = (b[j] >> 4) | ((LBO >> 4) << 16);
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) {
+        const uint32_t at = lo + (Y[i] * B_PLANE + k * B_STEP) / 16;
+        if (i + j + k) mma_ts<1>(d, a[j] + X[i] * a_plane + 8 * k, at, hi, idesc);
+        else mma_ts<0>(d, a[j] + X[i] * a_plane + 8 * k, at, hi, idesc);
+      }
     }
 }
 // an operand image of ROWS rows as rows x d (scores) and as d x rows (sums over the rows)
-template <int DP, int ROWS = SLOT, bool MORE = false>
+template <int DP, int ROWS = SLOT>
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<DP / 16, ROWS * DP * 2, 256, 128, DP * 16, MORE>(d, a, DP / 2, b, idesc_bf16(ROWS, 0));
+  mma_parts<1, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, {a}, DP / 2, {b}, idesc_bf16(ROWS, 0));
 }
-template <int DP, int ROWS = SLOT, bool MORE = false>
+template <int DP, int ROWS>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {
+  mma_parts<2, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, {a0, a1}, DP / 2, {b0, b1}, idesc_bf16(ROWS, 0));
+}
+template <int DP, int ROWS = SLOT>
 __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128, MORE>(d, a, ROWS / 2, b, idesc_bf16(DP, 1));
+  mma_parts<1, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, {a}, ROWS / 2, {b}, idesc_bf16(DP, 1));
+}
+template <int DP, int ROWS>
+__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {
+  mma_parts<2, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, {a0, a1}, ROWS / 2, {b0, b1}, idesc_bf16(DP, 1));
 }
 
 // the scores with the left operand's parts in shared memory too: 128 rows, planes of 128 DP 2 bytes

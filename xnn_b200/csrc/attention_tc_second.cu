@@ -97,14 +97,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
         if (elect()) {
           if (sum) {
             const uint32_t at = base + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0));
-            mma_sums<DP, HALF, true>(tmem + B::OUT, tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
+            mma_sums<DP, HALF>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0), tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
           }
           if (score) {
             const uint32_t at = base + i % 3 * B::STAGE;
             mma_scores<DP, HALF>(tmem + B::S, tmem, at);
-            mma_scores<DP, HALF>(tmem + B::T, tmem + B::P, at);
-            mma_scores<DP, HALF, true>(tmem + B::T, tmem, at + 2 * HB);
+            mma_scores<DP, HALF>(tmem + B::T, tmem + B::P, at, tmem, at + 2 * HB);
             mma_scores<DP, HALF>(tmem + B::DPO, tmem + 2 * B::P, at + HB);
             mma_scores<DP, HALF>(tmem + B::E, tmem + 2 * B::P, at + 3 * HB);
           }
@@ -309,15 +307,13 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
         if (elect()) {
           if (sum) {
             const uint32_t at = ring + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF>(tmem + B::K2, tmem + B::M, at);
-            mma_sums<DP, HALF, true>(tmem + B::K2, tmem + B::DS, at + 2 * HB);
+            mma_sums<DP, HALF>(tmem + B::K2, tmem + B::M, at, tmem + B::DS, at + 2 * HB);
             mma_sums<DP, HALF>(tmem + B::V2, tmem + B::PT, at + HB);
           }
           if (score) {
             const uint32_t at = ring + i % 3 * B::STAGE;
             mma_scores<DP, HALF>(tmem + B::S, tmem, at);
-            mma_scores<DP, HALF>(tmem + B::T, tmem, at + 2 * HB);
-            mma_scores<DP, HALF, true>(tmem + B::T, tmem + B::P, at);
+            mma_scores<DP, HALF>(tmem + B::T, tmem, at + 2 * HB, tmem + B::P, at);
             mma_scores_ss<DP, HALF>(tmem + B::DPO, base, at + HB);
             mma_scores_ss<DP, HALF>(tmem + B::E, base + B::BLOCK, at + HB);
           }
