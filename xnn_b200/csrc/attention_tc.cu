@@ -48,28 +48,30 @@ __global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const
 }
 
 // ------------------------------------------------------------------------------------------ forward
-// Warps 0-3 own a row each thread; a lane of warp 4 copies and issues. Tensor memory: the rows' parts, one
-// region that holds S and then the parts of P in its place, and the product P V of one tile, which the rows'
-// threads add to their accumulators in registers (rounded to nearest, which a sum over thousands of keys
-// inside the tensor core is not). At 64 columns that is 256 of 512 columns and 96 KB, so two blocks share an SM
-// and one's softmax runs under the other's products.
+// Eight warps of rows, two threads a row (half of a tile's keys and of the output's columns each), and a ninth that
+// copies and issues. Tensor memory: the rows' parts, one region that holds S and then the parts of P in its place, and
+// the product P V of one tile, which the rows' threads add to their accumulators in registers (rounded to nearest,
+// which a sum over thousands of keys inside the tensor core is not). At 64 columns that is 256 of 512 columns and
+// 97 KB, so two blocks share an SM and one's softmax runs under the other's products. One thread a row left the
+// tensor cores idle a third of the time: its 800 instructions a tile took longer than the other block's products.
 template <int DP>
 struct Fwd {
   static constexpr int Q = 0, S = 3 * DP / 2, O = S + 96, COLUMNS = O + DP <= 256 ? 256 : 512;
-  static constexpr int SMEM = 4 * Image<DP>::BYTES + 128;
+  static constexpr int BARS = 4 * Image<DP>::BYTES, TOPS = BARS + 128, SMEM = TOPS + 2 * 128 * 4;
   static constexpr int BLOCKS = COLUMNS == 256 ? 2 : 1;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Params<float> p, const Images ik, const Images iv,
-                                                                      int* status) {
+__global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Params<float> p, const Images ik,
+                                                                              const Images iv, int* status) {
   using F = Fwd<DP>;
-  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  constexpr int BYTES = Image<DP>::BYTES;
   extern __shared__ __align__(128) char smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 4 * BYTES);
-  uint64_t *full_k = bars, *full_v = bars + 2, *s_done = bars + 4, *p_ready = bars + 5;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 6);
-  volatile int* dead = reinterpret_cast<volatile int*>(bars + 7);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
+  uint64_t *full_k = bars, *full_v = bars + 2, *s_done = bars + 4, *o_done = bars + 5, *p_ready = bars + 6, *pair = bars + 7;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 12);
+  float* tops = reinterpret_cast<float*>(smem + F::TOPS);
   Part part;
   if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
   const int tid = threadIdx.x, warp = tid / 32;
@@ -77,19 +79,20 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
   const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
-  if (warp == 4) tmem_alloc(tmem_slot, F::COLUMNS);
+  if (warp == 8) tmem_alloc(tmem_slot, F::COLUMNS);
   if (tid == 0) {
-    for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
-    tc::mbar_init(p_ready, 4);
+    for (int i = 0; i < 6; ++i) tc::mbar_init(bars + i, 1);
+    tc::mbar_init(p_ready, 8);
+    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int row = part.row + tid;
-  const bool on = tid < 128 && row < part.hi;
+  const uint32_t tmem = *tmem_slot, lanes = tmem + ((uint32_t)(warp & 3) << 21);
+  const int r = tid & 127, row = part.row + r, half = warp / 4;
+  const bool on = warp < 8 && row < part.hi;
   const auto load = [&](uint64_t* bar, int at, const Images& im, int i) {
     if (elect()) {
       tc::mbar_arrive_expect_tx(bar, BYTES);
@@ -97,21 +100,25 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
     }
   };
   int loaded_k = min(n, 2), loaded_v = min(n, 2);
-  if (warp == 4) {                                      // the copies run while the other warps stage their rows
+  if (warp == 8) {                                      // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded_k; ++i) {
       load(full_k + i, i, ik, i);
       load(full_v + i, 2 + i, iv, i);
     }
   } else if (n > 0) {
-    stage_row<DP>(tmem + ((uint32_t)warp << 21) + F::Q, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D,
-                  p.scale * log2e<float>());
+    stage_row<DP, DP / 2>(lanes + F::Q, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D,
+                          p.scale * log2e<float>(), half * (DP / 2));
     tmem_st_wait();
     tc::tc_fence_before();
   }
   __syncthreads();
   tc::tc_fence_after();
+  bool ok = true;
+  float m = neg_inf<float>(), l = 0.f, acc[DP / 2];
+#pragma unroll
+  for (int d = 0; d < DP / 2; ++d) acc[d] = 0.f;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (n > 0) {
       const uint32_t sk = tc::smem_u32(smem), sv = sk + 2 * BYTES;
       const auto scores = [&](int i) {
@@ -120,7 +127,7 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
           tc::commit_to(s_done);
         }
       };
-      bool ok = wait_all(full_k, 0, dead, status);
+      ok = wait_all(full_k, 0, dead, status);
       if (ok) scores(0);
       for (int i = 0; ok && i < n; ++i) {
         // the probabilities of tile i are there, so S(i) and P V(i - 1) are done and their images free
@@ -129,12 +136,13 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
         if (i + 2 < n) { load(full_k + (i & 1), i & 1, ik, i + 2); loaded_k = i + 3; }
         if (i > 0 && i + 1 < n) { load(full_v + ((i + 1) & 1), 2 + ((i + 1) & 1), iv, i + 1); loaded_v = i + 2; }
         if (!(ok = wait_all(full_v + (i & 1), (i >> 1) & 1, dead, status))) break;
-        if (elect()) mma_sums<DP>(tmem + F::O, tmem + F::S, sv + (i & 1) * BYTES);
+        if (elect()) {
+          mma_sums<DP>(tmem + F::O, tmem + F::S, sv + (i & 1) * BYTES);
+          tc::commit_to(o_done);
+        }
         if (i + 1 < n) {
           if (!(ok = wait_all(full_k + ((i + 1) & 1), ((i + 1) >> 1) & 1, dead, status))) break;
           scores(i + 1);
-        } else if (elect()) {
-          tc::commit_to(s_done);
         }
       }
       if (!ok) {                                        // copies in flight must land before the block ends
@@ -144,36 +152,53 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
     }
     __syncwarp();
   } else {
-    const uint32_t lanes = tmem + ((uint32_t)warp << 21);
-    float m = neg_inf<float>(), l = 0.f, f = 1.f, acc[DP];
+    float f = 1.f;
+    const auto add = [&] {                              // P V of the tile before, relative to its maximum
 #pragma unroll
-    for (int d = 0; d < DP; ++d) acc[d] = 0.f;
-    bool ok = true;
+      for (int c = 0; c < DP / 2; c += 16) {
+        float o[16];
+        tmem_ld16(lanes + F::O + half * (DP / 2) + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
+      }
+    };
     for (int i = 0; i < n; ++i) {
-      const uint64_t bits = allowed_bits(k_lo + i * SLOT, k_hi, p.mask);
+      const uint32_t bits = (uint32_t)(allowed_bits(k_lo + i * SLOT, k_hi, p.mask) >> (32 * half));
+      if (i > 0) {                                      // under the scores of this tile
+        if (!(ok = wait_all(o_done, (i - 1) & 1, dead, status))) break;
+        tc::tc_fence_after();
+        add();
+      }
       if (!(ok = wait_all(s_done, i & 1, dead, status))) break;
       tc::tc_fence_after();
-      float s[SLOT];
-      tmem_ld32(lanes + F::S, s);
-      tmem_ld32(lanes + F::S + 32, s + 32);
+      float s[32];
+      tmem_ld32(lanes + F::S + 32 * half, s);
       tmem_ld_wait();
-      if (bits != ~0ull) {
+      if (bits != ~0u) {
 #pragma unroll
-        for (int j = 0; j < SLOT; ++j)
+        for (int j = 0; j < 32; ++j)
           if (!((bits >> j) & 1)) s[j] = neg_inf<float>();
       }
       float t0 = s[0], t1 = s[1], t2 = s[2], t3 = s[3];
 #pragma unroll
-      for (int j = 4; j < SLOT; j += 4) {
+      for (int j = 4; j < 32; j += 4) {
         t0 = fmaxf(t0, s[j]); t1 = fmaxf(t1, s[j + 1]); t2 = fmaxf(t2, s[j + 2]); t3 = fmaxf(t3, s[j + 3]);
       }
-      const float mn = fmaxf(m, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
+      const float mine = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+      tops[half * 128 + r] = mine;
+      tc::tc_fence_before();
+      arrive(pair + (warp & 3));
+      // the row's other half: its maximum, and it has read its scores before either writes over them
+      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
+      tc::tc_fence_after();
+      const float mn = fmaxf(m, fmaxf(mine, tops[(half ^ 1) * 128 + r]));
       const float base = mn == neg_inf<float>() ? 0.f : mn;
-      const float fn = ex2(m - base);
+      f = ex2(m - base);
       m = mn;
       float u0 = 0.f, u1 = 0.f;
 #pragma unroll
-      for (int c = 0; c < SLOT; c += 16) {
+      for (int c = 0; c < 32; c += 16) {
 #pragma unroll
         for (int j = c; j < c + 16; j += 2) {
           s[j] = ex2(s[j] - base);
@@ -181,51 +206,33 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
           u0 += s[j];
           u1 += s[j + 1];
         }
-        store_parts16(lanes + F::S + c / 2, SLOT / 2, s + c);
+        store_parts16(lanes + F::S + 16 * half + c / 2, SLOT / 2, s + c);
       }
-      l = fmaf(l, fn, u0 + u1);
-      if (i > 0) {                                      // P V of the tile before, relative to its maximum
-#pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-          float o[32];
-          tmem_ld32(lanes + F::O + c, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
-        }
-      }
-      f = fn;
+      l = fmaf(l, f, u0 + u1);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(p_ready);
     }
-    if (ok && n > 0 && (ok = wait_all(s_done, n & 1, dead, status))) {
+    if (ok && n > 0 && (ok = wait_all(o_done, (n - 1) & 1, dead, status))) {
       tc::tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        tmem_ld32(lanes + F::O + c, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
-      }
+      add();
     }
-    if (on) {
-      const bool none = m == neg_inf<float>() && l == 0.f;
-      const bool split = p.splits > 1;
-      const int64_t rows = (int64_t)p.H * p.N, at = blockIdx.z * rows + (int64_t)h * p.N + row;
-      const float g = !ok ? __int_as_float(0x7fc00000) : split ? 1.f : none ? 0.f : 1.f / l;
-      float* out = split ? p.work + at * p.D : p.out0 + ((int64_t)row * p.H + h) * p.D;
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp < 8) tops[half * 128 + r] = ok ? l : __int_as_float(0x7fc00000);
+  __syncthreads();
+  if (on) {
+    l = tops[r] + tops[128 + r];
+    const bool none = m == neg_inf<float>() && l == 0.f;
+    const bool split = p.splits > 1;
+    const int64_t rows = (int64_t)p.H * p.N, at = blockIdx.z * rows + (int64_t)h * p.N + row;
+    const float g = split ? 1.f : none ? 0.f : 1.f / l;
+    float* out = split ? p.work + at * p.D : p.out0 + ((int64_t)row * p.H + h) * p.D;
 #pragma unroll
-      for (int d = 0; d < DP; d += 4) {
-        if (p.D % 4 == 0) {
-          if (d < p.D) *reinterpret_cast<float4*>(out + d) = make_float4(g * acc[d], g * acc[d + 1], g * acc[d + 2], g * acc[d + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < p.D) out[d + e] = g * acc[d + e];
-        }
-      }
+    for (int d = 0; d < DP / 2; ++d) acc[d] *= g;
+    store_columns<DP / 2>(out, acc, half * (DP / 2), p.D);
+    if (half == 0) {
       if (split) {
         float* stats = p.work + p.splits * rows * p.D;
         stats[at] = m;
@@ -235,9 +242,7 @@ __global__ void __launch_bounds__(160, Fwd<DP>::BLOCKS) tc_fwd_kernel(const Para
       }
     }
   }
-  tc::tc_fence_before();
-  __syncthreads();
-  if (warp == 4) {
+  if (warp == 8) {
     tc::tc_fence_after();
     tmem_free(tmem, F::COLUMNS);
   }
@@ -658,7 +663,7 @@ cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStre
   cudaError_t e = write_images<DP>(p, src, 2, s);
   if (e != cudaSuccess) return e;
   if ((e = raise_smem_limit<tc_fwd_kernel<DP>>(Fwd<DP>::SMEM)) != cudaSuccess) return e;
-  tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), 160, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
+  tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
   return cudaGetLastError();
 }
 
