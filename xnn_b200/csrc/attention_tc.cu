@@ -68,9 +68,9 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   constexpr int BYTES = Image<DP>::BYTES;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
-  uint64_t *full_k = bars, *full_v = bars + 2, *s_done = bars + 4, *o_done = bars + 5, *p_ready = bars + 6, *pair = bars + 7;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
-  volatile int* dead = reinterpret_cast<volatile int*>(bars + 12);
+  uint64_t *full_k = bars, *full_v = bars + 2, *s_done = bars + 4, *o_done = bars + 5, *p_ready = bars + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7);
+  volatile int* dead = reinterpret_cast<volatile int*>(bars + 8);
   float* tops = reinterpret_cast<float*>(smem + F::TOPS);
   Part part;
   if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
@@ -83,7 +83,6 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(p_ready, 8);
-    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -133,17 +132,17 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
         // the probabilities of tile i are there, so S(i) and P V(i - 1) are done and their images free
         if (!(ok = wait_all(p_ready, i & 1, dead, status))) break;
         tc::tc_fence_after();
-        if (i + 2 < n) { load(full_k + (i & 1), i & 1, ik, i + 2); loaded_k = i + 3; }
-        if (i > 0 && i + 1 < n) { load(full_v + ((i + 1) & 1), 2 + ((i + 1) & 1), iv, i + 1); loaded_v = i + 2; }
         if (!(ok = wait_all(full_v + (i & 1), (i >> 1) & 1, dead, status))) break;
         if (elect()) {
-          mma_sums<DP>(tmem + F::O, tmem + F::S, sv + (i & 1) * BYTES);
+          mma_sums<DP, SLOT, OverScores>(tmem + F::O, tmem + F::S, sv + (i & 1) * BYTES);
           tc::commit_to(o_done);
         }
         if (i + 1 < n) {
           if (!(ok = wait_all(full_k + ((i + 1) & 1), ((i + 1) >> 1) & 1, dead, status))) break;
           scores(i + 1);
         }
+        if (i + 2 < n) { load(full_k + (i & 1), i & 1, ik, i + 2); loaded_k = i + 3; }
+        if (i > 0 && i + 1 < n) { load(full_v + ((i + 1) & 1), 2 + ((i + 1) & 1), iv, i + 1); loaded_v = i + 2; }
       }
       if (!ok) {                                        // copies in flight must land before the block ends
         for (int i = max(0, loaded_k - 2); i < loaded_k; ++i) tc::mbar_wait(full_k + (i & 1), (i >> 1) & 1, SPINS);
@@ -154,13 +153,15 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   } else {
     float f = 1.f;
     const auto add = [&] {                              // P V of the tile before, relative to its maximum
+      const Two ff = two(f, f);
 #pragma unroll
       for (int c = 0; c < DP / 2; c += 16) {
         float o[16];
         tmem_ld16(lanes + F::O + half * (DP / 2) + c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(acc[c + j], f, o[j]);
+        for (int j = 0; j < 16; j += 2)
+          get(fma2(two(acc[c + j], acc[c + j + 1]), ff, two(o[j], o[j + 1])), acc[c + j], acc[c + j + 1]);
       }
     };
     for (int i = 0; i < n; ++i) {
@@ -187,32 +188,32 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
       }
       const float mine = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
       tops[half * 128 + r] = mine;
-      tc::tc_fence_before();
-      arrive(pair + (warp & 3));
-      // the row's other half: its maximum, and it has read its scores before either writes over them
-      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
-      tc::tc_fence_after();
+      pair_sync(warp & 3);                              // the maximum of the row's other half of the keys
       const float mn = fmaxf(m, fmaxf(mine, tops[(half ^ 1) * 128 + r]));
       const float base = mn == neg_inf<float>() ? 0.f : mn;
       f = ex2(m - base);
       m = mn;
-      float u0 = 0.f, u1 = 0.f;
+      const Two down = two(-base, -base);
+      Two u = two(0.f, 0.f);
 #pragma unroll
       for (int c = 0; c < 32; c += 16) {
 #pragma unroll
         for (int j = c; j < c + 16; j += 2) {
-          s[j] = ex2(s[j] - base);
-          s[j + 1] = ex2(s[j + 1] - base);
-          u0 += s[j];
-          u1 += s[j + 1];
+          get(two(s[j], s[j + 1]) + down, s[j], s[j + 1]);
+          s[j] = ex2(s[j]);
+          s[j + 1] = ex2(s[j + 1]);
+          u = u + two(s[j], s[j + 1]);
         }
-        store_parts16(lanes + F::S + 16 * half + c / 2, SLOT / 2, s + c);
+        store_parts16<OverScores>(lanes + F::S, 2 * half + c / 16, s + c);
       }
+      float u0, u1;
+      get(u, u0, u1);
       l = fmaf(l, f, u0 + u1);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(p_ready);
     }
+    if (!ok) pair_leave(warp & 3);
     if (ok && n > 0 && (ok = wait_all(o_done, (n - 1) & 1, dead, status))) {
       tc::tc_fence_after();
       add();
@@ -313,8 +314,8 @@ __device__ __forceinline__ Block set_up(char* smem) {
   Block k;
   k.full = reinterpret_cast<uint64_t*>(smem + STAGES * Bwd<DP>::STAGE);
   k.bars = k.full + STAGES;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(k.bars + 8);
-  k.dead = reinterpret_cast<volatile int*>(k.bars + 9);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(k.bars + 4);
+  k.dead = reinterpret_cast<volatile int*>(k.bars + 5);
   k.warp = threadIdx.x / 32;
   if (k.warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
@@ -323,7 +324,6 @@ __device__ __forceinline__ Block set_up(char* smem) {
     tc::mbar_init(k.bars + 1, 1);
     tc::mbar_init(k.bars + 2, 8);
     tc::mbar_init(k.bars + 3, 8);
-    for (int i = 4; i < 8; ++i) tc::mbar_init(k.bars + i, 2);
     *k.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
         // dq of tile i - 1 is done: its stage is free
         if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
         if (elect()) {
-          mma_sums<DP>(k.tmem + B::Q_OUT, k.tmem + B::Q_DS, base + (i % STAGES) * B::STAGE);
+          mma_sums<DP, SLOT, Linear<SLOT / 2>>(k.tmem + B::Q_OUT, k.tmem + B::Q_DS, base + (i % STAGES) * B::STAGE);
           tc::commit_to(dq_done);
         }
       }
@@ -434,15 +434,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
 #pragma unroll
     for (int d = 0; d < DP / 2; ++d) acc[d] = 0.f;
     bool ok = true;
-    const auto add = [&] {
-#pragma unroll
-      for (int c = 0; c < DP / 2; c += 16) {
-        float o[16];
-        tc::tmem_ld16(lanes + B::Q_OUT + half * (DP / 2) + c, o);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
-      }
-    };
+    const auto add = [&] { add_columns<DP / 2>(lanes + B::Q_OUT + half * (DP / 2), acc); };
     for (int i = 0; i < n; ++i) {
       const uint32_t bits = (uint32_t)(allowed_bits(k_lo + i * SLOT, k_hi, p.mask) >> (32 * half));
       if (!(ok = wait_all(sd_done, i & 1, k.dead, status))) break;
@@ -453,8 +445,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
       tmem_ld_wait();
       tc::tc_fence_before();
       arrive(taken);
+      const Two low = two(-L, -L), down = two(-D, -D);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) s[j] = ex2(s[j] - L) * (dp[j] - D);
+      for (int j = 0; j < 32; j += 2) {
+        get(two(s[j], s[j + 1]) + low, s[j], s[j + 1]);
+        get(two(ex2(s[j]), ex2(s[j + 1])) * (two(dp[j], dp[j + 1]) + down), s[j], s[j + 1]);
+      }
       if (bits != ~0u) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -465,8 +461,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
         tc::tc_fence_after();
         add();
       }
-      store_parts16(lanes + B::Q_DS + 16 * half, SLOT / 2, s);
-      store_parts16(lanes + B::Q_DS + 16 * half + 8, SLOT / 2, s + 16);
+      store_parts16<Linear<SLOT / 2>>(lanes + B::Q_DS, 2 * half, s);
+      store_parts16<Linear<SLOT / 2>>(lanes + B::Q_DS, 2 * half + 1, s + 16);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ds_ready);
@@ -538,7 +534,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
       // a product of tile i and the score product of the next tile (or of none) behind it
       const auto step = [&](uint32_t sum, uint32_t a, uint32_t rows, uint32_t d, uint32_t parts, uint32_t image, bool next, uint64_t* bar) {
         if (elect()) {
-          mma_sums<DP>(sum, a, rows);
+          mma_sums<DP, SLOT, OverScores>(sum, a, rows);
           if (next) mma_scores<DP>(d, parts, image);
           tc::commit_to(bar);
         }
@@ -570,20 +566,11 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
   } else {
     const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
     const int half = k.warp / 4, row = part.row + (threadIdx.x & 127);
-    uint64_t* both = k.bars + 4 + (k.warp & 3);
     // the first half of the warps adds up dV, the second dK
     float acc[DP];
 #pragma unroll
     for (int d = 0; d < DP; ++d) acc[d] = 0.f;
-    const auto add = [&](int column) {
-#pragma unroll
-      for (int c = 0; c < DP; c += 16) {
-        float o[16];
-        tc::tmem_ld16(lanes + column + c, o);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
-      }
-    };
+    const auto add = [&](int column) { add_columns<DP>(lanes + column, acc); };
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const float* st = reinterpret_cast<const float*>(smem + (i % STAGES) * B::STAGE + 2 * BYTES) + 32 * half;
@@ -600,12 +587,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
         const float4 L = *reinterpret_cast<const float4*>(st + j);
         s[j] = ex2(s[j] - L.x); s[j + 1] = ex2(s[j + 1] - L.y); s[j + 2] = ex2(s[j + 2] - L.z); s[j + 3] = ex2(s[j + 3] - L.w);
       }
-      // the other half's warp of these lanes has read its S too before either writes P over it
-      arrive(both);
-      if (!(ok = wait_all(both, 0, k.dead, status))) break;
       if (half == 0 && i > 0) add(B::K_DV);
-      store_parts16(lanes + B::K_S + 16 * half, SLOT / 2, s);
-      store_parts16(lanes + B::K_S + 16 * half + 8, SLOT / 2, s + 16);
+      store_parts16<OverScores>(lanes + B::K_S, 2 * half, s);
+      store_parts16<OverScores>(lanes + B::K_S, 2 * half + 1, s + 16);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(p_ready);
@@ -618,11 +602,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
         const float4 D = *reinterpret_cast<const float4*>(st + SLOT + j);
         s[j] *= dp[j] - D.x; s[j + 1] *= dp[j + 1] - D.y; s[j + 2] *= dp[j + 2] - D.z; s[j + 3] *= dp[j + 3] - D.w;
       }
-      arrive(both);
-      if (!(ok = wait_all(both, 1, k.dead, status))) break;
       if (half == 1 && i > 0) add(B::K_DK);
-      store_parts16(lanes + B::K_DP + 16 * half, SLOT / 2, s);
-      store_parts16(lanes + B::K_DP + 16 * half + 8, SLOT / 2, s + 16);
+      store_parts16<OverScores>(lanes + B::K_DP, 2 * half, s);
+      store_parts16<OverScores>(lanes + B::K_DP, 2 * half + 1, s + 16);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ds_ready);

@@ -35,6 +35,30 @@ __device__ __forceinline__ const char* image(const Images& im, int head, int slo
 // the slot of a part's first rows (parts start at slots as they do at tiles of SLOT rows)
 __device__ __forceinline__ int first_slot(const Part& part) { return part.lo / SLOT + part.index; }
 
+// two float32 in a register pair: one instruction adds, multiplies or fuses both
+struct Two { uint64_t v; };
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void get(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // two numbers as three packed pairs of bf16, the first number in the low half
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -42,12 +66,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  const Two minus = two(-1.f, -1.f);
   p0 = pack_bf16(a, b);
-  a -= __uint_as_float(p0 << 16);
-  b -= __uint_as_float(p0 & 0xffff0000u);
+  Two x = fma2(two(__uint_as_float(p0 << 16), __uint_as_float(p0 & 0xffff0000u)), minus, two(a, b));
+  get(x, a, b);
   p1 = pack_bf16(a, b);
-  a -= __uint_as_float(p1 << 16);
-  b -= __uint_as_float(p1 & 0xffff0000u);
+  x = fma2(two(__uint_as_float(p1 << 16), __uint_as_float(p1 & 0xffff0000u)), minus, x);
+  get(x, a, b);
   p2 = pack_bf16(a, b);
 }
 
@@ -74,43 +99,65 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
       :: "r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(ACCUMULATE) : "memory");
 }
 
-// the six products of parts, smallest first: A's plane `x` at a + x a_plane columns, B's plane at b + y B_PLANE bytes,
-// 16 K elements a step of 8 columns of A and B_STEP bytes of B. With PAIRS = 2 the sum of two such products, part by
-// part: the tensor cores cut what a sum does not hold, so nothing small should come after something large.
-template <int PAIRS, int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO>
-__device__ __forceinline__ void mma_parts(uint32_t d, const uint32_t (&a)[PAIRS], uint32_t a_plane, const uint32_t (&b)[PAIRS],
-                                          uint32_t idesc) {
-  constexpr int X[6] = {2, 0, 1, 1, 0, 0}, Y[6] = {0, 2, 1, 0, 1, 0};
+// Where the parts of a left operand lie in tensor memory: the column of plane x, 16 K elements (8 columns) k.
+template <int PLANE> struct Linear {
+  static __host__ __device__ constexpr uint32_t col(int x, int k) { return x * PLANE + 8 * k; }
+};
+// Over 64 columns of scores and 32 more, each half of the keys (and of the threads of a row) in its own 32 columns and
+// its own 16 of the rest: no thread writes where another one's scores may still be.
+struct OverScores {
+  static __host__ __device__ constexpr uint32_t col(int x, int k) { return (x < 2 ? k / 2 * 32 + x * 16 : 64 + k / 2 * 16) + k % 2 * 8; }
+};
+// the same over regions of 32 columns, a half of the keys a step: plane x at Cx + Sx k
+template <int C0, int C1, int C2, int S0 = 16, int S1 = 16, int S2 = 16> struct OverHalves {
+  static __host__ __device__ constexpr uint32_t col(int x, int k) { return x == 0 ? C0 + S0 * k : x == 1 ? C1 + S1 * k : C2 + S2 * k; }
+};
+
+// one of the six products of parts: A's plane x, B's plane at b + y B_PLANE bytes, B_STEP bytes of B a step
+template <class A, int KSTEPS, int B_PLANE, int B_STEP, int LBO, int SBO>
+__device__ __forceinline__ void mma_part(uint32_t d, uint32_t a, uint32_t b, int x, int y, uint32_t idesc, bool first) {
   constexpr uint32_t hi = (SBO >> 4) | (1u << 14);      // bit 46: descriptor version
+  const uint32_t lo = (b >> 4) | ((LBO >> 4) << 16);
 #pragma unroll
-  for (int i = 0; i < 6; ++i)
-#pragma unroll
-    for (int j = 0; j < PAIRS; ++j) {
-      const uint32_t lo = (b[j] >> 4) | ((LBO >> 4) << 16);
-#pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        const uint32_t at = lo + (Y[i] * B_PLANE + k * B_STEP) / 16;
-        if (i + j + k) mma_ts<1>(d, a[j] + X[i] * a_plane + 8 * k, at, hi, idesc);
-        else mma_ts<0>(d, a[j] + X[i] * a_plane + 8 * k, at, hi, idesc);
-      }
-    }
+  for (int k = 0; k < KSTEPS; ++k) {
+    const uint32_t at = lo + (y * B_PLANE + k * B_STEP) / 16;
+    if (first && k == 0) mma_ts<0>(d, a + A::col(x, k), at, hi, idesc);
+    else mma_ts<1>(d, a + A::col(x, k), at, hi, idesc);
+  }
 }
-// an operand image of ROWS rows as rows x d (scores) and as d x rows (sums over the rows)
+// the six (x, y), smallest product first: (2 0) (0 2) (1 1) (1 0) (0 1) (0 0)
+__host__ __device__ constexpr int part_x(int i) { return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0; }
+__host__ __device__ constexpr int part_y(int i) { return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0; }
+// An operand image of ROWS rows as rows x d (scores) and as d x rows (sums over the rows); the forms with two operands
+// give the sum of two products, part by part: the tensor cores cut what a sum does not hold, so nothing small should
+// come after something large.
 template <int DP, int ROWS = SLOT>
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<1, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, {a}, DP / 2, {b}, idesc_bf16(ROWS, 0));
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+    mma_part<Linear<DP / 2>, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, a, b, part_x(i), part_y(i), idesc_bf16(ROWS, 0), i == 0);
 }
 template <int DP, int ROWS>
 __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {
-  mma_parts<2, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, {a0, a1}, DP / 2, {b0, b1}, idesc_bf16(ROWS, 0));
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    mma_part<Linear<DP / 2>, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, a0, b0, part_x(i), part_y(i), idesc_bf16(ROWS, 0), i == 0);
+    mma_part<Linear<DP / 2>, DP / 16, ROWS * DP * 2, 256, 128, DP * 16>(d, a1, b1, part_x(i), part_y(i), idesc_bf16(ROWS, 0), false);
+  }
 }
-template <int DP, int ROWS = SLOT>
+template <int DP, int ROWS, class A>
 __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b) {
-  mma_parts<1, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, {a}, ROWS / 2, {b}, idesc_bf16(DP, 1));
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+    mma_part<A, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, a, b, part_x(i), part_y(i), idesc_bf16(DP, 1), i == 0);
 }
-template <int DP, int ROWS>
+template <int DP, int ROWS, class A0, class A1>
 __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a0, uint32_t b0, uint32_t a1, uint32_t b1) {
-  mma_parts<2, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, {a0, a1}, ROWS / 2, {b0, b1}, idesc_bf16(DP, 1));
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    mma_part<A0, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, a0, b0, part_x(i), part_y(i), idesc_bf16(DP, 1), i == 0);
+    mma_part<A1, ROWS / 16, ROWS * DP * 2, DP * 32, DP * 16, 128>(d, a1, b1, part_x(i), part_y(i), idesc_bf16(DP, 1), false);
+  }
 }
 
 // the scores with the left operand's parts in shared memory too: 128 rows, planes of 128 DP 2 bytes
@@ -172,14 +219,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// sixteen neighbouring numbers of a row as three planes of eight columns
-__device__ __forceinline__ void store_parts16(uint32_t addr, uint32_t plane, const float* v) {
+// sixteen neighbouring numbers of a row (K elements 16 k ..) as three planes of eight columns in layout A
+template <class A>
+__device__ __forceinline__ void store_parts16(uint32_t addr, int k, const float* v) {
   uint32_t a[8], b[8], c[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) split_pair(v[2 * j], v[2 * j + 1], a[j], b[j], c[j]);
-  tmem_st8(addr, a);
-  tmem_st8(addr + plane, b);
-  tmem_st8(addr + 2 * plane, c);
+  tmem_st8(addr + A::col(0, k), a);
+  tmem_st8(addr + A::col(1, k), b);
+  tmem_st8(addr + A::col(2, k), c);
 }
 
 // N columns from c0 on of a row of D numbers times f (zero where `on` is false) as three planes of DP / 2 columns. The
@@ -207,7 +255,7 @@ __device__ __forceinline__ void stage_row(uint32_t addr, const float* row, bool 
       v[e] = f * x.x; v[e + 1] = f * x.y; v[e + 2] = f * x.z; v[e + 3] = f * x.w;
     }
 #pragma unroll
-    for (int e = 0; e < STEP; e += 16) store_parts16(addr + (c0 + b + e) / 2, DP / 2, v + e);
+    for (int e = 0; e < STEP; e += 16) store_parts16<Linear<DP / 2>>(addr, (c0 + b + e) / 16, v + e);
   }
 }
 
@@ -241,6 +289,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* dead, int* status) {
   return __all_sync(0xffffffffu, wait(bar, parity, dead, status));
 }
+
+// The two warps that share a quarter of the lanes (one half of a row's columns each) meet. No wait of their loops lies
+// between the meeting and the loop's next turn, so a warp that leaves its loop early owes its partner one arrival: the
+// partner then finds the block given up at its next wait.
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" :: "r"(quarter + 1) : "memory"); }
+__device__ __forceinline__ void pair_leave(int quarter) { asm volatile("bar.arrive %0, 64;" :: "r"(quarter + 1) : "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -312,7 +366,7 @@ __device__ __forceinline__ void add_columns(uint32_t addr, float* acc) {
     tmem_ld16(addr + c, o);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[c + j] += o[j];
+    for (int j = 0; j < 16; j += 2) get(two(acc[c + j], acc[c + j + 1]) + two(o[j], o[j + 1]), acc[c + j], acc[c + j + 1]);
   }
 }
 

@@ -22,6 +22,7 @@ template <int DP>
 struct Rows {
   static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = 3 * STAGE, SUMS = BARS + 128, SMEM = SUMS + 2 * 128 * 4;
   static constexpr int P = 3 * DP / 2, S = 3 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W0 = S, W1 = DPO, OUT = E + HALF;
+  using Weights = OverHalves<0, 8, HALF>;               // two planes over S or dP, one over T or E, each half over its own
   static_assert(OUT + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
 };
 
@@ -33,7 +34,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
-  uint64_t *full = bars, *done = bars + 3, *ready = bars + 4, *pair = bars + 5;
+  uint64_t *full = bars, *done = bars + 3, *ready = bars + 4;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 10);
   float* sums = reinterpret_cast<float*>(smem + B::SUMS);
@@ -47,7 +48,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
-    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
         if (elect()) {
           if (sum) {
             const uint32_t at = base + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0), tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
+            mma_sums<DP, HALF, typename B::Weights, typename B::Weights>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0), tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
           }
           if (score) {
             const uint32_t at = base + i % 3 * B::STAGE;
@@ -114,9 +114,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
       for (int i = 0; ok && i < n; ++i) {
         if (!(ok = wait_all(ready, i & 1, dead, status))) break;
         tc::tc_fence_after();
-        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }     // the sums of tile i - 1 are done
         if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
         step(i + 1, true, i + 1 < n);
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }     // the sums of tile i - 1 are done
       }
       if (!ok)
         for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
@@ -140,8 +140,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
       tmem_ld16(lanes + B::DPO + 16 * half, dp);
       tmem_ld16(lanes + B::E + 16 * half, e);
       tmem_ld_wait();
-      tc::tc_fence_before();
-      arrive(pair + (warp & 3));
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const bool in = (bits >> j) & 1;
@@ -157,11 +155,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
         }
       }
       if (i > 0) add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
-      // the other half's warp of these lanes has read its scores before either writes over them
-      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
-      tc::tc_fence_after();
-      store_parts16(lanes + B::W0 + 8 * half, HALF / 2, s);
-      store_parts16(lanes + B::W1 + 8 * half, HALF / 2, t);
+      store_parts16<typename B::Weights>(lanes + B::W0, half, s);
+      store_parts16<typename B::Weights>(lanes + B::W1, half, t);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ready);
@@ -231,9 +226,13 @@ template <int DP>
 struct Keys {
   static constexpr int HB = half_bytes<DP>(), BLOCK = PLANES * 128 * DP * 2, ST = 2 * BLOCK, STAGE = 3 * HB + KINDS * HALF * 4,
                        BARS = ST + 3 * STAGE, SMEM = BARS + 128;
-  static constexpr int P = 3 * DP / 2, S = 2 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W = 3 * HALF / 2, M = S, DS = M + W,
-                       PT = DS + W, K2 = PT + W, V2 = K2 + DP;
-  static_assert(V2 + DP <= 512 && K2 >= E + HALF && SMEM <= 232448, "tensor and shared memory");
+  static constexpr int P = 3 * DP / 2, S = 2 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, REST = E + HALF, K2 = REST + 16,
+                       V2 = K2 + DP;
+  // the parts of M, dS and P (T - r) over the four score regions and 16 columns more, each half over its own columns
+  using M = OverHalves<0, 8, HALF>;
+  using DS = OverHalves<HALF + 8, 2 * HALF, 2 * HALF + 8>;
+  using PT = OverHalves<3 * HALF, 3 * HALF + 8, 4 * HALF, 16, 16, 8>;
+  static_assert(V2 + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
 };
 
 template <int DP>
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
-  uint64_t *full = bars, *full_2 = bars + 3, *done = bars + 4, *ready = bars + 5, *pair = bars + 6;
+  uint64_t *full = bars, *full_2 = bars + 3, *done = bars + 4, *ready = bars + 5;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 10);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 11);
   Part part;
@@ -256,7 +255,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
-    for (int i = 0; i < 4; ++i) tc::mbar_init(pair + i, 2);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -307,8 +305,8 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
         if (elect()) {
           if (sum) {
             const uint32_t at = ring + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF>(tmem + B::K2, tmem + B::M, at, tmem + B::DS, at + 2 * HB);
-            mma_sums<DP, HALF>(tmem + B::V2, tmem + B::PT, at + HB);
+            mma_sums<DP, HALF, typename B::M, typename B::DS>(tmem + B::K2, tmem + B::S, at, tmem + B::S, at + 2 * HB);
+            mma_sums<DP, HALF, typename B::PT>(tmem + B::V2, tmem + B::S, at + HB);
           }
           if (score) {
             const uint32_t at = ring + i % 3 * B::STAGE;
@@ -325,9 +323,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
       for (int i = 0; ok && i < n; ++i) {
         if (!(ok = wait_all(ready, i & 1, dead, status))) break;
         tc::tc_fence_after();
-        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
         if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
         step(i + 1, true, i + 1 < n);
+        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
       }
       if (!ok) {
         tc::mbar_wait(full_2, 0, SPINS);
@@ -351,8 +349,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
       tmem_ld16(lanes + B::DPO + 16 * half, dp);
       tmem_ld16(lanes + B::E + 16 * half, e);
       tmem_ld_wait();
-      tc::tc_fence_before();
-      arrive(pair + (warp & 3));
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float pr = ex2(s[j] - st[j]), x = t[j] * LN2 - st[2 * HALF + j], y = dp[j] - st[HALF + j];
@@ -361,11 +357,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
         dp[j] = pr * x;
       }
       if (i > 0) add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
-      if (!(ok = wait_all(pair + (warp & 3), i & 1, dead, status))) break;
-      tc::tc_fence_after();
-      store_parts16(lanes + B::M + 8 * half, HALF / 2, s);
-      store_parts16(lanes + B::DS + 8 * half, HALF / 2, t);
-      store_parts16(lanes + B::PT + 8 * half, HALF / 2, dp);
+      store_parts16<typename B::M>(lanes + B::S, half, s);
+      store_parts16<typename B::DS>(lanes + B::S, half, t);
+      store_parts16<typename B::PT>(lanes + B::S, half, dp);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ready);

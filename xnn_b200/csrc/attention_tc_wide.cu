@@ -119,10 +119,10 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
         }
         if (!(ok = wait_all(ready, i & 1, dead, status))) break;
         tc::tc_fence_after();
-        if (i > 0 && i + 2 < n) { load(i + 2, true); loaded_y = i + 3; }
+        if (i > 0 && i + 2 < n) { load(i + 2, true); loaded_y = i + 3; }      // the sums of tile i - 1 are done
         if (!(ok = wait_all(full_y + i % 3, (i / 3) & 1, dead, status))) break;
         if (elect()) {
-          mma_sums<DP, HALF>(tmem + B::OUT, tmem + B::W, base + B::Y + i % 3 * B::HB);
+          mma_sums<DP, HALF, Linear<HALF / 2>>(tmem + B::OUT, tmem + B::W, base + B::Y + i % 3 * B::HB);
           tc::commit_to(summed);
         }
       }
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
         tc::tc_fence_after();
         add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
       }
-      store_parts16(lanes + B::W + 8 * half, HALF / 2, s);
+      store_parts16<Linear<HALF / 2>>(lanes + B::W, half, s);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ready);
