@@ -31,6 +31,8 @@ from ..data import AtomicGraph
 from ..nn import PolynomialCutoff
 from ..nn.radial import GaussianRBF
 from ..o3 import FromS2Grid, ToS2Grid, spherical_harmonics, wigner_3j
+from ..ops.dropout import CounterDropout
+from ..ops.embedding import ScaledEmbedding
 from ..ops.scatter import scatter_sum, segment_softmax
 from .equiformer import GraphDropPath, RadialMLP, SmoothLeakyReLU
 from .et import TransformerPotential
@@ -364,14 +366,16 @@ def make_norm(kind: str, lmax: int, channels: int) -> nn.Module:
 
 
 class EdgeScalars(nn.Module):
-    """Radial features, optionally with source and target element embeddings appended."""
+    """Radial features, optionally with source and target element embeddings appended
+    (``sorted_lookup``: their gradients summed over the edges sorted by element, in a fixed order)."""
 
-    def __init__(self, n_elements: int, channels: int, use_elements: bool):
+    def __init__(self, n_elements: int, channels: int, use_elements: bool, sorted_lookup: bool = False):
         super().__init__()
         self.source_embedding = self.target_embedding = None
         if use_elements:
-            self.source_embedding = nn.Embedding(n_elements, channels)
-            self.target_embedding = nn.Embedding(n_elements, channels)
+            table = ScaledEmbedding if sorted_lookup else nn.Embedding
+            self.source_embedding = table(n_elements, channels)
+            self.target_embedding = table(n_elements, channels)
             nn.init.uniform_(self.source_embedding.weight, -0.001, 0.001)
             nn.init.uniform_(self.target_embedding.weight, -0.001, 0.001)
 
@@ -389,13 +393,14 @@ class SO2GraphAttention(nn.Module):
     def __init__(self, channels: int, hidden_channels: int, num_heads: int, alpha_channels: int, value_channels: int,
                  out_channels: int, lmax: int, mmax: int, radial: List[int], n_elements: int,
                  use_atom_edge_embedding: bool, use_m_share_rad: bool, activation: str, use_attn_renorm: bool,
-                 resolution: Optional[int], alpha_drop: float = 0.0):
+                 resolution: Optional[int], alpha_drop: float = 0.0, dropout_rng: str = "torch",
+                 sorted_lookup: bool = False):
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
         self.num_heads, self.alpha_channels, self.lmax = int(num_heads), int(alpha_channels), int(lmax)
         radial = list(radial)
-        self.edge_scalars = EdgeScalars(n_elements, radial[-1], use_atom_edge_embedding)
+        self.edge_scalars = EdgeScalars(n_elements, radial[-1], use_atom_edge_embedding, sorted_lookup)
         if use_atom_edge_embedding:
             radial[0] += 2 * radial[-1]
         extra = num_heads * alpha_channels + {"gate": lmax * hidden_channels, "sep_s2": hidden_channels}.get(activation, 0)
@@ -412,7 +417,9 @@ class SO2GraphAttention(nn.Module):
         self.alpha_act = SmoothLeakyReLU(0.2)
         bound = 1.0 / math.sqrt(alpha_channels)
         self.alpha_dot = nn.Parameter(torch.empty(num_heads, alpha_channels).uniform_(-bound, bound))
-        self.alpha_dropout = nn.Dropout(alpha_drop) if alpha_drop > 0 else nn.Identity()
+        self.alpha_dropout = nn.Identity()
+        if alpha_drop > 0:
+            self.alpha_dropout = CounterDropout(alpha_drop) if dropout_rng == "counter" else nn.Dropout(alpha_drop)
         self.gate_act = self.s2_act = self.grid = None
         if activation == "gate":
             self.gate_act = GateActivation(lmax, mmax, hidden_channels)
@@ -490,15 +497,19 @@ class FeedForwardNetwork(nn.Module):
 
 
 class EquivariantDropout(nn.Module):
-    """One dropout mask per node and channel, shared by all coefficients."""
+    """One dropout mask per node and channel, shared by all coefficients. ``rng="counter"`` draws it from a counter
+    (:class:`~xnn_b200.ops.CounterDropout`: one pass each way, no mask in memory)."""
 
-    def __init__(self, p: float):
+    def __init__(self, p: float, rng: str = "torch"):
         super().__init__()
         self.p = float(p)
+        self.counter = CounterDropout(self.p, shared=(1,)) if rng == "counter" and self.p > 0 else None
 
     def forward(self, x: Tensor) -> Tensor:
         if not self.training or self.p == 0.0:
             return x
+        if self.counter is not None:
+            return self.counter(x)
         return x * F.dropout(x.new_ones((x.shape[0], 1, x.shape[2])), self.p, True)
 
 
@@ -507,14 +518,15 @@ class TransformerBlockV2(nn.Module):
                  attn_value_channels: int, ffn_hidden_channels: int, lmax: int, mmax: int, radial: List[int],
                  n_elements: int, use_atom_edge_embedding: bool, use_m_share_rad: bool, activation: str,
                  use_attn_renorm: bool, use_grid_mlp: bool, norm_type: str, resolution: Optional[int],
-                 alpha_drop: float, drop_path_rate: float, proj_drop: float):
+                 alpha_drop: float, drop_path_rate: float, proj_drop: float, dropout_rng: str = "torch",
+                 sorted_lookup: bool = False):
         super().__init__()
         self.norm_1 = make_norm(norm_type, lmax, channels)
         self.ga = SO2GraphAttention(channels, attn_hidden_channels, num_heads, attn_alpha_channels, attn_value_channels,
                                     channels, lmax, mmax, radial, n_elements, use_atom_edge_embedding, use_m_share_rad,
-                                    activation, use_attn_renorm, resolution, alpha_drop)
+                                    activation, use_attn_renorm, resolution, alpha_drop, dropout_rng, sorted_lookup)
         self.drop_path = GraphDropPath(drop_path_rate)
-        self.proj_drop = EquivariantDropout(proj_drop)
+        self.proj_drop = EquivariantDropout(proj_drop, dropout_rng)
         self.norm_2 = make_norm(norm_type, lmax, channels)
         self.ffn = FeedForwardNetwork(channels, ffn_hidden_channels, channels, lmax, activation, use_grid_mlp,
                                       resolution)
@@ -530,11 +542,11 @@ class EdgeDegreeEmbedding(nn.Module):
     of its frame's Wigner matrices (the frame rotated back), summed per receiver."""
 
     def __init__(self, channels: int, lmax: int, mmax: int, radial: List[int], n_elements: int,
-                 use_atom_edge_embedding: bool, avg_degree: float):
+                 use_atom_edge_embedding: bool, avg_degree: float, sorted_lookup: bool = False):
         super().__init__()
         self.lmax, self.channels = int(lmax), int(channels)
         radial = list(radial)
-        self.edge_scalars = EdgeScalars(n_elements, radial[-1], use_atom_edge_embedding)
+        self.edge_scalars = EdgeScalars(n_elements, radial[-1], use_atom_edge_embedding, sorted_lookup)
         if use_atom_edge_embedding:
             radial[0] += 2 * radial[-1]
         self.rad_func = RadialMLP(radial + [(lmax + 1) * channels])
@@ -573,7 +585,9 @@ def _init_weights(module: nn.Module, weight_init: str) -> None:
 @register_model("equiformer_v2")
 class EquiformerV2(TransformerPotential):
     """EquiformerV2 energy model (``direct_forces``: an extra attention block predicts forces from
-    its ``l = 1`` output; the energy is then not their potential)."""
+    its ``l = 1`` output; the energy is then not their potential). ``dropout_rng="counter"`` draws the attention and
+    projection dropout from a counter instead of PyTorch's generator; ``sorted_lookup`` sums the gradients of the
+    edges' element tables in sorted order (the same parameters and outputs, gradients to rounding)."""
     head_modules = ("energy_block", "energy_scale", "energy_shift", "atom_ref")
 
     def __init__(self, n_features: int = 96, n_interactions: int = 6, cutoff: float = 5.0, n_rbf: int = 128,
@@ -586,8 +600,10 @@ class EquiformerV2(TransformerPotential):
                  proj_drop: float = 0.0, avg_degree: float = AVG_DEGREE, avg_num_nodes: float = AVG_NUM_NODES,
                  direct_forces: bool = False, smooth_cutoff: bool = False, weight_init: str = "normal",
                  n_elements: int = 100, energy_shift: float = 0.0, energy_scale: float = 1.0, species=None,
-                 atomic_energies=None):
+                 atomic_energies=None, dropout_rng: str = "torch", sorted_lookup: bool = False):
         super().__init__()
+        if dropout_rng not in ("torch", "counter"):
+            raise ValueError(f"dropout_rng must be 'torch' or 'counter', got {dropout_rng!r}")
         if not 0 <= m_max <= l_max:
             raise ValueError(f"need 0 <= m_max <= l_max, got m_max={m_max}, l_max={l_max}")
         if norm_type not in NORMS:
@@ -605,7 +621,7 @@ class EquiformerV2(TransformerPotential):
         self.distance_expansion = GaussianRBF(n_rbf, cutoff, gamma=0.5 / (2.0 * spacing) ** 2)
         self.envelope = PolynomialCutoff(cutoff, p=6)
         radial = [n_rbf, edge_channels, edge_channels]
-        self.shared_edge_scalars = EdgeScalars(n_elements, edge_channels, share_atom_edge_embedding)
+        self.shared_edge_scalars = EdgeScalars(n_elements, edge_channels, share_atom_edge_embedding, sorted_lookup)
         per_block = use_atom_edge_embedding and not share_atom_edge_embedding
         if share_atom_edge_embedding:
             radial[0] += 2 * edge_channels
@@ -613,11 +629,11 @@ class EquiformerV2(TransformerPotential):
         self.frames = EdgeFrames(l_max)
         self.rotations = Rotations(l_max, m_max)
         self.edge_degree_embedding = EdgeDegreeEmbedding(n_features, l_max, m_max, radial, n_elements, per_block,
-                                                         avg_degree)
+                                                         avg_degree, sorted_lookup)
         self.blocks = nn.ModuleList(TransformerBlockV2(
             n_features, attn_hidden_channels, num_heads, attn_alpha_channels, attn_value_channels, ffn_hidden_channels,
             l_max, m_max, radial, n_elements, per_block, use_m_share_rad, activation, use_attn_renorm, use_grid_mlp,
-            norm_type, grid_resolution, alpha_drop, drop_path_rate, proj_drop) for _ in range(n_interactions))
+            norm_type, grid_resolution, alpha_drop, drop_path_rate, proj_drop, dropout_rng, sorted_lookup) for _ in range(n_interactions))
         self.norm = make_norm(norm_type, l_max, n_features)
         self.energy_block = FeedForwardNetwork(n_features, ffn_hidden_channels, 1, l_max, activation, use_grid_mlp,
                                                grid_resolution)
@@ -625,7 +641,8 @@ class EquiformerV2(TransformerPotential):
         if self.direct_forces:
             self.force_block = SO2GraphAttention(
                 n_features, attn_hidden_channels, num_heads, attn_alpha_channels, attn_value_channels, 1, l_max, m_max,
-                radial, n_elements, per_block, use_m_share_rad, activation, use_attn_renorm, grid_resolution, 0.0)
+                radial, n_elements, per_block, use_m_share_rad, activation, use_attn_renorm, grid_resolution, 0.0,
+                sorted_lookup=sorted_lookup)
         _init_weights(self, weight_init)
         self._init_energy_terms(n_elements, energy_scale, energy_shift, species, atomic_energies)
 
@@ -692,7 +709,7 @@ class EquiformerV2(TransformerPotential):
                           ("use_m_share_rad", bool), ("alpha_drop", float), ("drop_path_rate", float),
                           ("proj_drop", float), ("avg_degree", float), ("avg_num_nodes", float), ("direct_forces", bool),
                           ("smooth_cutoff", bool), ("weight_init", str), ("n_elements", int), ("energy_shift", float),
-                          ("energy_scale", float)):
+                          ("energy_scale", float), ("dropout_rng", str), ("sorted_lookup", bool)):
             if e.get(key) is not None:
                 kw[key] = kind(e[key])
         if "grid_resolution" in e:

@@ -25,6 +25,7 @@ from torch import Tensor, nn
 
 from ..data import AtomicGraph
 from ..nn.radial import ExponentialBernsteinRBF
+from ..ops.attention import structure_attention
 from ..ops.scatter import gather_rows, scatter_sum
 from .base import InteratomicPotential
 from .d4 import K4, K5, K6, KCN, CP_WEIGHTS
@@ -276,13 +277,35 @@ def structure_slots(batch: Tensor, num_graphs: int) -> Tuple[Tensor, int]:
     return slot, int(counts.max()) if counts.numel() else 0
 
 
+class PackedAtoms:
+    """The atoms ordered by structure: first row of each structure, the order (``None`` where the batch is
+    in it already), every atom's place in it, the largest structure."""
+
+    def __init__(self, batch: Tensor, num_graphs: int, slot: Tensor, n_max: int):
+        counts = torch.bincount(batch, minlength=num_graphs)
+        self.ptr = torch.cat([counts.new_zeros(1), torch.cumsum(counts, 0)])
+        self.n_max, self.order, self.place = int(n_max), None, None
+        if num_graphs > 1 and bool((batch[1:] < batch[:-1]).any()):
+            self.order = torch.argsort(batch, stable=True)
+            self.place = self.ptr[batch] + slot
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        if self.order is None:
+            return structure_attention(q, k, v, self.ptr, max_len=self.n_max)
+        o = structure_attention(*(t.index_select(0, self.order) for t in (q, k, v)), self.ptr, max_len=self.n_max)
+        return o.index_select(0, self.place)
+
+
 class NonlocalInteraction(nn.Module):
     """Self-attention over the atoms of each structure: FAVOR+ positive random features (``omega``
-    drawn once) or exact softmax (``n_random_features=None``)."""
+    drawn once), exact softmax with one maximum a structure and a damped denominator
+    (``n_random_features=None``), or, with ``heads``, the plain row softmax over that many heads
+    (:func:`~xnn_b200.ops.structure_attention`, which stores no pair of atoms)."""
 
     def __init__(self, n_features: int, n_residual: int, n_random_features: Optional[int],
-                 generator: Optional[torch.Generator] = None):
+                 generator: Optional[torch.Generator] = None, heads: int = 0):
         super().__init__()
+        self.heads = int(heads)
         self.resmlp_q = ResidualMLP(n_features, n_residual, zero_init=True)
         self.resmlp_k = ResidualMLP(n_features, n_residual, zero_init=True)
         self.resmlp_v = ResidualMLP(n_features, n_residual, zero_init=True)
@@ -295,8 +318,12 @@ class NonlocalInteraction(nn.Module):
         h = (x * x).sum(-1, keepdim=True) / (2.0 * math.sqrt(x.shape[-1]))
         return (torch.exp(u - h - shift) + 1e-4) / math.sqrt(self.omega.shape[-1])
 
-    def forward(self, x: Tensor, batch: Tensor, num_graphs: int, slot: Tensor, n_max: int) -> Tensor:
+    def forward(self, x: Tensor, batch: Tensor, num_graphs: int, slot: Tensor, n_max: int,
+                packed: Optional[PackedAtoms] = None) -> Tensor:
         q, k, v = residual_mlps(x, [self.resmlp_q, self.resmlp_k, self.resmlp_v])
+        if self.heads:
+            packed = packed or PackedAtoms(batch, num_graphs, slot, n_max)
+            return packed.attend(*(t.unflatten(-1, (self.heads, -1)) for t in (q, k, v))).flatten(1)
         flat = batch * n_max + slot
         if self.exact:
             return self._exact(q, k, v, flat, num_graphs, n_max)
@@ -327,21 +354,21 @@ class InteractionModule(nn.Module):
     """``x~ = residual(x)``, ``x' = residual(x~ + l + n)``, ``y = resmlp(x')``."""
 
     def __init__(self, n_features: int, n_rbf: int, n_residual: int, nonlocal_: bool,
-                 n_random_features: Optional[int], generator: Optional[torch.Generator]):
+                 n_random_features: Optional[int], generator: Optional[torch.Generator], heads: int = 0):
         super().__init__()
         self.residual_pre = nn.ModuleList(ResidualBlock(n_features) for _ in range(n_residual))
         self.local_interaction = LocalInteraction(n_features, n_rbf, n_residual)
-        self.nonlocal_interaction = (NonlocalInteraction(n_features, n_residual, n_random_features, generator)
+        self.nonlocal_interaction = (NonlocalInteraction(n_features, n_residual, n_random_features, generator, heads)
                                      if nonlocal_ else None)
         self.residual_post = nn.ModuleList(ResidualBlock(n_features) for _ in range(n_residual))
         self.resmlp_y = ResidualMLP(n_features, n_residual)
 
-    def forward(self, x, rho, y1, y2, src, dst, batch, num_graphs, slot, n_max, use_p, use_d, use_nonlocal):
+    def forward(self, x, rho, y1, y2, src, dst, batch, num_graphs, slot, n_max, use_p, use_d, use_nonlocal, packed=None):
         for block in self.residual_pre:
             x = block(x)
         h = x + self.local_interaction(x, rho, y1, y2, src, dst, use_p, use_d)
         if self.nonlocal_interaction is not None and use_nonlocal:
-            h = h + self.nonlocal_interaction(x, batch, num_graphs, slot, n_max)
+            h = h + self.nonlocal_interaction(x, batch, num_graphs, slot, n_max, packed)
         for block in self.residual_post:
             h = block(h)
         return h, self.resmlp_y(h)
@@ -488,6 +515,8 @@ class SpookyNet(InteratomicPotential):
     absent) and ``spin_multiplicity`` (singlet when absent). ``lr_cutoff`` truncates the
     electrostatics and dispersion (needed for periodic structures; otherwise they run over all
     pairs of each structure); ``ewald=True`` Ewald-sums the periodic structures' Coulomb part.
+    ``attention="softmax"`` attends with the plain softmax in ``attention_heads`` heads of up to 128
+    features, on CUDA without the pairs of atoms that ``"exact"`` holds in memory.
     """
 
     head_modules = ("output", "atom_ref", "charge_ref")
@@ -497,10 +526,15 @@ class SpookyNet(InteratomicPotential):
                  spin_embedding: bool = True, nonlocal_interactions: bool = True, attention: str = "favor",
                  n_random_features: Optional[int] = None, zbl_repulsion: bool = True, electrostatics: bool = True,
                  d4_dispersion: bool = True, exp_weighting: bool = False, ewald: bool = False,
-                 ewald_accuracy: float = 1.0e-6, seed: Optional[int] = None, species=None, atomic_energies=None):
+                 ewald_accuracy: float = 1.0e-6, seed: Optional[int] = None, species=None, atomic_energies=None,
+                 attention_heads: int = 1):
         super().__init__()
-        if attention not in ("favor", "exact"):
-            raise ValueError(f"attention must be 'favor' or 'exact', got {attention!r}")
+        if attention not in ("favor", "exact", "softmax"):
+            raise ValueError(f"attention must be 'favor', 'exact' or 'softmax', got {attention!r}")
+        heads = int(attention_heads)
+        if heads < 1 or n_features % heads or (heads != 1 and attention != "softmax"):
+            raise ValueError(f"attention_heads={heads} of {n_features} features with attention={attention!r}")
+        self.attention_heads = heads if attention == "softmax" else 0
         if ewald and lr_cutoff is None:
             raise ValueError("ewald=True needs lr_cutoff (the real-space cutoff)")
         self.local_cutoff = float(cutoff)
@@ -513,13 +547,13 @@ class SpookyNet(InteratomicPotential):
         self.ewald_alpha, self.ewald_k_cutoff = (ewald_parameters(self.lr_cutoff, float(ewald_accuracy))
                                                  if self.ewald else (0.0, 0.0))
         gen = torch.Generator().manual_seed(int(seed)) if seed is not None else None
-        m = None if attention == "exact" else int(n_random_features or n_features)
+        m = int(n_random_features or n_features) if attention == "favor" else None
         self.nuclear_embedding = NuclearEmbedding(n_features)
         self.charge_embedding = ElectronicEmbedding(n_features, n_residual, True) if charge_embedding else None
         self.spin_embedding = ElectronicEmbedding(n_features, n_residual, False) if spin_embedding else None
         self.radial_basis = ExponentialBernsteinRBF(n_rbf, exp_weighting=exp_weighting)
         self.interactions = nn.ModuleList(
-            InteractionModule(n_features, n_rbf, n_residual, nonlocal_interactions, m, gen)
+            InteractionModule(n_features, n_rbf, n_residual, nonlocal_interactions, m, gen, self.attention_heads)
             for _ in range(n_interactions))
         self.output = nn.Linear(n_features, 2, bias=False)
         glorot_orthogonal_(self.output.weight)
@@ -584,10 +618,11 @@ class SpookyNet(InteratomicPotential):
             slot, n_max = structure_slots(batch, num_graphs)
         else:
             slot, n_max = torch.arange(n, device=z.device), n
+        packed = PackedAtoms(batch, num_graphs, slot, n_max) if self.attention_heads and self.use_nonlocal else None
         f = torch.zeros_like(x)
         for module in self.interactions:
             x, y = module(x, rho, y1, y2, src, dst, batch, num_graphs, slot, n_max,
-                          self.use_p_orbitals, self.use_d_orbitals, self.use_nonlocal)
+                          self.use_p_orbitals, self.use_d_orbitals, self.use_nonlocal, packed)
             f = f + y
         out = self.output(f)
         e_nn = out[:, 0] + self.atom_ref(z).squeeze(-1)
@@ -655,7 +690,7 @@ class SpookyNet(InteratomicPotential):
         e = dict(cfg.extra or {})
         keys = ("lr_cutoff", "n_residual", "charge_embedding", "spin_embedding", "nonlocal_interactions", "attention",
                 "n_random_features", "zbl_repulsion", "electrostatics", "d4_dispersion", "exp_weighting", "ewald",
-                "ewald_accuracy", "seed", "species", "atomic_energies")
+                "ewald_accuracy", "seed", "species", "atomic_energies", "attention_heads")
         return cls(n_features=cfg.n_features, n_interactions=cfg.n_interactions, n_rbf=cfg.n_rbf, cutoff=cfg.cutoff,
                    **{k: e[k] for k in keys if k in e})
 
