@@ -140,14 +140,17 @@ __global__ void __launch_bounds__(128) join_kernel(const Params<T> p) {
   if (lane == 0 && p.lse) p.lse[at] = none ? -neg_inf<T>() : m + lg2(l);
 }
 
-// out[i] = sum of the splits' partial results in their order
+// out[i] = sum of the splits' partial results in their order, for one result or two whose splits follow each other
 template <typename T>
-__global__ void __launch_bounds__(256) sum_kernel(int64_t n, int splits, const T* __restrict__ work, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) sum_kernel(int64_t n, int splits, const T* __restrict__ work, T* __restrict__ out0,
+                                                  T* __restrict__ out1) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
+  work += blockIdx.y * splits * n;
   T a = T(0);
+#pragma unroll 4
   for (int z = 0; z < splits; ++z) a += work[z * n + i];
-  out[i] = a;
+  (blockIdx.y ? out1 : out0)[i] = a;
 }
 
 // ------------------------------------------------------------------------------------------ backward
@@ -603,8 +606,8 @@ cudaError_t forward_join(const Params<T>& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out, cudaStream_t s) {
-  sum_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(n, splits, work, out);
+cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out0, T* out1, cudaStream_t s) {
+  sum_kernel<T><<<dim3((unsigned)((n + 255) / 256), out1 ? 2 : 1), 256, 0, s>>>(n, splits, work, out0, out1);
   return cudaGetLastError();
 }
 template <typename T>
@@ -635,7 +638,7 @@ cudaError_t second_keys(const Params<T>& p, cudaStream_t s) {
 #define XNN_ATTN_INST(T)                                                                  \
   template cudaError_t forward<T>(const Params<T>&, cudaStream_t);                        \
   template cudaError_t forward_join<T>(const Params<T>&, cudaStream_t);                   \
-  template cudaError_t sum_splits<T>(int64_t, int, const T*, T*, cudaStream_t);           \
+  template cudaError_t sum_splits<T>(int64_t, int, const T*, T*, T*, cudaStream_t);       \
   template cudaError_t row_delta<T>(const Params<T>&, cudaStream_t);                      \
   template cudaError_t backward_short<T>(const Params<T>&, cudaStream_t);                 \
   template cudaError_t second_rows<T>(const Params<T>&, cudaStream_t);                    \

@@ -9,7 +9,7 @@ template <typename T> struct Params;
 
 template <typename T> cudaError_t forward(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t forward_join(const Params<T>&, cudaStream_t);
-template <typename T> cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out, cudaStream_t);
+template <typename T> cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out0, T* out1, cudaStream_t);
 template <typename T> cudaError_t row_delta(const Params<T>&, cudaStream_t);
 cudaError_t backward_dq(const Params<double>&, cudaStream_t);
 cudaError_t backward_dkv(const Params<double>&, cudaStream_t);

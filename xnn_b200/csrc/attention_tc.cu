@@ -13,14 +13,52 @@
 namespace attn {
 namespace {
 
-// writes the images of up to seven tensors: a block per (slot, head, tensor); zeros behind the structure's last
-// row, behind column D and where the mask is 0
+// L and D of the rows of a slot, D = do.o: `kinds` x 64 numbers a (head, slot), L = +inf behind the last row, so that P is
+// zero there. A warp takes eight rows at once, their loads overlap.
+__device__ __forceinline__ void slot_stats(const Params<float>& p, const Part& part, int h, float* at) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const bool vec = vec_ok(p.go, p.gos, p.goh, p.D) && vec_ok(p.o, p.os, p.oh, p.D);
+  float s[SLOT / 8], L[SLOT / 8];
+#pragma unroll
+  for (int i = 0; i < SLOT / 8; ++i) {
+    const int row = part.row + warp + 8 * i;
+    s[i] = 0.f;
+    L[i] = row < part.hi ? p.lse[(int64_t)h * p.N + row] : -neg_inf<float>();
+    if (row >= part.hi) continue;
+    const float *a = p.go + row * p.gos + h * p.goh, *b = p.o + row * p.os + h * p.oh;
+    if (vec) {
+      if (4 * lane < p.D) {
+        const float4 x = *reinterpret_cast<const float4*>(a + 4 * lane), y = *reinterpret_cast<const float4*>(b + 4 * lane);
+        s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, x.w * y.w)));
+      }
+    } else {
+      for (int d = lane; d < p.D; d += 32) s[i] = fmaf(a[d], b[d], s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < SLOT / 8; ++i) {
+    const float v = row_sum<32>(s[i]);
+    if (lane == 0) {
+      at[warp + 8 * i] = L[i];
+      at[SLOT + warp + 8 * i] = v;
+    }
+  }
+}
+
+// The images of up to seven tensors, and the rows' statistics where they are asked for: a block per (slot, head, tensor).
+// Zeros behind the structure's last row, behind column D and where the mask is 0.
 template <int DP>
-__global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const Sources src, int slots) {
-  const Source s = src.s[blockIdx.z];
-  if ((int)blockIdx.y >= s.heads) return;
+__global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const Sources src, int count, int slots, float* stats,
+                                                    int kinds) {
+  const bool rows = (int)blockIdx.z == count;
+  const Source s = src.s[rows ? 0 : blockIdx.z];
+  if (!rows && (int)blockIdx.y >= s.heads) return;
   Part part;
   if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
+  if (rows) {
+    slot_stats(p, part, blockIdx.y, stats + ((int64_t)blockIdx.y * slots + blockIdx.x) * kinds * SLOT);
+    return;
+  }
   const float* g = s.at + blockIdx.y * s.head;
   const bool vec = vec_ok(s.at, s.row, s.head, p.D);
   uint4* out = reinterpret_cast<uint4*>(s.out + ((int64_t)blockIdx.y * slots + blockIdx.x) * Image<DP>::BYTES);
@@ -250,41 +288,6 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
 }
 
 // ------------------------------------------------------------------------------------------ backward
-// L and D of the rows of a slot, D = do.o: 64 + 64 numbers a (head, slot), L = +inf behind the last row, so that P is zero there
-__global__ void __launch_bounds__(256) stats_kernel(const Params<float> p, float* __restrict__ out, int slots, int kinds) {
-  Part part;
-  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
-  const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  float* at = out + ((int64_t)h * slots + blockIdx.x) * kinds * SLOT;
-  // a warp's eight rows at once: their loads overlap
-  const bool vec = vec_ok(p.go, p.gos, p.goh, p.D) && vec_ok(p.o, p.os, p.oh, p.D);
-  float s[SLOT / 8], L[SLOT / 8];
-#pragma unroll
-  for (int i = 0; i < SLOT / 8; ++i) {
-    const int row = part.row + warp + 8 * i;
-    s[i] = 0.f;
-    L[i] = row < part.hi ? p.lse[(int64_t)h * p.N + row] : -neg_inf<float>();
-    if (row >= part.hi) continue;
-    const float *a = p.go + row * p.gos + h * p.goh, *b = p.o + row * p.os + h * p.oh;
-    if (vec) {
-      if (4 * lane < p.D) {
-        const float4 x = *reinterpret_cast<const float4*>(a + 4 * lane), y = *reinterpret_cast<const float4*>(b + 4 * lane);
-        s[i] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, x.w * y.w)));
-      }
-    } else {
-      for (int d = lane; d < p.D; d += 32) s[i] = fmaf(a[d], b[d], s[i]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < SLOT / 8; ++i) {
-    const float v = row_sum<32>(s[i]);
-    if (lane == 0) {
-      at[warp + 8 * i] = L[i];
-      at[SLOT + warp + 8 * i] = v;
-    }
-  }
-}
-
 // Eight warps of rows: warp w reaches the lanes 32 (w % 4) .. of tensor memory and takes half w / 4 of the columns;
 // a ninth copies and issues. A ring of three stages holds the streamed images.
 constexpr int BWD_THREADS = 288, STAGES = 3;
@@ -642,7 +645,7 @@ cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStre
   Sources src{};
   src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, ik};
   src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
-  cudaError_t e = write_images<DP>(p, src, 2, s);
+  cudaError_t e = write_images<DP>(p, src, 2, nullptr, 0, s);
   if (e != cudaSuccess) return e;
   if ((e = raise_smem_limit<tc_fwd_kernel<DP>>(Fwd<DP>::SMEM)) != cudaSuccess) return e;
   tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
@@ -658,8 +661,7 @@ cudaError_t prepare_dp(const Params<float>& p, char* work, cudaStream_t s) {
   src.s[1] = {p.v, p.vs, p.vh, p.HK, p.mask, iv};
   src.s[2] = {p.q, p.qs, p.qh, p.H, nullptr, iq};
   src.s[3] = {p.go, p.gos, p.goh, p.H, nullptr, io};
-  const cudaError_t e = write_images<DP>(p, src, 4, s);
-  return e != cudaSuccess ? e : write_stats(p, stats, 2, s);
+  return write_images<DP>(p, src, 4, stats, 2, s);
 }
 
 template <int DP>
@@ -687,18 +689,14 @@ cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t
 }  // namespace
 
 template <int DP>
-cudaError_t write_images(const Params<float>& p, const Sources& src, int count, cudaStream_t s) {
-  image_kernel<DP><<<dim3(p.N / SLOT + p.num + 2, p.H, count), 256, 0, s>>>(p, src, image_slots(p));
+cudaError_t write_images(const Params<float>& p, const Sources& src, int count, float* stats, int kinds, cudaStream_t s) {
+  const dim3 grid(p.N / SLOT + p.num + 2, p.H, count + (stats != nullptr));
+  image_kernel<DP><<<grid, 256, 0, s>>>(p, src, count, image_slots(p), stats, kinds);
   return cudaGetLastError();
 }
-template cudaError_t write_images<32>(const Params<float>&, const Sources&, int, cudaStream_t);
-template cudaError_t write_images<64>(const Params<float>&, const Sources&, int, cudaStream_t);
-template cudaError_t write_images<128>(const Params<float>&, const Sources&, int, cudaStream_t);
-
-cudaError_t write_stats(const Params<float>& p, float* out, int kinds, cudaStream_t s) {
-  stats_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H), 256, 0, s>>>(p, out, image_slots(p), kinds);
-  return cudaGetLastError();
-}
+template cudaError_t write_images<32>(const Params<float>&, const Sources&, int, float*, int, cudaStream_t);
+template cudaError_t write_images<64>(const Params<float>&, const Sources&, int, float*, int, cudaStream_t);
+template cudaError_t write_images<128>(const Params<float>&, const Sources&, int, float*, int, cudaStream_t);
 
 int64_t tc_forward_bytes(const Params<float>& p) {
   return 2 * (p.D <= 32 ? image_bytes<32>(p, p.HK) : p.D <= 64 ? image_bytes<64>(p, p.HK) : image_bytes<128>(p, p.HK));

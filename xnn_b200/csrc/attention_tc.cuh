@@ -377,8 +377,9 @@ struct Sources { Source s[MAX_SOURCES]; };
 
 inline int image_slots(const Params<float>& p) { return p.N / SLOT + p.num + 3; }   // the last: read behind the end by load_block
 template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { return (int64_t)heads * image_slots(p) * Image<DP>::BYTES; }
-template <int DP> cudaError_t write_images(const Params<float>& p, const Sources& src, int count, cudaStream_t s);
-// L, D (and room for two more) of the rows of each slot: `kinds` x SLOT numbers a (head, slot)
-cudaError_t write_stats(const Params<float>& p, float* out, int kinds, cudaStream_t s);
+// the images of `count` tensors and, with `stats`, L and D (and room for more) of the rows of each slot: `kinds` x SLOT
+// numbers a (head, slot)
+template <int DP>
+cudaError_t write_images(const Params<float>& p, const Sources& src, int count, float* stats, int kinds, cudaStream_t s);
 
 }  // namespace attn

@@ -18,9 +18,12 @@ constexpr int KINDS = 4;                                // L, D, r, c of a slot'
 
 struct Streams { Images a, b, c, d; };
 
+// the end of the part's last slot
+__device__ __forceinline__ int slots_end(const Part& part) { return part.lo + (part.hi - part.lo + SLOT - 1) / SLOT * SLOT; }
+
 template <int DP>
 struct Rows {
-  static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = 3 * STAGE, SUMS = BARS + 128, SMEM = SUMS + 2 * 128 * 4;
+  static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = 3 * STAGE, SUMS = BARS + 128, SMEM = SUMS + 4 * 128 * 4;
   static constexpr int P = 3 * DP / 2, S = 3 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W0 = S, W1 = DPO, OUT = E + HALF;
   using Weights = OverHalves<0, 8, HALF>;               // two planes over S or dP, one over T or E, each half over its own
   static_assert(OUT + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
@@ -28,7 +31,7 @@ struct Rows {
 
 template <int DP, int WALK>
 __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Params<float> p, const Streams im,
-                                                                     const float* __restrict__ stats, float* __restrict__ parts,
+                                                                     float* __restrict__ stats, float* __restrict__ parts,
                                                                      int* status) {
   using B = Rows<DP>;
   constexpr int HB = B::HB;
@@ -165,9 +168,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
       tc::tc_fence_after();
       add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
     }
-    if (WALK == 0 && half == 1) {
-      sums[threadIdx.x & 127] = ok ? R : __int_as_float(0x7fc00000);
-      sums[128 + (threadIdx.x & 127)] = U;
+    if (WALK == 0) {                                    // each half of a row's columns has its share of r and c
+      sums[128 * half + (threadIdx.x & 127)] = ok ? R : __int_as_float(0x7fc00000);
+      sums[256 + 128 * half + (threadIdx.x & 127)] = U;
     }
   }
   tc::tc_fence_before();
@@ -175,14 +178,35 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   if (on) {
     const int64_t rows = (int64_t)p.H * p.N, at = (int64_t)h * p.N + row;
     const float g = !ok ? __int_as_float(0x7fc00000) : WALK == 0 ? 1.f : p.scale;
+    float* out = p.splits > 1 ? p.work + (int64_t)blockIdx.z * rows * p.D : WALK == 0 ? p.out3 : p.out0;
+    if (WALK == 0) {
+      R = sums[threadIdx.x & 127] + sums[128 + (threadIdx.x & 127)];
+      U = sums[256 + (threadIdx.x & 127)] + sums[384 + (threadIdx.x & 127)];
+      if (p.splits > 1) {
+        if (half == 0) {
+          parts[(2 * (int64_t)blockIdx.z) * rows + at] = R;
+          parts[(2 * (int64_t)blockIdx.z + 1) * rows + at] = U;
+        }
+      } else if (part.keys) {                           // nothing to join: r, c and do' at once
+        float* st = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
+        if (half == 0) {
+          st[2 * SLOT] = R;
+          st[3 * SLOT] = U - st[SLOT] * R;
+        }
+        const float* o = p.o + row * p.os + h * p.oh + half * (DP / 2);
+#pragma unroll
+        for (int d = 0; d < DP / 2; ++d)
+          if (half * (DP / 2) + d < p.D) acc[d] -= R * o[d];
+      }
+    }
 #pragma unroll
     for (int d = 0; d < DP / 2; ++d) acc[d] *= g;
-    float* out = WALK == 1 && p.splits == 1 ? p.out0 : p.work + (int64_t)blockIdx.z * rows * p.D;
     store_columns<DP / 2>(out + ((int64_t)row * p.H + h) * p.D, acc, half * (DP / 2), p.D);
-    if (WALK == 0 && half == 0) {
-      parts[(2 * (int64_t)blockIdx.z) * rows + at] = R + sums[threadIdx.x];
-      parts[(2 * (int64_t)blockIdx.z + 1) * rows + at] = U + sums[128 + threadIdx.x];
-    }
+  } else if (WALK == 0 && warp < 8 && p.splits == 1 && part.keys && row < slots_end(part) && half == 0) {
+    // the rows behind the structure's last one in its last slot
+    float* st = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
+    st[2 * SLOT] = 0.f;
+    st[3 * SLOT] = 0.f;
   }
   if (warp == 8) {
     tc::tc_fence_after();
@@ -190,7 +214,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   }
 }
 
-// A warp per eight rows of a (slot, head), two rows at a time: r, c and do' from the splits; rows without keys give zero.
+// Two rows a warp of a quarter of a (slot, head): r, c and do' from the splits; rows without keys give zero.
 __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p, float* __restrict__ stats,
                                                           const float* __restrict__ parts, int slots) {
   Part part;
@@ -198,8 +222,8 @@ __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p,
   const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t rows = (int64_t)p.H * p.N;
   float* st = stats + ((int64_t)h * slots + blockIdx.x) * KINDS * SLOT;
-#pragma unroll 2
-  for (int i = warp; i < SLOT; i += 8) {
+#pragma unroll
+  for (int i = blockIdx.z * 16 + warp; i < (int)blockIdx.z * 16 + 16; i += 8) {
     const int row = part.row + i;
     const bool in = row < part.hi, live = in && part.keys;
     const int64_t at = (int64_t)h * p.N + (live ? row : 0);
@@ -414,8 +438,7 @@ cudaError_t prepare(const Params<float>& p, char* work, cudaStream_t s) {
   src.s[4] = {p.q, p.qs, p.qh, p.H, nullptr, w.at[4]};
   src.s[5] = {p.go, p.gos, p.goh, p.H, nullptr, w.at[5]};
   src.s[6] = {p.ca, p.cas, p.cah, p.H, nullptr, w.at[6]};
-  const cudaError_t e = write_images<DP>(p, src, 7, s);
-  return e != cudaSuccess ? e : write_stats(p, w.stats, KINDS, s);
+  return write_images<DP>(p, src, 7, w.stats, KINDS, s);
 }
 
 template <int DP, int WALK>
@@ -431,7 +454,7 @@ cudaError_t rows(const Params<float>& p, char* work, int* status, cudaStream_t s
 template <int DP>
 cudaError_t join(const Params<float>& p, char* work, cudaStream_t s) {
   const Layout<DP> w(p, work);
-  second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
+  second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H, 4), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
   return cudaGetLastError();
 }
 

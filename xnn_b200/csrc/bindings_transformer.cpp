@@ -199,7 +199,7 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
       XNN_OK(attn::tc_backward_prepare(pl, images, s));
       pl.splits = sq;
       XNN_OK(attn::tc_backward_dq(pl, images, status_of(status, q), s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
       pl.splits = sk;
       XNN_OK(attn::tc_backward_dkv(pl, images, status_of(status, q), s));
     } else {
@@ -208,14 +208,11 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
       XNN_OK(attn::row_delta<T>(pl, s));
       pl.splits = sq;
       XNN_OK(attn::backward_dq(pl, s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
       pl.splits = sk;
       XNN_OK(attn::backward_dkv(pl, s));
     }
-    if (sk > 1) {
-      XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, s));
-      XNN_OK(attn::sum_splits<T>(nk, sk, pl.work + (int64_t)sk * nk, p.out2, s));
-    }
+    if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, p.out2, s));
   }
   if (plan.short_ones) XNN_OK(attn::backward_short<T>(short_part(p, plan), s));
   return {dq, dk, dv};
@@ -249,22 +246,19 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
       const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
       const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
       auto images = bytes(attn::tc_second_bytes(pl) + (int64_t)sq * 2 * p.H * p.N * 4, q);
-      torch::Tensor work = torch::empty({std::max(sq * nq, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+      torch::Tensor work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
       char* im = static_cast<char*>(images.data_ptr());
       int* flag = status_of(status, q);
       pl.work = work.data_ptr<T>();
       pl.splits = sq;
       XNN_OK(attn::tc_second_prepare(pl, im, s));
       XNN_OK(attn::tc_second_rows(pl, im, 0, flag, s));
-      XNN_OK(attn::tc_second_join(pl, im, s));
+      if (sq > 1) XNN_OK(attn::tc_second_join(pl, im, s));
       XNN_OK(attn::tc_second_rows(pl, im, 1, flag, s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, s));
+      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
       pl.splits = sk;
       XNN_OK(attn::tc_second_keys(pl, im, flag, s));
-      if (sk > 1) {
-        XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, s));
-        XNN_OK(attn::sum_splits<T>(nk, sk, pl.work + (int64_t)sk * nk, p.out2, s));
-      }
+      if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, p.out2, s));
       rest = plan.short_ones;
       pr = short_part(p, plan);
     }
