@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(C::NT) dkv_kernel(const Params<T> p) {
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const bool vq = vec_ok(p.q, p.qs, p.qh, p.D), vo = vec_ok(p.go, p.gos, p.goh, p.D);
   int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
-  split_range<C::BK>(q_lo, q_hi, blockIdx.z, p.splits);
+  split_range<C::BK>(q_lo, q_hi, blockIdx.z, p.splits_k);
   const T c2 = p.scale * log2e<T>();
   T dk[C::RI][C::DP / C::TX], dv[C::RI][C::DP / C::TX];
   bool ok[C::RI];
@@ -289,9 +289,9 @@ __global__ void __launch_bounds__(C::NT) dkv_kernel(const Params<T> p) {
     if (row >= part.hi) continue;
     const int64_t at = ((int64_t)row * p.HK + hk) * p.D;
     T *ok_ = p.out1 + at, *ov_ = p.out2 + at;
-    if (p.splits > 1) {
-      ok_ = p.work + blockIdx.z * n + at;
-      ov_ = p.work + (p.splits + blockIdx.z) * n + at;
+    if (p.splits_k > 1) {
+      ok_ = p.work_k + blockIdx.z * n + at;
+      ov_ = p.work_k + (p.splits_k + blockIdx.z) * n + at;
     }
     store_row<T, C::DP, C::TX>(ok_, dk[r], p.scale, p.D, tx);
     store_row<T, C::DP, C::TX>(ov_, dv[r], T(1), p.D, tx);
@@ -568,12 +568,12 @@ __global__ void __launch_bounds__(C::NT) second_key_kernel(const Params<T> p) {
 
 // ------------------------------------------------------------------------------------------ launches
 template <typename T, typename C, auto KERNEL>
-cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s) {
+cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s, int splits = 1) {
   const size_t bytes = sizeof(T) * ((size_t)row_tiles * C::BQ * C::LD + (size_t)key_tiles * C::BK * C::LD +
                                     (size_t)squares * C::BQ * C::LDP);
   const cudaError_t e = raise_smem_limit<KERNEL>(bytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.N / C::BQ + p.num + 2, heads, p.splits);
+  const dim3 grid(p.N / C::BQ + p.num + 2, heads, splits);
   KERNEL<<<grid, C::NT, bytes, s>>>(p);
   return cudaGetLastError();
 }
@@ -597,7 +597,7 @@ template <> struct Second<double, 128> { using C = Cfg<double, 32, 16, 128, 2, 1
 
 template <typename T>
 cudaError_t forward(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s, p.splits)))
 }
 template <typename T>
 cudaError_t forward_join(const Params<T>& p, cudaStream_t s) {
@@ -617,10 +617,10 @@ cudaError_t row_delta(const Params<T>& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 cudaError_t backward_dq(const Params<double>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dq_kernel<double, C>>(p, p.H, 2, 2, 1, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dq_kernel<double, C>>(p, p.H, 2, 2, 1, s, p.splits)))
 }
 cudaError_t backward_dkv(const Params<double>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dkv_kernel<double, C>>(p, p.HK, 2, 2, 2, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dkv_kernel<double, C>>(p, p.HK, 2, 2, 2, s, p.splits_k)))
 }
 template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {

@@ -22,15 +22,9 @@ template <typename T> cudaError_t second_keys(const Params<T>&, cudaStream_t);
 int64_t tc_forward_bytes(const Params<float>&);
 int64_t tc_backward_bytes(const Params<float>&);
 cudaError_t tc_forward(const Params<float>&, char* work, int* status, cudaStream_t);
-cudaError_t tc_backward_prepare(const Params<float>&, char* work, cudaStream_t);
-cudaError_t tc_backward_dq(const Params<float>&, char* work, int* status, cudaStream_t);
-cudaError_t tc_backward_dkv(const Params<float>&, char* work, int* status, cudaStream_t);
-cudaError_t tc_wide_dq(const Params<float>&, char* work, int* status, cudaStream_t);      // 65 .. 128 columns
-cudaError_t tc_wide_dkv(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_backward(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_wide_backward(const Params<float>&, char* work, int* status, cudaStream_t);   // 65 .. 128 columns, images written
 int64_t tc_second_bytes(const Params<float>&);
-cudaError_t tc_second_prepare(const Params<float>&, char* work, cudaStream_t);
-cudaError_t tc_second_rows(const Params<float>&, char* work, int walk, int* status, cudaStream_t);
-cudaError_t tc_second_join(const Params<float>&, char* work, cudaStream_t);
-cudaError_t tc_second_keys(const Params<float>&, char* work, int* status, cudaStream_t);
+cudaError_t tc_second(const Params<float>&, char* work, int* status, cudaStream_t);          // up to 64 columns
 
 }  // namespace attn

@@ -16,9 +16,9 @@ struct Params {
   const uint8_t* mask;               // 1 where an atom may be attended to, or null
   T *out0, *out1, *out2, *out3;      // contiguous outputs
   T *lse, *delta, *r, *c;            // (H, N) row statistics
-  T* work;                           // partial results of split passes
+  T *work, *work_k;                  // partial results of split passes: over keys, over queries
   T scale;
-  int N, num, H, HK, D, splits;
+  int N, num, H, HK, D, splits, splits_k;
   int min_len, max_len;              // the lengths that this launch takes (others return at once)
 };
 

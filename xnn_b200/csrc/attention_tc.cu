@@ -261,17 +261,19 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   __syncthreads();
   if (warp < 8) tops[half * 128 + r] = ok ? l : __int_as_float(0x7fc00000);
   __syncthreads();
-  if (on) {
+  if (warp < 8) {
     l = tops[r] + tops[128 + r];
     const bool none = m == neg_inf<float>() && l == 0.f;
     const bool split = p.splits > 1;
     const int64_t rows = (int64_t)p.H * p.N, at = blockIdx.z * rows + (int64_t)h * p.N + row;
     const float g = split ? 1.f : none ? 0.f : 1.f / l;
-    float* out = split ? p.work + at * p.D : p.out0 + ((int64_t)row * p.H + h) * p.D;
+    const int row0 = part.row + 32 * (warp & 3);         // the warp's first row
+    float* out = split ? p.work + (blockIdx.z * rows + (int64_t)h * p.N + row0) * p.D : p.out0 + ((int64_t)row0 * p.H + h) * p.D;
 #pragma unroll
     for (int d = 0; d < DP / 2; ++d) acc[d] *= g;
-    store_columns<DP / 2>(out, acc, half * (DP / 2), p.D);
-    if (half == 0) {
+    store_rows<DP / 2>(scratch_of<DP / 2>(smem, warp), acc, out, split ? p.D : (int64_t)p.H * p.D, min(32, part.hi - row0),
+                       half * (DP / 2), p.D, ok);
+    if (half == 0 && on) {
       if (split) {
         float* stats = p.work + p.splits * rows * p.D;
         stats[at] = m;
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
 // ------------------------------------------------------------------------------------------ backward
 // Eight warps of rows: warp w reaches the lanes 32 (w % 4) .. of tensor memory and takes half w / 4 of the columns;
 // a ninth copies and issues. A ring of three stages holds the streamed images.
-constexpr int BWD_THREADS = 288, STAGES = 3;
+constexpr int STAGES = 3;
 
 template <int DP>
 struct Bwd {
@@ -337,15 +339,11 @@ __device__ __forceinline__ Block set_up(char* smem) {
   return k;
 }
 
-// the parts of the two resident operands: a (times af) by the first four warps, b by the others
+// the parts of the two resident operands: a by the first four warps, b by the others
 template <int DP>
-__device__ __forceinline__ void stage_rows(const Block& k, const Part& part, const float* a, int64_t as, bool av, float af,
-                                           const float* b, int64_t bs, bool bv, int D, const uint8_t* mask) {
-  const int row = part.row + (threadIdx.x & 127);
-  const bool on = row < part.hi && (mask == nullptr || mask[row]);
+__device__ __forceinline__ void stage_rows(const Block& k, const char* a, const char* b) {
   const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
-  if (k.warp < 4) stage_row<DP>(lanes, a + row * as, on, av, D, af);
-  else stage_row<DP>(lanes + Bwd<DP>::PARTS, b + row * bs, on, bv, D, 1.f);
+  stage_image<DP>(lanes + (k.warp < 4 ? 0 : Bwd<DP>::PARTS), k.warp < 4 ? a : b, threadIdx.x & 127);
   tmem_st_wait();
   tc::tc_fence_before();
 }
@@ -361,16 +359,14 @@ __device__ __forceinline__ void tear_down(const Block& k) {
 
 // dq of 128 queries. S and dP of the next tile run while the rows' threads form dS of this one.
 template <int DP>
-__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<float> p, const Images ik, const Images iv,
-                                                               const float* __restrict__ stats, int* status) {
+__device__ __forceinline__ void dq_block(const Params<float>& p, const Part& part, const Job& job, const Images& ik, const Images& iv,
+                                         const Images& iq, const Images& io, const float* __restrict__ stats, int* status) {
   using B = Bwd<DP>;
-  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  constexpr int BYTES = Image<DP>::BYTES;
   extern __shared__ __align__(128) char smem[];
-  Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int h = blockIdx.y, hk = h / (p.H / p.HK);
+  const int h = job.head, hk = h / (p.H / p.HK);
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
-  split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
+  split_range<SLOT>(k_lo, k_hi, job.split, job.splits);
   const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
   const Block k = set_up<DP>(smem);
   const auto load = [&](int i) {
@@ -385,8 +381,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
   if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    stage_rows<DP>(k, part, p.q + h * p.qh, p.qs, vec_ok(p.q, p.qs, p.qh, p.D), p.scale * log2e<float>(),
-                             p.go + h * p.goh, p.gos, vec_ok(p.go, p.gos, p.goh, p.D), p.D, nullptr);
+    const int own = first_slot(part) + (part.row - part.lo) / SLOT;
+    stage_rows<DP>(k, image<DP>(iq, h, own), image<DP>(io, h, own));
   }
   __syncthreads();
   tc::tc_fence_after();
@@ -428,6 +424,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
     const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
     const int half = k.warp / 4, r = threadIdx.x & 127, row = part.row + r;
     const bool on = row < part.hi;
+    const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, acc[DP / 2];
     if (on && n > 0) {
       const float* at = stats + ((int64_t)h * ik.slots + first_slot(part) + (row - part.lo) / SLOT) * 2 * SLOT;
@@ -448,10 +445,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
       tmem_ld_wait();
       tc::tc_fence_before();
       arrive(taken);
-      const Two low = two(-L, -L), down = two(-D, -D);
+      const Two low = two(-L, -L), down = two(-D, -D), by = two(c2, c2);
 #pragma unroll
       for (int j = 0; j < 32; j += 2) {
-        get(two(s[j], s[j + 1]) + low, s[j], s[j + 1]);
+        get(fma2(two(s[j], s[j + 1]), by, low), s[j], s[j + 1]);
         get(two(ex2(s[j]), ex2(s[j + 1])) * (two(dp[j], dp[j + 1]) + down), s[j], s[j + 1]);
       }
       if (bits != ~0u) {
@@ -474,21 +471,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
       tc::tc_fence_after();
       add();
     }
-    if (on) {
-      const float g = ok ? p.scale : __int_as_float(0x7fc00000);
-      float* out = (p.splits > 1 ? p.work + (int64_t)blockIdx.z * p.N * p.H * p.D : p.out0) + ((int64_t)row * p.H + h) * p.D;
 #pragma unroll
-      for (int d = 0; d < DP / 2; d += 4) {
-        const int c = half * (DP / 2) + d;
-        if (p.D % 4 == 0) {
-          if (c < p.D) *reinterpret_cast<float4*>(out + c) = make_float4(g * acc[d], g * acc[d + 1], g * acc[d + 2], g * acc[d + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < p.D) out[c + e] = g * acc[d + e];
-        }
-      }
-    }
+    for (int d = 0; d < DP / 2; ++d) acc[d] *= p.scale;
+    const int row0 = part.row + 32 * (k.warp & 3);
+    float* out = job.splits > 1 ? p.work + (int64_t)job.split * p.N * p.H * p.D : p.out0;
+    store_rows<DP / 2>(scratch_of<DP / 2>(smem, k.warp), acc, out + ((int64_t)row0 * p.H + h) * p.D, (int64_t)p.H * p.D,
+                       min(32, part.hi - row0), half * (DP / 2), p.D, ok);
   }
   tear_down(k);
 }
@@ -497,16 +485,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dq_kernel(const Params<floa
 // tensor cores: while the threads form P^T of a tile, dK of the tile before and dP^T of this one run; while they form
 // dS^T, dV of this tile and S^T of the next.
 template <int DP>
-__global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<float> p, const Images iq, const Images io,
-                                                                const float* __restrict__ stats, int* status) {
+__device__ __forceinline__ void dkv_block(const Params<float>& p, const Part& part, const Job& job, const Images& ik, const Images& iv,
+                                          const Images& iq, const Images& io, const float* __restrict__ stats, int* status) {
   using B = Bwd<DP>;
-  constexpr int BYTES = Image<DP>::BYTES, PLANE = Image<DP>::PLANE;
+  constexpr int BYTES = Image<DP>::BYTES;
   extern __shared__ __align__(128) char smem[];
-  Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int hk = blockIdx.y, group = p.H / p.HK;
+  const int hk = job.head, group = p.H / p.HK;
   int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
-  split_range<SLOT>(q_lo, q_hi, blockIdx.z, p.splits);
+  split_range<SLOT>(q_lo, q_hi, job.split, job.splits);
   const int tiles = (q_hi - q_lo + SLOT - 1) / SLOT, n = tiles * group, slot0 = first_slot(part) + (q_lo - part.lo) / SLOT;
   const Block k = set_up<DP>(smem);
   const auto load = [&](int i) {
@@ -524,8 +510,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
   if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    stage_rows<DP>(k, part, p.k + hk * p.kh, p.ks, vec_ok(p.k, p.ks, p.kh, p.D), p.scale * log2e<float>(),
-                             p.v + hk * p.vh, p.vs, vec_ok(p.v, p.vs, p.vh, p.D), p.D, p.mask);
+    const int own = first_slot(part) + (part.row - part.lo) / SLOT;
+    stage_rows<DP>(k, image<DP>(ik, hk, own), image<DP>(iv, hk, own));
   }
   __syncthreads();
   tc::tc_fence_after();
@@ -569,6 +555,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
   } else {
     const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
     const int half = k.warp / 4, row = part.row + (threadIdx.x & 127);
+    const float c2 = p.scale * log2e<float>();
     // the first half of the warps adds up dV, the second dK
     float acc[DP];
 #pragma unroll
@@ -588,7 +575,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
 #pragma unroll
       for (int j = 0; j < 32; j += 4) {
         const float4 L = *reinterpret_cast<const float4*>(st + j);
-        s[j] = ex2(s[j] - L.x); s[j + 1] = ex2(s[j + 1] - L.y); s[j + 2] = ex2(s[j + 2] - L.z); s[j + 3] = ex2(s[j + 3] - L.w);
+        s[j] = ex2(fmaf(s[j], c2, -L.x));
+        s[j + 1] = ex2(fmaf(s[j + 1], c2, -L.y));
+        s[j + 2] = ex2(fmaf(s[j + 2], c2, -L.z));
+        s[j + 3] = ex2(fmaf(s[j + 3], c2, -L.w));
       }
       if (half == 0 && i > 0) add(B::K_DV);
       store_parts16<OverScores>(lanes + B::K_S, 2 * half, s);
@@ -616,26 +606,27 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) tc_dkv_kernel(const Params<flo
       tc::tc_fence_after();
       add(half ? B::K_DK : B::K_DV);
     }
-    if (row < part.hi) {
-      const bool hidden = p.mask != nullptr && !p.mask[row];
-      const float g = !ok ? __int_as_float(0x7fc00000) : half ? p.scale : 1.f;
-      const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)row * p.HK + hk) * p.D;
-      float* out = p.splits > 1 ? p.work + ((half ? 0 : p.splits) + (int64_t)blockIdx.z) * all + at : (half ? p.out1 : p.out2) + at;
+    const bool hidden = row < part.hi && p.mask != nullptr && !p.mask[row];
 #pragma unroll
-      for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : g * acc[d];
-#pragma unroll
-      for (int d = 0; d < DP; d += 4) {
-        if (p.D % 4 == 0) {
-          if (d < p.D) *reinterpret_cast<float4*>(out + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < p.D) out[d + e] = acc[d + e];
-        }
-      }
-    }
+    for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : half ? p.scale * acc[d] : acc[d];
+    const int row0 = part.row + 32 * (k.warp & 3);
+    const int64_t all = (int64_t)p.N * p.HK * p.D;
+    float* out = job.splits > 1 ? p.work_k + ((half ? 0 : job.splits) + (int64_t)job.split) * all : half ? p.out1 : p.out2;
+    store_rows<DP>(scratch_of<DP>(smem, k.warp), acc, out + ((int64_t)row0 * p.HK + hk) * p.D, (int64_t)p.HK * p.D,
+                   min(32, part.hi - row0), 0, p.D, ok);
   }
   tear_down(k);
+}
+
+// Both in one launch, the longer blocks of the keys first, so that neither waits for the other's last blocks.
+template <int DP>
+__global__ void __launch_bounds__(ROW_THREADS, 1) tc_bwd_kernel(const Params<float> p, const Images ik, const Images iv, const Images iq,
+                                                                const Images io, const float* __restrict__ stats, int* status) {
+  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  if (rest < keys) dkv_block<DP>(p, part, {rest % p.HK, rest / p.HK, p.splits_k}, ik, iv, iq, io, stats, status);
+  else dq_block<DP>(p, part, {(rest - keys) % p.H, (rest - keys) / p.H, p.splits}, ik, iv, iq, io, stats, status);
 }
 
 template <int DP>
@@ -665,24 +656,15 @@ cudaError_t prepare_dp(const Params<float>& p, char* work, cudaStream_t s) {
 }
 
 template <int DP>
-cudaError_t dq_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+cudaError_t backward_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   const int slots = image_slots(p);
-  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK);
-  const float* stats = reinterpret_cast<const float*>(iv + image_bytes<DP>(p, p.HK) + 2 * image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit<tc_dq_kernel<DP>>(Bwd<DP>::SMEM);
-  if (e != cudaSuccess) return e;
-  tc_dq_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, stats, status);
-  return cudaGetLastError();
-}
-
-template <int DP>
-cudaError_t dkv_dp(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  const int slots = image_slots(p);
-  char *iq = work + 2 * image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
+  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit<tc_dkv_kernel<DP>>(Bwd<DP>::SMEM);
+  const cudaError_t e = raise_smem_limit<tc_bwd_kernel<DP>>(Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
-  tc_dkv_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), BWD_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{iq, slots}, Images{io, slots}, stats, status);
+  const int64_t blocks = (int64_t)(p.N / 128 + p.num + 2) * (p.HK * p.splits_k + p.H * p.splits);
+  tc_bwd_kernel<DP><<<(unsigned)blocks, ROW_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, Images{iq, slots},
+                                                                        Images{io, slots}, stats, status);
   return cudaGetLastError();
 }
 
@@ -708,14 +690,10 @@ int64_t tc_backward_bytes(const Params<float>& p) {
 cudaError_t tc_forward(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   return p.D <= 32 ? forward_dp<32>(p, work, status, s) : p.D <= 64 ? forward_dp<64>(p, work, status, s) : forward_dp<128>(p, work, status, s);
 }
-cudaError_t tc_backward_prepare(const Params<float>& p, char* work, cudaStream_t s) {
-  return p.D <= 32 ? prepare_dp<32>(p, work, s) : p.D <= 64 ? prepare_dp<64>(p, work, s) : prepare_dp<128>(p, work, s);
-}
-cudaError_t tc_backward_dq(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  return p.D <= 32 ? dq_dp<32>(p, work, status, s) : p.D <= 64 ? dq_dp<64>(p, work, status, s) : tc_wide_dq(p, work, status, s);
-}
-cudaError_t tc_backward_dkv(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  return p.D <= 32 ? dkv_dp<32>(p, work, status, s) : p.D <= 64 ? dkv_dp<64>(p, work, status, s) : tc_wide_dkv(p, work, status, s);
+cudaError_t tc_backward(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  cudaError_t e = p.D <= 32 ? prepare_dp<32>(p, work, s) : p.D <= 64 ? prepare_dp<64>(p, work, s) : prepare_dp<128>(p, work, s);
+  if (e != cudaSuccess) return e;
+  return p.D <= 32 ? backward_dp<32>(p, work, status, s) : p.D <= 64 ? backward_dp<64>(p, work, status, s) : tc_wide_backward(p, work, status, s);
 }
 
 }  // namespace attn

@@ -317,6 +317,8 @@ __device__ __forceinline__ uint64_t allowed_bits(int k0, int hi, const uint8_t* 
 
 // ---- kernels that stream halves of images: eight warps of rows, a ninth that copies and issues ----
 constexpr int HALF = SLOT / 2, ROW_THREADS = 288;
+// which head and which share of the other axis a block takes
+struct Job { int head, split, splits; };
 template <int DP> constexpr int half_bytes() { return PLANES * HALF * DP * 2; }
 
 // half `half` of an image: its planes one behind the other
@@ -342,20 +344,49 @@ __device__ __forceinline__ uint32_t allowed_half(int k0, int hi, const uint8_t* 
   return __ballot_sync(0xffffffffu, k < hi && (mask == nullptr || mask[k]));
 }
 
-// N neighbouring columns of a row, guarded by D
+// N columns from c0 on of row r of a block of 128 rows, from the images of its slots: neighbouring lanes read neighbouring
+// 16 bytes, where rows of the tensor itself would be a line of memory apart
+template <int DP, int N = DP>
+__device__ __forceinline__ void stage_image(uint32_t addr, const char* im, int r, int c0 = 0) {
+  const char* at = im + r / SLOT * Image<DP>::BYTES + r % SLOT / 8 * (DP * 16) + r % 8 * 16 + c0 * 16;
+  uint4 v[PLANES][N / 8];
+#pragma unroll
+  for (int x = 0; x < PLANES; ++x)
+#pragma unroll
+    for (int c = 0; c < N / 8; ++c) v[x][c] = *reinterpret_cast<const uint4*>(at + x * Image<DP>::PLANE + c * 128);
+#pragma unroll
+  for (int x = 0; x < PLANES; ++x)
+#pragma unroll
+    for (int c = 0; c < N / 8; c += 2)
+      tmem_st8(addr + x * (DP / 2) + c0 / 2 + c * 4, reinterpret_cast<const uint32_t*>(&v[x][c]));
+}
+
+// N columns from c0 on of a warp's 32 rows (a lane has a row), through shared memory so that whole lines are written;
+// `rows` of them exist. NaN where the block gave up.
 template <int N>
-__device__ __forceinline__ void store_columns(float* out, const float* v, int c0, int D) {
+__device__ __forceinline__ void store_rows(float* scratch, const float* v, float* out, int64_t stride, int rows, int c0, int D, bool ok) {
+  constexpr int LD = N + 4, PER = N / 4;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int d = 0; d < N; d += 4) {
+  for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(scratch + lane * LD + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  __syncwarp();
+  const int c = lane % PER * 4;
+  for (int r = lane / PER; r < rows; r += 32 / PER) {
+    float4 x = *reinterpret_cast<const float4*>(scratch + r * LD + c);
+    if (!ok) x.x = x.y = x.z = x.w = __int_as_float(0x7fc00000);
+    float* to = out + r * stride + c0 + c;
     if (D % 4 == 0) {
-      if (c0 + d < D) *reinterpret_cast<float4*>(out + c0 + d) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+      if (c0 + c < D) *reinterpret_cast<float4*>(to) = x;
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c0 + d + e < D) out[c0 + d + e] = v[d + e];
+      if (c0 + c < D) to[0] = x.x;
+      if (c0 + c + 1 < D) to[1] = x.y;
+      if (c0 + c + 2 < D) to[2] = x.z;
+      if (c0 + c + 3 < D) to[3] = x.w;
     }
   }
 }
+template <int N>
+__device__ __forceinline__ float* scratch_of(char* smem, int warp) { return reinterpret_cast<float*>(smem) + warp * 32 * (N + 4); }
 
 // acc += N columns of tensor memory
 template <int N>

@@ -13,7 +13,6 @@
 namespace attn {
 namespace {
 
-constexpr float LN2 = 0.6931471805599453f;              // the staged rows carry log2 e: T times it comes out of the products
 constexpr int KINDS = 4;                                // L, D, r, c of a slot's rows
 
 struct Streams { Images a, b, c, d; };
@@ -30,9 +29,8 @@ struct Rows {
 };
 
 template <int DP, int WALK>
-__global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Params<float> p, const Streams im,
-                                                                     float* __restrict__ stats, float* __restrict__ parts,
-                                                                     int* status) {
+__device__ __forceinline__ void rows_block(const Params<float>& p, const Part& part, const Job& job, const Streams& im, const Streams& own,
+                                           float* __restrict__ stats, float* __restrict__ parts, int* status) {
   using B = Rows<DP>;
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
@@ -41,11 +39,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 10);
   float* sums = reinterpret_cast<float*>(smem + B::SUMS);
-  Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int warp = threadIdx.x / 32, h = blockIdx.y, hk = h / (p.H / p.HK);
+  const int warp = threadIdx.x / 32, h = job.head, hk = h / (p.H / p.HK);
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
-  split_range<SLOT>(lo, hi, blockIdx.z, p.splits);
+  split_range<SLOT>(lo, hi, job.split, job.splits);
   const int n = (hi - lo + HALF - 1) / HALF, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
@@ -75,13 +71,13 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   if (warp == 8) {                                      // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    const float c2 = p.scale * log2e<float>();
+    const int mine = first_slot(part) + (part.row - part.lo) / SLOT;   // own: q, A and do
     if (half == 0) {
-      stage_row<DP>(lanes, p.q + row * p.qs + h * p.qh, on, vec_ok(p.q, p.qs, p.qh, p.D), p.D, c2);
+      stage_image<DP>(lanes, image<DP>(own.a, h, mine), threadIdx.x & 127);
     } else {
-      stage_row<DP>(lanes + B::P, p.ca + row * p.cas + h * p.cah, on, vec_ok(p.ca, p.cas, p.cah, p.D), p.D, c2);
-      stage_row<DP>(lanes + 2 * B::P, p.go + row * p.gos + h * p.goh, on, vec_ok(p.go, p.gos, p.goh, p.D), p.D, 1.f);
+      stage_image<DP>(lanes + B::P, image<DP>(own.b, h, mine), threadIdx.x & 127);
     }
+    stage_image<DP, DP / 2>(lanes + 2 * B::P, image<DP>(own.c, h, mine), threadIdx.x & 127, half * (DP / 2));
     tmem_st_wait();
     tc::tc_fence_before();
   }
@@ -126,6 +122,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
     }
     __syncwarp();
   } else {
+    const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, r = 0.f, c = 0.f;
     if (on && n > 0) {
       const float* at = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
@@ -146,7 +143,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const bool in = (bits >> j) & 1;
-        const float pr = in ? ex2(s[j] - L) : 0.f, tt = t[j] * LN2;
+        const float pr = in ? ex2(fmaf(s[j], c2, -L)) : 0.f, tt = t[j] * p.scale;
         if (WALK == 0) {
           s[j] = in ? pr * tt : 0.f;
           t[j] = pr;
@@ -175,38 +172,38 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_rows_kernel(const Param
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (on) {
+  if (warp < 8) {
     const int64_t rows = (int64_t)p.H * p.N, at = (int64_t)h * p.N + row;
-    const float g = !ok ? __int_as_float(0x7fc00000) : WALK == 0 ? 1.f : p.scale;
-    float* out = p.splits > 1 ? p.work + (int64_t)blockIdx.z * rows * p.D : WALK == 0 ? p.out3 : p.out0;
+    float* out = job.splits > 1 ? p.work + (int64_t)job.split * rows * p.D : WALK == 0 ? p.out3 : p.out0;
     if (WALK == 0) {
       R = sums[threadIdx.x & 127] + sums[128 + (threadIdx.x & 127)];
       U = sums[256 + (threadIdx.x & 127)] + sums[384 + (threadIdx.x & 127)];
-      if (p.splits > 1) {
-        if (half == 0) {
-          parts[(2 * (int64_t)blockIdx.z) * rows + at] = R;
-          parts[(2 * (int64_t)blockIdx.z + 1) * rows + at] = U;
+      if (job.splits > 1) {
+        if (on && half == 0) {
+          parts[(2 * (int64_t)job.split) * rows + at] = R;
+          parts[(2 * (int64_t)job.split + 1) * rows + at] = U;
         }
-      } else if (part.keys) {                           // nothing to join: r, c and do' at once
+      } else if (part.keys && row < slots_end(part)) {  // nothing to join: r, c and do' at once, zeros behind the last row
         float* st = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
         if (half == 0) {
-          st[2 * SLOT] = R;
-          st[3 * SLOT] = U - st[SLOT] * R;
+          st[2 * SLOT] = on ? R : 0.f;
+          st[3 * SLOT] = on ? U - st[SLOT] * R : 0.f;
         }
-        const float* o = p.o + row * p.os + h * p.oh + half * (DP / 2);
+        if (on) {
+          const float* o = p.o + row * p.os + h * p.oh + half * (DP / 2);
 #pragma unroll
-        for (int d = 0; d < DP / 2; ++d)
-          if (half * (DP / 2) + d < p.D) acc[d] -= R * o[d];
+          for (int d = 0; d < DP / 2; ++d)
+            if (half * (DP / 2) + d < p.D) acc[d] -= R * o[d];
+        }
       }
     }
+    if (WALK == 1) {
 #pragma unroll
-    for (int d = 0; d < DP / 2; ++d) acc[d] *= g;
-    store_columns<DP / 2>(out + ((int64_t)row * p.H + h) * p.D, acc, half * (DP / 2), p.D);
-  } else if (WALK == 0 && warp < 8 && p.splits == 1 && part.keys && row < slots_end(part) && half == 0) {
-    // the rows behind the structure's last one in its last slot
-    float* st = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
-    st[2 * SLOT] = 0.f;
-    st[3 * SLOT] = 0.f;
+      for (int d = 0; d < DP / 2; ++d) acc[d] *= p.scale;
+    }
+    const int row0 = part.row + 32 * (warp & 3);
+    store_rows<DP / 2>(scratch_of<DP / 2>(smem, warp), acc, out + ((int64_t)row0 * p.H + h) * p.D, (int64_t)p.H * p.D,
+                       min(32, part.hi - row0), half * (DP / 2), p.D, ok);
   }
   if (warp == 8) {
     tc::tc_fence_after();
@@ -260,8 +257,8 @@ struct Keys {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Params<float> p, const Images iv, const Images ic,
-                                                                     const Streams im, const float* __restrict__ stats, int* status) {
+__device__ __forceinline__ void keys_block(const Params<float>& p, const Part& part, const Job& job, const Streams& own, const Streams& im,
+                                           const float* __restrict__ stats, int* status) {
   using B = Keys<DP>;
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
@@ -269,11 +266,10 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   uint64_t *full = bars, *full_2 = bars + 3, *done = bars + 4, *ready = bars + 5;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 10);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 11);
-  Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int warp = threadIdx.x / 32, hk = blockIdx.y, group = p.H / p.HK;
+  const int warp = threadIdx.x / 32, hk = job.head, group = p.H / p.HK;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
-  split_range<SLOT>(lo, hi, blockIdx.z, p.splits);
+  split_range<SLOT>(lo, hi, job.split, job.splits);
+  const int mine = first_slot(part) + (part.row - part.lo) / SLOT;     // own: k, v, B, C
   const int tiles = (hi - lo + HALF - 1) / HALF, n = tiles * group, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
@@ -304,18 +300,14 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   int loaded = min(n, 3);
   if (warp == 8 && n > 0) {
     if (elect()) {
-      const int s = first_slot(part) + (part.row - part.lo) / SLOT;
       tc::mbar_arrive_expect_tx(full_2, 2 * B::BLOCK);
-      load_block<DP>(smem, image<DP>(iv, hk, s), full_2);
-      load_block<DP>(smem + B::BLOCK, image<DP>(ic, hk, s), full_2);
+      load_block<DP>(smem, image<DP>(own.b, hk, mine), full_2);
+      load_block<DP>(smem + B::BLOCK, image<DP>(own.d, hk, mine), full_2);
     }
     __syncwarp();
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    const bool on = row < part.hi && (p.mask == nullptr || p.mask[row]);
-    const float c2 = p.scale * log2e<float>();
-    if (half == 0) stage_row<DP>(lanes, p.k + row * p.ks + hk * p.kh, on, vec_ok(p.k, p.ks, p.kh, p.D), p.D, c2);
-    else stage_row<DP>(lanes + B::P, p.cb + row * p.cbs + hk * p.cbh, on, vec_ok(p.cb, p.cbs, p.cbh, p.D), p.D, c2);
+    stage_image<DP>(lanes + (half ? B::P : 0), image<DP>(half ? own.c : own.a, hk, mine), threadIdx.x & 127);
     tmem_st_wait();
     tc::tc_fence_before();
   }
@@ -358,6 +350,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
     }
     __syncwarp();
   } else {
+    const float c2 = p.scale * log2e<float>();
     float acc[DP];                                      // the first half of the warps adds up k', the second v'
 #pragma unroll
     for (int d = 0; d < DP; ++d) acc[d] = 0.f;
@@ -375,7 +368,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const float pr = ex2(s[j] - st[j]), x = t[j] * LN2 - st[2 * HALF + j], y = dp[j] - st[HALF + j];
+        const float pr = ex2(fmaf(s[j], c2, -st[j])), x = fmaf(t[j], p.scale, -st[2 * HALF + j]), y = dp[j] - st[HALF + j];
         s[j] = pr * (fmaf(x, y, e[j]) - st[3 * HALF + j]);
         t[j] = pr * y;
         dp[j] = pr * x;
@@ -392,15 +385,14 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
       tc::tc_fence_after();
       add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
     }
-    if (row < part.hi) {
-      const bool hidden = p.mask != nullptr && !p.mask[row];
-      const float g = !ok ? __int_as_float(0x7fc00000) : half ? 1.f : p.scale;
+    const bool hidden = row < part.hi && p.mask != nullptr && !p.mask[row];
 #pragma unroll
-      for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : g * acc[d];
-      const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)row * p.HK + hk) * p.D;
-      float* out = p.splits > 1 ? p.work + ((half ? p.splits : 0) + (int64_t)blockIdx.z) * all + at : (half ? p.out2 : p.out1) + at;
-      store_columns<DP>(out, acc, 0, p.D);
-    }
+    for (int d = 0; d < DP; ++d) acc[d] = hidden ? 0.f : half ? acc[d] : p.scale * acc[d];
+    const int row0 = part.row + 32 * (warp & 3);
+    const int64_t all = (int64_t)p.N * p.HK * p.D;
+    float* out = job.splits > 1 ? p.work_k + ((half ? job.splits : 0) + (int64_t)job.split) * all : half ? p.out2 : p.out1;
+    store_rows<DP>(scratch_of<DP>(smem, warp), acc, out + ((int64_t)row0 * p.HK + hk) * p.D, (int64_t)p.HK * p.D,
+                   min(32, part.hi - row0), 0, p.D, ok);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -410,7 +402,26 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_keys_kernel(const Param
   }
 }
 
-// where things lie in the workspace: images of k, v, B, C, then q, do, A, the statistics, the splits' r and c
+template <int DP>
+__global__ void __launch_bounds__(ROW_THREADS, 1) second_first_kernel(const Params<float> p, const Streams k, const Streams q,
+                                                                      float* __restrict__ stats, float* __restrict__ parts, int* status) {
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  rows_block<DP, 0>(p, part, {(int)blockIdx.y, (int)blockIdx.z, p.splits}, k, q, stats, parts, status);
+}
+
+// what needs r and c, in one launch: the longer blocks of the keys first, then the second walk of the rows
+template <int DP>
+__global__ void __launch_bounds__(ROW_THREADS, 1) second_last_kernel(const Params<float> p, const Streams k, const Streams q,
+                                                                     float* __restrict__ stats, float* __restrict__ parts, int* status) {
+  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  if (rest < keys) keys_block<DP>(p, part, {rest % p.HK, rest / p.HK, p.splits_k}, k, {q.a, q.c, q.b, q.b}, stats, status);
+  else rows_block<DP, 1>(p, part, {(rest - keys) % p.H, (rest - keys) / p.H, p.splits}, k, q, stats, parts, status);
+}
+
+// where things lie in the workspace: images of k, v, B, C, then q, A, do, the statistics, the splits' r and c
 template <int DP>
 struct Layout {
   char* at[7];
@@ -428,7 +439,7 @@ struct Layout {
 };
 
 template <int DP>
-cudaError_t prepare(const Params<float>& p, char* work, cudaStream_t s) {
+cudaError_t second(const Params<float>& p, char* work, int* status, cudaStream_t s) {
   const Layout<DP> w(p, work);
   Sources src{};
   src.s[0] = {p.k, p.ks, p.kh, p.HK, p.mask, w.at[0]};
@@ -436,59 +447,36 @@ cudaError_t prepare(const Params<float>& p, char* work, cudaStream_t s) {
   src.s[2] = {p.cb, p.cbs, p.cbh, p.HK, p.mask, w.at[2]};
   src.s[3] = {p.cc, p.ccs, p.cch, p.HK, p.mask, w.at[3]};
   src.s[4] = {p.q, p.qs, p.qh, p.H, nullptr, w.at[4]};
-  src.s[5] = {p.go, p.gos, p.goh, p.H, nullptr, w.at[5]};
-  src.s[6] = {p.ca, p.cas, p.cah, p.H, nullptr, w.at[6]};
-  return write_images<DP>(p, src, 7, w.stats, KINDS, s);
-}
-
-template <int DP, int WALK>
-cudaError_t rows(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  const Layout<DP> w(p, work);
-  const cudaError_t e = raise_smem_limit<second_rows_kernel<DP, WALK>>(Rows<DP>::SMEM);
-  if (e != cudaSuccess) return e;
-  second_rows_kernel<DP, WALK><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Rows<DP>::SMEM, s>>>(
-      p, Streams{w[0], w[1], w[2], w[3]}, w.stats, w.parts, status);
-  return cudaGetLastError();
-}
-
-template <int DP>
-cudaError_t join(const Params<float>& p, char* work, cudaStream_t s) {
-  const Layout<DP> w(p, work);
-  second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H, 4), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
-  return cudaGetLastError();
-}
-
-template <int DP>
-cudaError_t keys(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  const Layout<DP> w(p, work);
-  const cudaError_t e = raise_smem_limit<second_keys_kernel<DP>>(Keys<DP>::SMEM);
-  if (e != cudaSuccess) return e;
-  second_keys_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.HK, p.splits), ROW_THREADS, Keys<DP>::SMEM, s>>>(
-      p, w[1], w[3], Streams{w[4], w[5], w[6], w[6]}, w.stats, status);
+  src.s[5] = {p.ca, p.cas, p.cah, p.H, nullptr, w.at[5]};
+  src.s[6] = {p.go, p.gos, p.goh, p.H, nullptr, w.at[6]};
+  cudaError_t e = write_images<DP>(p, src, 7, w.stats, KINDS, s);
+  constexpr int SMEM = Rows<DP>::SMEM > Keys<DP>::SMEM ? Rows<DP>::SMEM : Keys<DP>::SMEM;
+  if (e != cudaSuccess || (e = raise_smem_limit<second_first_kernel<DP>>(Rows<DP>::SMEM)) != cudaSuccess ||
+      (e = raise_smem_limit<second_last_kernel<DP>>(SMEM)) != cudaSuccess)
+    return e;
+  const int tiles = p.N / 128 + p.num + 2;
+  const Streams k{w[0], w[1], w[2], w[3]}, q{w[4], w[5], w[6], w[6]};
+  second_first_kernel<DP><<<dim3(tiles, p.H, p.splits), ROW_THREADS, Rows<DP>::SMEM, s>>>(p, k, q, w.stats, w.parts, status);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (p.splits > 1) {
+    second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H, 4), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  const int64_t blocks = (int64_t)tiles * (p.HK * p.splits_k + p.H * p.splits);
+  second_last_kernel<DP><<<(unsigned)blocks, ROW_THREADS, SMEM, s>>>(p, k, q, w.stats, w.parts, status);
   return cudaGetLastError();
 }
 
 template <int DP>
 int64_t bytes(const Params<float>& p) {
-  return image_bytes<DP>(p, 4 * p.HK + 3 * p.H) + (int64_t)p.H * image_slots(p) * KINDS * SLOT * 4;
+  return image_bytes<DP>(p, 4 * p.HK + 3 * p.H) + (int64_t)p.H * (image_slots(p) * KINDS * SLOT + 2 * (int64_t)p.splits * p.N) * 4;
 }
 
 }  // namespace
 
-// without the splits' r and c, two numbers a row, head and split, which follow
 int64_t tc_second_bytes(const Params<float>& p) { return p.D <= 32 ? bytes<32>(p) : bytes<64>(p); }
-cudaError_t tc_second_prepare(const Params<float>& p, char* work, cudaStream_t s) {
-  return p.D <= 32 ? prepare<32>(p, work, s) : prepare<64>(p, work, s);
-}
-cudaError_t tc_second_rows(const Params<float>& p, char* work, int walk, int* status, cudaStream_t s) {
-  if (p.D <= 32) return walk == 0 ? rows<32, 0>(p, work, status, s) : rows<32, 1>(p, work, status, s);
-  return walk == 0 ? rows<64, 0>(p, work, status, s) : rows<64, 1>(p, work, status, s);
-}
-cudaError_t tc_second_join(const Params<float>& p, char* work, cudaStream_t s) {
-  return p.D <= 32 ? join<32>(p, work, s) : join<64>(p, work, s);
-}
-cudaError_t tc_second_keys(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  return p.D <= 32 ? keys<32>(p, work, status, s) : keys<64>(p, work, status, s);
+cudaError_t tc_second(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  return p.D <= 32 ? second<32>(p, work, status, s) : second<64>(p, work, status, s);
 }
 
 }  // namespace attn

@@ -25,11 +25,11 @@ struct Wide {
   static_assert(OUT + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
 };
 
+// first, second: images of the owned rows' operands, a, b: of the streamed ones
 template <int DP, int MODE>
-__global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float> p, const Images first, const Images second,
-                                                              const Images a, const Images b, const float* __restrict__ stats,
-                                                              int* status) {
-  // first, second: images of the owned rows' operands (only the second's are read), a, b: of the streamed ones
+__device__ __forceinline__ void wide_block(const Params<float>& p, const Part& part, const Job& job, const Images& first,
+                                           const Images& second, const Images& a, const Images& b, const float* __restrict__ stats,
+                                           int* status) {
   using B = Wide<DP, MODE>;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
@@ -37,13 +37,11 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
            *ready = bars + 9;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 10);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 11);
-  Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
-  const int warp = threadIdx.x / 32, group = p.H / p.HK, own = blockIdx.y;
+  const int warp = threadIdx.x / 32, group = p.H / p.HK, own = job.head;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
-  split_range<SLOT>(lo, hi, blockIdx.z, p.splits);
+  split_range<SLOT>(lo, hi, job.split, job.splits);
   const int tiles = (hi - lo + HALF - 1) / HALF, n = MODE == DQ ? tiles : tiles * group;
-  const int slot0 = first_slot(part) + (lo - part.lo) / SLOT;
+  const int slot0 = first_slot(part) + (lo - part.lo) / SLOT, own_slot = first_slot(part) + (part.row - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) tc::mbar_init(bars + i, 1);
@@ -77,17 +75,14 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
   if (warp == 8 && n > 0) {                             // the copies run while the other warps stage their rows
     if (MODE != DV && elect()) {
       tc::mbar_arrive_expect_tx(full_2, B::SECOND);
-      load_block<DP>(smem, image<DP>(second, own, first_slot(part) + (part.row - part.lo) / SLOT), full_2);
+      load_block<DP>(smem, image<DP>(second, own, own_slot), full_2);
     }
     __syncwarp();
     for (int i = 0; i < loaded_x; ++i) load(i, false);
     for (int i = 0; i < loaded_y; ++i) load(i, true);
   } else if (n > 0) {
-    const int row = part.row + (threadIdx.x & 127);
-    const bool on = row < part.hi && (MODE == DQ || p.mask == nullptr || p.mask[row]);
-    const float* x = MODE == DQ ? p.q + row * p.qs + own * p.qh : p.k + row * p.ks + own * p.kh;
-    const bool vec = MODE == DQ ? vec_ok(p.q, p.qs, p.qh, p.D) : vec_ok(p.k, p.ks, p.kh, p.D);
-    stage_row<DP, DP / 2>(tmem + ((uint32_t)(warp & 3) << 21), x, on, vec, p.D, p.scale * log2e<float>(), warp / 4 * (DP / 2));
+    stage_image<DP, DP / 2>(tmem + ((uint32_t)(warp & 3) << 21), image<DP>(first, own, own_slot), threadIdx.x & 127,
+                            warp / 4 * (DP / 2));
     tmem_st_wait();
     tc::tc_fence_before();
   }
@@ -137,6 +132,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp / 4, row = part.row + (threadIdx.x & 127);
     const bool on = row < part.hi;
+    const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, acc[DP / 2];
     if (MODE == DQ && on && n > 0) {
       const float* at = stats + ((int64_t)own * a.slots + first_slot(part) + (row - part.lo) / SLOT) * 2 * SLOT;
@@ -159,12 +155,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
       arrive(taken);
       if (MODE == DQ) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = (bits >> j) & 1 ? ex2(s[j] - L) * (dp[j] - D) : 0.f;
+        for (int j = 0; j < 16; ++j) s[j] = (bits >> j) & 1 ? ex2(fmaf(s[j], c2, -L)) * (dp[j] - D) : 0.f;
       } else {
         const float* st = reinterpret_cast<const float*>(smem + B::ST + i % 3 * (2 * HALF * 4)) + 16 * half;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          s[j] = ex2(s[j] - st[j]);
+          s[j] = ex2(fmaf(s[j], c2, -st[j]));
           if (MODE == DK) s[j] *= dp[j] - st[HALF + j];
         }
       }
@@ -182,17 +178,15 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
       tc::tc_fence_after();
       add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
     }
-    if (on) {
-      const bool hidden = MODE != DQ && p.mask != nullptr && !p.mask[row];
-      const float g = !ok ? __int_as_float(0x7fc00000) : MODE == DV ? 1.f : p.scale;
+    const bool hidden = MODE != DQ && on && p.mask != nullptr && !p.mask[row];
 #pragma unroll
-      for (int d = 0; d < DP / 2; ++d) acc[d] = hidden ? 0.f : g * acc[d];
-      const int heads = MODE == DQ ? p.H : p.HK;
-      const int64_t all = (int64_t)p.N * heads * p.D, at = ((int64_t)row * heads + own) * p.D;
-      float* out = p.splits > 1 ? p.work + ((MODE == DV ? p.splits : 0) + (int64_t)blockIdx.z) * all + at
-                                : (MODE == DQ ? p.out0 : MODE == DK ? p.out1 : p.out2) + at;
-      store_columns<DP / 2>(out, acc, half * (DP / 2), p.D);
-    }
+    for (int d = 0; d < DP / 2; ++d) acc[d] = hidden ? 0.f : MODE == DV ? acc[d] : p.scale * acc[d];
+    const int heads = MODE == DQ ? p.H : p.HK, row0 = part.row + 32 * (warp & 3);
+    const int64_t all = (int64_t)p.N * heads * p.D;
+    float* out = MODE == DQ ? p.out0 : MODE == DK ? p.out1 : p.out2;
+    if (job.splits > 1) out = (MODE == DQ ? p.work : p.work_k) + ((MODE == DV ? job.splits : 0) + (int64_t)job.split) * all;
+    store_rows<DP / 2>(scratch_of<DP / 2>(smem, warp), acc, out + ((int64_t)row0 * heads + own) * p.D, (int64_t)heads * p.D,
+                       min(32, part.hi - row0), half * (DP / 2), p.D, ok);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -202,27 +196,32 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float
   }
 }
 
-template <int MODE>
-cudaError_t launch_wide(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  constexpr int DP = 128;
-  const int slots = image_slots(p);
-  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
-  const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
-  const cudaError_t e = raise_smem_limit<wide_kernel<DP, MODE>>(Wide<DP, MODE>::SMEM);
-  if (e != cudaSuccess) return e;
-  const Images q{iq, slots}, k{ik, slots}, v{iv, slots}, o{io, slots};
-  const dim3 grid(p.N / 128 + p.num + 2, MODE == DQ ? p.H : p.HK, p.splits);
-  if (MODE == DQ) wide_kernel<DP, MODE><<<grid, ROW_THREADS, Wide<DP, MODE>::SMEM, s>>>(p, q, o, k, v, stats, status);
-  else wide_kernel<DP, MODE><<<grid, ROW_THREADS, Wide<DP, MODE>::SMEM, s>>>(p, k, v, q, o, stats, status);
-  return cudaGetLastError();
+// the three in one launch: the blocks of the keys first
+template <int DP>
+__global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float> p, const Images k, const Images v, const Images q,
+                                                              const Images o, const float* __restrict__ stats, int* status) {
+  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  Part part;
+  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  const Job job{rest % keys % p.HK, rest % keys / p.HK, p.splits_k};
+  if (rest < keys) wide_block<DP, DK>(p, part, job, k, v, q, o, stats, status);
+  else if (rest < 2 * keys) wide_block<DP, DV>(p, part, job, k, v, q, o, stats, status);
+  else wide_block<DP, DQ>(p, part, {(rest - 2 * keys) % p.H, (rest - 2 * keys) / p.H, p.splits}, q, o, k, v, stats, status);
 }
 
 }  // namespace
 
-cudaError_t tc_wide_dq(const Params<float>& p, char* work, int* status, cudaStream_t s) { return launch_wide<DQ>(p, work, status, s); }
-cudaError_t tc_wide_dkv(const Params<float>& p, char* work, int* status, cudaStream_t s) {
-  const cudaError_t e = launch_wide<DK>(p, work, status, s);
-  return e != cudaSuccess ? e : launch_wide<DV>(p, work, status, s);
+cudaError_t tc_wide_backward(const Params<float>& p, char* work, int* status, cudaStream_t s) {
+  constexpr int DP = 128, SMEM = Wide<DP, DQ>::SMEM;     // of the three the first two need most
+  const int slots = image_slots(p);
+  char *ik = work, *iv = ik + image_bytes<DP>(p, p.HK), *iq = iv + image_bytes<DP>(p, p.HK), *io = iq + image_bytes<DP>(p, p.H);
+  const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
+  const cudaError_t e = raise_smem_limit<wide_kernel<DP>>(SMEM);
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = (int64_t)(p.N / 128 + p.num + 2) * (2 * p.HK * p.splits_k + p.H * p.splits);
+  wide_kernel<DP><<<(unsigned)blocks, ROW_THREADS, SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, Images{iq, slots},
+                                                             Images{io, slots}, stats, status);
+  return cudaGetLastError();
 }
 
 }  // namespace attn

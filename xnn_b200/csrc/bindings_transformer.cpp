@@ -190,29 +190,24 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
     const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
     torch::Tensor work, scratch;
     if (sq > 1 || sk > 1) {
-      work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
+      work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
       pl.work = work.data_ptr<T>();
+      pl.work_k = pl.work + (sq > 1 ? sq * nq : 0);
     }
+    pl.splits = sq;
+    pl.splits_k = sk;
     if constexpr (sizeof(T) == 4) {
       scratch = bytes(attn::tc_backward_bytes(pl), q);
-      char* images = static_cast<char*>(scratch.data_ptr());
-      XNN_OK(attn::tc_backward_prepare(pl, images, s));
-      pl.splits = sq;
-      XNN_OK(attn::tc_backward_dq(pl, images, status_of(status, q), s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
-      pl.splits = sk;
-      XNN_OK(attn::tc_backward_dkv(pl, images, status_of(status, q), s));
+      XNN_OK(attn::tc_backward(pl, static_cast<char*>(scratch.data_ptr()), status_of(status, q), s));
     } else {
       scratch = torch::empty({p.H, p.N}, q.options());
       pl.delta = scratch.data_ptr<T>();
       XNN_OK(attn::row_delta<T>(pl, s));
-      pl.splits = sq;
       XNN_OK(attn::backward_dq(pl, s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
-      pl.splits = sk;
       XNN_OK(attn::backward_dkv(pl, s));
     }
-    if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, p.out2, s));
+    if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
+    if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work_k, p.out1, p.out2, s));
   }
   if (plan.short_ones) XNN_OK(attn::backward_short<T>(short_part(p, plan), s));
   return {dq, dk, dv};
@@ -245,20 +240,18 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
       auto pl = long_part(p, plan);
       const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
       const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
-      auto images = bytes(attn::tc_second_bytes(pl) + (int64_t)sq * 2 * p.H * p.N * 4, q);
-      torch::Tensor work = torch::empty({std::max(sq > 1 ? sq * nq : 0, sk > 1 ? 2 * sk * nk : 0)}, q.options());
-      char* im = static_cast<char*>(images.data_ptr());
-      int* flag = status_of(status, q);
-      pl.work = work.data_ptr<T>();
+      torch::Tensor work;
+      if (sq > 1 || sk > 1) {
+        work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
+        pl.work = work.data_ptr<T>();
+        pl.work_k = pl.work + (sq > 1 ? sq * nq : 0);
+      }
       pl.splits = sq;
-      XNN_OK(attn::tc_second_prepare(pl, im, s));
-      XNN_OK(attn::tc_second_rows(pl, im, 0, flag, s));
-      if (sq > 1) XNN_OK(attn::tc_second_join(pl, im, s));
-      XNN_OK(attn::tc_second_rows(pl, im, 1, flag, s));
+      pl.splits_k = sk;
+      auto images = bytes(attn::tc_second_bytes(pl), q);
+      XNN_OK(attn::tc_second(pl, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
       if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
-      pl.splits = sk;
-      XNN_OK(attn::tc_second_keys(pl, im, flag, s));
-      if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work, p.out1, p.out2, s));
+      if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work_k, p.out1, p.out2, s));
       rest = plan.short_ones;
       pr = short_part(p, plan);
     }
