@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
       for (int n = 0; n < C::DP / C::TX; ++n) acc[r][n] *= f;
     }
     __syncthreads();
-    tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sP, i0, sV, tx);
+    tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sP, i0, sV, tx, k_hi - k0);
     __syncthreads();
   }
   const int64_t rows = (int64_t)p.H * p.N;
@@ -360,9 +360,9 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
         }
       }
       __syncthreads();
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dq, sS, i0, sK, tx);
-      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sS, i0, sQ, tx);
-      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dv, sP, i0, sO, tx);
+      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dq, sS, i0, sK, tx, part.hi - part.row);
+      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sS, i0, sQ, tx, part.hi - part.row);
+      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dv, sP, i0, sO, tx, part.hi - part.row);
       __syncthreads();
     }
 #pragma unroll
@@ -578,11 +578,17 @@ cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, 
   return cudaGetLastError();
 }
 
-// The square tiles of 32 rows; double: two rows and columns a thread (four would need 128 registers for the
-// accumulators alone at 128 columns).
+// The square tiles of 32 rows. float: a 2 x 4 corner of the scores a thread (one molecule of 21 atoms at 64 columns:
+// 6.1 us with 128 threads, 9.1 with 64 and 4 x 4 corners; 4000 x 4 heads: 236 and 279 us). double: 2 x 2, since the
+// accumulators of 4 x 4 alone would take 128 registers at 128 columns.
 template <typename T, int DP> struct Small;
-template <int DP> struct Small<float, DP> { using C = Cfg<float, 32, 32, DP, 4, 8>; };
+template <int DP> struct Small<float, DP> { using C = Cfg<float, 32, 32, DP, 2, 8>; };
 template <int DP> struct Small<double, DP> { using C = Cfg<double, 32, 32, DP, 2, 16>; };
+// The short backward pass has five products on a tile and reads less of it with 4 x 4 corners, up to 64 columns (64: 532
+// and 565 us for 4000 x 4 heads; 128: 186 and, with 256 threads, 153 us for 2000).
+template <typename T, int DP> struct Short { using C = typename Small<T, DP>::C; };
+template <int DP> struct Short<float, DP> { using C = Cfg<float, 32, 32, DP, 4, 8>; };
+template <> struct Short<float, 128> { using C = Cfg<float, 32, 32, 128, 2, 16>; };
 // the second derivative holds seven tiles: 128 double columns leave room for 16 streamed rows
 template <typename T, int DP> struct Second { using C = typename Small<T, DP>::C; };
 template <int DP> struct Second<float, DP> { using C = Cfg<float, 32, 64, DP, 2, 16>; };
@@ -624,7 +630,7 @@ cudaError_t backward_dkv(const Params<double>& p, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, bwd_short_kernel<T, C>>(p, p.HK, 2, 2, 2, s)))
+  XNN_ATTN_DIM(p.D, using C = typename Short<T, DP>::C; return (launch<T, C, bwd_short_kernel<T, C>>(p, p.HK, 2, 2, 2, s)))
 }
 template <typename T>
 cudaError_t second_rows(const Params<T>& p, cudaStream_t s) {

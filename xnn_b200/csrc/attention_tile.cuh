@@ -141,13 +141,14 @@ struct Cols {
   static constexpr int NC = PER / VW;
 };
 
-// acc[r][.] += sum_{j < J} P[i0 + r][j] V[j][columns of tx]
+// acc[r][.] += sum_{j < J} P[i0 + r][j] V[j][columns of tx]; from the first `used` on, P is zero
 template <typename T, int RI, int J, int TX, int DP, int LDP, int LD>
-__device__ __forceinline__ void tile_nn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx) {
+__device__ __forceinline__ void tile_nn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx, int used = J) {
   using C = Cols<T, DP, TX>;
   constexpr int W = Vec<T>::W;
+  const int end = used < J ? used : J;
 #pragma unroll 2
-  for (int j = 0; j < J; j += W) {
+  for (int j = 0; j < end; j += W) {
     V16<T> p[RI];
 #pragma unroll
     for (int r = 0; r < RI; ++r) p[r] = *reinterpret_cast<const V16<T>*>(P + (i0 + r) * LDP + j);
@@ -174,11 +175,12 @@ __device__ __forceinline__ void tile_nn(T (&acc)[RI][DP / TX], const T* P, int i
 
 // acc[r][.] += sum_{j < J} P[j][i0 + r] V[j][columns of tx] (P read transposed; RI neighbouring columns)
 template <typename T, int RI, int J, int TX, int DP, int LDP, int LD>
-__device__ __forceinline__ void tile_tn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx) {
+__device__ __forceinline__ void tile_tn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx, int used = J) {
   using C = Cols<T, DP, TX>;
   constexpr int W = Vec<T>::W;
+  const int end = used < J ? used : J;
 #pragma unroll 4
-  for (int j = 0; j < J; ++j) {
+  for (int j = 0; j < end; ++j) {
     T p[RI];
 #pragma unroll
     for (int r = 0; r < RI; r += W) *reinterpret_cast<V16<T>*>(p + r) = *reinterpret_cast<const V16<T>*>(P + j * LDP + i0 + r);
