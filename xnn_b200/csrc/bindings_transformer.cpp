@@ -4,6 +4,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <array>
+#include <cmath>
 #include <limits>
 
 #include "attention.h"
@@ -282,6 +284,16 @@ Tensors attention_forward(const torch::Tensor& q, const torch::Tensor& k, const 
   return r;
 }
 
+Tensors attention_backward(const torch::Tensor& go, const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                           const torch::Tensor& o, const torch::Tensor& lse, const torch::Tensor& ptr,
+                           const c10::optional<torch::Tensor>& mask, int64_t max_len, double scale, const torch::Tensor& status) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensors r;
+  AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward",
+                             [&] { r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale, status); });
+  return r;
+}
+
 torch::Tensor rows(const torch::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
 c10::optional<torch::Tensor> maybe(const torch::Tensor& t) {
@@ -323,12 +335,7 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
     ctx->save_for_backward({go, q, k, v, o, lse, ptr, mask.value_or(Variable())});
     ctx->saved_data["status"] = status;
     keep(ctx, {max_len, scale});
-    const c10::cuda::CUDAGuard guard(q.device());
-    Tensors r;
-    AT_DISPATCH_FLOATING_TYPES(q.scalar_type(), "structure attention backward", [&] {
-      r = backward_typed<scalar_t>(go, q, k, v, o, lse, ptr, mask, max_len, scale, status);
-    });
-    return r;
+    return attention_backward(go, q, k, v, o, lse, ptr, mask, max_len, scale, status);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
@@ -351,6 +358,12 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const auto set = kept(ctx);
+    if (!torch::GradMode::is_enabled()) {              // no graph of this pass is asked for
+      auto r = attention_backward(rows(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), set.max_len, set.scale,
+                                  ctx->saved_data["status"].toTensor());
+      r.resize(8);
+      return r;
+    }
     // o without its graph: the second derivative holds what goes through it
     auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3].detach(), s[4], s[5], maybe(s[6]),
                                   ctx->saved_data["status"].toTensor(), set.max_len, set.scale);
@@ -359,14 +372,44 @@ struct Attention : torch::autograd::Function<Attention> {
   }
 };
 
+// The arguments are checked here, not in Python: for the smallest structures the call costs more than its kernel.
+template <typename... A>
+void require(bool ok, const A&... what) {
+  if (!ok) throw pybind11::value_error(c10::str(what...));
+}
+template <typename... A>
+void require_type(bool ok, const A&... what) {
+  if (!ok) throw pybind11::type_error(c10::str(what...));
+}
+bool floating(const torch::Tensor& t) { return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kFloat64; }
+
 torch::Tensor structure_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor ptr,
-                                  c10::optional<torch::Tensor> mask, int64_t max_len, double scale, torch::Tensor status) {
+                                  c10::optional<int64_t> max_len, c10::optional<double> scale, c10::optional<torch::Tensor> mask,
+                                  const torch::Tensor& status) {
+  require(q.dim() == 3, "q must be (atoms, heads, width), got ", q.sizes());
+  require(k.dim() == 3 && v.dim() == 3, "k and v must be (atoms, key heads, width), got ", k.sizes(), " and ", v.sizes());
+  require_type(floating(q) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                   v.device() == q.device(),
+               "q, k and v must all be float32 or all float64 on one device, got ", q.scalar_type(), ", ", k.scalar_type(), " and ",
+               v.scalar_type());
+  const int64_t n = q.size(0), h = q.size(1), d = q.size(2);
+  require(k.size(0) == n && k.size(2) == d && v.sizes() == k.sizes(), "k and v must be (", n, ", key heads, ", d, "), got ", k.sizes(),
+          " and ", v.sizes());
+  require(h > 0 && d > 0 && k.size(1) > 0 && h % k.size(1) == 0, "the ", k.size(1), " key heads must divide the ", h, " query heads");
+  require(ptr.dim() == 1 && ptr.numel() >= 1 && ptr.scalar_type() == torch::kInt64 && ptr.device() == q.device(),
+          "ptr must be int64 (structures + 1) on ", q.device(), ", got ", ptr.scalar_type(), " ", ptr.sizes(), " on ", ptr.device());
+  require(!mask.has_value() || (mask->scalar_type() == torch::kBool && mask->dim() == 1 && mask->size(0) == n && mask->device() == q.device()),
+          "key_mask must be bool (", n, ") on ", q.device());
+  require(max_len.value_or(0) >= 0, "max_len must not be negative, got ", max_len.value_or(0));
+  require(d <= 128, "head width ", d, ": the kernels take up to 128");
+  const int64_t most = max_len.value_or(n);
+  const double f = scale.value_or(1.0 / std::sqrt((double)d));
   q = rows(q); k = rows(k); v = rows(v);
   ptr = ptr.contiguous();
   if (mask.has_value()) mask = mask->contiguous();
   if (torch::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
-    return Attention::apply(q, k, v, ptr, mask, status, max_len, scale);
-  return attention_forward(q, k, v, ptr, mask, max_len, scale, false, status)[0];
+    return Attention::apply(q, k, v, ptr, mask, status, most, f);
+  return attention_forward(q, k, v, ptr, mask, most, f, false, status)[0];
 }
 
 // x (outer, shared, inner) contiguous; rng int64 (seed, offset) on x's device
@@ -396,16 +439,47 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto n = ctx->saved_data["sizes"].toIntVector();
+    if (!torch::GradMode::is_enabled())
+      return {dropout_raw(g[0].contiguous(), n[0], n[1], n[2], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]),
+              Variable(), Variable(), Variable(), Variable(), Variable()};
     return {Dropout::apply(g[0].contiguous(), ctx->get_saved_variables()[0], n[0], n[1], n[2], ctx->saved_data["p"].toDouble()),
             Variable(), Variable(), Variable(), Variable(), Variable()};
   }
 };
 
-torch::Tensor dropout_op(torch::Tensor x, int64_t outer, int64_t shared, int64_t inner, double p, torch::Tensor rng) {
+// the sizes in front of, in and behind the dimensions that share a mask entry
+std::array<int64_t, 3> shared_sizes(const torch::Tensor& x, const std::vector<int64_t>& shared) {
+  std::array<int64_t, 3> n{1, 1, 1};
+  if (shared.empty()) return {x.numel(), 1, 1};
+  uint64_t set = 0;
+  for (const int64_t s : shared) {
+    require(s >= -x.dim() && s < x.dim() && x.dim() <= 64, "shared dimension ", s, " of a tensor with ", x.dim(), " dimensions");
+    set |= 1ull << (s < 0 ? s + x.dim() : s);
+  }
+  int stage = 0;
+  for (int64_t i = 0; i < x.dim(); ++i) {
+    if (x.size(i) == 1) continue;
+    if (set >> i & 1) {
+      require(stage < 2, "the shared dimensions ", shared, " of shape ", x.sizes(), " must be neighbours");
+      stage = 1;
+    } else if (stage == 1) {
+      stage = 2;
+    }
+    n[stage] *= x.size(i);
+  }
+  return n;
+}
+
+torch::Tensor dropout_op(torch::Tensor x, double p, torch::Tensor rng, const std::vector<int64_t>& shared) {
+  require_type(floating(x), "counter_dropout takes float32 or float64, got ", x.scalar_type());
+  require(p >= 0.0 && p <= 1.0, "the dropout probability must be in [0, 1], got ", p);
+  require(rng.scalar_type() == torch::kInt64 && rng.dim() == 1 && rng.size(0) == 2 && rng.device() == x.device(),
+          "rng must be two int64 numbers (seed, offset) on ", x.device());
+  const auto n = shared_sizes(x, shared);
   x = x.contiguous();
   rng = rng.contiguous();
-  if (torch::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, rng, outer, shared, inner, p);
-  return dropout_raw(x, outer, shared, inner, p, rng);
+  if (torch::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, rng, n[0], n[1], n[2], p);
+  return dropout_raw(x, n[0], n[1], n[2], p, rng);
 }
 
 void check_ids(const torch::Tensor& ids, const torch::Tensor& like) {
@@ -472,6 +546,9 @@ struct Lookup : torch::autograd::Function<Lookup> {
     return lookup_raw(table, ids, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!torch::GradMode::is_enabled())
+      return {lookup_grad_raw(ctx->get_saved_variables()[0], g[0].contiguous(), ctx->saved_data["rows"].toInt(),
+                              ctx->saved_data["scale"].toDouble()), Variable(), Variable()};
     return {LookupGrad::apply(g[0].contiguous(), ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
                               ctx->saved_data["scale"].toDouble()), Variable(), Variable()};
   }
@@ -487,6 +564,11 @@ variable_list LookupGrad::backward(AutogradContext* ctx, variable_list t) {
 }
 
 torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
+  require_type(table.dim() == 2 && floating(table), "table must be (rows, width) float32 or float64, got ", table.scalar_type(), " ",
+               table.sizes());
+  require_type(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ",
+               ids.scalar_type());
+  require(ids.device() == table.device(), "table on ", table.device(), ", ids on ", ids.device());
   table = table.contiguous();
   ids = ids.contiguous();
   if (torch::GradMode::is_enabled() && table.requires_grad()) return Lookup::apply(table, ids, scale);

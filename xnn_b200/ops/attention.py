@@ -27,15 +27,20 @@ from torch import Tensor
 from .. import _ext
 from .gemm import _status
 
-MAX_WIDTH = 128
 _TYPES = (torch.float32, torch.float64)
 
 
-def _kernels():
-    mod = _ext.ops()
-    if not hasattr(mod, "structure_attention"):
-        raise RuntimeError("xnn_b200 extension without the attention kernels: rebuild it (xnn_b200.build)")
-    return mod
+_KERNEL = None
+
+
+def _kernel():
+    global _KERNEL
+    if _KERNEL is None:
+        mod = _ext.ops()
+        if not hasattr(mod, "structure_attention"):
+            raise RuntimeError("xnn_b200 extension without the attention kernels: rebuild it (xnn_b200.build)")
+        _KERNEL = mod.structure_attention
+    return _KERNEL
 
 
 def _formula(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, mask: Optional[Tensor], scale: float) -> Tensor:
@@ -74,6 +79,8 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, max_len: O
     (``N`` when omitted; a smaller bound lets short structures take the kernels made for them; where it
     is exceeded, gradients are NaN). ``scale``: ``D ** -0.5`` when omitted. ``key_mask``: bool ``(N)``, false
     for atoms that nobody attends to. Differentiable twice on CUDA, to any order on the CPU."""
+    if q.is_cuda:                                # the arguments are checked there
+        return _kernel()(q, k, v, ptr, max_len, scale, key_mask, _status(q.device))
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"{name} must be (atoms, heads, width), got {tuple(t.shape)}")
@@ -94,12 +101,8 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, max_len: O
     if max_len < 0:
         raise ValueError(f"max_len must not be negative, got {max_len}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not q.is_cuda:
-        if int(ptr[0]) < 0 or int(ptr[-1]) > n or bool((ptr[1:] < ptr[:-1]).any()):
-            raise ValueError(f"ptr must ascend within 0 .. {n}")
-        if ptr.numel() > 1 and int((ptr[1:] - ptr[:-1]).max()) > max_len:
-            raise ValueError(f"a structure has more than max_len={max_len} atoms")
-        return _formula(q, k, v, ptr, key_mask, scale)
-    if d > MAX_WIDTH:
-        raise ValueError(f"head width {d}: the kernels take up to {MAX_WIDTH}")
-    return _kernels().structure_attention(q, k, v, ptr, key_mask, max_len, scale, _status(q.device))
+    if int(ptr[0]) < 0 or int(ptr[-1]) > n or bool((ptr[1:] < ptr[:-1]).any()):
+        raise ValueError(f"ptr must ascend within 0 .. {n}")
+    if ptr.numel() > 1 and int((ptr[1:] - ptr[:-1]).max()) > max_len:
+        raise ValueError(f"a structure has more than max_len={max_len} atoms")
+    return _formula(q, k, v, ptr, key_mask, scale)

@@ -83,11 +83,17 @@ class _Dropout(Function):
         return _Dropout.apply(g, ctx.p, ctx.saved_tensors[0], ctx.sizes), None, None, None
 
 
-def _kernels():
-    mod = _ext.ops()
-    if not hasattr(mod, "counter_dropout"):
-        raise RuntimeError("xnn_b200 extension without the dropout kernel: rebuild it (xnn_b200.build)")
-    return mod
+_KERNEL = None
+
+
+def _kernel():
+    global _KERNEL
+    if _KERNEL is None:
+        mod = _ext.ops()
+        if not hasattr(mod, "counter_dropout"):
+            raise RuntimeError("xnn_b200 extension without the dropout kernel: rebuild it (xnn_b200.build)")
+        _KERNEL = mod.counter_dropout
+    return _KERNEL
 
 
 def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -> Tensor:
@@ -95,6 +101,10 @@ def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -
     order. ``rng = (seed, offset)``: two integers, or an int64 tensor of them on ``x``'s device (it is read
     when the kernels run, and again in the backward pass: advance a copy, not the tensor itself).
     ``shared``: neighbouring dimensions over which the mask is the same."""
+    if not isinstance(rng, Tensor):
+        rng = torch.tensor([int(rng[0]), int(rng[1])], dtype=torch.int64, device=x.device)
+    if x.is_cuda:                                # the arguments are checked there
+        return _kernel()(x, p, rng, shared)
     if x.dtype not in (torch.float32, torch.float64):
         raise TypeError(f"counter_dropout takes float32 or float64, got {x.dtype}")
     p = float(p)
@@ -102,16 +112,10 @@ def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -
         raise ValueError(f"the dropout probability must be in [0, 1], got {p}")
     if any(not -x.dim() <= int(d) < x.dim() for d in shared):
         raise ValueError(f"shared dimensions {tuple(shared)} of a tensor with {x.dim()} dimensions")
-    if not isinstance(rng, Tensor):
-        rng = torch.tensor([int(rng[0]), int(rng[1])], dtype=torch.int64, device=x.device)
-    elif rng.dtype != torch.int64 or rng.shape != (2,) or rng.device != x.device:
+    if rng.dtype != torch.int64 or rng.shape != (2,) or rng.device != x.device:
         raise ValueError(f"rng must be two int64 numbers (seed, offset) on {x.device}")
     sizes = _split(x.shape, tuple(int(d) % x.dim() for d in shared))
-    if 0 in x.shape:
-        return x.clone()
-    if x.is_cuda:
-        return _kernels().counter_dropout(x, *sizes, p, rng)
-    return _Dropout.apply(x, p, rng, sizes)
+    return x.clone() if 0 in x.shape else _Dropout.apply(x, p, rng, sizes)
 
 
 class CounterDropout(nn.Module):

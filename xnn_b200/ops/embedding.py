@@ -15,11 +15,17 @@ from torch.autograd import Function
 from .. import _ext
 
 
-def _kernels():
-    mod = _ext.ops()
-    if not hasattr(mod, "embedding_lookup"):
-        raise RuntimeError("xnn_b200 extension without the lookup kernels: rebuild it (xnn_b200.build)")
-    return mod
+_KERNEL = None
+
+
+def _kernel():
+    global _KERNEL
+    if _KERNEL is None:
+        mod = _ext.ops()
+        if not hasattr(mod, "embedding_lookup"):
+            raise RuntimeError("xnn_b200 extension without the lookup kernels: rebuild it (xnn_b200.build)")
+        _KERNEL = mod.embedding_lookup
+    return _KERNEL
 
 
 class _Lookup(Function):
@@ -52,14 +58,14 @@ class _LookupGrad(Function):
 
 def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0) -> Tensor:
     """``scale * table[ids]``, ``(*ids.shape, width)``, with zero rows for ids outside ``0 .. rows - 1``."""
+    if table.is_cuda:                            # the arguments are checked there
+        return _kernel()(table, ids, scale)
     if table.dim() != 2 or table.dtype not in (torch.float32, torch.float64):
         raise TypeError(f"table must be (rows, width) float32 or float64, got {table.dtype} {tuple(table.shape)}")
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"ids must be int64 or int32, got {ids.dtype}")
     if ids.device != table.device:
         raise ValueError(f"table on {table.device}, ids on {ids.device}")
-    if table.is_cuda:
-        return _kernels().embedding_lookup(table, ids, float(scale))
     return _Lookup.apply(table, ids, float(scale))
 
 
