@@ -216,6 +216,24 @@ def test_strides(dtype, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("lens", [[33] + [2] * 40, [3] * 500 + [1000] + [1] * 300 + [33, 34, 0, 64, 65, 32, 128, 129], [4] * 90 + [70, 0, 63]])
+@pytest.mark.parametrize("before", [0, 5, 70])
+def test_few_long_among_many_short(dtype, lens, before):
+    """Both classes in one batch, with rows in front of the first structure and behind the last."""
+    h, d, behind = 2, 16, 40
+    n = before + sum(lens) + behind
+    ptr = torch.tensor([before] + lens).cumsum(0).cuda()
+    g = torch.Generator("cuda").manual_seed(2)
+    q, k, v, do, a, b, c = (torch.randn(n, h, d, generator=g, device="cuda", dtype=dtype) for _ in range(7))
+    got = _all(lambda *t: structure_attention(*t, ptr, max_len=max(lens)), q, k, v, do, a, b, c)
+    inner = slice(before, n - behind)
+    want = _all(lambda *t: _definition(*t, ptr - before, None, d ** -0.5), *(t[inner].double() for t in (q, k, v, do, a, b, c)))
+    _check([x[inner] for x in got], want, dtype, COUNTS)
+    assert not any(x[:before].any() or x[n - behind:].any() for x in got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[12, 30], [40, 600], [500, 900]])
 def test_wrong_bound_is_loud_or_right(lens):
     """A structure longer than ``max_len``: its gradients are right or NaN, the others' are right."""

@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
   T* sV = sK + C::BK * C::LD;
   T* sP = sV + C::BK * C::LD;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const T *gq = p.q + h * p.qh, *gk = p.k + hk * p.kh, *gv = p.v + hk * p.vh;
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(C::NT) dq_kernel(const Params<T> p) {
   T* sV = sK + C::BK * C::LD;
   T* sP = sV + C::BK * C::LD;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const T *gk = p.k + hk * p.kh, *gv = p.v + hk * p.vh;
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(C::NT) dkv_kernel(const Params<T> p) {
   T* sP = sO + C::BK * C::LD;
   T* sS = sP + C::BQ * C::LDP;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int hk = blockIdx.y, group = p.H / p.HK;
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const bool vq = vec_ok(p.q, p.qs, p.qh, p.D), vo = vec_ok(p.go, p.gos, p.goh, p.D);
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
   T* sP = sO + C::BK * C::LD;
   T* sS = sP + C::BQ * C::LDP;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int hk = blockIdx.y, group = p.H / p.HK;
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const T c2 = p.scale * log2e<T>();
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(C::NT) second_row_kernel(const Params<T> p) {
   T* sP = sC + C::BK * C::LD;
   T* sS = sP + C::BQ * C::LDP;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(C::NT) second_key_kernel(const Params<T> p) {
   T* sS = sM + C::BQ * C::LDP;
   T* sT = sS + C::BQ * C::LDP;
   Part part;
-  if (!find_part<C::BQ>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
   const int hk = blockIdx.y, group = p.H / p.HK;
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
@@ -573,7 +573,7 @@ cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, 
                                     (size_t)squares * C::BQ * C::LDP);
   const cudaError_t e = raise_smem_limit<KERNEL>(bytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.N / C::BQ + p.num + 2, heads, splits);
+  const dim3 grid(part_blocks(p, C::BQ), heads, splits);
   KERNEL<<<grid, C::NT, bytes, s>>>(p);
   return cudaGetLastError();
 }

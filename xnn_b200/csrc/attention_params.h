@@ -20,6 +20,8 @@ struct Params {
   T scale;
   int N, num, H, HK, D, splits, splits_k;
   int min_len, max_len;              // the lengths that this launch takes (others return at once)
+  int rest;                          // whether it takes the rows of no structure too
+  int compact;                       // only structures of more than 32 atoms, blocks numbered by windows of 32 rows
 };
 
 }  // namespace attn

@@ -54,14 +54,15 @@ __global__ void __launch_bounds__(256) image_kernel(const Params<float> p, const
   const Source s = src.s[rows ? 0 : blockIdx.z];
   if (!rows && (int)blockIdx.y >= s.heads) return;
   Part part;
-  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part) || !part.keys) return;
+  if (!find_part<SLOT>(p, blockIdx.x, part) || !part.keys) return;
+  const int64_t slot = (int64_t)blockIdx.y * slots + first_slot(p, part) + (part.row - part.lo) / SLOT;
   if (rows) {
-    slot_stats(p, part, blockIdx.y, stats + ((int64_t)blockIdx.y * slots + blockIdx.x) * kinds * SLOT);
+    slot_stats(p, part, blockIdx.y, stats + slot * kinds * SLOT);
     return;
   }
   const float* g = s.at + blockIdx.y * s.head;
   const bool vec = vec_ok(s.at, s.row, s.head, p.D);
-  uint4* out = reinterpret_cast<uint4*>(s.out + ((int64_t)blockIdx.y * slots + blockIdx.x) * Image<DP>::BYTES);
+  uint4* out = reinterpret_cast<uint4*>(s.out + slot * Image<DP>::BYTES);
 #pragma unroll 2
   for (int i = threadIdx.x; i < SLOT * DP / 8; i += 256) {
     const int r = i / DP * 8 + i % 8, c = i / 8 % (DP / 8) * 8, row = part.row + r;
@@ -111,12 +112,12 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 8);
   float* tops = reinterpret_cast<float*>(smem + F::TOPS);
   Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<128>(p, blockIdx.x, part)) return;
   const int tid = threadIdx.x, warp = tid / 32;
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(k_lo, k_hi, blockIdx.z, p.splits);
-  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
+  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(p, part) + (k_lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(tmem_slot, F::COLUMNS);
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) tc::mbar_init(bars + i, 1);
@@ -367,7 +368,7 @@ __device__ __forceinline__ void dq_block(const Params<float>& p, const Part& par
   const int h = job.head, hk = h / (p.H / p.HK);
   int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(k_lo, k_hi, job.split, job.splits);
-  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(part) + (k_lo - part.lo) / SLOT;
+  const int n = (k_hi - k_lo + SLOT - 1) / SLOT, slot0 = first_slot(p, part) + (k_lo - part.lo) / SLOT;
   const Block k = set_up<DP>(smem);
   const auto load = [&](int i) {
     if (elect()) {
@@ -381,7 +382,7 @@ __device__ __forceinline__ void dq_block(const Params<float>& p, const Part& par
   if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    const int own = first_slot(part) + (part.row - part.lo) / SLOT;
+    const int own = first_slot(p, part) + (part.row - part.lo) / SLOT;
     stage_rows<DP>(k, image<DP>(iq, h, own), image<DP>(io, h, own));
   }
   __syncthreads();
@@ -427,7 +428,7 @@ __device__ __forceinline__ void dq_block(const Params<float>& p, const Part& par
     const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, acc[DP / 2];
     if (on && n > 0) {
-      const float* at = stats + ((int64_t)h * ik.slots + first_slot(part) + (row - part.lo) / SLOT) * 2 * SLOT;
+      const float* at = stats + ((int64_t)h * ik.slots + first_slot(p, part) + (row - part.lo) / SLOT) * 2 * SLOT;
       L = at[(row - part.lo) % SLOT];
       D = at[SLOT + (row - part.lo) % SLOT];
     }
@@ -493,7 +494,7 @@ __device__ __forceinline__ void dkv_block(const Params<float>& p, const Part& pa
   const int hk = job.head, group = p.H / p.HK;
   int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(q_lo, q_hi, job.split, job.splits);
-  const int tiles = (q_hi - q_lo + SLOT - 1) / SLOT, n = tiles * group, slot0 = first_slot(part) + (q_lo - part.lo) / SLOT;
+  const int tiles = (q_hi - q_lo + SLOT - 1) / SLOT, n = tiles * group, slot0 = first_slot(p, part) + (q_lo - part.lo) / SLOT;
   const Block k = set_up<DP>(smem);
   const auto load = [&](int i) {
     if (elect()) {
@@ -510,7 +511,7 @@ __device__ __forceinline__ void dkv_block(const Params<float>& p, const Part& pa
   if (k.warp == 8) {                                    // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    const int own = first_slot(part) + (part.row - part.lo) / SLOT;
+    const int own = first_slot(p, part) + (part.row - part.lo) / SLOT;
     stage_rows<DP>(k, image<DP>(ik, hk, own), image<DP>(iv, hk, own));
   }
   __syncthreads();
@@ -622,9 +623,9 @@ __device__ __forceinline__ void dkv_block(const Params<float>& p, const Part& pa
 template <int DP>
 __global__ void __launch_bounds__(ROW_THREADS, 1) tc_bwd_kernel(const Params<float> p, const Images ik, const Images iv, const Images iq,
                                                                 const Images io, const float* __restrict__ stats, int* status) {
-  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  const int tiles = part_blocks(p, 128), rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
   Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  if (!find_part<128>(p, blockIdx.x % tiles, part)) return;
   if (rest < keys) dkv_block<DP>(p, part, {rest % p.HK, rest / p.HK, p.splits_k}, ik, iv, iq, io, stats, status);
   else dq_block<DP>(p, part, {(rest - keys) % p.H, (rest - keys) / p.H, p.splits}, ik, iv, iq, io, stats, status);
 }
@@ -639,7 +640,7 @@ cudaError_t forward_dp(const Params<float>& p, char* work, int* status, cudaStre
   cudaError_t e = write_images<DP>(p, src, 2, nullptr, 0, s);
   if (e != cudaSuccess) return e;
   if ((e = raise_smem_limit<tc_fwd_kernel<DP>>(Fwd<DP>::SMEM)) != cudaSuccess) return e;
-  tc_fwd_kernel<DP><<<dim3(p.N / 128 + p.num + 2, p.H, p.splits), ROW_THREADS, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
+  tc_fwd_kernel<DP><<<dim3(part_blocks(p, 128), p.H, p.splits), ROW_THREADS, Fwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, status);
   return cudaGetLastError();
 }
 
@@ -662,7 +663,7 @@ cudaError_t backward_dp(const Params<float>& p, char* work, int* status, cudaStr
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
   const cudaError_t e = raise_smem_limit<tc_bwd_kernel<DP>>(Bwd<DP>::SMEM);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = (int64_t)(p.N / 128 + p.num + 2) * (p.HK * p.splits_k + p.H * p.splits);
+  const int64_t blocks = (int64_t)(part_blocks(p, 128)) * (p.HK * p.splits_k + p.H * p.splits);
   tc_bwd_kernel<DP><<<(unsigned)blocks, ROW_THREADS, Bwd<DP>::SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, Images{iq, slots},
                                                                         Images{io, slots}, stats, status);
   return cudaGetLastError();
@@ -672,7 +673,7 @@ cudaError_t backward_dp(const Params<float>& p, char* work, int* status, cudaStr
 
 template <int DP>
 cudaError_t write_images(const Params<float>& p, const Sources& src, int count, float* stats, int kinds, cudaStream_t s) {
-  const dim3 grid(p.N / SLOT + p.num + 2, p.H, count + (stats != nullptr));
+  const dim3 grid(part_blocks(p, SLOT), p.H, count + (stats != nullptr));
   image_kernel<DP><<<grid, 256, 0, s>>>(p, src, count, image_slots(p), stats, kinds);
   return cudaGetLastError();
 }

@@ -33,7 +33,9 @@ __device__ __forceinline__ const char* image(const Images& im, int head, int slo
 }
 
 // the slot of a part's first rows (parts start at slots as they do at tiles of SLOT rows)
-__device__ __forceinline__ int first_slot(const Part& part) { return part.lo / SLOT + part.index; }
+__device__ __forceinline__ int first_slot(const Params<float>& p, const Part& part) {
+  return p.compact ? part.lo / 32 : part.lo / SLOT + part.index;
+}
 
 // two float32 in a register pair: one instruction adds, multiplies or fuses both
 struct Two { uint64_t v; };
@@ -406,7 +408,7 @@ struct Source { const float* at; int64_t row, head; int heads; const uint8_t* ma
 constexpr int MAX_SOURCES = 7;
 struct Sources { Source s[MAX_SOURCES]; };
 
-inline int image_slots(const Params<float>& p) { return p.N / SLOT + p.num + 3; }   // the last: read behind the end by load_block
+inline int image_slots(const Params<float>& p) { return part_blocks(p, SLOT) + 1; }   // the last: read behind the end by load_block
 template <int DP> int64_t image_bytes(const Params<float>& p, int heads) { return (int64_t)heads * image_slots(p) * Image<DP>::BYTES; }
 // the images of `count` tensors and, with `stats`, L and D (and room for more) of the rows of each slot: `kinds` x SLOT
 // numbers a (head, slot)

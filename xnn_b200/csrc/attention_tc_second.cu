@@ -42,7 +42,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   const int warp = threadIdx.x / 32, h = job.head, hk = h / (p.H / p.HK);
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(lo, hi, job.split, job.splits);
-  const int n = (hi - lo + HALF - 1) / HALF, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
+  const int n = (hi - lo + HALF - 1) / HALF, slot0 = first_slot(p, part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) tc::mbar_init(bars + i, 1);
@@ -71,7 +71,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   if (warp == 8) {                                      // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
-    const int mine = first_slot(part) + (part.row - part.lo) / SLOT;   // own: q, A and do
+    const int mine = first_slot(p, part) + (part.row - part.lo) / SLOT;   // own: q, A and do
     if (half == 0) {
       stage_image<DP>(lanes, image<DP>(own.a, h, mine), threadIdx.x & 127);
     } else {
@@ -125,7 +125,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
     const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, r = 0.f, c = 0.f;
     if (on && n > 0) {
-      const float* at = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
+      const float* at = stats + ((int64_t)h * im.a.slots + first_slot(p, part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
       L = at[0];
       D = at[SLOT];
       if (WALK == 1) { r = at[2 * SLOT]; c = at[3 * SLOT]; }
@@ -184,7 +184,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
           parts[(2 * (int64_t)job.split + 1) * rows + at] = U;
         }
       } else if (part.keys && row < slots_end(part)) {  // nothing to join: r, c and do' at once, zeros behind the last row
-        float* st = stats + ((int64_t)h * im.a.slots + first_slot(part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
+        float* st = stats + ((int64_t)h * im.a.slots + first_slot(p, part) + (row - part.lo) / SLOT) * KINDS * SLOT + (row - part.lo) % SLOT;
         if (half == 0) {
           st[2 * SLOT] = on ? R : 0.f;
           st[3 * SLOT] = on ? U - st[SLOT] * R : 0.f;
@@ -215,10 +215,10 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
 __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p, float* __restrict__ stats,
                                                           const float* __restrict__ parts, int slots) {
   Part part;
-  if (!find_part<SLOT>(p.ptr, p.num, p.N, blockIdx.x, part)) return;
+  if (!find_part<SLOT>(p, blockIdx.x, part)) return;
   const int h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t rows = (int64_t)p.H * p.N;
-  float* st = stats + ((int64_t)h * slots + blockIdx.x) * KINDS * SLOT;
+  float* st = stats + ((int64_t)h * slots + first_slot(p, part) + (part.row - part.lo) / SLOT) * KINDS * SLOT;
 #pragma unroll
   for (int i = blockIdx.z * 16 + warp; i < (int)blockIdx.z * 16 + 16; i += 8) {
     const int row = part.row + i;
@@ -269,8 +269,8 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   const int warp = threadIdx.x / 32, hk = job.head, group = p.H / p.HK;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(lo, hi, job.split, job.splits);
-  const int mine = first_slot(part) + (part.row - part.lo) / SLOT;     // own: k, v, B, C
-  const int tiles = (hi - lo + HALF - 1) / HALF, n = tiles * group, slot0 = first_slot(part) + (lo - part.lo) / SLOT;
+  const int mine = first_slot(p, part) + (part.row - part.lo) / SLOT;     // own: k, v, B, C
+  const int tiles = (hi - lo + HALF - 1) / HALF, n = tiles * group, slot0 = first_slot(p, part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
@@ -406,7 +406,7 @@ template <int DP>
 __global__ void __launch_bounds__(ROW_THREADS, 1) second_first_kernel(const Params<float> p, const Streams k, const Streams q,
                                                                       float* __restrict__ stats, float* __restrict__ parts, int* status) {
   Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x, part) || !takes(p, part)) return;
+  if (!find_part<128>(p, blockIdx.x, part)) return;
   rows_block<DP, 0>(p, part, {(int)blockIdx.y, (int)blockIdx.z, p.splits}, k, q, stats, parts, status);
 }
 
@@ -414,9 +414,9 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) second_first_kernel(const Para
 template <int DP>
 __global__ void __launch_bounds__(ROW_THREADS, 1) second_last_kernel(const Params<float> p, const Streams k, const Streams q,
                                                                      float* __restrict__ stats, float* __restrict__ parts, int* status) {
-  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  const int tiles = part_blocks(p, 128), rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
   Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  if (!find_part<128>(p, blockIdx.x % tiles, part)) return;
   if (rest < keys) keys_block<DP>(p, part, {rest % p.HK, rest / p.HK, p.splits_k}, k, {q.a, q.c, q.b, q.b}, stats, status);
   else rows_block<DP, 1>(p, part, {(rest - keys) % p.H, (rest - keys) / p.H, p.splits}, k, q, stats, parts, status);
 }
@@ -454,12 +454,12 @@ cudaError_t second(const Params<float>& p, char* work, int* status, cudaStream_t
   if (e != cudaSuccess || (e = raise_smem_limit<second_first_kernel<DP>>(Rows<DP>::SMEM)) != cudaSuccess ||
       (e = raise_smem_limit<second_last_kernel<DP>>(SMEM)) != cudaSuccess)
     return e;
-  const int tiles = p.N / 128 + p.num + 2;
+  const int tiles = part_blocks(p, 128);
   const Streams k{w[0], w[1], w[2], w[3]}, q{w[4], w[5], w[6], w[6]};
   second_first_kernel<DP><<<dim3(tiles, p.H, p.splits), ROW_THREADS, Rows<DP>::SMEM, s>>>(p, k, q, w.stats, w.parts, status);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (p.splits > 1) {
-    second_join_kernel<<<dim3(p.N / SLOT + p.num + 2, p.H, 4), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
+    second_join_kernel<<<dim3(part_blocks(p, SLOT), p.H, 4), 256, 0, s>>>(p, w.stats, w.parts, w.slots);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   const int64_t blocks = (int64_t)tiles * (p.HK * p.splits_k + p.H * p.splits);

@@ -41,7 +41,7 @@ __device__ __forceinline__ void wide_block(const Params<float>& p, const Part& p
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
   split_range<SLOT>(lo, hi, job.split, job.splits);
   const int tiles = (hi - lo + HALF - 1) / HALF, n = MODE == DQ ? tiles : tiles * group;
-  const int slot0 = first_slot(part) + (lo - part.lo) / SLOT, own_slot = first_slot(part) + (part.row - part.lo) / SLOT;
+  const int slot0 = first_slot(p, part) + (lo - part.lo) / SLOT, own_slot = first_slot(p, part) + (part.row - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 8; ++i) tc::mbar_init(bars + i, 1);
@@ -135,7 +135,7 @@ __device__ __forceinline__ void wide_block(const Params<float>& p, const Part& p
     const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, acc[DP / 2];
     if (MODE == DQ && on && n > 0) {
-      const float* at = stats + ((int64_t)own * a.slots + first_slot(part) + (row - part.lo) / SLOT) * 2 * SLOT;
+      const float* at = stats + ((int64_t)own * a.slots + first_slot(p, part) + (row - part.lo) / SLOT) * 2 * SLOT;
       L = at[(row - part.lo) % SLOT];
       D = at[SLOT + (row - part.lo) % SLOT];
     }
@@ -200,9 +200,9 @@ __device__ __forceinline__ void wide_block(const Params<float>& p, const Part& p
 template <int DP>
 __global__ void __launch_bounds__(ROW_THREADS, 1) wide_kernel(const Params<float> p, const Images k, const Images v, const Images q,
                                                               const Images o, const float* __restrict__ stats, int* status) {
-  const int tiles = p.N / 128 + p.num + 2, rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
+  const int tiles = part_blocks(p, 128), rest = blockIdx.x / tiles, keys = p.HK * p.splits_k;
   Part part;
-  if (!find_part<128>(p.ptr, p.num, p.N, blockIdx.x % tiles, part) || !takes(p, part)) return;
+  if (!find_part<128>(p, blockIdx.x % tiles, part)) return;
   const Job job{rest % keys % p.HK, rest % keys / p.HK, p.splits_k};
   if (rest < keys) wide_block<DP, DK>(p, part, job, k, v, q, o, stats, status);
   else if (rest < 2 * keys) wide_block<DP, DV>(p, part, job, k, v, q, o, stats, status);
@@ -218,7 +218,7 @@ cudaError_t tc_wide_backward(const Params<float>& p, char* work, int* status, cu
   const float* stats = reinterpret_cast<const float*>(io + image_bytes<DP>(p, p.H));
   const cudaError_t e = raise_smem_limit<wide_kernel<DP>>(SMEM);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = (int64_t)(p.N / 128 + p.num + 2) * (2 * p.HK * p.splits_k + p.H * p.splits);
+  const int64_t blocks = (int64_t)(part_blocks(p, 128)) * (2 * p.HK * p.splits_k + p.H * p.splits);
   wide_kernel<DP><<<(unsigned)blocks, ROW_THREADS, SMEM, s>>>(p, Images{ik, slots}, Images{iv, slots}, Images{iq, slots},
                                                              Images{io, slots}, stats, status);
   return cudaGetLastError();

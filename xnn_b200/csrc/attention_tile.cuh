@@ -26,38 +26,50 @@ __device__ __forceinline__ int part_bound(const int64_t* ptr, int num, int N, in
   return (int)(v < 0 ? 0 : (v > N ? N : v));
 }
 
-// the part and first row of tile `t` (tiles of Q rows); false where the tile number is one of the unused
-// ones. All lanes of a warp call it together.
-template <int Q>
-__device__ __forceinline__ bool find_part(const int64_t* ptr, int num, int N, int t, Part& out) {
+// the last part p of 0 .. num + 1 for which ok(p) holds (it holds up to some part and from there on no more). All lanes of
+// a warp call it together.
+template <typename F>
+__device__ __forceinline__ int last_part(int num, F ok) {
   const int lane = threadIdx.x & 31;
   int at = 0, n = num + 2;
   while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int i = lane * step;
-    const bool ok = i < n && part_bound(ptr, num, N, at + i) / Q + at + i <= t;
-    const unsigned b = __ballot_sync(0xffffffffu, ok);
+    const int step = (n + 31) / 32, i = lane * step;
+    const unsigned b = __ballot_sync(0xffffffffu, i < n && ok(at + i));
     const int c = max(__popc(b) - 1, 0);
     at += c * step;
     n = min(step, n - c * step);
   }
-  out.lo = part_bound(ptr, num, N, at);
-  out.hi = max(part_bound(ptr, num, N, at + 1), out.lo);
-  out.index = at;
-  out.keys = at > 0 && at <= num;
-  const int64_t row = (int64_t)out.lo + (int64_t)(t - at - out.lo / Q) * Q;
-  out.row = (int)row;
-  return row >= out.lo && row < out.hi;
+  return at;
 }
+
+// The part and first row of block `t` of Q rows; false where the number is one of the unused ones.
+template <int Q, typename T>
+__device__ __forceinline__ bool find_part(const Params<T>& p, int t, Part& out) {
+  const int64_t* ptr = p.ptr;
+  const int num = p.num, N = p.N;
+  if (p.compact) {
+    // Structures of more than 32 atoms alone, numbered from floor(start / 32): floor(x / 32) >= ceil(x / 64) numbers lie
+    // before the next one, however many short structures there are. Row 32 t + 31 is in the structure that owns t.
+    out.index = last_part(num, [&](int i) { return part_bound(ptr, num, N, i) <= min(32 * (int64_t)t + 31, (int64_t)N - 1); });
+  } else {
+    out.index = last_part(num, [&](int i) { return part_bound(ptr, num, N, i) / Q + i <= t; });
+  }
+  out.lo = part_bound(ptr, num, N, out.index);
+  out.hi = max(part_bound(ptr, num, N, out.index + 1), out.lo);
+  out.keys = out.index > 0 && out.index <= num;
+  const int first = p.compact ? out.lo / 32 : out.lo / Q + out.index;
+  const int64_t row = (int64_t)out.lo + (int64_t)(t - first) * Q;
+  out.row = (int)row;
+  const int len = out.hi - out.lo;
+  if (p.compact && len <= 32) return false;
+  return row >= out.lo && row < out.hi && (out.keys ? len >= p.min_len && len <= p.max_len : p.rest != 0);
+}
+
+// how many blocks of Q rows there may be
+template <typename T>
+__host__ __device__ __forceinline__ int part_blocks(const Params<T>& p, int Q) { return p.compact ? p.N / 32 + 1 : p.N / Q + p.num + 2; }
 
 template <typename T> __device__ __forceinline__ T log2e() { return T(1.4426950408889634074); }
-
-template <typename T>
-__device__ __forceinline__ bool takes(const Params<T>& p, const Part& part) {
-  const int len = part.hi - part.lo;
-  // the parts without keys go with the longest lengths
-  return part.keys ? (len >= p.min_len && len <= p.max_len) : p.max_len == std::numeric_limits<int>::max();
-}
 
 // the share of split z of the tiles of `B` rows in [lo, hi)
 template <int B>

@@ -54,6 +54,8 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
   check_rows(v, q, N, HK, D, "v");
   TORCH_CHECK(ptr.device() == q.device() && ptr.scalar_type() == torch::kInt64 && ptr.dim() == 1 && ptr.is_contiguous() &&
                   ptr.numel() >= 1 && ptr.numel() < (1 << 30), "structure attention: ptr must be int64 (structures + 1) on ", q.device());
+  TORCH_CHECK((N / SHORT + ptr.numel() + 2) * 3 * H < std::numeric_limits<int>::max(),
+              "structure attention: more structures and heads than a launch can number");
   attn::Params<T> p{};
   p.q = q.data_ptr<T>(); p.qs = q.stride(0); p.qh = q.stride(1);
   p.k = k.data_ptr<T>(); p.ks = k.stride(0); p.kh = k.stride(1);
@@ -67,8 +69,8 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
   p.scale = (T)scale;
   p.N = (int)N; p.num = (int)ptr.numel() - 1; p.H = (int)H; p.HK = (int)HK; p.D = (int)D;
   p.splits = 1;
-  p.min_len = 0;
   p.max_len = ANY_LENGTH;
+  p.rest = 1;
   return p;
 }
 
@@ -91,16 +93,20 @@ Plan choose(const attn::Params<T>& p, int64_t max_len, bool covered) {
   return {true, (int64_t)p.N < TC_AVERAGE * (int64_t)p.num};
 }
 
-// the parameters of the two launches: the long structures (with the rows of none), the short ones
+// The parameters of the two launches: the long structures, the short ones (with the rows of none, where both run). The
+// tensor cores' blocks and workspace are then numbered without regard to the short ones, of which there may be many.
 template <typename T>
 attn::Params<T> long_part(attn::Params<T> p, const Plan& plan) {
-  p.min_len = plan.short_ones ? SHORT + 1 : 0;
+  if (plan.short_ones) {
+    p.min_len = SHORT + 1;
+    p.rest = 0;
+    p.compact = sizeof(T) == 4;
+  }
   return p;
 }
 template <typename T>
 attn::Params<T> short_part(attn::Params<T> p, const Plan& plan) {
   if (plan.long_ones) p.max_len = SHORT;
-  p.splits = 1;
   return p;
 }
 
@@ -116,7 +122,9 @@ int choose_splits(int64_t row_blocks, int64_t max_len, int tile) {
 template <typename T>
 int splits_of(const attn::Params<T>& p, int heads, int64_t max_len) {
   const int rows = sizeof(T) == 4 ? TC_ROWS : SHORT;
-  return choose_splits(((int64_t)p.N / rows + std::max(p.num, 1)) * heads, max_len, sizeof(T) == 4 ? TC_TILE : SHORT);
+  const int64_t structures = p.min_len > 0 ? std::min(p.num, p.N / p.min_len) : p.num;
+  const int64_t blocks = ((int64_t)p.N / rows + std::max<int64_t>(structures, 1)) * heads;
+  return choose_splits(blocks, std::min<int64_t>(max_len, p.N), sizeof(T) == 4 ? TC_TILE : SHORT);
 }
 
 torch::Tensor bytes(int64_t n, const torch::Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kUInt8)); }
@@ -143,7 +151,7 @@ std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Te
   if (sizeof(T) == 8 && plan.long_ones) plan.short_ones = false;         // one tile for every length
   if (plan.long_ones) {
     auto pl = long_part(p, plan);
-    pl.splits = splits_of(p, p.H, max_len);
+    pl.splits = splits_of(pl, p.H, max_len);
     torch::Tensor work, images;
     if (pl.splits > 1) {
       work = torch::empty({(int64_t)pl.splits * p.H * p.N * (p.D + 2)}, q.options());
@@ -189,7 +197,7 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
   if (plan.long_ones) {
     auto pl = long_part(p, plan);
     const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
-    const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
+    const int sq = splits_of(pl, p.H, max_len), sk = splits_of(pl, p.HK, max_len);
     torch::Tensor work, scratch;
     if (sq > 1 || sk > 1) {
       work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
@@ -241,7 +249,7 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
     if (plan.long_ones && p.D <= TC_SECOND_WIDTH) {
       auto pl = long_part(p, plan);
       const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
-      const int sq = splits_of(p, p.H, max_len), sk = splits_of(p, p.HK, max_len);
+      const int sq = splits_of(pl, p.H, max_len), sk = splits_of(pl, p.HK, max_len);
       torch::Tensor work;
       if (sq > 1 || sk > 1) {
         work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
