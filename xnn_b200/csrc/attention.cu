@@ -43,8 +43,7 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
   const T *gq = p.q + h * p.qh, *gk = p.k + hk * p.kh, *gv = p.v + hk * p.vh;
   const bool vq = vec_ok(p.q, p.qs, p.qh, p.D), vk = vec_ok(p.k, p.ks, p.kh, p.D), vv = vec_ok(p.v, p.vs, p.vh, p.D);
-  int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
-  split_range<C::BK>(k_lo, k_hi, blockIdx.z, p.splits);
+  const int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   const T c2 = p.scale * log2e<T>();
   T m[C::RI], l[C::RI], acc[C::RI][C::DP / C::TX];
 #pragma unroll
@@ -92,24 +91,13 @@ __global__ void __launch_bounds__(C::NT) fwd_kernel(const Params<T> p) {
     tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sP, i0, sV, tx, k_hi - k0);
     __syncthreads();
   }
-  const int64_t rows = (int64_t)p.H * p.N;
 #pragma unroll
   for (int r = 0; r < C::RI; ++r) {
     const int row = part.row + i0 + r;
     if (row >= part.hi) continue;
-    if (p.splits > 1) {
-      const int64_t at = blockIdx.z * rows + (int64_t)h * p.N + row;
-      store_row<T, C::DP, C::TX>(p.work + at * p.D, acc[r], T(1), p.D, tx);
-      if (tx == 0) {
-        T* stats = p.work + p.splits * rows * p.D;
-        stats[at] = m[r];
-        stats[p.splits * rows + at] = l[r];
-      }
-    } else {
-      const bool none = m[r] == neg_inf<T>() && l[r] == T(0);   // NaN scores are not an empty row
-      store_row<T, C::DP, C::TX>(p.out0 + ((int64_t)row * p.H + h) * p.D, acc[r], none ? T(0) : T(1) / l[r], p.D, tx);
-      if (tx == 0 && p.lse) p.lse[(int64_t)h * p.N + row] = none ? -neg_inf<T>() : m[r] + lg2(l[r]);
-    }
+    const bool none = m[r] == neg_inf<T>() && l[r] == T(0);   // NaN scores are not an empty row
+    store_row<T, C::DP, C::TX>(p.out0 + ((int64_t)row * p.H + h) * p.D, acc[r], none ? T(0) : T(1) / l[r], p.D, tx);
+    if (tx == 0 && p.lse) p.lse[(int64_t)h * p.N + row] = none ? -neg_inf<T>() : m[r] + lg2(l[r]);
   }
 }
 
@@ -166,136 +154,6 @@ __global__ void __launch_bounds__(128) delta_kernel(const Params<T> p) {
   for (int d = lane; d < p.D; d += 32) s += a[d] * b[d];
   s = row_sum<32>(s);
   if (lane == 0) p.delta[(int64_t)h * p.N + row] = s;
-}
-
-template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT) dq_kernel(const Params<T> p) {
-  extern __shared__ __align__(16) char smem_raw[];
-  T* sQ = reinterpret_cast<T*>(smem_raw);
-  T* sO = sQ + C::BQ * C::LD;
-  T* sK = sO + C::BQ * C::LD;
-  T* sV = sK + C::BK * C::LD;
-  T* sP = sV + C::BK * C::LD;
-  Part part;
-  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
-  const int h = blockIdx.y, hk = h / (p.H / p.HK);
-  const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
-  const T *gk = p.k + hk * p.kh, *gv = p.v + hk * p.vh;
-  const bool vk = vec_ok(p.k, p.ks, p.kh, p.D), vv = vec_ok(p.v, p.vs, p.vh, p.D);
-  int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
-  split_range<C::BK>(k_lo, k_hi, blockIdx.z, p.splits);
-  const T c2 = p.scale * log2e<T>();
-  T L[C::RI], D[C::RI], acc[C::RI][C::DP / C::TX];
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) {
-    const int row = part.row + i0 + r;
-    L[r] = row < part.hi ? p.lse[(int64_t)h * p.N + row] : T(0);
-    D[r] = row < part.hi ? p.delta[(int64_t)h * p.N + row] : T(0);
-#pragma unroll
-    for (int n = 0; n < C::DP / C::TX; ++n) acc[r][n] = T(0);
-  }
-  if (k_lo < k_hi) {
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sQ, p.q + h * p.qh, p.qs, part.row, part.hi, p.D, vec_ok(p.q, p.qs, p.qh, p.D));
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sO, p.go + h * p.goh, p.gos, part.row, part.hi, p.D, vec_ok(p.go, p.gos, p.goh, p.D));
-  }
-  for (int k0 = k_lo; k0 < k_hi; k0 += C::BK) {
-    load_tile<T, C::BK, C::DP, C::LD, C::NT>(sK, gk, p.ks, k0, k_hi, p.D, vk, p.mask);
-    load_tile<T, C::BK, C::DP, C::LD, C::NT>(sV, gv, p.vs, k0, k_hi, p.D, vv, p.mask);
-    __syncthreads();
-    T s[C::RI][C::RJ] = {}, dp[C::RI][C::RJ] = {};
-    tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, sQ, i0, sK, tx);
-    tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, sO, i0, sV, tx);
-#pragma unroll
-    for (int c = 0; c < C::RJ; ++c) {
-      const bool ok = allowed(k0 + tx + C::TX * c, k_hi, p.mask);
-#pragma unroll
-      for (int r = 0; r < C::RI; ++r)
-        sP[(i0 + r) * C::LDP + tx + C::TX * c] = ok ? pow2(s[r][c] * c2 - L[r]) * (dp[r][c] - D[r]) : T(0);
-    }
-    __syncthreads();
-    tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sP, i0, sK, tx);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) {
-    const int row = part.row + i0 + r;
-    if (row >= part.hi) continue;
-    T* out = (p.splits > 1 ? p.work + (int64_t)blockIdx.z * p.N * p.H * p.D : p.out0) + ((int64_t)row * p.H + h) * p.D;
-    store_row<T, C::DP, C::TX>(out, acc[r], p.scale, p.D, tx);
-  }
-}
-
-// a block owns BQ keys of one key head and walks the queries of every head that shares it
-template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT) dkv_kernel(const Params<T> p) {
-  extern __shared__ __align__(16) char smem_raw[];
-  T* sK = reinterpret_cast<T*>(smem_raw);
-  T* sV = sK + C::BQ * C::LD;
-  T* sQ = sV + C::BQ * C::LD;
-  T* sO = sQ + C::BK * C::LD;
-  T* sP = sO + C::BK * C::LD;
-  T* sS = sP + C::BQ * C::LDP;
-  Part part;
-  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
-  const int hk = blockIdx.y, group = p.H / p.HK;
-  const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
-  const bool vq = vec_ok(p.q, p.qs, p.qh, p.D), vo = vec_ok(p.go, p.gos, p.goh, p.D);
-  int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
-  split_range<C::BK>(q_lo, q_hi, blockIdx.z, p.splits_k);
-  const T c2 = p.scale * log2e<T>();
-  T dk[C::RI][C::DP / C::TX], dv[C::RI][C::DP / C::TX];
-  bool ok[C::RI];
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) {
-    ok[r] = allowed(part.row + i0 + r, part.hi, p.mask);
-#pragma unroll
-    for (int n = 0; n < C::DP / C::TX; ++n) dk[r][n] = dv[r][n] = T(0);
-  }
-  if (q_lo < q_hi) {
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sK, p.k + hk * p.kh, p.ks, part.row, part.hi, p.D, vec_ok(p.k, p.ks, p.kh, p.D), p.mask);
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sV, p.v + hk * p.vh, p.vs, part.row, part.hi, p.D, vec_ok(p.v, p.vs, p.vh, p.D), p.mask);
-  }
-  for (int g = 0; g < group; ++g) {
-    const int h = hk * group + g;
-    for (int q0 = q_lo; q0 < q_hi; q0 += C::BK) {
-      load_tile<T, C::BK, C::DP, C::LD, C::NT>(sQ, p.q + h * p.qh, p.qs, q0, q_hi, p.D, vq);
-      load_tile<T, C::BK, C::DP, C::LD, C::NT>(sO, p.go + h * p.goh, p.gos, q0, q_hi, p.D, vo);
-      __syncthreads();
-      T s[C::RI][C::RJ] = {}, dp[C::RI][C::RJ] = {};
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, sK, i0, sQ, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, sV, i0, sO, tx);
-#pragma unroll
-      for (int c = 0; c < C::RJ; ++c) {
-        const int row = q0 + tx + C::TX * c;
-        const bool in = row < q_hi;
-        const T L = in ? p.lse[(int64_t)h * p.N + row] : T(0), D = in ? p.delta[(int64_t)h * p.N + row] : T(0);
-#pragma unroll
-        for (int r = 0; r < C::RI; ++r) {
-          const T e = in && ok[r] ? pow2(s[r][c] * c2 - L) : T(0);
-          sP[(i0 + r) * C::LDP + tx + C::TX * c] = e;
-          sS[(i0 + r) * C::LDP + tx + C::TX * c] = in && ok[r] ? e * (dp[r][c] - D) : T(0);
-        }
-      }
-      __syncthreads();
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dv, sP, i0, sO, tx);
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sS, i0, sQ, tx);
-      __syncthreads();
-    }
-  }
-  const int64_t n = (int64_t)p.N * p.HK * p.D;
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) {
-    const int row = part.row + i0 + r;
-    if (row >= part.hi) continue;
-    const int64_t at = ((int64_t)row * p.HK + hk) * p.D;
-    T *ok_ = p.out1 + at, *ov_ = p.out2 + at;
-    if (p.splits_k > 1) {
-      ok_ = p.work_k + blockIdx.z * n + at;
-      ov_ = p.work_k + (p.splits_k + blockIdx.z) * n + at;
-    }
-    store_row<T, C::DP, C::TX>(ok_, dk[r], p.scale, p.D, tx);
-    store_row<T, C::DP, C::TX>(ov_, dv[r], T(1), p.D, tx);
-  }
 }
 
 // structures of at most BQ atoms: one block holds the whole probability matrix of a head, so that the
@@ -568,12 +426,12 @@ __global__ void __launch_bounds__(C::NT) second_key_kernel(const Params<T> p) {
 
 // ------------------------------------------------------------------------------------------ launches
 template <typename T, typename C, auto KERNEL>
-cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s, int splits = 1) {
+cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, int squares, cudaStream_t s) {
   const size_t bytes = sizeof(T) * ((size_t)row_tiles * C::BQ * C::LD + (size_t)key_tiles * C::BK * C::LD +
                                     (size_t)squares * C::BQ * C::LDP);
   const cudaError_t e = raise_smem_limit<KERNEL>(bytes);
   if (e != cudaSuccess) return e;
-  const dim3 grid(part_blocks(p, C::BQ), heads, splits);
+  const dim3 grid(part_blocks(p, C::BQ), heads);
   KERNEL<<<grid, C::NT, bytes, s>>>(p);
   return cudaGetLastError();
 }
@@ -603,7 +461,7 @@ template <> struct Second<double, 128> { using C = Cfg<double, 32, 16, 128, 2, 1
 
 template <typename T>
 cudaError_t forward(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s, p.splits)))
+  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, fwd_kernel<T, C>>(p, p.H, 1, 2, 1, s)))
 }
 template <typename T>
 cudaError_t forward_join(const Params<T>& p, cudaStream_t s) {
@@ -621,12 +479,6 @@ cudaError_t row_delta(const Params<T>& p, cudaStream_t s) {
   const int64_t rows = (int64_t)p.H * p.N;
   delta_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
   return cudaGetLastError();
-}
-cudaError_t backward_dq(const Params<double>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dq_kernel<double, C>>(p, p.H, 2, 2, 1, s, p.splits)))
-}
-cudaError_t backward_dkv(const Params<double>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Small<double, DP>::C; return (launch<double, C, dkv_kernel<double, C>>(p, p.HK, 2, 2, 2, s, p.splits_k)))
 }
 template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {

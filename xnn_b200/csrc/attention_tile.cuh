@@ -82,6 +82,7 @@ __device__ __forceinline__ void split_range(int& lo, int& hi, int z, int splits)
 
 template <typename T> struct Vec { static constexpr int W = 16 / sizeof(T); };
 template <typename T> struct alignas(16) V16 { T x[16 / sizeof(T)]; };
+template <typename T> struct alignas(2 * sizeof(T)) V2 { T x, y; };
 
 __device__ __forceinline__ float pow2(float x) { return exp2f(x); }
 __device__ __forceinline__ double pow2(double x) { return exp2(x); }

@@ -81,15 +81,14 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
 //                               backward / second: 11 / 26 / 61 us, short and 64-row FP32 tiles 14 / 44 / 50; of 48-80
 //                               atoms 14 / 33 / 79 and 16 / 48 / 146; 400 x 2 heads of 24-40: 38 / 131 / 274 and 32 / 102 / 298
 //   otherwise                   tensor cores for the structures above SHORT, then the short kernels for the rest
-// float64 has no tensor-core form: 32-row tiles, for short structures with the whole backward pass in one kernel.
+// float64 goes by the same rule between its short kernels and the FP64 tensor instructions.
 constexpr int TC_AVERAGE = 32, TC_WIDTH = 128, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
 
 struct Plan { bool long_ones, short_ones; };
 
 template <typename T>
-Plan choose(const attn::Params<T>& p, int64_t max_len, bool covered) {
+Plan choose(const attn::Params<T>& p, int64_t max_len) {
   if (max_len <= SHORT) return {false, true};
-  if (sizeof(T) == 8 || !covered) return {true, (int64_t)p.N < 48 * (int64_t)p.num};
   return {true, (int64_t)p.N < TC_AVERAGE * (int64_t)p.num};
 }
 
@@ -110,21 +109,28 @@ attn::Params<T> short_part(attn::Params<T> p, const Plan& plan) {
   return p;
 }
 
-// Few row blocks and long structures: the walk over the other axis is shared out among up to 16 blocks
-// and their results added in order, until there are two blocks a multiprocessor; a share has four tiles
-// at least, or the second pass over the partial results costs what it saves.
-int choose_splits(int64_t row_blocks, int64_t max_len, int tile) {
+// How many blocks share the walk over the other axis (their partial results are added in order). With `slots` blocks running
+// at a time, z shares take ceil(blocks z / slots) rounds of walk / z tiles and a fixed part of about two tiles (staging,
+// storing); up to 16 shares, of two tiles at least, and only for a tenth less time, as the sums are another pass.
+int choose_splits(int64_t row_blocks, int64_t max_len, int tile, int slots) {
   const int64_t walk = (max_len + tile - 1) / tile;
-  int64_t s = 2 * SMS / std::max<int64_t>(row_blocks, 1);
-  s = std::min({s, walk / 4, (int64_t)16});
-  return (int)std::max<int64_t>(s, 1);
+  int best = 1;
+  double least = 0;
+  for (int z = 1; z <= 16 && (z == 1 || walk >= 2 * z); ++z) {
+    const double cost = (double)((row_blocks * z + slots - 1) / slots) * (double)((walk + z - 1) / z + 2);
+    if (z == 1 || cost < 0.9 * least) {
+      best = z;
+      least = cost;
+    }
+  }
+  return best;
 }
 template <typename T>
-int splits_of(const attn::Params<T>& p, int heads, int64_t max_len) {
-  const int rows = sizeof(T) == 4 ? TC_ROWS : SHORT;
+int splits_of(const attn::Params<T>& p, int heads, int64_t max_len, bool tc = sizeof(T) == 4, int resident = 1) {
+  const int rows = tc ? TC_ROWS : SHORT;
   const int64_t structures = p.min_len > 0 ? std::min(p.num, p.N / p.min_len) : p.num;
   const int64_t blocks = ((int64_t)p.N / rows + std::max<int64_t>(structures, 1)) * heads;
-  return choose_splits(blocks, std::min<int64_t>(max_len, p.N), sizeof(T) == 4 ? TC_TILE : SHORT);
+  return choose_splits(blocks, std::min<int64_t>(max_len, p.N), TC_TILE, SMS * resident);
 }
 
 torch::Tensor bytes(int64_t n, const torch::Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kUInt8)); }
@@ -147,11 +153,10 @@ std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Te
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = out.data_ptr<T>();
   p.lse = want_stats ? lse.data_ptr<T>() : nullptr;
-  auto plan = choose(p, max_len, true);
-  if (sizeof(T) == 8 && plan.long_ones) plan.short_ones = false;         // one tile for every length
+  const auto plan = choose(p, max_len);
   if (plan.long_ones) {
     auto pl = long_part(p, plan);
-    pl.splits = splits_of(pl, p.H, max_len);
+    pl.splits = splits_of(pl, p.H, max_len, sizeof(T) == 4, p.D <= 64 ? 2 : 1);
     torch::Tensor work, images;
     if (pl.splits > 1) {
       work = torch::empty({(int64_t)pl.splits * p.H * p.N * (p.D + 2)}, q.options());
@@ -161,7 +166,7 @@ std::vector<torch::Tensor> forward_typed(const torch::Tensor& q, const torch::Te
       images = bytes(attn::tc_forward_bytes(pl), q);
       XNN_OK(attn::tc_forward(pl, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
     } else {
-      XNN_OK(attn::forward<T>(pl, s));
+      XNN_OK(attn::forward64(pl, s));
     }
     if (pl.splits > 1) XNN_OK(attn::forward_join<T>(pl, s));             // short structures' rows hold nothing yet
   }
@@ -193,7 +198,7 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
   if (p.N == 0) return {dq, dk, dv};
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = dq.data_ptr<T>(); p.out1 = dk.data_ptr<T>(); p.out2 = dv.data_ptr<T>();
-  const auto plan = choose(p, max_len, true);
+  const auto plan = choose(p, max_len);
   if (plan.long_ones) {
     auto pl = long_part(p, plan);
     const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
@@ -212,9 +217,7 @@ std::vector<torch::Tensor> backward_typed(const torch::Tensor& go, const torch::
     } else {
       scratch = torch::empty({p.H, p.N}, q.options());
       pl.delta = scratch.data_ptr<T>();
-      XNN_OK(attn::row_delta<T>(pl, s));
-      XNN_OK(attn::backward_dq(pl, s));
-      XNN_OK(attn::backward_dkv(pl, s));
+      XNN_OK(attn::backward64(pl, s));
     }
     if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
     if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work_k, p.out1, p.out2, s));
@@ -242,38 +245,43 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
   if (p.N == 0) return {q2, k2, v2, do2};
   const auto s = at::cuda::getCurrentCUDAStream();
   p.out0 = q2.data_ptr<T>(); p.out1 = k2.data_ptr<T>(); p.out2 = v2.data_ptr<T>(); p.out3 = do2.data_ptr<T>();
-  bool rest = true;                                    // what the FP32 / FP64 pipes take
-  auto pr = p;
-  if constexpr (sizeof(T) == 4) {
-    const auto plan = choose(p, max_len, p.D <= TC_SECOND_WIDTH);
-    if (plan.long_ones && p.D <= TC_SECOND_WIDTH) {
-      auto pl = long_part(p, plan);
-      const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
-      const int sq = splits_of(pl, p.H, max_len), sk = splits_of(pl, p.HK, max_len);
-      torch::Tensor work;
-      if (sq > 1 || sk > 1) {
-        work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
-        pl.work = work.data_ptr<T>();
-        pl.work_k = pl.work + (sq > 1 ? sq * nq : 0);
+  const auto plan = choose(p, max_len);
+  if (plan.long_ones) {
+    const bool tc = sizeof(T) == 4 && p.D <= TC_SECOND_WIDTH;
+    auto pl = long_part(p, plan);
+    if (!tc) pl.compact = 0;
+    const int sq = splits_of(pl, p.H, max_len, tc), sk = splits_of(pl, p.HK, max_len, tc);
+    const int64_t nq = (int64_t)p.N * p.H * p.D, nk = (int64_t)p.N * p.HK * p.D;
+    pl.splits = sq;
+    pl.splits_k = sk;
+    if constexpr (sizeof(T) == 4) {
+      if (tc) {
+        torch::Tensor work;
+        if (sq > 1 || sk > 1) {
+          work = torch::empty({(sq > 1 ? sq * nq : 0) + (sk > 1 ? 2 * sk * nk : 0)}, q.options());
+          pl.work = work.data_ptr<T>();
+          pl.work_k = pl.work + (sq > 1 ? sq * nq : 0);
+        }
+        auto images = bytes(attn::tc_second_bytes(pl), q);
+        XNN_OK(attn::tc_second(pl, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
+        if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
+        if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work_k, p.out1, p.out2, s));
       }
-      pl.splits = sq;
-      pl.splits_k = sk;
-      auto images = bytes(attn::tc_second_bytes(pl), q);
-      XNN_OK(attn::tc_second(pl, static_cast<char*>(images.data_ptr()), status_of(status, q), s));
-      if (sq > 1) XNN_OK(attn::sum_splits<T>(nq, sq, pl.work, p.out0, nullptr, s));
-      if (sk > 1) XNN_OK(attn::sum_splits<T>(nk, sk, pl.work_k, p.out1, p.out2, s));
-      rest = plan.short_ones;
-      pr = short_part(p, plan);
+    }
+    if (!tc) {
+      torch::Tensor work = torch::empty({attn::second64_words<T>(pl)}, q.options().dtype(torch::kFloat64));
+      XNN_OK(attn::second64<T>(pl, work.data_ptr<double>(), s));
     }
   }
-  if (rest) {
+  if (plan.short_ones) {
+    auto ps = short_part(p, plan);
     torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
-    pr.delta = stats.data_ptr<T>();
-    pr.r = pr.delta + (int64_t)p.H * p.N;
-    pr.c = pr.r + (int64_t)p.H * p.N;
-    XNN_OK(attn::row_delta<T>(pr, s));
-    XNN_OK(attn::second_rows<T>(pr, s));
-    XNN_OK(attn::second_keys<T>(pr, s));
+    ps.delta = stats.data_ptr<T>();
+    ps.r = ps.delta + (int64_t)p.H * p.N;
+    ps.c = ps.r + (int64_t)p.H * p.N;
+    XNN_OK(attn::row_delta<T>(ps, s));
+    XNN_OK(attn::second_rows<T>(ps, s));
+    XNN_OK(attn::second_keys<T>(ps, s));
   }
   return {q2, k2, v2, do2};
 }
