@@ -28,28 +28,41 @@ __device__ __forceinline__ void mma(double (&c)[2], double a, double b) {
   asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-// `rows` rows of g from row0 on, widened; zero behind `end`, behind column D (up to the next multiple of 8) and where masked
+// `rows` rows of g from row0 (< end) on, widened; zero behind `end`, behind column D (up to the next multiple of 8) and where
+// masked. Eight loads are in flight a thread: they go to addresses that exist and what is not wanted is dropped
+// afterwards, since a load under a condition waits for the one before.
 template <typename IN, int THREADS>
 __device__ __forceinline__ void load_rows(double* s, int ld, const IN* g, int64_t stride, int64_t head, int row0, int rows, int end,
                                           int D, const uint8_t* mask = nullptr) {
   const bool vec = reinterpret_cast<uintptr_t>(g) % (2 * sizeof(IN)) == 0 && stride % 2 == 0 && head % 2 == 0 && D % 2 == 0;
   const uint32_t pairs = (D + 7) / 8 * 4, by = ((1u << 20) + pairs - 1) / pairs;      // i / pairs = i by / 2^20 for i < 2^13
-#pragma unroll 8
-  for (uint32_t i = threadIdx.x; i < rows * pairs; i += THREADS) {
-    const int r = i * by >> 20, c = (i - r * pairs) * 2, row = row0 + r;
-    double x = 0.0, y = 0.0;
-    if (row < end && c < D && (mask == nullptr || mask[row])) {
-      const IN* p = g + row * stride + c;
+  const uint32_t n = rows * pairs;
+  constexpr int U = 8;
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += U * THREADS) {
+    V2<IN> v[U];
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = min(i0 + u * THREADS, n - 1);
+      const int r = i * by >> 20, c = (i - r * pairs) * 2, row = min(row0 + r, end - 1);
+      on[u] = row0 + r < end && c < D;
+      const IN* p = g + row * stride + (c < D ? c : 0);
       if (vec) {
-        const V2<IN> v = *reinterpret_cast<const V2<IN>*>(p);
-        x = (double)v.x;
-        y = (double)v.y;
+        v[u] = *reinterpret_cast<const V2<IN>*>(p);
       } else {
-        x = (double)p[0];
-        if (c + 1 < D) y = (double)p[1];
+        v[u].x = p[0];
+        v[u].y = c + 1 < D ? p[1] : IN(0);
+      }
+      if (mask) on[u] = on[u] && mask[row];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * THREADS;
+      if (i < n) {
+        const int r = i * by >> 20, c = (i - r * pairs) * 2;
+        *reinterpret_cast<double2*>(s + r * ld + c) = on[u] ? make_double2((double)v[u].x, (double)v[u].y) : make_double2(0.0, 0.0);
       }
     }
-    *reinterpret_cast<double2*>(s + r * ld + c) = make_double2(x, y);
   }
 }
 

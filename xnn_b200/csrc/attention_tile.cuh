@@ -99,29 +99,42 @@ __host__ __device__ __forceinline__ bool vec_ok(const T* p, int64_t rs, int64_t 
   return (reinterpret_cast<uintptr_t>(p) % 16 == 0) && rs % W == 0 && hs % W == 0 && D % W == 0;
 }
 
-// rows row0 .. row0 + ROWS of g into s (row stride LD), zero behind `end`, behind column D and where the
-// mask is 0: what is masked or belongs to another structure never enters a product, NaN included
+// Rows row0 (< end) .. row0 + ROWS of g into s (row stride LD), zero behind `end`, behind column D and where the mask is 0:
+// what is masked or belongs to another structure never enters a product, NaN included. Eight loads are in flight a
+// thread: they go to addresses that exist and what is not wanted is dropped afterwards, since a load under a condition
+// waits for the one before.
 template <typename T, int ROWS, int DP, int LD, int NT>
 __device__ __forceinline__ void load_tile(T* s, const T* g, int64_t stride, int row0, int end, int D, bool vec,
                                           const uint8_t* mask = nullptr) {
-  constexpr int W = Vec<T>::W, CH = DP / W;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < ROWS * CH; i += NT) {
-    const int r = i / CH, c = (i % CH) * W, row = row0 + r;
-    V16<T> v;
+  constexpr int W = Vec<T>::W, CH = DP / W, N = ROWS * CH, U = N / NT < 8 ? (N / NT < 1 ? 1 : N / NT) : 8;
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < N; i0 += U * NT) {
+    V16<T> v[U];
+    bool on[U];
 #pragma unroll
-    for (int e = 0; e < W; ++e) v.x[e] = T(0);
-    if (row < end && c < D && (mask == nullptr || mask[row])) {
-      const T* p = g + (int64_t)row * stride + c;
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * NT, N - 1), r = i / CH, c = (i % CH) * W, row = min(row0 + r, end - 1);
+      on[u] = row0 + r < end && c < D;
+      const T* p = g + (int64_t)row * stride + (c < D ? c : 0);
       if (vec) {
-        v = *reinterpret_cast<const V16<T>*>(p);
+        v[u] = *reinterpret_cast<const V16<T>*>(p);
       } else {
 #pragma unroll
+        for (int e = 0; e < W; ++e) v[u].x[e] = p[c + e < D ? e : 0];
+      }
+      if (mask) on[u] = on[u] && mask[row];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      if (i < N) {
+        const int c = (i % CH) * W;
+#pragma unroll
         for (int e = 0; e < W; ++e)
-          if (c + e < D) v.x[e] = p[e];
+          if (!on[u] || c + e >= D) v[u].x[e] = T(0);
+        *reinterpret_cast<V16<T>*>(s + i / CH * LD + c) = v[u];
       }
     }
-    *reinterpret_cast<V16<T>*>(s + r * LD + c) = v;
   }
 }
 
