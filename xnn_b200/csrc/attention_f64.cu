@@ -3,12 +3,16 @@
 // more than 64 columns a head, whose parts the FP16-type tensor cores' memory does not hold (the operands are widened
 // as they are read; 64-bit products run at half the FP32 pipes' rate but need a third of their shared-memory traffic).
 //
+// The streamed tiles come by asynchronous copies in two groups: those that a walk only takes for one kind of product are
+// free while the others are at work, so the next tile's copies run under the products without a second set of buffers.
+//
 // A block owns 32 rows and streams tiles of the other side through shared memory. Its warps are RG groups of rows by KG
 // groups of the streamed rows: a warp forms the weights of its 8 RB rows and its own slice of each tile, multiplies
 // them on at once, and the KG partial results (with their own running maxima in the forward pass) are joined at the
 // end. With m8n8k4 products a lane holds, of 8 x 8 scores, row lane / 4 and columns 2 (lane % 4) + {0, 1}; the next
 // product takes a row's weights as they lie, four columns at a time: step s takes column 2 t + (s ^ t / 2) from lane t,
-// so that the four matching rows of the other operand fall into different banks (rows are 4 mod 16 numbers long).
+// so that the four matching rows of the other operand fall into different banks (rows are 4 mod 16 numbers long; float32
+// rows, 4 mod 32 long, are conflict-free with column 2 t + s).
 #include "attention.h"
 #include "attention_tile.cuh"
 
@@ -22,46 +26,48 @@ struct Shape {
   static_assert(ROWS == 32, "a block owns 32 rows");
 };
 
-__host__ __device__ constexpr int row_length(int D) { return (D + 15) / 16 * 16 + 4; }
+template <typename IN>
+__host__ __device__ constexpr int row_length(int D) {
+  return sizeof(IN) == 8 ? (D + 15) / 16 * 16 + 4 : (D + 31) / 32 * 32 + 4;
+}
 
 __device__ __forceinline__ void mma(double (&c)[2], double a, double b) {
   asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
 }
 
-// `rows` rows of g from row0 (< end) on, widened; zero behind `end`, behind column D (up to the next multiple of 8) and where
-// masked. Eight loads are in flight a thread: they go to addresses that exist and what is not wanted is dropped
-// afterwards, since a load under a condition waits for the one before.
-template <typename IN, int THREADS>
-__device__ __forceinline__ void load_rows(double* s, int ld, const IN* g, int64_t stride, int64_t head, int row0, int rows, int end,
-                                          int D, const uint8_t* mask = nullptr) {
+// BYTES to shared memory, zero if not `on`
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* s, const void* g, bool on) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(s);
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(g), "n"(BYTES), "r"(on ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits for the copies of all groups but the latest LEFT, the whole block's
+template <int LEFT>
+__device__ __forceinline__ void arrive() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+  __syncthreads();
+}
+
+// starts the copies of `rows` rows of g from row0 (< end) on; zero behind `end`, behind column D (up to the next multiple of
+// 8) and where masked
+template <int THREADS, typename IN>
+__device__ __forceinline__ void copy_rows(IN* s, int ld, const IN* g, int64_t stride, int64_t head, int row0, int rows, int end, int D,
+                                          const uint8_t* mask = nullptr) {
   const bool vec = reinterpret_cast<uintptr_t>(g) % (2 * sizeof(IN)) == 0 && stride % 2 == 0 && head % 2 == 0 && D % 2 == 0;
   const uint32_t pairs = (D + 7) / 8 * 4, by = ((1u << 20) + pairs - 1) / pairs;      // i / pairs = i by / 2^20 for i < 2^13
   const uint32_t n = rows * pairs;
-  constexpr int U = 8;
-  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += U * THREADS) {
-    V2<IN> v[U];
-    bool on[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t i = min(i0 + u * THREADS, n - 1);
-      const int r = i * by >> 20, c = (i - r * pairs) * 2, row = min(row0 + r, end - 1);
-      on[u] = row0 + r < end && c < D;
-      const IN* p = g + row * stride + (c < D ? c : 0);
-      if (vec) {
-        v[u] = *reinterpret_cast<const V2<IN>*>(p);
-      } else {
-        v[u].x = p[0];
-        v[u].y = c + 1 < D ? p[1] : IN(0);
-      }
-      if (mask) on[u] = on[u] && mask[row];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t i = i0 + u * THREADS;
-      if (i < n) {
-        const int r = i * by >> 20, c = (i - r * pairs) * 2;
-        *reinterpret_cast<double2*>(s + r * ld + c) = on[u] ? make_double2((double)v[u].x, (double)v[u].y) : make_double2(0.0, 0.0);
-      }
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+    const int r = i * by >> 20, c = (i - r * pairs) * 2, row = min(row0 + r, end - 1);
+    const bool on = row0 + r < end && c < D && (mask == nullptr || mask[row]);
+    const IN* p = g + row * stride + (c < D ? c : 0);
+    IN* to = s + r * ld + c;
+    if (vec) {
+      copy_async<2 * sizeof(IN)>(to, p, on);
+    } else {
+      copy_async<sizeof(IN)>(to, p, on);
+      copy_async<sizeof(IN)>(to + 1, p + (c + 1 < D), on && c + 1 < D);
     }
   }
 }
@@ -70,7 +76,7 @@ __device__ __forceinline__ void load_rows(double* s, int ld, const IN* g, int64_
 template <class S>
 struct Lane {
   int g, t, rg, kg, ld;
-  __device__ __forceinline__ explicit Lane(int D) : g(threadIdx.x % 32 / 4), t(threadIdx.x % 4), ld(row_length(D)) {
+  __device__ __forceinline__ explicit Lane(int ld_) : g(threadIdx.x % 32 / 4), t(threadIdx.x % 4), ld(ld_) {
     rg = threadIdx.x / 32 / S::KG;
     kg = threadIdx.x / 32 % S::KG;
   }
@@ -97,15 +103,15 @@ __device__ __forceinline__ void clear(Sums<S>& x) {
 }
 
 // x += own rows of A times streamed rows of B
-template <class S>
-__device__ __forceinline__ void scores(Scores<S>& x, const Lane<S>& l, const double* A, const double* B, int D) {
+template <class S, typename IN>
+__device__ __forceinline__ void scores(Scores<S>& x, const Lane<S>& l, const IN* A, const IN* B, int D) {
 #pragma unroll 4
   for (int k = 0; k < D; k += 4) {
     double a[S::RB], b[S::NT];
 #pragma unroll
-    for (int rb = 0; rb < S::RB; ++rb) a[rb] = A[l.own(rb) * l.ld + k + l.t];
+    for (int rb = 0; rb < S::RB; ++rb) a[rb] = (double)A[l.own(rb) * l.ld + k + l.t];
 #pragma unroll
-    for (int nt = 0; nt < S::NT; ++nt) b[nt] = B[(l.col(nt) + l.g) * l.ld + k + l.t];
+    for (int nt = 0; nt < S::NT; ++nt) b[nt] = (double)B[(l.col(nt) + l.g) * l.ld + k + l.t];
 #pragma unroll
     for (int rb = 0; rb < S::RB; ++rb)
 #pragma unroll
@@ -114,21 +120,21 @@ __device__ __forceinline__ void scores(Scores<S>& x, const Lane<S>& l, const dou
 }
 
 // acc += weights (own rows x streamed rows) times streamed rows of V
-template <class S>
-__device__ __forceinline__ void sums(Sums<S>& acc, const Lane<S>& l, const Scores<S>& w, const double* V, int D) {
+template <class S, typename IN>
+__device__ __forceinline__ void sums(Sums<S>& acc, const Lane<S>& l, const Scores<S>& w, const IN* V, int D) {
 #pragma unroll
   for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int e = s ^ (l.t >> 1);
-      const double* row = V + (l.col(nt) + 2 * l.t + e) * l.ld + l.g;
+      const int e = sizeof(IN) == 8 ? s ^ (l.t >> 1) : s;
+      const IN* row = V + (l.col(nt) + 2 * l.t + e) * l.ld + l.g;
       double a[S::RB];
 #pragma unroll
       for (int rb = 0; rb < S::RB; ++rb) a[rb] = e ? w[rb][nt][1] : w[rb][nt][0];
 #pragma unroll
       for (int n = 0; n < S::DP / 8; ++n) {
         if (n * 8 < D) {
-          const double b = row[n * 8];
+          const double b = (double)row[n * 8];
 #pragma unroll
           for (int rb = 0; rb < S::RB; ++rb) mma(acc[rb][n], a[rb], b);
         }
@@ -141,20 +147,21 @@ __device__ __forceinline__ void sums(Sums<S>& acc, const Lane<S>& l, const Score
 template <class S, typename OUT>
 __device__ __forceinline__ void join_rows(double* red, const Lane<S>& l, const Sums<S>& acc, const double (&f)[S::RB], OUT* out,
                                           int64_t stride, int rows, int D, double scale) {
+  const int ld = row_length<double>(D);
   __syncthreads();
 #pragma unroll
   for (int rb = 0; rb < S::RB; ++rb)
 #pragma unroll
     for (int n = 0; n < S::DP / 8; ++n)
       if (n * 8 < D)
-        *reinterpret_cast<double2*>(red + (l.kg * 32 + l.own(rb)) * l.ld + n * 8 + 2 * l.t) =
+        *reinterpret_cast<double2*>(red + (l.kg * 32 + l.own(rb)) * ld + n * 8 + 2 * l.t) =
             make_double2(f[rb] * acc[rb][n][0], f[rb] * acc[rb][n][1]);
   __syncthreads();
   for (int i = threadIdx.x; i < rows * D; i += S::THREADS) {
     const int r = i / D, d = i - r * D;
     double x = 0.0;
 #pragma unroll
-    for (int kg = 0; kg < S::KG; ++kg) x += red[(kg * 32 + r) * l.ld + d];
+    for (int kg = 0; kg < S::KG; ++kg) x += red[(kg * 32 + r) * ld + d];
     out[r * stride + d] = (OUT)(scale * x);
   }
 }
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(S::THREADS) fwd64_kernel(const Params<double> 
   __shared__ double top[S::KG][32], total[S::KG][32];
   Part part;
   if (!find_part<32>(p, blockIdx.x, part)) return;
-  const Lane<S> l(p.D);
+  const Lane<S> l(row_length<double>(p.D));
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   double *sQ = smem64, *sK = sQ + 32 * l.ld, *sV = sK + S::TILE * l.ld;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
@@ -187,12 +194,19 @@ __global__ void __launch_bounds__(S::THREADS) fwd64_kernel(const Params<double> 
     m[rb] = neg_inf<double>();
     sum[rb] = 0.0;
   }
-  if (lo < hi) load_rows<double, S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
+  const auto next_k = [&](int k0) {
+    if (k0 < hi) copy_rows<S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
+    end_group();
+  };
+  const auto next_v = [&](int k0) {
+    if (k0 < hi) copy_rows<S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
+    end_group();
+  };
+  if (lo < hi) copy_rows<S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
+  next_k(lo);
+  next_v(lo);
   for (int k0 = lo; k0 < hi; k0 += S::TILE) {
-    __syncthreads();
-    load_rows<double, S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
-    load_rows<double, S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
-    __syncthreads();
+    arrive<1>();
     Scores<S> s;
     zero<S>(s);
     scores<S>(s, l, sQ, sK, p.D);
@@ -228,7 +242,11 @@ __global__ void __launch_bounds__(S::THREADS) fwd64_kernel(const Params<double> 
         acc[rb][n][1] *= f;
       }
     }
+    arrive<0>();
+    next_k(k0 + S::TILE);
     sums<S>(acc, l, s, sV, p.D);
+    __syncthreads();
+    next_v(k0 + S::TILE);
   }
   if (l.t == 0) {
 #pragma unroll
@@ -273,7 +291,7 @@ __global__ void __launch_bounds__(S::THREADS) dq64_kernel(const Params<double> p
   extern __shared__ __align__(16) double smem64[];
   Part part;
   if (!find_part<32>(p, blockIdx.x, part)) return;
-  const Lane<S> l(p.D);
+  const Lane<S> l(row_length<double>(p.D));
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
   double *sQ = smem64, *sO = sQ + 32 * l.ld, *sK = sO + 32 * l.ld, *sV = sK + S::TILE * l.ld;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
@@ -289,20 +307,29 @@ __global__ void __launch_bounds__(S::THREADS) dq64_kernel(const Params<double> p
     D[rb] = row < part.hi ? p.delta[(int64_t)h * p.N + row] : 0.0;
     one[rb] = 1.0;
   }
+  const auto next_k = [&](int k0) {
+    if (k0 < hi) copy_rows<S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
+    end_group();
+  };
+  const auto next_v = [&](int k0) {
+    if (k0 < hi) copy_rows<S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
+    end_group();
+  };
   if (lo < hi) {
-    load_rows<double, S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
-    load_rows<double, S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, part.row, 32, part.hi, p.D);
+    copy_rows<S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
+    copy_rows<S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, part.row, 32, part.hi, p.D);
   }
+  next_v(lo);
+  next_k(lo);
   for (int k0 = lo; k0 < hi; k0 += S::TILE) {
-    __syncthreads();
-    load_rows<double, S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
-    load_rows<double, S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
-    __syncthreads();
+    arrive<1>();
     Scores<S> s, dp;
     zero<S>(s);
     zero<S>(dp);
-    scores<S>(s, l, sQ, sK, p.D);
     scores<S>(dp, l, sO, sV, p.D);
+    arrive<0>();
+    next_v(k0 + S::TILE);
+    scores<S>(s, l, sQ, sK, p.D);
 #pragma unroll
     for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -312,6 +339,8 @@ __global__ void __launch_bounds__(S::THREADS) dq64_kernel(const Params<double> p
         for (int rb = 0; rb < S::RB; ++rb) s[rb][nt][e] = ok ? exp2(s[rb][nt][e] * c2 - L[rb]) * (dp[rb][nt][e] - D[rb]) : 0.0;
       }
     sums<S>(acc, l, s, sK, p.D);
+    __syncthreads();
+    next_k(k0 + S::TILE);
   }
   double* out = p.splits > 1 ? p.work + (int64_t)blockIdx.z * p.N * p.H * p.D : p.out0;
   join_rows<S, double>(smem64, l, acc, one, out + ((int64_t)part.row * p.H + h) * p.D, (int64_t)p.H * p.D, min(32, part.hi - part.row),
@@ -323,7 +352,7 @@ __global__ void __launch_bounds__(S::THREADS) dkv64_kernel(const Params<double> 
   extern __shared__ __align__(16) double smem64[];
   Part part;
   if (!find_part<32>(p, blockIdx.x, part)) return;
-  const Lane<S> l(p.D);
+  const Lane<S> l(row_length<double>(p.D));
   const int hk = blockIdx.y, group = p.H / p.HK;
   double *sK = smem64, *sV = sK + 32 * l.ld, *sQ = sV + 32 * l.ld, *sO = sQ + S::TILE * l.ld;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
@@ -340,21 +369,31 @@ __global__ void __launch_bounds__(S::THREADS) dkv64_kernel(const Params<double> 
     one[rb] = 1.0;
   }
   if (lo < hi) {
-    load_rows<double, S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, part.row, 32, part.hi, p.D, p.mask);
-    load_rows<double, S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, part.row, 32, part.hi, p.D, p.mask);
   }
+  const auto next_q = [&](int h, int q0) {
+    if (q0 < hi) copy_rows<S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, q0, S::TILE, hi, p.D);
+    end_group();
+  };
+  const auto next_o = [&](int h, int q0) {
+    if (q0 < hi) copy_rows<S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, q0, S::TILE, hi, p.D);
+    end_group();
+  };
+  next_o(hk * group, lo);
+  next_q(hk * group, lo);
   for (int gh = 0; gh < group; ++gh) {
     const int h = hk * group + gh;
     for (int q0 = lo; q0 < hi; q0 += S::TILE) {
-      __syncthreads();
-      load_rows<double, S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, q0, S::TILE, hi, p.D);
-      load_rows<double, S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, q0, S::TILE, hi, p.D);
-      __syncthreads();
+      const bool last = q0 + S::TILE >= hi;                                // the next tile is the next head's first, or none
+      const int h1 = last ? h + 1 : h, q1 = !last ? q0 + S::TILE : gh + 1 < group ? lo : hi;
+      arrive<1>();
       Scores<S> s, dp;
       zero<S>(s);
       zero<S>(dp);
-      scores<S>(s, l, sK, sQ, p.D);
       scores<S>(dp, l, sV, sO, p.D);
+      arrive<0>();
+      scores<S>(s, l, sK, sQ, p.D);
 #pragma unroll
       for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -371,7 +410,11 @@ __global__ void __launch_bounds__(S::THREADS) dkv64_kernel(const Params<double> 
           }
         }
       sums<S>(dv, l, s, sO, p.D);
+      __syncthreads();
+      next_o(h1, q1);
       sums<S>(dk, l, dp, sQ, p.D);
+      __syncthreads();
+      next_q(h1, q1);
     }
   }
   const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)part.row * p.HK + hk) * p.D;
@@ -394,10 +437,10 @@ __global__ void __launch_bounds__(S::THREADS) rows64_kernel(const Params<IN> p, 
   __shared__ double share[2][S::KG][32];
   Part part;
   if (!find_part<32>(p, blockIdx.x, part)) return;
-  const Lane<S> l(p.D);
+  const Lane<S> l(row_length<IN>(p.D));
   const int h = blockIdx.y, hk = h / (p.H / p.HK);
-  double *sQ = smem64, *sO = sQ + 32 * l.ld, *sA = sO + 32 * l.ld, *sK = sA + 32 * l.ld, *sV = sK + S::TILE * l.ld,
-         *sB = sV + S::TILE * l.ld, *sC = sB + S::TILE * l.ld;
+  IN *sQ = reinterpret_cast<IN*>(smem64), *sO = sQ + 32 * l.ld, *sA = sO + 32 * l.ld, *sK = sA + 32 * l.ld, *sV = sK + S::TILE * l.ld,
+     *sB = sV + S::TILE * l.ld, *sC = sB + S::TILE * l.ld;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
   split_range<S::TILE>(lo, hi, blockIdx.z, p.splits);
   const double scale = (double)p.scale, c2 = scale * log2e<double>();
@@ -417,28 +460,54 @@ __global__ void __launch_bounds__(S::THREADS) rows64_kernel(const Params<IN> p, 
     R[rb] = U[rb] = 0.0;
     one[rb] = 1.0;
   }
+  const auto next_kb = [&](int k0) {
+    if (k0 < hi) {
+      copy_rows<S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
+      copy_rows<S::THREADS>(sB, l.ld, p.cb + hk * p.cbh, p.cbs, p.cbh, k0, S::TILE, hi, p.D, p.mask);
+    }
+    end_group();
+  };
+  const auto next_vc = [&](int k0) {
+    if (k0 < hi) {
+      copy_rows<S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
+      copy_rows<S::THREADS>(sC, l.ld, p.cc + hk * p.cch, p.ccs, p.cch, k0, S::TILE, hi, p.D, p.mask);
+    }
+    end_group();
+  };
+  // the pair that the walk's last products do not take comes first
+  const auto first = [&](int k0) {
+    if (WALK == 0) next_kb(k0); else next_vc(k0);
+  };
+  const auto second = [&](int k0) {
+    if (WALK == 0) next_vc(k0); else next_kb(k0);
+  };
   if (lo < hi) {
-    load_rows<IN, S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
-    load_rows<IN, S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, part.row, 32, part.hi, p.D);
-    load_rows<IN, S::THREADS>(sA, l.ld, p.ca + h * p.cah, p.cas, p.cah, part.row, 32, part.hi, p.D);
+    copy_rows<S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, part.row, 32, part.hi, p.D);
+    copy_rows<S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, part.row, 32, part.hi, p.D);
+    copy_rows<S::THREADS>(sA, l.ld, p.ca + h * p.cah, p.cas, p.cah, part.row, 32, part.hi, p.D);
   }
+  first(lo);
+  second(lo);
   for (int k0 = lo; k0 < hi; k0 += S::TILE) {
-    __syncthreads();
-    load_rows<IN, S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, k0, S::TILE, hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, k0, S::TILE, hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sB, l.ld, p.cb + hk * p.cbh, p.cbs, p.cbh, k0, S::TILE, hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sC, l.ld, p.cc + hk * p.cch, p.ccs, p.cch, k0, S::TILE, hi, p.D, p.mask);
-    __syncthreads();
+    arrive<1>();
     Scores<S> s, t, dp, e;
     zero<S>(s);
     zero<S>(t);
     zero<S>(dp);
     zero<S>(e);
-    scores<S>(s, l, sQ, sK, p.D);
-    scores<S>(t, l, sA, sK, p.D);
-    scores<S>(t, l, sQ, sB, p.D);
-    scores<S>(dp, l, sO, sV, p.D);
-    scores<S>(e, l, sO, sC, p.D);
+    const auto with_kb = [&] {
+      scores<S>(s, l, sQ, sK, p.D);
+      scores<S>(t, l, sA, sK, p.D);
+      scores<S>(t, l, sQ, sB, p.D);
+    };
+    const auto with_vc = [&] {
+      scores<S>(dp, l, sO, sV, p.D);
+      scores<S>(e, l, sO, sC, p.D);
+    };
+    if (WALK == 0) with_kb(); else with_vc();
+    arrive<0>();
+    first(k0 + S::TILE);
+    if (WALK == 0) with_vc(); else with_kb();
 #pragma unroll
     for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -460,6 +529,8 @@ __global__ void __launch_bounds__(S::THREADS) rows64_kernel(const Params<IN> p, 
       }
     sums<S>(acc, l, s, WALK == 0 ? sV : sK, p.D);
     sums<S>(acc, l, t, WALK == 0 ? sC : sB, p.D);
+    __syncthreads();
+    second(k0 + S::TILE);
   }
   const int rows = min(32, part.hi - part.row);
   if (WALK == 0) {
@@ -544,10 +615,10 @@ __global__ void __launch_bounds__(S::THREADS) keys64_kernel(const Params<IN> p, 
   extern __shared__ __align__(16) double smem64[];
   Part part;
   if (!find_part<32>(p, blockIdx.x, part)) return;
-  const Lane<S> l(p.D);
+  const Lane<S> l(row_length<IN>(p.D));
   const int hk = blockIdx.y, group = p.H / p.HK;
-  double *sK = smem64, *sV = sK + 32 * l.ld, *sB = sV + 32 * l.ld, *sC = sB + 32 * l.ld, *sQ = sC + 32 * l.ld,
-         *sO = sQ + S::TILE * l.ld, *sA = sO + S::TILE * l.ld;
+  IN *sK = reinterpret_cast<IN*>(smem64), *sV = sK + 32 * l.ld, *sB = sV + 32 * l.ld, *sC = sB + 32 * l.ld, *sQ = sC + 32 * l.ld,
+     *sO = sQ + S::TILE * l.ld, *sA = sO + S::TILE * l.ld;
   int lo = part.lo, hi = part.keys ? part.hi : part.lo;
   split_range<S::TILE>(lo, hi, blockIdx.z, p.splits_k);
   const double scale = (double)p.scale, c2 = scale * log2e<double>();
@@ -563,29 +634,41 @@ __global__ void __launch_bounds__(S::THREADS) keys64_kernel(const Params<IN> p, 
     one[rb] = 1.0;
   }
   if (lo < hi) {
-    load_rows<IN, S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, part.row, 32, part.hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, part.row, 32, part.hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sB, l.ld, p.cb + hk * p.cbh, p.cbs, p.cbh, part.row, 32, part.hi, p.D, p.mask);
-    load_rows<IN, S::THREADS>(sC, l.ld, p.cc + hk * p.cch, p.ccs, p.cch, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sK, l.ld, p.k + hk * p.kh, p.ks, p.kh, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sV, l.ld, p.v + hk * p.vh, p.vs, p.vh, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sB, l.ld, p.cb + hk * p.cbh, p.cbs, p.cbh, part.row, 32, part.hi, p.D, p.mask);
+    copy_rows<S::THREADS>(sC, l.ld, p.cc + hk * p.cch, p.ccs, p.cch, part.row, 32, part.hi, p.D, p.mask);
   }
+  const auto next_qa = [&](int h, int q0) {
+    if (q0 < hi) {
+      copy_rows<S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, q0, S::TILE, hi, p.D);
+      copy_rows<S::THREADS>(sA, l.ld, p.ca + h * p.cah, p.cas, p.cah, q0, S::TILE, hi, p.D);
+    }
+    end_group();
+  };
+  const auto next_o = [&](int h, int q0) {
+    if (q0 < hi) copy_rows<S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, q0, S::TILE, hi, p.D);
+    end_group();
+  };
+  next_o(hk * group, lo);
+  next_qa(hk * group, lo);
   for (int gh = 0; gh < group; ++gh) {
     const int h = hk * group + gh;
     for (int q0 = lo; q0 < hi; q0 += S::TILE) {
-      __syncthreads();
-      load_rows<IN, S::THREADS>(sQ, l.ld, p.q + h * p.qh, p.qs, p.qh, q0, S::TILE, hi, p.D);
-      load_rows<IN, S::THREADS>(sO, l.ld, p.go + h * p.goh, p.gos, p.goh, q0, S::TILE, hi, p.D);
-      load_rows<IN, S::THREADS>(sA, l.ld, p.ca + h * p.cah, p.cas, p.cah, q0, S::TILE, hi, p.D);
-      __syncthreads();
+      const bool last = q0 + S::TILE >= hi;                                // the next tile is the next head's first, or none
+      const int h1 = last ? h + 1 : h, q1 = !last ? q0 + S::TILE : gh + 1 < group ? lo : hi;
+      arrive<1>();
       Scores<S> s, t, dp, e;
       zero<S>(s);
       zero<S>(t);
       zero<S>(dp);
       zero<S>(e);
+      scores<S>(dp, l, sV, sO, p.D);
+      scores<S>(e, l, sC, sO, p.D);
+      arrive<0>();
       scores<S>(s, l, sK, sQ, p.D);
       scores<S>(t, l, sK, sA, p.D);
       scores<S>(t, l, sB, sQ, p.D);
-      scores<S>(dp, l, sV, sO, p.D);
-      scores<S>(e, l, sC, sO, p.D);
 #pragma unroll
       for (int nt = 0; nt < S::NT; ++nt)
 #pragma unroll
@@ -603,9 +686,13 @@ __global__ void __launch_bounds__(S::THREADS) keys64_kernel(const Params<IN> p, 
             dp[rb][nt][x] = on ? pr * tt : 0.0;
           }
         }
+      sums<S>(dv, l, dp, sO, p.D);
+      __syncthreads();
+      next_o(h1, q1);
       sums<S>(dk, l, s, sQ, p.D);
       sums<S>(dk, l, t, sA, p.D);
-      sums<S>(dv, l, dp, sO, p.D);
+      __syncthreads();
+      next_qa(h1, q1);
     }
   }
   const int64_t n = (int64_t)p.N * p.HK * p.D, at = ((int64_t)part.row * p.HK + hk) * p.D;
@@ -621,15 +708,15 @@ __global__ void __launch_bounds__(S::THREADS) keys64_kernel(const Params<IN> p, 
 
 // ------------------------------------------------------------------------------------------ launches
 // shared memory: the tiles, or the KG partial results that replace them in the end
-template <class S>
+template <class S, typename IN>
 size_t smem_bytes(int D, int own, int streamed) {
-  const int tiles = own * 32 + streamed * S::TILE, ends = S::KG * 32;
-  return sizeof(double) * row_length(D) * (tiles > ends ? tiles : ends);
+  const size_t tiles = sizeof(IN) * row_length<IN>(D) * (own * 32 + streamed * S::TILE), ends = sizeof(double) * row_length<double>(D) * S::KG * 32;
+  return tiles > ends ? tiles : ends;
 }
 
 template <class S, auto KERNEL, typename T, typename... A>
 cudaError_t launch64(const Params<T>& p, int heads, int splits, int own, int streamed, cudaStream_t s, A... more) {
-  const size_t bytes = smem_bytes<S>(p.D, own, streamed);
+  const size_t bytes = smem_bytes<S, T>(p.D, own, streamed);
   const cudaError_t e = raise_smem_limit<KERNEL>(232448 - 4096);       // the kernels' own static arrays stay below 4 KB
   if (e != cudaSuccess) return e;
   KERNEL<<<dim3(part_blocks(p, 32), heads, splits), S::THREADS, bytes, s>>>(p, more...);
@@ -667,7 +754,7 @@ int64_t second64_words(const Params<IN>& p) {
 
 template <typename IN, int DP, bool NARROW>
 cudaError_t second64_dp(const Params<IN>& p, double* work, cudaStream_t s) {
-  // 113 .. 128 columns: three slices of the keys and half the queries a tile, so that seven tiles fit
+  // float64 of 113 .. 128 columns: three slices of the keys and half the queries a tile, so that seven tiles fit
   using R = Shape<DP, 2, 2, NARROW ? 3 : 4, 1>;
   using K = Shape<DP, 1, 4, 2, NARROW ? 1 : 2>;
   const int64_t rows = (int64_t)p.H * p.N, nq = rows * p.D, nk = (int64_t)p.N * p.HK * p.D;
@@ -692,7 +779,7 @@ cudaError_t second64_dp(const Params<IN>& p, double* work, cudaStream_t s) {
 
 template <typename IN>
 cudaError_t second64(const Params<IN>& p, double* work, cudaStream_t s) {
-  if (p.D > 112) return second64_dp<IN, 128, true>(p, work, s);
+  if (sizeof(IN) == 8 && p.D > 112) return second64_dp<IN, 128, sizeof(IN) == 8>(p, work, s);
   XNN_F64_DIM(p.D, return (second64_dp<IN, DP, false>(p, work, s)))
 }
 
