@@ -234,6 +234,14 @@ def test_few_long_among_many_short(dtype, lens, before):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("width", [3, 31, 64, 65, 96, 113, 128])
+@pytest.mark.parametrize("heads", [(1, 1), (6, 2)])
+def test_short_structures_at_every_width(dtype, width, heads):
+    _run(([3, 32, 1, 17, 0, 30, 8], *heads, width, 0.2, 2), dtype, "cuda")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[12, 30], [40, 600], [500, 900]])
 def test_wrong_bound_is_loud_or_right(lens):
     """A structure longer than ``max_len``: its gradients are right or NaN, the others' are right."""

@@ -203,13 +203,18 @@ __device__ __forceinline__ void tile_nn(T (&acc)[RI][DP / TX], const T* P, int i
 template <typename T, int RI, int J, int TX, int DP, int LDP, int LD>
 __device__ __forceinline__ void tile_tn(T (&acc)[RI][DP / TX], const T* P, int i0, const T* V, int tx, int used = J) {
   using C = Cols<T, DP, TX>;
-  constexpr int W = Vec<T>::W;
+  constexpr int G = RI < Vec<T>::W ? RI : Vec<T>::W;       // columns a load takes
+  struct alignas(G * sizeof(T)) Group { T x[G]; };
   const int end = used < J ? used : J;
 #pragma unroll 4
   for (int j = 0; j < end; ++j) {
     T p[RI];
 #pragma unroll
-    for (int r = 0; r < RI; r += W) *reinterpret_cast<V16<T>*>(p + r) = *reinterpret_cast<const V16<T>*>(P + j * LDP + i0 + r);
+    for (int r = 0; r < RI; r += G) {
+      const Group at = *reinterpret_cast<const Group*>(P + j * LDP + i0 + r);
+#pragma unroll
+      for (int x = 0; x < G; ++x) p[r + x] = at.x[x];
+    }
     const T* row = V + j * LD + tx * C::VW;
 #pragma unroll
     for (int n = 0; n < C::NC; ++n) {
