@@ -185,6 +185,27 @@ def test_hidden_values_do_not_spread(device, lens):
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("lens,width", [([20, 11], 16), ([90, 70], 16), ([90, 70], 72), ([400], 64)])
+def test_no_gradient_where_no_key_is(device, dtype, lens, width):
+    """Rows without an allowed key, with NaN as queries and as incoming gradients (0 / 0 of a padded row), get zeros, and
+    so do masked keys next to valid ones."""
+    q, k, v, do, a, b, c, ptr, _ = _inputs((lens, 2, 1, width, 0.0, 0), dtype, device)
+    mask = torch.ones(sum(lens), dtype=torch.bool, device=device)
+    mask[:lens[0]] = False                       # the first structure has no key
+    mask[lens[0] + 1::3] = False
+    q[:lens[0]], do[:lens[0]] = float("nan"), float("nan")
+    run = lambda *t: structure_attention(*t, ptr, max_len=max(lens), key_mask=mask)  # noqa: E731
+    _, *first = _all(run, q, k, v, do, a, b, c, second=False)
+    _, *both = _all(run, q, k, v, do, a, b, c)
+    for x in first + both:
+        assert not x[:lens[0]].any() and not x.isnan().any()
+    do[lens[0]:] = float("nan")                  # what a masked key hides from the queries, it does not take from them
+    for x in _all(run, q, k, v, do, a, b, c, second=False)[2:]:
+        assert not x[~mask].any()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_large_scores(device):
     """Scores of thousands: the running maximum keeps every power in range, and one key takes all."""
     q, k, v, do, *_, ptr, _ = _inputs(([150, 40], 1, 1, 32, 0.0, 0), torch.float64, device)

@@ -1,5 +1,6 @@
-// Softmax attention over the atoms of each structure of a packed batch, its backward pass and the
-// backward pass of that, on the FP32 / FP64 pipes; the matrix of probabilities never leaves the chip.
+// Softmax attention over the atoms of each structure of a packed batch, its backward pass and the backward pass of that:
+// the formulas, the kernels of short structures on the FP32 / FP64 pipes (attention_tc*.cu and attention_f64.cu hold those of
+// the long ones) and the joins of split walks. The matrix of probabilities never leaves the chip.
 //
 // With S = scale q k^T over the allowed keys of a row's structure (x = S log2 e, so that powers of two
 // serve), P = softmax_row(S), O = P V:
@@ -27,6 +28,16 @@ struct Cfg {
 
 __device__ __forceinline__ bool allowed(int j, int hi, const uint8_t* mask) {
   return j < hi && (mask == nullptr || mask[j]);
+}
+
+// a masked key's gradients are zero whatever its queries hold (0 NaN is NaN)
+template <typename T, int N>
+__device__ __forceinline__ void hide(T (&a)[N], T (&b)[N], bool hidden) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    a[n] = hidden ? T(0) : a[n];
+    b[n] = hidden ? T(0) : b[n];
+  }
 }
 
 // ------------------------------------------------------------------------------------------ forward
@@ -142,23 +153,9 @@ __global__ void __launch_bounds__(256) sum_kernel(int64_t n, int splits, const T
 }
 
 // ------------------------------------------------------------------------------------------ backward
-// D = do.o per row and head: a warp each
-template <typename T>
-__global__ void __launch_bounds__(128) delta_kernel(const Params<T> p) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (i >= (int64_t)p.H * p.N) return;
-  const int h = (int)(i % p.H), row = (int)(i / p.H);
-  const T *a = p.go + (int64_t)row * p.gos + h * p.goh, *b = p.o + (int64_t)row * p.os + h * p.oh;
-  T s = T(0);
-  for (int d = lane; d < p.D; d += 32) s += a[d] * b[d];
-  s = row_sum<32>(s);
-  if (lane == 0) p.delta[(int64_t)h * p.N + row] = s;
-}
-
 // structures of at most BQ atoms: one block holds the whole probability matrix of a head, so that the
 // softmax is formed at once (neither the forward output nor its statistics are read) and dq, dk, dv
-// come from one launch and one reading of the inputs
+// come from one launch and one reading of the inputs (4000 structures of 8-31 atoms x 4 heads x 64: 505 us)
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
   static_assert(C::BQ == C::BK, "square tiles");
@@ -192,12 +189,15 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
       T s[C::RI][C::RJ] = {}, dp[C::RI][C::RJ] = {};
       tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, sQ, i0, sK, tx);
       tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, sO, i0, sV, tx);
+      bool ok[C::RJ];
+#pragma unroll
+      for (int c = 0; c < C::RJ; ++c) ok[c] = allowed(part.row + tx + C::TX * c, part.hi, p.mask);
 #pragma unroll
       for (int r = 0; r < C::RI; ++r) {
         T top = neg_inf<T>();
 #pragma unroll
         for (int c = 0; c < C::RJ; ++c) {
-          s[r][c] = allowed(part.row + tx + C::TX * c, part.hi, p.mask) ? s[r][c] * c2 : neg_inf<T>();
+          s[r][c] = ok[c] ? s[r][c] * c2 : neg_inf<T>();
           top = s[r][c] > top ? s[r][c] : top;
         }
         top = row_max<C::TX>(top);
@@ -206,10 +206,14 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
 #pragma unroll
         for (int c = 0; c < C::RJ; ++c) { s[r][c] = pow2(s[r][c] - base); sum += s[r][c]; }
         sum = row_sum<C::TX>(sum);
-        const T inv = top == neg_inf<T>() || part.row + i0 + r >= part.hi ? T(0) : T(1) / sum;
+        const T inv = (top == neg_inf<T>() && sum == T(0)) || part.row + i0 + r >= part.hi ? T(0) : T(1) / sum;
         T D = T(0);
 #pragma unroll
-        for (int c = 0; c < C::RJ; ++c) { s[r][c] *= inv; D += s[r][c] * dp[r][c]; }
+        for (int c = 0; c < C::RJ; ++c) {
+          s[r][c] = ok[c] ? s[r][c] * inv : T(0);
+          dp[r][c] = ok[c] ? dp[r][c] : T(0);
+          D += s[r][c] * dp[r][c];
+        }
         D = row_sum<C::TX>(D);
 #pragma unroll
         for (int c = 0; c < C::RJ; ++c) {
@@ -233,6 +237,7 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
   for (int r = 0; r < C::RI; ++r) {
     const int row = part.row + i0 + r;
     if (row >= part.hi) continue;
+    hide(dk[r], dv[r], p.mask != nullptr && !p.mask[row]);
     const int64_t at = ((int64_t)row * p.HK + hk) * p.D;
     store_row<T, C::DP, C::TX>(p.out1 + at, dk[r], p.scale * good, p.D, tx);
     store_row<T, C::DP, C::TX>(p.out2 + at, dv[r], good, p.D, tx);
@@ -240,187 +245,125 @@ __global__ void __launch_bounds__(C::NT) bwd_short_kernel(const Params<T> p) {
 }
 
 // ------------------------------------------------------------------------------------------ second derivative
-// rows: q' and do'; the first walk over the keys gives r, c and do', the second q'
+// Structures of at most BQ atoms, as in bwd_short_kernel: 12 products on a structure instead of the 22 of separate walks
+// for do', q' and the keys, no statistics from memory. Four tiles of shared memory serve seven operands: q, k, A, B for the
+// scores, do, v, C in place of the first three for the products with them, then q, k, A again (from L2), which keeps four
+// blocks of 128 threads an SM at 64 columns. 64 structures of 9-30 atoms x 4 heads x 64: 25 us (80 in separate walks), 4000:
+// 1.22 ms (3.91).
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT) second_row_kernel(const Params<T> p) {
+__global__ void __launch_bounds__(C::NT) second_short_kernel(const Params<T> p) {
+  static_assert(C::BQ == C::BK, "square tiles");
   extern __shared__ __align__(16) char smem_raw[];
-  T* sQ = reinterpret_cast<T*>(smem_raw);
-  T* sO = sQ + C::BQ * C::LD;
-  T* sA = sO + C::BQ * C::LD;
-  T* sK = sA + C::BQ * C::LD;
-  T* sV = sK + C::BK * C::LD;
-  T* sB = sV + C::BK * C::LD;
-  T* sC = sB + C::BK * C::LD;
-  T* sP = sC + C::BK * C::LD;
-  T* sS = sP + C::BQ * C::LDP;
+  T* s0 = reinterpret_cast<T*>(smem_raw);
+  T* s1 = s0 + C::BQ * C::LD;
+  T* s2 = s1 + C::BQ * C::LD;
+  T* sB = s2 + C::BQ * C::LD;
+  T* sP = sB + C::BQ * C::LD;                            // P, P (T - r), M, P (dP - D)
+  T* sT = sP + C::BQ * C::LDP;
+  T* sM = sT + C::BQ * C::LDP;
+  T* sS = sM + C::BQ * C::LDP;
   Part part;
   if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
-  const int h = blockIdx.y, hk = h / (p.H / p.HK);
+  const int hk = blockIdx.y, group = p.H / p.HK, used = part.hi - part.row;
   const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
-  const int k_lo = part.lo, k_hi = part.keys ? part.hi : part.lo;
   const T c2 = p.scale * log2e<T>();
-  T L[C::RI], D[C::RI], R[C::RI], U[C::RI], acc[C::RI][C::DP / C::TX];
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) {
-    const int row = part.row + i0 + r;
-    L[r] = row < part.hi ? p.lse[(int64_t)h * p.N + row] : T(0);
-    D[r] = row < part.hi ? p.delta[(int64_t)h * p.N + row] : T(0);
-    R[r] = U[r] = T(0);
-#pragma unroll
-    for (int n = 0; n < C::DP / C::TX; ++n) acc[r][n] = T(0);
-  }
-  if (k_lo < k_hi) {
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sQ, p.q + h * p.qh, p.qs, part.row, part.hi, p.D, vec_ok(p.q, p.qs, p.qh, p.D));
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sO, p.go + h * p.goh, p.gos, part.row, part.hi, p.D, vec_ok(p.go, p.gos, p.goh, p.D));
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sA, p.ca + h * p.cah, p.cas, part.row, part.hi, p.D, vec_ok(p.ca, p.cas, p.cah, p.D));
-  }
-  const bool one = k_hi - k_lo <= C::BK;                 // the second walk finds the keys still in place
-  for (int walk = 0; walk < 2; ++walk) {
-    for (int k0 = k_lo; k0 < k_hi; k0 += C::BK) {
-      if (walk == 0 || !one) {
-        load_tile<T, C::BK, C::DP, C::LD, C::NT>(sK, p.k + hk * p.kh, p.ks, k0, k_hi, p.D, vec_ok(p.k, p.ks, p.kh, p.D), p.mask);
-        load_tile<T, C::BK, C::DP, C::LD, C::NT>(sV, p.v + hk * p.vh, p.vs, k0, k_hi, p.D, vec_ok(p.v, p.vs, p.vh, p.D), p.mask);
-        load_tile<T, C::BK, C::DP, C::LD, C::NT>(sB, p.cb + hk * p.cbh, p.cbs, k0, k_hi, p.D, vec_ok(p.cb, p.cbs, p.cbh, p.D), p.mask);
-        load_tile<T, C::BK, C::DP, C::LD, C::NT>(sC, p.cc + hk * p.cch, p.ccs, k0, k_hi, p.D, vec_ok(p.cc, p.ccs, p.cch, p.D), p.mask);
-      }
+  const bool keys = part.keys;
+  const T good = keys && part.hi - part.lo > C::BQ ? std::numeric_limits<T>::quiet_NaN() : T(1);
+  T dk[C::RI][C::DP / C::TX] = {}, dv[C::RI][C::DP / C::TX] = {};
+  const auto tile = [&](T* to, const T* g, int64_t rs, int64_t hs, int head, const uint8_t* mask) {
+    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(to, g + head * hs, rs, part.row, part.hi, p.D, vec_ok(g, rs, hs, p.D), mask);
+  };
+  if (keys) tile(sB, p.cb, p.cbs, p.cbh, hk, p.mask);
+  for (int g = 0; g < group; ++g) {
+    const int h = hk * group + g;
+    T dq[C::RI][C::DP / C::TX] = {}, dout[C::RI][C::DP / C::TX] = {};
+    if (keys) {
+      tile(s0, p.q, p.qs, p.qh, h, nullptr);
+      tile(s1, p.k, p.ks, p.kh, hk, p.mask);
+      tile(s2, p.ca, p.cas, p.cah, h, nullptr);
       __syncthreads();
       T s[C::RI][C::RJ] = {}, t[C::RI][C::RJ] = {}, dp[C::RI][C::RJ] = {}, e[C::RI][C::RJ] = {};
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, sQ, i0, sK, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, sA, i0, sK, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, sQ, i0, sB, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, sO, i0, sV, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(e, sO, i0, sC, tx);
+      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, s0, i0, s1, tx);
+      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, s2, i0, s1, tx);
+      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, s0, i0, sB, tx);
+      __syncthreads();
+      tile(s0, p.go, p.gos, p.goh, h, nullptr);
+      tile(s1, p.v, p.vs, p.vh, hk, p.mask);
+      tile(s2, p.cc, p.ccs, p.cch, hk, p.mask);
+      __syncthreads();
+      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, s0, i0, s1, tx);
+      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(e, s0, i0, s2, tx);
+      bool ok[C::RJ];
 #pragma unroll
-      for (int c = 0; c < C::RJ; ++c) {
-        const bool ok = allowed(k0 + tx + C::TX * c, k_hi, p.mask);
+      for (int c = 0; c < C::RJ; ++c) ok[c] = allowed(part.row + tx + C::TX * c, part.hi, p.mask);
 #pragma unroll
-        for (int r = 0; r < C::RI; ++r) {
-          const T pr = ok ? pow2(s[r][c] * c2 - L[r]) : T(0);
-          const T tt = t[r][c] * p.scale;
-          T a, b;
-          if (walk == 0) {
-            a = pr * tt;
-            b = pr;
-            R[r] += a;
-            U[r] += pr * (tt * dp[r][c] + e[r][c]);
-          } else {
-            a = pr * ((tt - R[r]) * (dp[r][c] - D[r]) + e[r][c] - U[r]);
-            b = pr * (dp[r][c] - D[r]);
-          }
-          sP[(i0 + r) * C::LDP + tx + C::TX * c] = ok ? a : T(0);
-          sS[(i0 + r) * C::LDP + tx + C::TX * c] = ok ? b : T(0);
+      for (int r = 0; r < C::RI; ++r) {
+        T top = neg_inf<T>();
+#pragma unroll
+        for (int c = 0; c < C::RJ; ++c) {
+          s[r][c] = ok[c] ? s[r][c] * c2 : neg_inf<T>();
+          top = s[r][c] > top ? s[r][c] : top;
+        }
+        top = row_max<C::TX>(top);
+        const T base = top == neg_inf<T>() ? T(0) : top;
+        T sum = T(0);
+#pragma unroll
+        for (int c = 0; c < C::RJ; ++c) { s[r][c] = pow2(s[r][c] - base); sum += s[r][c]; }
+        sum = row_sum<C::TX>(sum);
+        const T inv = (top == neg_inf<T>() && sum == T(0)) || part.row + i0 + r >= part.hi ? T(0) : T(1) / sum;
+        T D = T(0), R = T(0), U = T(0);
+#pragma unroll
+        for (int c = 0; c < C::RJ; ++c) {
+          s[r][c] = ok[c] ? s[r][c] * inv : T(0);
+          t[r][c] *= p.scale;
+          D += ok[c] ? s[r][c] * dp[r][c] : T(0);
+          R += ok[c] ? s[r][c] * t[r][c] : T(0);
+          U += ok[c] ? s[r][c] * (t[r][c] * dp[r][c] + e[r][c]) : T(0);
+        }
+        D = row_sum<C::TX>(D);
+        R = row_sum<C::TX>(R);
+        U = row_sum<C::TX>(U) - D * R;
+#pragma unroll
+        for (int c = 0; c < C::RJ; ++c) {
+          const int w = (i0 + r) * C::LDP + tx + C::TX * c;
+          sP[w] = s[r][c];
+          sT[w] = ok[c] ? s[r][c] * (t[r][c] - R) : T(0);
+          sM[w] = ok[c] ? s[r][c] * ((t[r][c] - R) * (dp[r][c] - D) + e[r][c] - U) : T(0);
+          sS[w] = ok[c] ? s[r][c] * (dp[r][c] - D) : T(0);
         }
       }
       __syncthreads();
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sP, i0, walk == 0 ? sV : sK, tx);
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(acc, sS, i0, walk == 0 ? sC : sB, tx);
+      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dout, sT, i0, s1, tx, used);
+      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dout, sP, i0, s2, tx, used);
+      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dv, sT, i0, s0, tx, used);
+      __syncthreads();
+      tile(s0, p.q, p.qs, p.qh, h, nullptr);
+      tile(s1, p.k, p.ks, p.kh, hk, p.mask);
+      tile(s2, p.ca, p.cas, p.cah, h, nullptr);
+      __syncthreads();
+      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dq, sM, i0, s1, tx, used);
+      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dq, sS, i0, sB, tx, used);
+      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sM, i0, s0, tx, used);
+      tile_tn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sS, i0, s2, tx, used);
       __syncthreads();
     }
 #pragma unroll
     for (int r = 0; r < C::RI; ++r) {
       const int row = part.row + i0 + r;
-      const bool in = row < part.hi;
-      T* out = (walk == 0 ? p.out3 : p.out0) + ((int64_t)row * p.H + h) * p.D;
-      if (walk == 0) {
-        R[r] = row_sum<C::TX>(R[r]);
-        U[r] = row_sum<C::TX>(U[r]) - D[r] * R[r];
-        if (in) {
-          using K = Cols<T, C::DP, C::TX>;
-          const T* o = p.o + (int64_t)row * p.os + h * p.oh;
-#pragma unroll
-          for (int n = 0; n < K::NC; ++n)
-#pragma unroll
-            for (int w = 0; w < K::VW; ++w) {
-              const int d = n * C::TX * K::VW + tx * K::VW + w;
-              if (d < p.D) acc[r][n * K::VW + w] -= R[r] * o[d];
-            }
-          if (tx == 0) {
-            p.r[(int64_t)h * p.N + row] = R[r];
-            p.c[(int64_t)h * p.N + row] = U[r];
-          }
-        }
-      }
-      if (in) store_row<T, C::DP, C::TX>(out, acc[r], walk == 0 ? T(1) : p.scale, p.D, tx);
-#pragma unroll
-      for (int n = 0; n < C::DP / C::TX; ++n) acc[r][n] = T(0);
-    }
-  }
-}
-
-// keys: k' and v' of BQ keys of one key head, over the queries of every head that shares it
-template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT) second_key_kernel(const Params<T> p) {
-  extern __shared__ __align__(16) char smem_raw[];
-  T* sK = reinterpret_cast<T*>(smem_raw);
-  T* sV = sK + C::BQ * C::LD;
-  T* sB = sV + C::BQ * C::LD;
-  T* sC = sB + C::BQ * C::LD;
-  T* sQ = sC + C::BQ * C::LD;
-  T* sO = sQ + C::BK * C::LD;
-  T* sA = sO + C::BK * C::LD;
-  T* sM = sA + C::BK * C::LD;
-  T* sS = sM + C::BQ * C::LDP;
-  T* sT = sS + C::BQ * C::LDP;
-  Part part;
-  if (!find_part<C::BQ>(p, blockIdx.x, part)) return;
-  const int hk = blockIdx.y, group = p.H / p.HK;
-  const int tx = threadIdx.x % C::TX, i0 = threadIdx.x / C::TX * C::RI;
-  const int q_lo = part.lo, q_hi = part.keys ? part.hi : part.lo;
-  const T c2 = p.scale * log2e<T>();
-  T dk[C::RI][C::DP / C::TX] = {}, dv[C::RI][C::DP / C::TX] = {};
-  bool ok[C::RI];
-#pragma unroll
-  for (int r = 0; r < C::RI; ++r) ok[r] = allowed(part.row + i0 + r, part.hi, p.mask);
-  if (q_lo < q_hi) {
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sK, p.k + hk * p.kh, p.ks, part.row, part.hi, p.D, vec_ok(p.k, p.ks, p.kh, p.D), p.mask);
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sV, p.v + hk * p.vh, p.vs, part.row, part.hi, p.D, vec_ok(p.v, p.vs, p.vh, p.D), p.mask);
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sB, p.cb + hk * p.cbh, p.cbs, part.row, part.hi, p.D, vec_ok(p.cb, p.cbs, p.cbh, p.D), p.mask);
-    load_tile<T, C::BQ, C::DP, C::LD, C::NT>(sC, p.cc + hk * p.cch, p.ccs, part.row, part.hi, p.D, vec_ok(p.cc, p.ccs, p.cch, p.D), p.mask);
-  }
-  for (int g = 0; g < group; ++g) {
-    const int h = hk * group + g;
-    for (int q0 = q_lo; q0 < q_hi; q0 += C::BK) {
-      load_tile<T, C::BK, C::DP, C::LD, C::NT>(sQ, p.q + h * p.qh, p.qs, q0, q_hi, p.D, vec_ok(p.q, p.qs, p.qh, p.D));
-      load_tile<T, C::BK, C::DP, C::LD, C::NT>(sO, p.go + h * p.goh, p.gos, q0, q_hi, p.D, vec_ok(p.go, p.gos, p.goh, p.D));
-      load_tile<T, C::BK, C::DP, C::LD, C::NT>(sA, p.ca + h * p.cah, p.cas, q0, q_hi, p.D, vec_ok(p.ca, p.cas, p.cah, p.D));
-      __syncthreads();
-      T s[C::RI][C::RJ] = {}, t[C::RI][C::RJ] = {}, dp[C::RI][C::RJ] = {}, e[C::RI][C::RJ] = {};
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(s, sK, i0, sQ, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, sK, i0, sA, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(t, sB, i0, sQ, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(dp, sV, i0, sO, tx);
-      tile_nt<T, C::RI, C::RJ, C::TX, C::DP, C::LD>(e, sC, i0, sO, tx);
-#pragma unroll
-      for (int c = 0; c < C::RJ; ++c) {
-        const int row = q0 + tx + C::TX * c;
-        const bool in = row < q_hi;
-        const int64_t at = (int64_t)h * p.N + (in ? row : q_lo);
-        const T L = p.lse[at], D = p.delta[at], R = p.r[at], U = p.c[at];
-#pragma unroll
-        for (int r = 0; r < C::RI; ++r) {
-          const bool on = in && ok[r];
-          const T pr = on ? pow2(s[r][c] * c2 - L) : T(0);
-          const T tt = t[r][c] * p.scale;
-          const int w = (i0 + r) * C::LDP + tx + C::TX * c;
-          sM[w] = on ? pr * ((tt - R) * (dp[r][c] - D) + e[r][c] - U) : T(0);
-          sS[w] = on ? pr * (dp[r][c] - D) : T(0);
-          sT[w] = on ? pr * (tt - R) : T(0);
-        }
-      }
-      __syncthreads();
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sM, i0, sQ, tx);
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dk, sS, i0, sA, tx);
-      tile_nn<T, C::RI, C::BK, C::TX, C::DP, C::LDP, C::LD>(dv, sT, i0, sO, tx);
-      __syncthreads();
+      if (row >= part.hi) continue;
+      const int64_t at = ((int64_t)row * p.H + h) * p.D;
+      store_row<T, C::DP, C::TX>(p.out0 + at, dq[r], p.scale * good, p.D, tx);
+      store_row<T, C::DP, C::TX>(p.out3 + at, dout[r], good, p.D, tx);
     }
   }
 #pragma unroll
   for (int r = 0; r < C::RI; ++r) {
     const int row = part.row + i0 + r;
     if (row >= part.hi) continue;
+    hide(dk[r], dv[r], p.mask != nullptr && !p.mask[row]);
     const int64_t at = ((int64_t)row * p.HK + hk) * p.D;
-    store_row<T, C::DP, C::TX>(p.out1 + at, dk[r], p.scale, p.D, tx);
-    store_row<T, C::DP, C::TX>(p.out2 + at, dv[r], T(1), p.D, tx);
+    store_row<T, C::DP, C::TX>(p.out1 + at, dk[r], p.scale * good, p.D, tx);
+    store_row<T, C::DP, C::TX>(p.out2 + at, dv[r], good, p.D, tx);
   }
 }
 
@@ -436,21 +379,17 @@ cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, 
   return cudaGetLastError();
 }
 
-// The square tiles of 32 rows. float: a 2 x 4 corner of the scores a thread (one molecule of 21 atoms at 64 columns:
-// 6.1 us with 128 threads, 9.1 with 64 and 4 x 4 corners; 4000 x 4 heads: 236 and 279 us). double: 2 x 2, since the
-// accumulators of 4 x 4 alone would take 128 registers at 128 columns.
+// The square tiles of 32 rows. float: a 2 x 4 corner of the scores a thread (one molecule of 21 atoms at 64 columns: 5 us with
+// 128 threads, 9 with 64 and 4 x 4 corners; 4000 x 4 heads: 253 and 279 us, of 97 to move the data: what is read from shared
+// memory bounds it). double: 2 x 2, since the accumulators of 4 x 4 alone would take 128 registers at 128 columns.
 template <typename T, int DP> struct Small;
 template <int DP> struct Small<float, DP> { using C = Cfg<float, 32, 32, DP, 2, 8>; };
 template <int DP> struct Small<double, DP> { using C = Cfg<double, 32, 32, DP, 2, 16>; };
-// The short backward pass has five products on a tile and reads less of it with 4 x 4 corners, up to 64 columns (64: 532
-// and 565 us for 4000 x 4 heads; 128: 186 and, with 256 threads, 153 us for 2000).
+// the short backward pass at 128 float columns: 256 threads (2000 structures: 138 us against 186 with 128 threads). Corners of
+// 4 x 4 read less of the tiles, but leave half the warps (64 columns, 4000 x 4 heads: 531 us against 505; 512 structures of one
+// head: 27 and 23).
 template <typename T, int DP> struct Short { using C = typename Small<T, DP>::C; };
-template <int DP> struct Short<float, DP> { using C = Cfg<float, 32, 32, DP, 4, 8>; };
 template <> struct Short<float, 128> { using C = Cfg<float, 32, 32, 128, 2, 16>; };
-// the second derivative holds seven tiles: 128 double columns leave room for 16 streamed rows
-template <typename T, int DP> struct Second { using C = typename Small<T, DP>::C; };
-template <int DP> struct Second<float, DP> { using C = Cfg<float, 32, 64, DP, 2, 16>; };
-template <> struct Second<double, 128> { using C = Cfg<double, 32, 16, 128, 2, 16>; };
 
 #define XNN_ATTN_DIM(D_, ...)                            \
   if ((D_) <= 32) { constexpr int DP = 32; __VA_ARGS__; } \
@@ -475,32 +414,20 @@ cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out0, T* out1, c
   return cudaGetLastError();
 }
 template <typename T>
-cudaError_t row_delta(const Params<T>& p, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.H * p.N;
-  delta_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
-  return cudaGetLastError();
-}
-template <typename T>
 cudaError_t backward_short(const Params<T>& p, cudaStream_t s) {
   XNN_ATTN_DIM(p.D, using C = typename Short<T, DP>::C; return (launch<T, C, bwd_short_kernel<T, C>>(p, p.HK, 2, 2, 2, s)))
 }
 template <typename T>
-cudaError_t second_rows(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C, second_row_kernel<T, C>>(p, p.H, 3, 4, 2, s)))
-}
-template <typename T>
-cudaError_t second_keys(const Params<T>& p, cudaStream_t s) {
-  XNN_ATTN_DIM(p.D, using C = typename Second<T, DP>::C; return (launch<T, C, second_key_kernel<T, C>>(p, p.HK, 4, 3, 3, s)))
+cudaError_t second_short(const Params<T>& p, cudaStream_t s) {
+  XNN_ATTN_DIM(p.D, using C = typename Small<T, DP>::C; return (launch<T, C, second_short_kernel<T, C>>(p, p.HK, 2, 2, 4, s)))
 }
 
 #define XNN_ATTN_INST(T)                                                                  \
   template cudaError_t forward<T>(const Params<T>&, cudaStream_t);                        \
   template cudaError_t forward_join<T>(const Params<T>&, cudaStream_t);                   \
   template cudaError_t sum_splits<T>(int64_t, int, const T*, T*, T*, cudaStream_t);       \
-  template cudaError_t row_delta<T>(const Params<T>&, cudaStream_t);                      \
   template cudaError_t backward_short<T>(const Params<T>&, cudaStream_t);                 \
-  template cudaError_t second_rows<T>(const Params<T>&, cudaStream_t);                    \
-  template cudaError_t second_keys<T>(const Params<T>&, cudaStream_t);
+  template cudaError_t second_short<T>(const Params<T>&, cudaStream_t);
 XNN_ATTN_INST(float)
 XNN_ATTN_INST(double)
 

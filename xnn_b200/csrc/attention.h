@@ -10,10 +10,8 @@ template <typename T> struct Params;
 template <typename T> cudaError_t forward(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t forward_join(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t sum_splits(int64_t n, int splits, const T* work, T* out0, T* out1, cudaStream_t);
-template <typename T> cudaError_t row_delta(const Params<T>&, cudaStream_t);
 template <typename T> cudaError_t backward_short(const Params<T>&, cudaStream_t);
-template <typename T> cudaError_t second_rows(const Params<T>&, cudaStream_t);
-template <typename T> cudaError_t second_keys(const Params<T>&, cudaStream_t);
+template <typename T> cudaError_t second_short(const Params<T>&, cudaStream_t);
 
 // float64 on the FP64 tensor instructions, and the second derivative of wide float32 heads in 64 bits (attention_f64.cu)
 cudaError_t forward64(const Params<double>&, cudaStream_t);

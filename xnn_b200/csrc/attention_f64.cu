@@ -102,6 +102,18 @@ __device__ __forceinline__ void clear(Sums<S>& x) {
     for (int n = 0; n < S::DP / 8; ++n) x[rb][n][0] = x[rb][n][1] = 0.0;
 }
 
+// a masked key's gradients are zero whatever its queries hold (0 NaN is NaN)
+template <class S>
+__device__ __forceinline__ void hide(Sums<S>& x, const bool (&ok)[S::RB]) {
+#pragma unroll
+  for (int rb = 0; rb < S::RB; ++rb)
+#pragma unroll
+    for (int n = 0; n < S::DP / 8; ++n) {
+      x[rb][n][0] = ok[rb] ? x[rb][n][0] : 0.0;
+      x[rb][n][1] = ok[rb] ? x[rb][n][1] : 0.0;
+    }
+}
+
 // x += own rows of A times streamed rows of B
 template <class S, typename IN>
 __device__ __forceinline__ void scores(Scores<S>& x, const Lane<S>& l, const IN* A, const IN* B, int D) {
@@ -417,6 +429,8 @@ __global__ void __launch_bounds__(S::THREADS) dkv64_kernel(const Params<double> 
       next_q(h1, q1);
     }
   }
+  hide<S>(dk, ok);
+  hide<S>(dv, ok);
   const int64_t all = (int64_t)p.N * p.HK * p.D, at = ((int64_t)part.row * p.HK + hk) * p.D;
   double *ok_ = p.out1, *ov_ = p.out2;
   if (p.splits_k > 1) {
@@ -695,6 +709,8 @@ __global__ void __launch_bounds__(S::THREADS) keys64_kernel(const Params<IN> p, 
       next_qa(h1, q1);
     }
   }
+  hide<S>(dk, ok);
+  hide<S>(dv, ok);
   const int64_t n = (int64_t)p.N * p.HK * p.D, at = ((int64_t)part.row * p.HK + hk) * p.D;
   const int rows = min(32, part.hi - part.row);
   if (p.splits_k == 1) {

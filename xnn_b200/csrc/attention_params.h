@@ -15,7 +15,7 @@ struct Params {
   const int64_t* ptr;
   const uint8_t* mask;               // 1 where an atom may be attended to, or null
   T *out0, *out1, *out2, *out3;      // contiguous outputs
-  T *lse, *delta, *r, *c;            // (H, N) row statistics
+  T *lse, *delta;                    // (H, N) row statistics
   T *work, *work_k;                  // partial results of split passes: over keys, over queries
   T scale;
   int N, num, H, HK, D, splits, splits_k;

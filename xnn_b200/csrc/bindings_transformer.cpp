@@ -273,16 +273,7 @@ std::vector<torch::Tensor> second_typed(const torch::Tensor& a, const torch::Ten
       XNN_OK(attn::second64<T>(pl, work.data_ptr<double>(), s));
     }
   }
-  if (plan.short_ones) {
-    auto ps = short_part(p, plan);
-    torch::Tensor stats = torch::empty({3, p.H, p.N}, q.options());
-    ps.delta = stats.data_ptr<T>();
-    ps.r = ps.delta + (int64_t)p.H * p.N;
-    ps.c = ps.r + (int64_t)p.H * p.N;
-    XNN_OK(attn::row_delta<T>(ps, s));
-    XNN_OK(attn::second_rows<T>(ps, s));
-    XNN_OK(attn::second_keys<T>(ps, s));
-  }
+  if (plan.short_ones) XNN_OK(attn::second_short<T>(short_part(p, plan), s));
   return {q2, k2, v2, do2};
 }
 
