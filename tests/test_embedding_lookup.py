@@ -83,6 +83,13 @@ def test_refusals(device):
             embedding_lookup(table, ids.cpu())
 
 
+def test_module_refuses_what_it_would_ignore():
+    for wrong in (dict(padding_idx=0), dict(padding_idx=2), dict(max_norm=1.0), dict(sparse=True), dict(scale_grad_by_freq=True)):
+        with pytest.raises(ValueError):
+            ScaledEmbedding(3, 4, **wrong)
+    assert ScaledEmbedding(3, 4, padding_idx=None, sparse=False).weight.shape == (3, 4)
+
+
 def test_module_keeps_the_parameter_name():
     m = ScaledEmbedding(5, 3, scale=2.0)
     assert list(m.state_dict()) == ["weight"]

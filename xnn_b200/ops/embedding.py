@@ -74,7 +74,7 @@ class ScaledEmbedding(nn.Embedding):
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, **kwargs):
         for name in ("padding_idx", "max_norm", "sparse", "scale_grad_by_freq"):
-            if kwargs.get(name):
+            if kwargs.get(name) is not None and kwargs[name] is not False:      # padding_idx=0 is a request too
                 raise ValueError(f"ScaledEmbedding does not take {name}")
         super().__init__(num_embeddings, embedding_dim, **kwargs)
         self.scale = float(scale)
