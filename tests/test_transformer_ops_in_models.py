@@ -6,7 +6,7 @@ from torch import nn
 from xnn_b200.data import collate, structure_to_graph, synthetic
 from xnn_b200.models import ForceStressOutput
 from xnn_b200.models.equiformer_v2 import EquiformerV2
-from xnn_b200.models.spookynet import NonlocalInteraction, SpookyNet, structure_slots
+from xnn_b200.models.spookynet import NonlocalInteraction, PackedAtoms, SpookyNet, structure_slots
 from xnn_b200.ops import CounterDropout, ScaledEmbedding, structure_attention
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -117,6 +117,38 @@ def test_nonlocal_interaction(device, heads):
             on = b == s
             w = torch.softmax(torch.einsum("ihc,jhc->hij", q[on], k[on]) / (16 // heads) ** 0.5, -1)
             assert torch.allclose(got[on], torch.einsum("hij,jhc->ihc", w, v[on]).flatten(1), rtol=0, atol=1e-12)
+
+
+def test_packed_atoms():
+    """First rows, order and places, for one structure without reading anything back."""
+    one = PackedAtoms(torch.zeros(5, dtype=torch.long), 1, torch.arange(5), 5)
+    assert one.ptr.tolist() == [0, 5] and one.ptr.dtype == torch.int64 and one.order is None
+    mixed = PackedAtoms(torch.tensor([1, 0, 1, 2, 0]), 4, torch.tensor([0, 0, 1, 0, 1]), 2)
+    assert mixed.ptr.tolist() == [0, 2, 4, 5, 5]
+    assert mixed.order.tolist() == [1, 4, 0, 2, 3] and mixed.place.tolist() == [2, 0, 3, 4, 1]
+
+
+@pytest.mark.gpu
+def test_one_structure_is_captured():
+    torch.manual_seed(3)
+    layer = NonlocalInteraction(16, 1, None, heads=2).cuda()
+    for mlp in (layer.resmlp_q, layer.resmlp_k, layer.resmlp_v):
+        for p in mlp.parameters():
+            torch.nn.init.normal_(p, std=0.3)
+    x, batch, slot = torch.randn(40, 16, device="cuda"), torch.zeros(40, dtype=torch.long, device="cuda"), torch.arange(40, device="cuda")
+    run = lambda: layer(x, batch, 1, slot, 40)  # noqa: E731
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        x.copy_(torch.randn(40, 16, device="cuda"))
+        graph.replay()
+        assert torch.equal(out, run()) and bool(out.any())
 
 
 def test_spookynet_options():

@@ -282,10 +282,13 @@ class PackedAtoms:
     in it already), every atom's place in it, the largest structure."""
 
     def __init__(self, batch: Tensor, num_graphs: int, slot: Tensor, n_max: int):
+        self.n_max, self.order, self.place = int(n_max), None, None
+        if num_graphs == 1:                          # nothing is read back: a single structure's step can be captured
+            self.ptr = torch.arange(2, device=batch.device) * batch.shape[0]
+            return
         counts = torch.bincount(batch, minlength=num_graphs)
         self.ptr = torch.cat([counts.new_zeros(1), torch.cumsum(counts, 0)])
-        self.n_max, self.order, self.place = int(n_max), None, None
-        if num_graphs > 1 and bool((batch[1:] < batch[:-1]).any()):
+        if bool((batch[1:] < batch[:-1]).any()):
             self.order = torch.argsort(batch, stable=True)
             self.place = self.ptr[batch] + slot
 
