@@ -121,7 +121,8 @@ def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -
 class CounterDropout(nn.Module):
     """:func:`counter_dropout` in training mode with its own seed (drawn from PyTorch's generator when
     omitted) and an offset that each call advances. The two numbers live on the module's device, so a
-    captured training step draws a new mask at every replay."""
+    captured training step draws a new mask at every replay. Processes that start from one seed draw the
+    same masks, each for its own rows."""
 
     def __init__(self, p: float, shared: Sequence[int] = (), seed: Optional[int] = None):
         super().__init__()
