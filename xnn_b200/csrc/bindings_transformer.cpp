@@ -74,22 +74,23 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
   return p;
 }
 
-// Which kernels take a call. Structures of at most SHORT atoms fill a square tile of the FP32 pipes; the tensor cores
-// own 128 rows at a time, most of them empty for such a structure, but cost little more for the first 128. float32:
-//   all within SHORT            the short kernels
-//   TC_AVERAGE atoms on average the tensor cores for all; 64 structures of 24-40 atoms at 64 columns, forward /
-//                               backward / second: 11 / 26 / 61 us, short and 64-row FP32 tiles 14 / 44 / 50; of 48-80
-//                               atoms 14 / 33 / 79 and 16 / 48 / 146; 400 x 2 heads of 24-40: 38 / 131 / 274 and 32 / 102 / 298
-//   otherwise                   tensor cores for the structures above SHORT, then the short kernels for the rest
-// float64 goes by the same rule between its short kernels and the FP64 tensor instructions.
-constexpr int TC_AVERAGE = 32, TC_WIDTH = 128, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
+// Which kernels take a call. Structures of at most SHORT atoms fill a square tile of the FP32 / FP64 pipes; the tensor cores
+// own 128 rows at a time (float64: 32), most of them empty for such a structure.
+//   all within SHORT                       the short kernels
+//   one wave of structures and heads, or
+//   LONG_AVERAGE atoms on average          the tensor cores for all
+//   otherwise                              the tensor cores for the structures above SHORT, the short kernels for the rest
+// Both ways, for all / in two launches, forward, backward, second derivative at 64 columns in us: 64 structures of 9-40 atoms,
+// one head 11, 17, 39 / 16, 27, 55; of 400 x 2 heads 37, 138, 259 / 35, 77, 172; of 20-60 atoms 41, 149, 306 / 47, 135, 278.
+// float64: 11, 29, 73 / 20, 44, 105; 74, 183, 371 / 66, 142, 343; 103, 263, 618 / 108, 253, 615.
+constexpr int LONG_AVERAGE = 40, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
 
 struct Plan { bool long_ones, short_ones; };
 
 template <typename T>
 Plan choose(const attn::Params<T>& p, int64_t max_len) {
   if (max_len <= SHORT) return {false, true};
-  return {true, (int64_t)p.N < TC_AVERAGE * (int64_t)p.num};
+  return {true, (int64_t)p.N < LONG_AVERAGE * (int64_t)p.num && (int64_t)p.num * p.H > SMS};
 }
 
 // The parameters of the two launches: the long structures, the short ones (with the rows of none, where both run). The
