@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(p_ready, 8);
+    tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(ROW_THREADS, Fwd<DP>::BLOCKS) tc_fwd_kernel(co
         for (int i = max(0, loaded_v - 2); i < loaded_v; ++i) tc::mbar_wait(full_v + (i & 1), (i >> 1) & 1, SPINS);
       }
     }
-    __syncwarp();
+    drain(bars + DRAINED);
   } else {
     float f = 1.f;
     const auto add = [&] {                              // P V of the tile before, relative to its maximum
@@ -330,6 +331,7 @@ __device__ __forceinline__ Block set_up(char* smem) {
     tc::mbar_init(k.bars + 1, 1);
     tc::mbar_init(k.bars + 2, 8);
     tc::mbar_init(k.bars + 3, 8);
+    tc::mbar_init(k.full + DRAINED, 1);
     *k.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -420,7 +422,7 @@ __device__ __forceinline__ void dq_block(const Params<float>& p, const Part& par
       if (!ok)
         for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);
     }
-    __syncwarp();
+    drain(k.full + DRAINED);
   } else {
     const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
     const int half = k.warp / 4, r = threadIdx.x & 127, row = part.row + r;
@@ -552,7 +554,7 @@ __device__ __forceinline__ void dkv_block(const Params<float>& p, const Part& pa
       if (!ok)
         for (int i = max(0, loaded - STAGES); i < loaded; ++i) tc::mbar_wait(k.full + i % STAGES, (i / STAGES) & 1, SPINS);
     }
-    __syncwarp();
+    drain(k.full + DRAINED);
   } else {
     const uint32_t lanes = k.tmem + ((uint32_t)(k.warp & 3) << 21);
     const int half = k.warp / 4, row = part.row + (threadIdx.x & 127);

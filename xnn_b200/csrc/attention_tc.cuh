@@ -292,6 +292,15 @@ __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, wait(bar, parity, dead, status));
 }
 
+// The issuing warp's last step: all its products are complete (or a limit ran out), whoever gave up, so that tensor memory
+// may be freed and the images overwritten. The barrier takes the last eight of the 128 bytes that each block has for them.
+constexpr int DRAINED = 15;
+__device__ __forceinline__ void drain(uint64_t* bar) {
+  if (elect()) tc::commit_to(bar);
+  __syncwarp();
+  tc::mbar_wait(bar, 0, SPINS);
+}
+
 // The two warps that share a quarter of the lanes (one half of a row's columns each) meet. No wait of their loops lies
 // between the meeting and the loop's next turn, so a warp that leaves its loop early owes its partner one arrival: the
 // partner then finds the block given up at its next wait.

@@ -47,6 +47,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
+    tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -120,7 +121,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
       if (!ok)
         for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
     }
-    __syncwarp();
+    drain(bars + DRAINED);
   } else {
     const float c2 = p.scale * log2e<float>();
     float L = -neg_inf<float>(), D = 0.f, r = 0.f, c = 0.f;
@@ -275,6 +276,7 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   if (threadIdx.x == 0) {
     for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
+    tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -348,7 +350,7 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
         for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
       }
     }
-    __syncwarp();
+    drain(bars + DRAINED);
   } else {
     const float c2 = p.scale * log2e<float>();
     float acc[DP];                                      // the first half of the warps adds up k', the second v'

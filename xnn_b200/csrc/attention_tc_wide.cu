@@ -47,6 +47,7 @@ __device__ __forceinline__ void wide_block(const Params<float>& p, const Part& p
     for (int i = 0; i < 8; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(taken, 8);
     tc::mbar_init(ready, 8);
+    tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -127,7 +128,7 @@ __device__ __forceinline__ void wide_block(const Params<float>& p, const Part& p
         for (int i = max(0, loaded_y - 3); i < loaded_y; ++i) tc::mbar_wait(full_y + i % 3, (i / 3) & 1, SPINS);
       }
     }
-    __syncwarp();
+    drain(bars + DRAINED);
   } else {
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
     const int half = warp / 4, row = part.row + (threadIdx.x & 127);
