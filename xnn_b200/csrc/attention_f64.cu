@@ -746,8 +746,10 @@ cudaError_t launch64(const Params<T>& p, int heads, int splits, int own, int str
 
 }  // namespace
 
+template <int DP, int NT> using Wider = std::conditional_t<DP == 128, Shape<DP, 1, 4, 4, NT>, Shape<DP, 2, 2, 4, NT>>;
+
 cudaError_t forward64(const Params<double>& p, cudaStream_t s) {
-  XNN_F64_DIM(p.D, using S = Shape<DP, 2, 2, 4, 2>; return (launch64<S, fwd64_kernel<S>>(p, p.H, p.splits, 1, 2, s)))
+  XNN_F64_DIM(p.D, using S = Wider<DP, 2>; return (launch64<S, fwd64_kernel<S>>(p, p.H, p.splits, 1, 2, s)))
 }
 
 cudaError_t backward64(const Params<double>& p, cudaStream_t s) {
@@ -755,7 +757,7 @@ cudaError_t backward64(const Params<double>& p, cudaStream_t s) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // dk and dv take one block of rows a warp: two would need 256 registers for the sums
-  XNN_F64_DIM(p.D, using S = Shape<DP, 2, 2, 4, 2>; using K = Shape<DP, 1, 4, 2, 4>;
+  XNN_F64_DIM(p.D, using S = Wider<DP, 2>; using K = Shape<DP, 1, 4, 2, 4>;
               if ((e = launch64<S, dq64_kernel<S>>(p, p.H, p.splits, 2, 2, s)) != cudaSuccess) return e;
               return (launch64<K, dkv64_kernel<K>>(p, p.HK, p.splits_k, 2, 2, s)))
 }
@@ -771,7 +773,7 @@ int64_t second64_words(const Params<IN>& p) {
 template <typename IN, int DP, bool NARROW>
 cudaError_t second64_dp(const Params<IN>& p, double* work, cudaStream_t s) {
   // float64 of 113 .. 128 columns: three slices of the keys and half the queries a tile, so that seven tiles fit
-  using R = Shape<DP, 2, 2, NARROW ? 3 : 4, 1>;
+  using R = std::conditional_t<DP == 128, Shape<DP, 1, 4, NARROW ? 3 : 4, 1>, Shape<DP, 2, 2, 4, 1>>;
   using K = Shape<DP, 1, 4, 2, NARROW ? 1 : 2>;
   const int64_t rows = (int64_t)p.H * p.N, nq = rows * p.D, nk = (int64_t)p.N * p.HK * p.D;
   double *stats = work, *rc = stats + 3 * rows, *out = rc + 2 * p.splits * rows;
