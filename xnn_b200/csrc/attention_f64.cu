@@ -13,6 +13,8 @@
 // product takes a row's weights as they lie, four columns at a time: step s takes column 2 t + (s ^ t / 2) from lane t,
 // so that the four matching rows of the other operand fall into different banks (rows are 4 mod 16 numbers long; float32
 // rows, 4 mod 32 long, are conflict-free with column 2 t + s).
+#include <type_traits>
+
 #include "attention.h"
 #include "attention_tile.cuh"
 
@@ -746,18 +748,22 @@ cudaError_t launch64(const Params<T>& p, int heads, int splits, int own, int str
 
 }  // namespace
 
-template <int DP, int NT> using Wider = std::conditional_t<DP == 128, Shape<DP, 1, 4, 4, NT>, Shape<DP, 2, 2, 4, NT>>;
+// Two blocks of rows a warp read less of the streamed tile, one leaves registers for twice the warps: 16 an SM instead of 8
+// at 65-128 columns, where the forward pass takes 259 us instead of 391 (1500 atoms x 4 heads x 96). At 33-64 columns the
+// forward pass (two blocks of eight warps fit) is 4% faster with two, the others up to a quarter slower.
+template <int DP, int NT, int FROM>
+using Rows64 = std::conditional_t<DP >= FROM, Shape<DP, 1, 4, 4, NT>, Shape<DP, 2, 2, 4, NT>>;
 
 cudaError_t forward64(const Params<double>& p, cudaStream_t s) {
-  XNN_F64_DIM(p.D, using S = Wider<DP, 2>; return (launch64<S, fwd64_kernel<S>>(p, p.H, p.splits, 1, 2, s)))
+  XNN_F64_DIM(p.D, using S = Rows64<DP, 2, 128>; return (launch64<S, fwd64_kernel<S>>(p, p.H, p.splits, 1, 2, s)))
 }
 
 cudaError_t backward64(const Params<double>& p, cudaStream_t s) {
   delta64_kernel<double><<<(unsigned)(((int64_t)p.H * p.N + 3) / 4), 128, 0, s>>>(p, p.delta);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // dk and dv take one block of rows a warp: two would need 256 registers for the sums
-  XNN_F64_DIM(p.D, using S = Wider<DP, 2>; using K = Shape<DP, 1, 4, 2, 4>;
+  // two sums of 128 columns leave no registers for more than eight warps
+  XNN_F64_DIM(p.D, using S = Rows64<DP, 2, 64>; using K = std::conditional_t<DP == 64, Shape<DP, 1, 4, 4, 2>, Shape<DP, 1, 4, 2, 4>>;
               if ((e = launch64<S, dq64_kernel<S>>(p, p.H, p.splits, 2, 2, s)) != cudaSuccess) return e;
               return (launch64<K, dkv64_kernel<K>>(p, p.HK, p.splits_k, 2, 2, s)))
 }
@@ -773,8 +779,8 @@ int64_t second64_words(const Params<IN>& p) {
 template <typename IN, int DP, bool NARROW>
 cudaError_t second64_dp(const Params<IN>& p, double* work, cudaStream_t s) {
   // float64 of 113 .. 128 columns: three slices of the keys and half the queries a tile, so that seven tiles fit
-  using R = std::conditional_t<DP == 128, Shape<DP, 1, 4, NARROW ? 3 : 4, 1>, Shape<DP, 2, 2, 4, 1>>;
-  using K = Shape<DP, 1, 4, 2, NARROW ? 1 : 2>;
+  using R = std::conditional_t<NARROW, Shape<DP, 1, 4, 3, 1>, Rows64<DP, 1, 64>>;
+  using K = std::conditional_t<DP == 64, Shape<DP, 1, 4, 4, 1>, Shape<DP, 1, 4, 2, NARROW ? 1 : 2>>;
   const int64_t rows = (int64_t)p.H * p.N, nq = rows * p.D, nk = (int64_t)p.N * p.HK * p.D;
   double *stats = work, *rc = stats + 3 * rows, *out = rc + 2 * p.splits * rows;
   const unsigned row_warps = (unsigned)((rows + 3) / 4);
