@@ -5,8 +5,9 @@
 //        Between them a small kernel joins the splits: r, c and do' = sum - r O.
 // keys   a block owns 128 keys with the parts of k and B in tensor memory, those of v and C in shared memory, and streams
 //        q, do and A: k' and v'.
-// The score products of a tile follow the sums of the tile before in one stretch (the weights' parts take the
-// scores' place in tensor memory, which at 64 columns is full), so the threads' work is not hidden under them.
+// The weights' parts take the scores' place in tensor memory. At 64 columns that memory is full: the score products of a
+// tile follow the sums of the tile before in one stretch, and the threads' work is not hidden under them. Up to 32 columns
+// it holds two sets of scores, and those of the next tile run while the threads form the weights of this one.
 #include "attention.h"
 #include "attention_tc.cuh"
 
@@ -15,6 +16,9 @@ namespace {
 
 constexpr int KINDS = 4;                                // L, D, r, c of a slot's rows
 
+template <int DP> constexpr int SETS = DP <= 32 ? 2 : 1;  // sets of scores in tensor memory
+template <int DP> constexpr int RING = SETS<DP> + 2;      // images: of the tiles with scores, of the sums before, on the way
+
 struct Streams { Images a, b, c, d; };
 
 // the end of the part's last slot
@@ -22,11 +26,42 @@ __device__ __forceinline__ int slots_end(const Part& part) { return part.lo + (p
 
 template <int DP>
 struct Rows {
-  static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = 3 * STAGE, SUMS = BARS + 128, SMEM = SUMS + 4 * 128 * 4;
-  static constexpr int P = 3 * DP / 2, S = 3 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W0 = S, W1 = DPO, OUT = E + HALF;
+  static constexpr int HB = half_bytes<DP>(), STAGE = 4 * HB, BARS = RING<DP> * STAGE, SUMS = BARS + 128, SMEM = SUMS + 4 * 128 * 4;
+  static constexpr int P = 3 * DP / 2, S = 3 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, W0 = S, W1 = DPO, SET = 4 * HALF,
+                       OUT = S + SETS<DP> * SET;
   using Weights = OverHalves<0, 8, HALF>;               // two planes over S or dP, one over T or E, each half over its own
   static_assert(OUT + DP <= 512 && SMEM <= 232448, "tensor and shared memory");
 };
+
+// copies in flight must land before the block ends
+template <int DP>
+__device__ __forceinline__ void give_up(int loaded, uint64_t* full, uint64_t* more = nullptr) {
+  if (more) tc::mbar_wait(more, 0, SPINS);
+  for (int i = max(0, loaded - RING<DP>); i < loaded; ++i) tc::mbar_wait(full + i % RING<DP>, i / RING<DP> & 1, SPINS);
+}
+
+// The ninth warp's turns. Products run in the order of their issue, so the scores of tile i + SETS may be issued behind the
+// sums of tile i, whose weights they overwrite; the weights of tile i come after the threads have the sums of tile i - 1,
+// whose images are then free.
+template <int DP, class Load, class Score, class Sum>
+__device__ __forceinline__ void issue(int n, int loaded, uint64_t* full, uint64_t* ready, volatile int* dead, int* status, const Load& load,
+                                      const Score& score, const Sum& sum) {
+  bool ok = true;
+  for (int i = 0; ok && i < SETS<DP> && i < n; ++i)
+    if ((ok = wait_all(full + i, 0, dead, status))) score(i);
+  for (int i = 0; ok && i < n; ++i) {
+    if (!(ok = wait_all(ready, i & 1, dead, status))) break;
+    tc::tc_fence_after();
+    sum(i);
+    const int next = i + SETS<DP>;
+    if (next < n) {
+      if (!(ok = wait_all(full + next % RING<DP>, next / RING<DP> & 1, dead, status))) break;
+      score(next);
+    }
+    if (i > 0 && i - 1 + RING<DP> < n) { load(i - 1 + RING<DP>); loaded = i + RING<DP>; }
+  }
+  if (!ok) give_up<DP>(loaded, full);
+}
 
 template <int DP, int WALK>
 __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& part, const Job& job, const Streams& im, const Streams& own,
@@ -35,7 +70,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
-  uint64_t *full = bars, *done = bars + 3, *ready = bars + 4;
+  uint64_t *full = bars, *scored = bars + 4, *summed = bars + 6, *ready = bars + 7;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 9);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 10);
   float* sums = reinterpret_cast<float*>(smem + B::SUMS);
@@ -45,7 +80,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   const int n = (hi - lo + HALF - 1) / HALF, slot0 = first_slot(p, part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) tc::mbar_init(bars + i, 1);
+    for (int i = 0; i < 7; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
     tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
@@ -59,8 +94,8 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   const bool on = warp < 8 && row < part.hi;
   const auto load = [&](int i) {
     if (elect()) {
-      char* to = smem + i % 3 * B::STAGE;
-      uint64_t* bar = full + i % 3;
+      char* to = smem + i % RING<DP> * B::STAGE;
+      uint64_t* bar = full + i % RING<DP>;
       tc::mbar_arrive_expect_tx(bar, B::STAGE);
       load_half<DP>(to, image<DP>(im.a, hk, slot0 + i / 2), i % 2, bar);
       load_half<DP>(to + HB, image<DP>(im.b, hk, slot0 + i / 2), i % 2, bar);
@@ -68,7 +103,7 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
       load_half<DP>(to + 3 * HB, image<DP>(im.d, hk, slot0 + i / 2), i % 2, bar);
     }
   };
-  int loaded = min(n, 3);
+  int loaded = min(n, RING<DP>);
   if (warp == 8) {                                      // the copies run while the other warps stage their rows
     for (int i = 0; i < loaded; ++i) load(i);
   } else if (n > 0) {
@@ -92,34 +127,25 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
   if (warp == 8) {
     if (n > 0) {
       const uint32_t base = tc::smem_u32(smem);
-      // the sums of tile i - 1 and the scores of tile i, whichever of them there are
-      const auto step = [&](int i, bool sum, bool score) {
+      const auto score = [&](int i) {
         if (elect()) {
-          if (sum) {
-            const uint32_t at = base + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF, typename B::Weights, typename B::Weights>(tmem + B::OUT, tmem + B::W0, at + (WALK == 0 ? HB : 0), tmem + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
-          }
-          if (score) {
-            const uint32_t at = base + i % 3 * B::STAGE;
-            mma_scores<DP, HALF>(tmem + B::S, tmem, at);
-            mma_scores<DP, HALF>(tmem + B::T, tmem + B::P, at, tmem, at + 2 * HB);
-            mma_scores<DP, HALF>(tmem + B::DPO, tmem + 2 * B::P, at + HB);
-            mma_scores<DP, HALF>(tmem + B::E, tmem + 2 * B::P, at + 3 * HB);
-          }
-          tc::commit_to(done);
+          const uint32_t at = base + i % RING<DP> * B::STAGE, set = tmem + i % SETS<DP> * B::SET;
+          mma_scores<DP, HALF>(set + B::S, tmem, at);
+          mma_scores<DP, HALF>(set + B::T, tmem + B::P, at, tmem, at + 2 * HB);
+          mma_scores<DP, HALF>(set + B::DPO, tmem + 2 * B::P, at + HB);
+          mma_scores<DP, HALF>(set + B::E, tmem + 2 * B::P, at + 3 * HB);
+          tc::commit_to(scored + i % SETS<DP>);
         }
       };
-      ok = wait_all(full, 0, dead, status);
-      if (ok) step(0, false, true);
-      for (int i = 0; ok && i < n; ++i) {
-        if (!(ok = wait_all(ready, i & 1, dead, status))) break;
-        tc::tc_fence_after();
-        if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
-        step(i + 1, true, i + 1 < n);
-        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }     // the sums of tile i - 1 are done
-      }
-      if (!ok)
-        for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
+      const auto sum = [&](int i) {
+        if (elect()) {
+          const uint32_t at = base + i % RING<DP> * B::STAGE, set = tmem + i % SETS<DP> * B::SET;
+          mma_sums<DP, HALF, typename B::Weights, typename B::Weights>(tmem + B::OUT, set + B::W0, at + (WALK == 0 ? HB : 0),
+                                                                       set + B::W1, at + (WALK == 0 ? 3 * HB : 2 * HB));
+          tc::commit_to(summed);
+        }
+      };
+      issue<DP>(n, loaded, full, ready, dead, status, load, score, sum);
     }
     drain(bars + DRAINED);
   } else {
@@ -133,13 +159,14 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
     }
     for (int i = 0; i < n; ++i) {
       const uint32_t bits = allowed_half(lo + i * HALF, hi, p.mask) >> (16 * half);
-      if (!(ok = wait_all(done, i & 1, dead, status))) break;
+      if (!(ok = wait_all(scored + i % SETS<DP>, i / SETS<DP> & 1, dead, status))) break;
       tc::tc_fence_after();
+      const uint32_t set = lanes + i % SETS<DP> * B::SET;
       float s[16], t[16], dp[16], e[16];
-      tmem_ld16(lanes + B::S + 16 * half, s);
-      tmem_ld16(lanes + B::T + 16 * half, t);
-      tmem_ld16(lanes + B::DPO + 16 * half, dp);
-      tmem_ld16(lanes + B::E + 16 * half, e);
+      tmem_ld16(set + B::S + 16 * half, s);
+      tmem_ld16(set + B::T + 16 * half, t);
+      tmem_ld16(set + B::DPO + 16 * half, dp);
+      tmem_ld16(set + B::E + 16 * half, e);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -155,14 +182,18 @@ __device__ __forceinline__ void rows_block(const Params<float>& p, const Part& p
           t[j] = in ? pr * (dp[j] - D) : 0.f;
         }
       }
-      if (i > 0) add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
-      store_parts16<typename B::Weights>(lanes + B::W0, half, s);
-      store_parts16<typename B::Weights>(lanes + B::W1, half, t);
+      if (i > 0) {
+        if (!(ok = wait_all(summed, (i - 1) & 1, dead, status))) break;
+        tc::tc_fence_after();
+        add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
+      }
+      store_parts16<typename B::Weights>(set + B::W0, half, s);
+      store_parts16<typename B::Weights>(set + B::W1, half, t);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ready);
     }
-    if (ok && n > 0 && (ok = wait_all(done, n & 1, dead, status))) {
+    if (ok && n > 0 && (ok = wait_all(summed, (n - 1) & 1, dead, status))) {
       tc::tc_fence_after();
       add_columns<DP / 2>(lanes + B::OUT + half * (DP / 2), acc);
     }
@@ -247,9 +278,9 @@ __global__ void __launch_bounds__(256) second_join_kernel(const Params<float> p,
 template <int DP>
 struct Keys {
   static constexpr int HB = half_bytes<DP>(), BLOCK = PLANES * 128 * DP * 2, ST = 2 * BLOCK, STAGE = 3 * HB + KINDS * HALF * 4,
-                       BARS = ST + 3 * STAGE, SMEM = BARS + 128;
-  static constexpr int P = 3 * DP / 2, S = 2 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, REST = E + HALF, K2 = REST + 16,
-                       V2 = K2 + DP;
+                       BARS = ST + RING<DP> * STAGE, SMEM = BARS + 128;
+  static constexpr int P = 3 * DP / 2, S = 2 * P, T = S + HALF, DPO = T + HALF, E = DPO + HALF, SET = 4 * HALF + 16,
+                       K2 = S + SETS<DP> * SET, V2 = K2 + DP;
   // the parts of M, dS and P (T - r) over the four score regions and 16 columns more, each half over its own columns
   using M = OverHalves<0, 8, HALF>;
   using DS = OverHalves<HALF + 8, 2 * HALF, 2 * HALF + 8>;
@@ -264,7 +295,7 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   constexpr int HB = B::HB;
   extern __shared__ __align__(128) char smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + B::BARS);
-  uint64_t *full = bars, *full_2 = bars + 3, *done = bars + 4, *ready = bars + 5;
+  uint64_t *full = bars, *full_2 = bars + 4, *scored = bars + 5, *summed = bars + 7, *ready = bars + 8;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 10);
   volatile int* dead = reinterpret_cast<volatile int*>(bars + 11);
   const int warp = threadIdx.x / 32, hk = job.head, group = p.H / p.HK;
@@ -274,7 +305,7 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   const int tiles = (hi - lo + HALF - 1) / HALF, n = tiles * group, slot0 = first_slot(p, part) + (lo - part.lo) / SLOT;
   if (warp == 8) tmem_alloc(slot, 512);
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 5; ++i) tc::mbar_init(bars + i, 1);
+    for (int i = 0; i < 8; ++i) tc::mbar_init(bars + i, 1);
     tc::mbar_init(ready, 8);
     tc::mbar_init(bars + DRAINED, 1);
     *dead = 0;
@@ -287,8 +318,8 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   const int row = part.row + (threadIdx.x & 127), half = warp / 4;
   const auto load = [&](int i) {                    // q, do, A and the statistics of tile i
     if (elect()) {
-      char* to = smem + B::ST + i % 3 * B::STAGE;
-      uint64_t* bar = full + i % 3;
+      char* to = smem + B::ST + i % RING<DP> * B::STAGE;
+      uint64_t* bar = full + i % RING<DP>;
       const int head = hk * group + i / tiles, t = i % tiles;
       tc::mbar_arrive_expect_tx(bar, B::STAGE);
       load_half<DP>(to, image<DP>(im.a, head, slot0 + t / 2), t % 2, bar);
@@ -299,7 +330,7 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
       for (int x = 0; x < KINDS; ++x) tc::bulk_g2s(to + 3 * HB + x * HALF * 4, st + x * SLOT, HALF * 4, bar);
     }
   };
-  int loaded = min(n, 3);
+  int loaded = min(n, RING<DP>);
   if (warp == 8 && n > 0) {
     if (elect()) {
       tc::mbar_arrive_expect_tx(full_2, 2 * B::BLOCK);
@@ -319,36 +350,26 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
   if (warp == 8) {
     if (n > 0) {
       const uint32_t base = tc::smem_u32(smem), ring = base + B::ST;
-      const auto step = [&](int i, bool sum, bool score) {
+      const auto score = [&](int i) {
         if (elect()) {
-          if (sum) {
-            const uint32_t at = ring + (i + 2) % 3 * B::STAGE;
-            mma_sums<DP, HALF, typename B::M, typename B::DS>(tmem + B::K2, tmem + B::S, at, tmem + B::S, at + 2 * HB);
-            mma_sums<DP, HALF, typename B::PT>(tmem + B::V2, tmem + B::S, at + HB);
-          }
-          if (score) {
-            const uint32_t at = ring + i % 3 * B::STAGE;
-            mma_scores<DP, HALF>(tmem + B::S, tmem, at);
-            mma_scores<DP, HALF>(tmem + B::T, tmem, at + 2 * HB, tmem + B::P, at);
-            mma_scores_ss<DP, HALF>(tmem + B::DPO, base, at + HB);
-            mma_scores_ss<DP, HALF>(tmem + B::E, base + B::BLOCK, at + HB);
-          }
-          tc::commit_to(done);
+          const uint32_t at = ring + i % RING<DP> * B::STAGE, set = tmem + i % SETS<DP> * B::SET;
+          mma_scores<DP, HALF>(set + B::S, tmem, at);
+          mma_scores<DP, HALF>(set + B::T, tmem, at + 2 * HB, tmem + B::P, at);
+          mma_scores_ss<DP, HALF>(set + B::DPO, base, at + HB);
+          mma_scores_ss<DP, HALF>(set + B::E, base + B::BLOCK, at + HB);
+          tc::commit_to(scored + i % SETS<DP>);
         }
       };
-      bool ok = wait_all(full_2, 0, dead, status) && wait_all(full, 0, dead, status);
-      if (ok) step(0, false, true);
-      for (int i = 0; ok && i < n; ++i) {
-        if (!(ok = wait_all(ready, i & 1, dead, status))) break;
-        tc::tc_fence_after();
-        if (i + 1 < n && !(ok = wait_all(full + (i + 1) % 3, ((i + 1) / 3) & 1, dead, status))) break;
-        step(i + 1, true, i + 1 < n);
-        if (i > 0 && i + 2 < n) { load(i + 2); loaded = i + 3; }
-      }
-      if (!ok) {
-        tc::mbar_wait(full_2, 0, SPINS);
-        for (int i = max(0, loaded - 3); i < loaded; ++i) tc::mbar_wait(full + i % 3, (i / 3) & 1, SPINS);
-      }
+      const auto sum = [&](int i) {
+        if (elect()) {
+          const uint32_t at = ring + i % RING<DP> * B::STAGE, set = tmem + i % SETS<DP> * B::SET;
+          mma_sums<DP, HALF, typename B::M, typename B::DS>(tmem + B::K2, set + B::S, at, set + B::S, at + 2 * HB);
+          mma_sums<DP, HALF, typename B::PT>(tmem + B::V2, set + B::S, at + HB);
+          tc::commit_to(summed);
+        }
+      };
+      if (wait_all(full_2, 0, dead, status)) issue<DP>(n, loaded, full, ready, dead, status, load, score, sum);
+      else give_up<DP>(loaded, full, full_2);
     }
     drain(bars + DRAINED);
   } else {
@@ -358,15 +379,16 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
     for (int d = 0; d < DP; ++d) acc[d] = 0.f;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      if (!(ok = wait_all(done, i & 1, dead, status))) break;
-      if (!(ok = wait_all(full + i % 3, (i / 3) & 1, dead, status))) break;
+      if (!(ok = wait_all(scored + i % SETS<DP>, i / SETS<DP> & 1, dead, status))) break;
+      if (!(ok = wait_all(full + i % RING<DP>, i / RING<DP> & 1, dead, status))) break;
       tc::tc_fence_after();
-      const float* st = reinterpret_cast<const float*>(smem + B::ST + i % 3 * B::STAGE + 3 * HB) + 16 * half;
+      const float* st = reinterpret_cast<const float*>(smem + B::ST + i % RING<DP> * B::STAGE + 3 * HB) + 16 * half;
+      const uint32_t set = lanes + i % SETS<DP> * B::SET;
       float s[16], t[16], dp[16], e[16];
-      tmem_ld16(lanes + B::S + 16 * half, s);
-      tmem_ld16(lanes + B::T + 16 * half, t);
-      tmem_ld16(lanes + B::DPO + 16 * half, dp);
-      tmem_ld16(lanes + B::E + 16 * half, e);
+      tmem_ld16(set + B::S + 16 * half, s);
+      tmem_ld16(set + B::T + 16 * half, t);
+      tmem_ld16(set + B::DPO + 16 * half, dp);
+      tmem_ld16(set + B::E + 16 * half, e);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -375,15 +397,19 @@ __device__ __forceinline__ void keys_block(const Params<float>& p, const Part& p
         t[j] = pr * y;
         dp[j] = pr * x;
       }
-      if (i > 0) add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
-      store_parts16<typename B::M>(lanes + B::S, half, s);
-      store_parts16<typename B::DS>(lanes + B::S, half, t);
-      store_parts16<typename B::PT>(lanes + B::S, half, dp);
+      if (i > 0) {
+        if (!(ok = wait_all(summed, (i - 1) & 1, dead, status))) break;
+        tc::tc_fence_after();
+        add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
+      }
+      store_parts16<typename B::M>(set + B::S, half, s);
+      store_parts16<typename B::DS>(set + B::S, half, t);
+      store_parts16<typename B::PT>(set + B::S, half, dp);
       tmem_st_wait();
       tc::tc_fence_before();
       arrive(ready);
     }
-    if (ok && n > 0 && (ok = wait_all(done, n & 1, dead, status))) {
+    if (ok && n > 0 && (ok = wait_all(summed, (n - 1) & 1, dead, status))) {
       tc::tc_fence_after();
       add_columns<DP>(lanes + (half ? B::V2 : B::K2), acc);
     }
