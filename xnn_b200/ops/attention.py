@@ -14,8 +14,9 @@ neither outputs nor gradients, and no structure's values reach another's.
 
 On CUDA tensors (float32, float64; ``D <= 128``) this package's sm_100a kernels run
 (``csrc/attention.cu``), on the calling thread's current stream, without a host synchronisation, so
-they can be captured into a CUDA graph; results do not depend on the launch (no atomics). On the CPU the
-padded formula runs, differentiable to any order.
+they can be captured into a CUDA graph; results do not depend on the launch (no atomics). float32 structures of
+more than 32 atoms run as products of exact parts, so an infinite operand that no mask hides gives NaN. On the
+CPU the padded formula runs, differentiable to any order.
 """
 from __future__ import annotations
 
