@@ -113,3 +113,17 @@ def test_captured_replays_draw_new_masks():
         assert torch.equal(y, counter_dropout(x, 0.5, (9, step)))
         seen.append(y.detach().clone())
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_module_refuses_a_recomputed_pass():
+    """The second run of a checkpointed pass would meet another offset; the function with its numbers repeats its mask."""
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(64, requires_grad=True)
+    drop = CounterDropout(0.5, seed=3)
+    y = checkpoint(lambda t: drop(t).square(), x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="counter_dropout"):
+        y.sum().backward()
+    y = checkpoint(lambda t: counter_dropout(t, 0.5, (3, 7)).square(), x, use_reentrant=False)
+    (g,) = torch.autograd.grad(y.sum(), x)
+    kept = counter_dropout(torch.ones(64), 0.5, (3, 7))
+    assert torch.equal(g, 2 * x.detach() * kept * kept)

@@ -122,7 +122,8 @@ class CounterDropout(nn.Module):
     """:func:`counter_dropout` in training mode with its own seed (drawn from PyTorch's generator when
     omitted) and an offset that each call advances. The two numbers live on the module's device, so a
     captured training step draws a new mask at every replay. Processes that start from one seed draw the
-    same masks, each for its own rows."""
+    same masks, each for its own rows. Inside an activation checkpoint it is refused: the recomputed pass
+    would meet another offset."""
 
     def __init__(self, p: float, shared: Sequence[int] = (), seed: Optional[int] = None):
         super().__init__()
@@ -135,6 +136,9 @@ class CounterDropout(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         if not self.training or self.p == 0.0:
             return x
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("CounterDropout in a forward pass that a backward pass runs again (activation checkpointing) "
+                               "would draw another mask: call counter_dropout with the numbers of the first pass")
         now = self.rng.clone()
         self.rng[1] += 1
         return counter_dropout(x, self.p, now, self.shared)
