@@ -29,7 +29,8 @@ def _mask(shape, p, rng, shared):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
 @pytest.mark.parametrize("shape,shared", [((1,), ()), ((7,), ()), ((33, 8), ()), ((1201, 8), ()), ((5, 49, 128), (1,)),
                                           ((6, 9, 13), (1,)), ((300, 4, 3), (1,)), ((4, 5, 6, 7), (1, 2)), ((2, 1, 9), (1,)),
-                                          ((40, 16), (1,)), ((40, 16), (0,)), ((3, 2), (0, 1)), ((5000, 49, 4), (1,))])
+                                          ((40, 16), (1,)), ((40, 16), (0,)), ((3, 2), (0, 1)), ((5000, 49, 4), (1,)),
+                                          ((4099,), ()), ((129, 3, 37), (1,)), ((3, 2, 301), (1,))])
 def test_values_and_gradients(device, dtype, shape, shared):
     rng = (2 ** 61 + 12345, 2 ** 40 + 7)
     x = torch.randn(shape, dtype=dtype, device=device, requires_grad=True)

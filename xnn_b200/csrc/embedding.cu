@@ -25,9 +25,10 @@ __device__ __forceinline__ int64_t row_of(const I* ids, int64_t n, int64_t V) {
 // written is not read again here, so it goes past the caches. 400000 rows of 128 floats: 34 us, 6.1 TB/s written.
 constexpr int LOOKUPS = 4;
 
-template <typename T, typename I, int W>
+template <typename T, typename I>
 __global__ void __launch_bounds__(256) lookup_kernel(uint32_t items, uint32_t per, int64_t V, int C, const T* __restrict__ table,
                                                      const I* __restrict__ ids, T scale, T* __restrict__ out) {
+  constexpr int W = 16 / sizeof(T);
   const uint32_t first = blockIdx.x * (256u * LOOKUPS) + threadIdx.x;
   int64_t v[LOOKUPS];
   uint32_t n[LOOKUPS], c[LOOKUPS];
@@ -38,24 +39,49 @@ __global__ void __launch_bounds__(256) lookup_kernel(uint32_t items, uint32_t pe
     c[u] = (i - n[u] * per) * W;
     v[u] = i < items ? row_of(ids, n[u], V) : -1;
   }
-  if constexpr (W == 1) {
+  Pack<T> a[LOOKUPS];
 #pragma unroll
-    for (int u = 0; u < LOOKUPS; ++u)
-      if (first + u * 256u < items) out[(int64_t)n[u] * C + c[u]] = v[u] < 0 ? T(0) : scale * table[v[u] * C + c[u]];
+  for (int u = 0; u < LOOKUPS; ++u) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) a[u].x[e] = T(0);
+    if (v[u] >= 0) a[u] = *reinterpret_cast<const Pack<T>*>(table + v[u] * C + c[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < LOOKUPS; ++u) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) a[u].x[e] *= scale;
+    if (first + u * 256u < items) __stcs(reinterpret_cast<float4*>(out + (int64_t)n[u] * C + c[u]), *reinterpret_cast<float4*>(&a[u]));
+  }
+}
+
+// Rows that are no whole number of 16 bytes (or not on such boundaries): a thread writes 16 bytes of the output, whatever rows
+// they are of. 400000 rows of 127 floats: 61 us (97 with single
+// elements, each with its own division).
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) lookup_odd_kernel(uint32_t items, uint32_t C, int64_t V, const T* __restrict__ table,
+                                                         const I* __restrict__ ids, T scale, T* __restrict__ out) {
+  constexpr int W = 16 / sizeof(T);
+  const uint32_t e0 = (blockIdx.x * 256u + threadIdx.x) * W;
+  if (e0 >= items) return;
+  uint32_t n = e0 / C, c = e0 - n * C;
+  int64_t v = row_of(ids, n, V);
+  Pack<T> a;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    a.x[e] = v < 0 ? T(0) : table[v * C + c];
+    if (++c == C && e0 + e + 1 < items) {
+      c = 0;
+      v = row_of(ids, ++n, V);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < W; ++e) a.x[e] *= scale;
+  if (e0 + W <= items) {
+    __stcs(reinterpret_cast<float4*>(out + e0), *reinterpret_cast<float4*>(&a));
   } else {
-    Pack<T> a[LOOKUPS];
 #pragma unroll
-    for (int u = 0; u < LOOKUPS; ++u) {
-#pragma unroll
-      for (int e = 0; e < W; ++e) a[u].x[e] = T(0);
-      if (v[u] >= 0) a[u] = *reinterpret_cast<const Pack<T>*>(table + v[u] * C + c[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < LOOKUPS; ++u) {
-#pragma unroll
-      for (int e = 0; e < W; ++e) a[u].x[e] *= scale;
-      if (first + u * 256u < items) __stcs(reinterpret_cast<float4*>(out + (int64_t)n[u] * C + c[u]), *reinterpret_cast<float4*>(&a[u]));
-    }
+    for (int e = 0; e < W; ++e)
+      if (e0 + e < items) out[e0 + e] = a.x[e];
   }
 }
 
@@ -255,56 +281,58 @@ __device__ __forceinline__ void run_part(const T* part, int c0, int j0, int j1, 
   }
 }
 
-// A warp per table row: zeros where no id came, the partials of a run over several chunks added up. Rows of more
-// than MANY partials (the few elements that most atoms are) are left to the whole block. A block's eight rows lie
-// gridDim apart, so that the popular ids, which are neighbours, meet in different blocks.
+// A warp per table row and 32 W columns: zeros where no id came, the partials of a run over several chunks added up. Rows of
+// more than MANY partials (the few elements that most atoms are) are left to the whole block. A block's rows lie gridDim.x
+// apart, so that the popular ids, which are neighbours, meet in different blocks; a table of at most a row an SM has a block
+// of 32 warps a row (gradient of 400000 ids of 5 elements, 512 columns: 163 us, 747 with eight rows in one block).
 constexpr int MANY = 32;
 
-template <typename T, int W>
-__global__ void __launch_bounds__(256) rows_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
-                                                   const T* __restrict__ part, T scale, T* __restrict__ table) {
-  __shared__ T sums[8][32 * W];
-  __shared__ int heavy_first[8], heavy_count[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, v = blockIdx.x + warp * gridDim.x;
-  int n = 0, c0 = 0;
+template <typename T, int W, int WARPS, int ROWS>
+__global__ void __launch_bounds__(32 * WARPS) rows_kernel(int N, int V, int C, int R, const int* __restrict__ keys,
+                                                          const T* __restrict__ part, T scale, T* __restrict__ table) {
+  __shared__ T sums[WARPS][32 * W];
+  __shared__ int heavy_first[ROWS], heavy_count[ROWS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (blockIdx.y * 32 + lane) * W;
   T s[W];
-  if (v < V) {
-    const int a = lower_bound(keys, N, v), b = lower_bound(keys, N, v + 1);
-    T* out = table + (int64_t)v * C;
-    if (a == b) {
-      for (int c = lane; c < C; c += 32) out[c] = T(0);
-    } else {
-      c0 = a / R;
-      n = (b - 1) / R - c0 + 1;                         // 1: one chunk had the whole run and has written it
-      if (n > 1 && n <= MANY)
-        for (int c = lane * W; c < C; c += 32 * W) {
+  if (warp < ROWS) {
+    const int v = blockIdx.x + warp * gridDim.x;
+    int n = 0, c0 = 0;
+    if (v < V) {
+      const int a = lower_bound(keys, N, v), b = lower_bound(keys, N, v + 1);
+      T* out = table + (int64_t)v * C;
+      if (a == b) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) s[e] = T(0);
+        put<T, W>(out, s, scale, c, C);
+      } else {
+        c0 = a / R;
+        n = (b - 1) / R - c0 + 1;                       // 1: one chunk had the whole run and has written it
+        if (n > 1 && n <= MANY) {
           run_part<T, W>(part, c0, 0, n, C, c, s);
           put<T, W>(out, s, scale, c, C);
         }
+      }
+    }
+    if (lane == 0) {
+      heavy_first[warp] = c0;
+      heavy_count[warp] = n > MANY ? n : 0;
     }
   }
-  if (lane == 0) {
-    heavy_first[warp] = c0;
-    heavy_count[warp] = n > MANY ? n : 0;
-  }
   __syncthreads();
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < ROWS; ++w) {
     const int m = heavy_count[w];
     if (m == 0) continue;
-    const int per = (m + 7) / 8;
-    for (int cb = 0; cb < C; cb += 32 * W) {
-      const int c = cb + lane * W;
-      run_part<T, W>(part, heavy_first[w], warp * per, min(m, (warp + 1) * per), C, c, s);
-      __syncthreads();
+    const int per = (m + WARPS - 1) / WARPS;
+    run_part<T, W>(part, heavy_first[w], min(m, warp * per), min(m, (warp + 1) * per), C, c, s);
+    __syncthreads();
 #pragma unroll
-      for (int e = 0; e < W; ++e) sums[warp][lane * W + e] = s[e];
-      __syncthreads();
-      if (warp == 0) {
-        for (int k = 1; k < 8; ++k)
+    for (int e = 0; e < W; ++e) sums[warp][lane * W + e] = s[e];
+    __syncthreads();
+    if (warp == 0) {
+      for (int k = 1; k < WARPS; ++k)
 #pragma unroll
-          for (int e = 0; e < W; ++e) s[e] += sums[k][lane * W + e];
-        put<T, W>(table + (int64_t)(blockIdx.x + w * gridDim.x) * C, s, scale, c, C);
-      }
+        for (int e = 0; e < W; ++e) s[e] += sums[k][lane * W + e];
+      put<T, W>(table + (int64_t)(blockIdx.x + w * gridDim.x) * C, s, scale, c, C);
     }
   }
 }
@@ -370,6 +398,13 @@ int run_chunk(int64_t N) {
 }
 bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 22; }
 
+template <typename T, int W>
+void add_partials(int N, int V, int C, int R, const int* keys, const T* part, T scale, T* table, cudaStream_t s) {
+  const unsigned columns = (unsigned)((C + 32 * W - 1) / (32 * W));
+  if (V <= 148) rows_kernel<T, W, 32, 1><<<dim3(V, columns), 1024, 0, s>>>(N, V, C, R, keys, part, scale, table);
+  else rows_kernel<T, W, 8, 8><<<dim3((V + 7) / 8, columns), 256, 0, s>>>(N, V, C, R, keys, part, scale, table);
+}
+
 }  // namespace
 
 template <typename T, typename I>
@@ -377,14 +412,14 @@ cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const 
   constexpr int W = 16 / sizeof(T);
   const bool vec = C % W == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   const int64_t per = vec ? C / W : C;
-  // pieces are counted in 32 bits: rows in groups that fit
-  const int64_t group = ((int64_t)1 << 31) / per;
+  // pieces are counted in 32 bits: rows in groups that fit, each on a 16-byte boundary of the output
+  const int64_t group = ((int64_t)1 << 31) / per / W * W;
   for (int64_t n0 = 0; n0 < N; n0 += group) {
     const int64_t n = N - n0 < group ? N - n0 : group;
     const uint32_t items = (uint32_t)(n * per);
-    const unsigned grid = (unsigned)(((int64_t)items + 256 * LOOKUPS - 1) / (256 * LOOKUPS));
-    if (vec) lookup_kernel<T, I, W><<<grid, 256, 0, s>>>(items, (uint32_t)per, V, C, table, ids + n0, (T)scale, out + n0 * C);
-    else lookup_kernel<T, I, 1><<<grid, 256, 0, s>>>(items, (uint32_t)per, V, C, table, ids + n0, (T)scale, out + n0 * C);
+    const unsigned each = vec ? 256 * LOOKUPS : 256 * W, grid = (unsigned)(((int64_t)items + each - 1) / each);
+    if (vec) lookup_kernel<T, I><<<grid, 256, 0, s>>>(items, (uint32_t)per, V, C, table, ids + n0, (T)scale, out + n0 * C);
+    else lookup_odd_kernel<T, I><<<grid, 256, 0, s>>>(items, (uint32_t)C, V, table, ids + n0, (T)scale, out + n0 * C);
   }
   return cudaGetLastError();
 }
@@ -430,10 +465,9 @@ cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g
   const dim3 grid((chunks + 3) / 4, (C + cols - 1) / cols);
   if (vec) runs_kernel<T, W><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
   else runs_kernel<T, 1><<<grid, 128, 0, s>>>((int)N, (int)V, C, R, k, r, g, (T)scale, table, partials);
-  const unsigned row_blocks = (unsigned)((V + 7) / 8);
   // partial rows start on 16-byte boundaries where a whole number of vectors makes a row
-  if (C % W == 0) rows_kernel<T, W><<<row_blocks, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
-  else rows_kernel<T, 1><<<row_blocks, 256, 0, s>>>((int)N, (int)V, C, R, k, partials, (T)scale, table);
+  if (C % W == 0) add_partials<T, W>((int)N, (int)V, C, R, k, partials, (T)scale, table, s);
+  else add_partials<T, 1>((int)N, (int)V, C, R, k, partials, (T)scale, table, s);
   return cudaGetLastError();
 }
 
