@@ -396,7 +396,7 @@ int run_chunk(int64_t N) {
   const int64_t r = (N + 148 * 24 - 1) / (148 * 24);
   return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
-bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 22; }
+bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 23; }
 
 template <typename T, int W>
 void add_partials(int N, int V, int C, int R, const int* keys, const T* part, T scale, T* table, cudaStream_t s) {
@@ -439,8 +439,8 @@ int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C) {
 template <typename T, typename I>
 cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g, double scale, int* ints, T* partials,
                            T* table, cudaStream_t s) {
-  // collecting costs N V id reads in all and sums a row's entries in one block; the sort costs four to ten
-  // launches: below some thousand entries the former is one short launch
+  // collecting costs N V id reads in all and sums a row's entries in one block; the sort costs four to ten launches. 4096
+  // ids of 1100 rows: 13 us on the device against 23, of 2000: 20 and 24, of 8000: 70 and 29
   if (collects(N, V)) {
     collect_kernel<T, I><<<(unsigned)V, 256, 256 * sizeof(T) + sizeof(int) * (size_t)N, s>>>((int)N, V, C, ids, g, (T)scale, table);
     return cudaGetLastError();
