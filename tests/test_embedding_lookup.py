@@ -28,7 +28,8 @@ def _ids(n, rows, kind, g):
     (1, 1, 1, "same"), (5, 3, 7, "outside"), (611, 87, 64, "any"), (4096, 100, 33, "few"), (4097, 100, 32, "few"),
     (4500, 87, 64, "same"), (5000, 255, 128, "any"), (5000, 256, 20, "outside"), (9000, 257, 130, "sorted"),
     (20000, 7569, 16, "any"), (30011, 70000, 4, "outside"), (40000, 5, 300, "few"), (700, 9000, 12, "any"), (60000, 148, 130, "any"),
-    (60000, 149, 3, "few"), (50001, 4, 257, "same")])
+    (60000, 149, 3, "few"), (50001, 4, 257, "same"),
+    (8192, 2000, 16, "any"), (8192, 40, 16, "same"), (8192, 40, 17, "same"), (8193, 5, 3, "few"), (1023, 30, 128, "few")])
 def test_values_and_gradients(device, dtype, n, rows, width, kind):
     g = torch.Generator().manual_seed(n + rows)
     table = torch.randn(rows, width, generator=g, dtype=torch.float64).to(dtype).to(device).requires_grad_()

@@ -19,7 +19,7 @@ cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const 
 template <typename T, typename I>
 cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g, double scale, int* ints, T* partials,
                            T* table, cudaStream_t s);
-int64_t embedding_grad_ints(int64_t N, int64_t V);
+int64_t embedding_grad_ints(int64_t N, int64_t V, int64_t C);
 int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C);
 
 namespace {
@@ -528,7 +528,7 @@ torch::Tensor lookup_grad_raw(const torch::Tensor& ids, const torch::Tensor& g, 
   if (out.numel() == 0) return out;
   if (N == 0) return out.zero_();
   const auto s = at::cuda::getCurrentCUDAStream();
-  auto ints = torch::empty({embedding_grad_ints(N, rows)}, g.options().dtype(torch::kInt32));
+  auto ints = torch::empty({embedding_grad_ints(N, rows, C)}, g.options().dtype(torch::kInt32));
   auto parts = torch::empty({embedding_grad_partials(N, rows, C)}, g.options());
   AT_DISPATCH_FLOATING_TYPES(g.scalar_type(), "embedding_lookup gradient", [&] {
     if (ids.scalar_type() == torch::kInt64)

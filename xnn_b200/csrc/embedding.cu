@@ -8,7 +8,7 @@
 // goes to the table; the part of a run that began before the chunk, and the one that goes on behind it, are
 // written to one of the chunk's two partial rows. A warp (or, for long runs, a block) per table row then adds the partials of its run in their order
 // and writes zeros where no id came. Every sum has a fixed order; there are no atomics on values.
-// Small inputs (rule at `embedding_grad`) skip the sort: a block per table row collects its ids itself.
+// Small inputs (rule at `collects`) skip the sort: a block per table row collects its ids itself.
 #include "common.cuh"
 
 namespace {
@@ -347,19 +347,31 @@ __global__ void __launch_bounds__(256) collect_kernel(int N, int64_t V, int C, c
   __shared__ int warp_n[8];
   const int v = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int n = 0;
-  for (int i0 = 0; i0 < N; i0 += 256) {
-    const int i = i0 + t;
-    const bool hit = i < N && (int64_t)ids[i] == v;
-    const unsigned b = __ballot_sync(0xffffffffu, hit);
-    if (lane == 0) warp_n[warp] = __popc(b);
+  // four neighbouring ids a thread, so that a turn with its two meetings covers 1024
+  const unsigned before = (1u << lane) - 1;
+  for (int i0 = 0; i0 < N; i0 += 1024) {
+    const int i = i0 + 4 * t;
+    bool hit[4];
+    int mine = 0, all = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) hit[j] = i + j < N && (int64_t)ids[min(i + j, N - 1)] == v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned b = __ballot_sync(0xffffffffu, hit[j]);
+      mine += __popc(b & before);
+      all += __popc(b);
+    }
+    if (lane == 0) warp_n[warp] = all;
     __syncthreads();
-    int at = n;
+    int at = n + mine;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
       at += w < warp ? warp_n[w] : 0;
       n += warp_n[w];
     }
-    if (hit) list[at + __popc(b & ((1u << lane) - 1))] = i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (hit[j]) list[at++] = i + j;
     __syncthreads();
   }
   T* out = table + (int64_t)v * C;
@@ -383,7 +395,7 @@ __global__ void __launch_bounds__(256) collect_kernel(int N, int64_t V, int C, c
   }
 }
 
-constexpr int SMALL_ROWS = 4096;
+constexpr int SMALL_ROWS = 8192;                        // the list of a row's entries is in shared memory
 
 // pairs a sort block takes: at most 148 blocks (each reads every block's counts), 1024 pairs at least
 int sort_tile(int64_t N) {
@@ -396,7 +408,12 @@ int run_chunk(int64_t N) {
   const int64_t r = (N + 148 * 24 - 1) / (148 * 24);
   return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
-bool collects(int64_t N, int64_t V) { return N <= SMALL_ROWS && N * V <= (int64_t)1 << 23; }
+// Collecting costs N V id reads in all and sums a row's entries, in the worst case all of them, in one block; the sort costs four
+// to ten launches, 15-25 us on the device and as much of the host. Collecting, device: 4868 ids of 1777 rows, 11 columns 16
+// us, 8192 ids of 4000 rows 48, 8192 ids of 4 rows x 128 columns 80, x 512 306; 8192 of 1000, 64 columns 18, 611 of 87 x 64 4.
+bool collects(int64_t N, int64_t V, int64_t C) {
+  return N <= SMALL_ROWS && N * V <= (int64_t)1 << 24 && N * C <= (int64_t)1 << 17;
+}
 
 template <typename T, int W>
 void add_partials(int N, int V, int C, int R, const int* keys, const T* part, T scale, T* table, cudaStream_t s) {
@@ -425,13 +442,13 @@ cudaError_t embedding_lookup(int64_t N, int64_t V, int C, const T* table, const 
 }
 
 // int32 words of workspace for the sort, and elements of T for the partial rows
-int64_t embedding_grad_ints(int64_t N, int64_t V) {
-  if (collects(N, V)) return 0;
+int64_t embedding_grad_ints(int64_t N, int64_t V, int64_t C) {
+  if (collects(N, V, C)) return 0;
   const int64_t tile = sort_tile(N);
   return 4 * N + (N + tile - 1) / tile * 256;
 }
 int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C) {
-  if (collects(N, V)) return 0;
+  if (collects(N, V, C)) return 0;
   const int64_t R = run_chunk(N);
   return (N + R - 1) / R * 2 * C;
 }
@@ -439,9 +456,7 @@ int64_t embedding_grad_partials(int64_t N, int64_t V, int64_t C) {
 template <typename T, typename I>
 cudaError_t embedding_grad(int64_t N, int64_t V, int C, const I* ids, const T* g, double scale, int* ints, T* partials,
                            T* table, cudaStream_t s) {
-  // collecting costs N V id reads in all and sums a row's entries in one block; the sort costs four to ten launches. 4096
-  // ids of 1100 rows: 13 us on the device against 23, of 2000: 20 and 24, of 8000: 70 and 29
-  if (collects(N, V)) {
+  if (collects(N, V, C)) {
     collect_kernel<T, I><<<(unsigned)V, 256, 256 * sizeof(T) + sizeof(int) * (size_t)N, s>>>((int)N, V, C, ids, g, (T)scale, table);
     return cudaGetLastError();
   }
