@@ -10,16 +10,11 @@
 // and writes zeros where no id came. Every sum has a fixed order; there are no atomics on values.
 // Small inputs (rule at `collects`) skip the sort: a block per table row collects its ids itself.
 #include "common.cuh"
+#include "embedding_impl.h"
 
 namespace {
 
 template <typename T> struct alignas(16) Pack { T x[16 / sizeof(T)]; };
-
-template <typename I>
-__device__ __forceinline__ int64_t row_of(const I* ids, int64_t n, int64_t V) {
-  const int64_t v = (int64_t)ids[n];
-  return v >= 0 && v < V ? v : -1;
-}
 
 // A thread takes LOOKUPS pieces of 16 bytes, a block apart, so that its id and row loads overlap; what is
 // written is not read again here, so it goes past the caches. 400000 rows of 128 floats: 34 us, 6.1 TB/s written.
@@ -63,25 +58,15 @@ __global__ void __launch_bounds__(256) lookup_odd_kernel(uint32_t items, uint32_
   constexpr int W = 16 / sizeof(T);
   const uint32_t e0 = (blockIdx.x * 256u + threadIdx.x) * W;
   if (e0 >= items) return;
-  uint32_t n = e0 / C, c = e0 - n * C;
-  int64_t v = row_of(ids, n, V);
-  Pack<T> a;
-#pragma unroll
-  for (int e = 0; e < W; ++e) {
-    a.x[e] = v < 0 ? T(0) : table[v * C + c];
-    if (++c == C && e0 + e + 1 < items) {
-      c = 0;
-      v = row_of(ids, ++n, V);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < W; ++e) a.x[e] *= scale;
   if (e0 + W <= items) {
+    Pack<T> a;
+    walk_elements<W, true>(e0, items, C, V, ids, [&](int e, int64_t v, uint32_t c) { a.x[e] = v < 0 ? T(0) : table[v * C + c]; });
+#pragma unroll
+    for (int e = 0; e < W; ++e) a.x[e] *= scale;
     __stcs(reinterpret_cast<float4*>(out + e0), *reinterpret_cast<float4*>(&a));
   } else {
-#pragma unroll
-    for (int e = 0; e < W; ++e)
-      if (e0 + e < items) out[e0 + e] = a.x[e];
+    walk_elements<W, false>(e0, items, C, V, ids,
+                            [&](int e, int64_t v, uint32_t c) { out[e0 + e] = v < 0 ? T(0) : scale * table[v * C + c]; });
   }
 }
 
