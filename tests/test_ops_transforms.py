@@ -1,0 +1,61 @@
+"""Derivatives and transforms that the CUDA kernels of the transformer operators do not have are refused, not dropped."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from xnn_b200.ops import counter_dropout, embedding_lookup, structure_attention
+
+
+def _calls(device):
+    ptr = torch.tensor([0, 9, 50], device=device)
+    ids = torch.tensor([3, 0, 3, -1], device=device)
+    other = torch.randn(50, 2, 16, device=device)
+    return {"attention": (lambda t: structure_attention(t, t, t, ptr), (50, 2, 16)),
+            "attention_keys": (lambda t: structure_attention(other, t, other, ptr), (50, 2, 16)),
+            "attention_values": (lambda t: structure_attention(other, other, t, ptr), (50, 2, 16)),
+            "dropout": (lambda t: counter_dropout(t, 0.3, (1, 2)), (50, 2, 16)),
+            "lookup": (lambda t: embedding_lookup(t, ids), (5, 16))}
+
+
+NAMES = ["attention", "attention_keys", "attention_values", "dropout", "lookup"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("leaf", [False, True])
+def test_tangents_are_refused(name, leaf):
+    fn, shape = _calls("cuda")[name]
+    x = torch.randn(shape, device="cuda").requires_grad_(leaf)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            fn(forward_ad.make_dual(x, torch.ones_like(x)))
+    assert fn(x).shape[-1] == 16                # an ordinary call afterwards is served
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("graph", [False, True])
+def test_tangents_of_incoming_gradients_are_refused(name, graph):
+    fn, shape = _calls("cuda")[name]
+    x = torch.randn(shape, device="cuda", requires_grad=True)
+    y = fn(x)
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.randn_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(y, x, g, create_graph=graph)
+
+
+def test_tangents_on_the_cpu():
+    """The formula of attention carries them, the other two refuse them."""
+    calls = _calls("cpu")
+    fn, shape = calls["attention"]
+    x, u = torch.randn(shape, dtype=torch.float64), torch.randn(shape, dtype=torch.float64)
+    with forward_ad.dual_level():
+        tangent = forward_ad.unpack_dual(fn(forward_ad.make_dual(x, u))).tangent
+    step = 1e-6
+    # central differences: the remainder is of size step^2, a value's rounding is divided by step
+    assert float((tangent - (fn(x + step * u) - fn(x - step * u)) / (2 * step)).abs().max()) < 1e-8
+    for name in ("dropout", "lookup"):
+        fn, shape = calls[name]
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            fn(forward_ad.make_dual(torch.randn(shape), torch.ones(shape)))

@@ -30,6 +30,12 @@ namespace {
     TORCH_CHECK(err_ == cudaSuccess, #call, " failed: ", cudaGetErrorString(err_));           \
   } while (0)
 
+// The kernels carry no tangents: a call or a backward pass over a dual tensor would drop them without a word.
+void no_tangents(const char* what, std::initializer_list<torch::Tensor> tensors) {
+  for (const auto& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " on CUDA has no forward-mode derivative");
+}
+
 constexpr int ANY_LENGTH = std::numeric_limits<int>::max();
 constexpr int SHORT = 32;            // rows of the square tiles that hold a short structure whole
 constexpr int SMS = 148;
@@ -366,6 +372,7 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const auto set = kept(ctx);
+    no_tangents("structure_attention", {g[0]});
     if (!torch::GradMode::is_enabled()) {              // no graph of this pass is asked for
       auto r = attention_backward(rows(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], maybe(s[6]), set.max_len, set.scale,
                                   ctx->saved_data["status"].toTensor());
@@ -409,6 +416,7 @@ torch::Tensor structure_attention(torch::Tensor q, torch::Tensor k, torch::Tenso
   require(!mask.has_value() || (mask->scalar_type() == torch::kBool && mask->dim() == 1 && mask->size(0) == n && mask->device() == q.device()),
           "key_mask must be bool (", n, ") on ", q.device());
   require(max_len.value_or(0) >= 0, "max_len must not be negative, got ", max_len.value_or(0));
+  no_tangents("structure_attention", {q, k, v});
   require(d <= 128, "head width ", d, ": the kernels take up to 128");
   const int64_t most = max_len.value_or(n);
   const double f = scale.value_or(1.0 / std::sqrt((double)d));
@@ -447,6 +455,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto n = ctx->saved_data["sizes"].toIntVector();
+    no_tangents("counter_dropout", {g[0]});
     if (!torch::GradMode::is_enabled())
       return {dropout_raw(g[0].contiguous(), n[0], n[1], n[2], ctx->saved_data["p"].toDouble(), ctx->get_saved_variables()[0]),
               Variable(), Variable(), Variable(), Variable(), Variable()};
@@ -483,6 +492,7 @@ torch::Tensor dropout_op(torch::Tensor x, double p, torch::Tensor rng, const std
   require(p >= 0.0 && p <= 1.0, "the dropout probability must be in [0, 1], got ", p);
   require(rng.scalar_type() == torch::kInt64 && rng.dim() == 1 && rng.size(0) == 2 && rng.device() == x.device(),
           "rng must be two int64 numbers (seed, offset) on ", x.device());
+  no_tangents("counter_dropout", {x});
   const auto n = shared_sizes(x, shared);
   x = x.contiguous();
   rng = rng.contiguous();
@@ -554,6 +564,7 @@ struct Lookup : torch::autograd::Function<Lookup> {
     return lookup_raw(table, ids, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_tangents("embedding_lookup", {g[0]});
     if (!torch::GradMode::is_enabled())
       return {lookup_grad_raw(ctx->get_saved_variables()[0], g[0].contiguous(), ctx->saved_data["rows"].toInt(),
                               ctx->saved_data["scale"].toDouble()), Variable(), Variable()};
@@ -577,6 +588,7 @@ torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
   require_type(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ",
                ids.scalar_type());
   require(ids.device() == table.device(), "table on ", table.device(), ", ids on ", ids.device());
+  no_tangents("embedding_lookup", {table});
   table = table.contiguous();
   ids = ids.contiguous();
   if (torch::GradMode::is_enabled() && table.requires_grad()) return Lookup::apply(table, ids, scale);

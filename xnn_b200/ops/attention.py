@@ -79,7 +79,8 @@ def structure_attention(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, max_len: O
     rows outside ``ptr[0] .. ptr[-1]`` belong to none). ``max_len``: no structure has more atoms
     (``N`` when omitted; a smaller bound lets short structures take the kernels made for them; where a structure
     exceeds it, the CPU refuses and on CUDA its gradients are NaN unless they are right). ``scale``: ``D ** -0.5`` when omitted. ``key_mask``: bool ``(N)``, false
-    for atoms that nobody attends to. Differentiable twice on CUDA, to any order on the CPU."""
+    for atoms that nobody attends to. Differentiable twice on CUDA, to any order (and in forward mode) on
+    the CPU; what CUDA has no derivative for raises an error."""
     if q.is_cuda:                                # the arguments are checked there
         return _kernel()(q, k, v, ptr, max_len, scale, key_mask, _status(q.device))
     for name, t in (("q", q), ("k", k), ("v", v)):

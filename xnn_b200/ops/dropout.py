@@ -98,7 +98,7 @@ def _kernel():
 
 def counter_dropout(x: Tensor, p: float, rng: Rng, shared: Sequence[int] = ()) -> Tensor:
     """``x`` with entries dropped with probability ``p``, the others divided by ``1 - p``; differentiable to any
-    order. ``rng = (seed, offset)``: two integers, or an int64 tensor of them on ``x``'s device (it is read
+    order in reverse mode. ``rng = (seed, offset)``: two integers, or an int64 tensor of them on ``x``'s device (it is read
     when the kernels run, and again in the backward pass: advance a copy, not the tensor itself).
     ``shared``: neighbouring dimensions over which the mask is the same."""
     if not isinstance(rng, Tensor):
