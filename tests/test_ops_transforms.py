@@ -59,3 +59,15 @@ def test_tangents_on_the_cpu():
         fn, shape = calls[name]
         with forward_ad.dual_level(), pytest.raises(NotImplementedError):
             fn(forward_ad.make_dual(torch.randn(shape), torch.ones(shape)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("leaf", [False, True])
+def test_traces_are_refused(name, leaf):
+    """A trace would keep the example's result whatever its inputs are later."""
+    fn, shape = _calls("cuda")[name]
+    x = torch.randn(shape, device="cuda").requires_grad_(leaf)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: fn(t) + t.sum(), (x,), check_trace=False)
+    assert fn(x).shape[-1] == 16

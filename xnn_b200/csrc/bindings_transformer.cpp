@@ -2,6 +2,7 @@
 // launched on the current stream of the operands' device; workspaces come from the caching allocator on that stream.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -34,6 +35,11 @@ namespace {
 void no_tangents(const char* what, std::initializer_list<torch::Tensor> tensors) {
   for (const auto& t : tensors)
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " on CUDA has no forward-mode derivative");
+}
+
+// A trace records operators that PyTorch knows; a result of these kernels would become a constant in it.
+void not_traced(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " on CUDA cannot be traced (torch.jit.trace)");
 }
 
 constexpr int ANY_LENGTH = std::numeric_limits<int>::max();
@@ -417,6 +423,7 @@ torch::Tensor structure_attention(torch::Tensor q, torch::Tensor k, torch::Tenso
           "key_mask must be bool (", n, ") on ", q.device());
   require(max_len.value_or(0) >= 0, "max_len must not be negative, got ", max_len.value_or(0));
   no_tangents("structure_attention", {q, k, v});
+  not_traced("structure_attention");
   require(d <= 128, "head width ", d, ": the kernels take up to 128");
   const int64_t most = max_len.value_or(n);
   const double f = scale.value_or(1.0 / std::sqrt((double)d));
@@ -493,6 +500,7 @@ torch::Tensor dropout_op(torch::Tensor x, double p, torch::Tensor rng, const std
   require(rng.scalar_type() == torch::kInt64 && rng.dim() == 1 && rng.size(0) == 2 && rng.device() == x.device(),
           "rng must be two int64 numbers (seed, offset) on ", x.device());
   no_tangents("counter_dropout", {x});
+  not_traced("counter_dropout");
   const auto n = shared_sizes(x, shared);
   x = x.contiguous();
   rng = rng.contiguous();
@@ -589,6 +597,7 @@ torch::Tensor lookup_op(torch::Tensor table, torch::Tensor ids, double scale) {
                ids.scalar_type());
   require(ids.device() == table.device(), "table on ", table.device(), ", ids on ", ids.device());
   no_tangents("embedding_lookup", {table});
+  not_traced("embedding_lookup");
   table = table.contiguous();
   ids = ids.contiguous();
   if (torch::GradMode::is_enabled() && table.requires_grad()) return Lookup::apply(table, ids, scale);
