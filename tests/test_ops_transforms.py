@@ -71,3 +71,14 @@ def test_traces_are_refused(name, leaf):
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda t: fn(t) + t.sum(), (x,), check_trace=False)
     assert fn(x).shape[-1] == 16
+
+
+def test_traced_attention_on_the_cpu():
+    """Longer structures than the example's, shorter ones and other counts."""
+    def inputs(lens):
+        n = sum(lens)
+        return (torch.randn(n, 2, 4), torch.randn(n, 1, 4), torch.randn(n, 1, 4), torch.tensor([0] + lens).cumsum(0))
+    traced = torch.jit.trace(structure_attention, inputs([5, 3]), check_trace=False)
+    for lens in ([5, 3], [9, 2, 7], [1], [4, 0, 2, 30]):
+        args = inputs(lens)
+        assert torch.equal(traced(*args), structure_attention(*args))

@@ -47,7 +47,9 @@ def _kernel():
 def _formula(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, mask: Optional[Tensor], scale: float) -> Tensor:
     """The same over padded structures ``(B, H, L, D)``."""
     n, heads, _ = q.shape
-    length = int((ptr[1:] - ptr[:-1]).max()) if ptr.numel() > 1 else 0
+    length = (ptr[1:] - ptr[:-1]).max() if ptr.numel() > 1 else 0
+    if not torch.jit.is_tracing():              # a trace keeps the length of its own inputs' structures
+        length = int(length)
     out = q.new_zeros(n, heads, q.shape[2])
     if n == 0 or length == 0:
         return out + 0.0 * (q.sum() + k.sum() + v.sum())
