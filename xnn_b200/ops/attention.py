@@ -52,7 +52,7 @@ def _formula(q: Tensor, k: Tensor, v: Tensor, ptr: Tensor, mask: Optional[Tensor
         length = int(length)
     out = q.new_zeros(n, heads, q.shape[2])
     if n == 0 or length == 0:
-        return out + 0.0 * (q.sum() + k.sum() + v.sum())
+        return out + (q[:0].sum() + k[:0].sum() + v[:0].sum())      # zero, with a graph
     slot = ptr[:-1, None] + torch.arange(length, device=q.device)
     on = slot < ptr[1:, None]
     row = slot.clamp(max=n - 1)
