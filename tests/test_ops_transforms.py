@@ -82,3 +82,19 @@ def test_traced_attention_on_the_cpu():
     for lens in ([5, 3], [9, 2, 7], [1], [4, 0, 2, 30]):
         args = inputs(lens)
         assert torch.equal(traced(*args), structure_attention(*args))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("lens", [[9, 20], [50]])
+def test_third_derivative_through_the_incoming_gradient_is_refused(turned, lens):
+    """Refused on the path through the cotangent of the output too, contiguous or not."""
+    n = sum(lens)
+    ptr = torch.tensor([0] + lens).cumsum(0).cuda()
+    q, k, v = (torch.randn(n, 2, 16, device="cuda", requires_grad=True) for _ in range(3))
+    y = torch.randn((16, 2, n) if turned else (n, 2, 16), device="cuda", requires_grad=True)
+    do = y.square().permute(2, 1, 0) if turned else y.square()
+    (dq,) = torch.autograd.grad(structure_attention(q, k, v, ptr), q, do, create_graph=True)
+    second = torch.autograd.grad(dq, (q, k, v), torch.ones_like(dq), create_graph=True)
+    with pytest.raises(RuntimeError, match="not three times"):
+        torch.autograd.grad(sum(t.sum() for t in second), y, allow_unused=True)

@@ -351,7 +351,6 @@ struct AttentionSecond : torch::autograd::Function<AttentionSecond> {
 struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
   static variable_list forward(AutogradContext* ctx, Variable go, Variable q, Variable k, Variable v, Variable o, Variable lse,
                                Variable ptr, c10::optional<Variable> mask, Variable status, int64_t max_len, double scale) {
-    go = rows(go);
     ctx->save_for_backward({go, q, k, v, o, lse, ptr, mask.value_or(Variable())});
     ctx->saved_data["status"] = status;
     keep(ctx, {max_len, scale});
@@ -386,7 +385,8 @@ struct Attention : torch::autograd::Function<Attention> {
       return r;
     }
     // o without its graph: the second derivative holds what goes through it
-    auto r = AttentionGrad::apply(g[0], s[0], s[1], s[2], s[3].detach(), s[4], s[5], maybe(s[6]),
+    // (the gradient's rows are laid out here, where that is recorded: the copy belongs to the graph)
+    auto r = AttentionGrad::apply(rows(g[0]), s[0], s[1], s[2], s[3].detach(), s[4], s[5], maybe(s[6]),
                                   ctx->saved_data["status"].toTensor(), set.max_len, set.scale);
     r.resize(8);
     return r;
