@@ -122,7 +122,8 @@ class CounterDropout(nn.Module):
     """:func:`counter_dropout` in training mode with its own seed (drawn from PyTorch's generator when
     omitted) and an offset that each call advances. The two numbers live on the module's device, so a
     captured training step draws a new mask at every replay. Processes that start from one seed draw the
-    same masks, each for its own rows. Inside an activation checkpoint it is refused: the recomputed pass
+    same masks, each for its own rows, unless :meth:`set_rank` tells them apart (the trainer does). The state dict
+    does not hold the numbers: a run that starts again draws from its seed's first mask on. Inside an activation checkpoint it is refused: the recomputed pass
     would meet another offset."""
 
     def __init__(self, p: float, shared: Sequence[int] = (), seed: Optional[int] = None):
@@ -132,6 +133,10 @@ class CounterDropout(nn.Module):
         self.p, self.shared = float(p), tuple(int(d) for d in shared)
         seed = int(torch.randint(0, 2 ** 62, ())) if seed is None else int(seed)
         self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+
+    def set_rank(self, rank: int) -> None:
+        """Masks of rank ``rank``'s own: the offset counts from ``rank * 2^40`` on (rank 0 as without ranks)."""
+        self.rng[1] = (self.rng[1] & ((1 << 40) - 1)) | (int(rank) << 40)
 
     def forward(self, x: Tensor) -> Tensor:
         if not self.training or self.p == 0.0:

@@ -33,6 +33,7 @@ from torch import Tensor, nn
 
 from ..data import AtomicGraph, collate
 from ..models import ForceStressOutput, prepare_model
+from ..ops.dropout import CounterDropout
 from ..ops.modes import params_only
 from ..parallel import distributed as D
 from ..parallel.grad_sync import GradSync
@@ -108,9 +109,13 @@ class Trainer:
         self.grad_sync = GradSync(self.params, backend=self._grad_backend)
         # same starting weights on every rank
         if self.world > 1:
+            drops = [m for m in self.module.modules() if isinstance(m, CounterDropout)]
+            own = {id(m.rng) for m in drops}
             with torch.no_grad():
-                for t in list(self.module.parameters()) + list(self.module.buffers()):
+                for t in list(self.module.parameters()) + [b for b in self.module.buffers() if id(b) not in own]:
                     torch.distributed.broadcast(t, 0)
+            for m in drops:                     # but dropout masks of its own (a seed that a rank was given stays)
+                m.set_rank(self.rank)
         graphs = bool(cfg.trainer.cuda_graph) and self.device.type == "cuda"
         self.use_graphs = graphs
         lr = torch.tensor(o.lr, device=self.device) if graphs else o.lr
