@@ -537,6 +537,8 @@ class SpookyNet(InteratomicPotential):
         heads = int(attention_heads)
         if heads < 1 or n_features % heads or (heads != 1 and attention != "softmax"):
             raise ValueError(f"attention_heads={heads} of {n_features} features with attention={attention!r}")
+        if attention == "softmax" and n_features // heads > 128:
+            raise ValueError(f"attention='softmax' takes heads of up to 128 features, got {n_features} in {heads}")
         self.attention_heads = heads if attention == "softmax" else 0
         if ewald and lr_cutoff is None:
             raise ValueError("ewald=True needs lr_cutoff (the real-space cutoff)")
