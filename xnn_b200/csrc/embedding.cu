@@ -393,11 +393,14 @@ int run_chunk(int64_t N) {
   const int64_t r = (N + 148 * 24 - 1) / (148 * 24);
   return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
-// Collecting costs N V id reads in all and sums a row's entries, in the worst case all of them, in one block; the sort costs four
-// to ten launches, 15-25 us on the device and as much of the host. Collecting, device: 4868 ids of 1777 rows, 11 columns 16
-// us, 8192 ids of 4000 rows 48, 8192 ids of 4 rows x 128 columns 80, x 512 306; 8192 of 1000, 64 columns 18, 611 of 87 x 64 4.
+// Collecting costs N V id reads in all, a block a table row, and sums a row's entries, in the worst case all of them, in one
+// block; the sort costs four to ten launches, 15-25 us on the device and as much of the host. Collecting, device: 4868 ids of
+// 1777 rows, 11 columns 16 us, 8192 ids of 4000 rows 48, 8192 ids of 4 rows x 128 columns 80, x 512 306; 8192 of 1000, 64
+// columns 18, 611 of 87 x 64 4. The blocks alone: 16 ids x 64 columns, collected and sorted, of 8192 rows 18 and 17 us on the
+// device (the call 53 and 71), of 16384 34 and 18 (53 and 71), of 32768 66 and 22 (72 and 72), of 2^20 2058 and 223.
+constexpr int64_t COLLECTED_ROWS = 16384;
 bool collects(int64_t N, int64_t V, int64_t C) {
-  return N <= SMALL_ROWS && N * V <= (int64_t)1 << 24 && N * C <= (int64_t)1 << 17;
+  return N <= SMALL_ROWS && V <= COLLECTED_ROWS && N * V <= (int64_t)1 << 24 && N * C <= (int64_t)1 << 17;
 }
 
 template <typename T, int W>
