@@ -803,8 +803,12 @@ cudaError_t second64_dp(const Params<IN>& p, double* work, cudaStream_t s) {
 
 template <typename IN>
 cudaError_t second64(const Params<IN>& p, double* work, cudaStream_t s) {
-  if (sizeof(IN) == 8 && p.D > 112) return second64_dp<IN, 128, sizeof(IN) == 8>(p, work, s);
-  XNN_F64_DIM(p.D, return (second64_dp<IN, DP, false>(p, work, s)))
+  if constexpr (sizeof(IN) == 4) {
+    return second64_dp<IN, 128, false>(p, work, s);      // up to 64 columns are attention_tc_second.cu's
+  } else {
+    if (p.D > 112) return second64_dp<IN, 128, true>(p, work, s);
+    XNN_F64_DIM(p.D, return (second64_dp<IN, DP, false>(p, work, s)))
+  }
 }
 
 template int64_t second64_words<float>(const Params<float>&);

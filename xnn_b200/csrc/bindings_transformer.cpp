@@ -94,7 +94,9 @@ attn::Params<T> make_params(const torch::Tensor& q, const torch::Tensor& k, cons
 //   otherwise                              the tensor cores for the structures above SHORT, the short kernels for the rest
 // Both ways, for all / in two launches, forward, backward, second derivative at 64 columns in us: 64 structures of 9-40 atoms,
 // one head 11, 17, 39 / 16, 27, 55; of 400 x 2 heads 37, 138, 259 / 35, 77, 172; of 20-60 atoms 41, 149, 306 / 47, 135, 278.
-// float64: 11, 29, 73 / 20, 44, 105; 74, 183, 371 / 66, 142, 343; 103, 263, 618 / 108, 253, 615.
+// float64: 11, 29, 73 / 20, 44, 105; 74, 183, 371 / 66, 142, 343; 103, 263, 618 / 108, 253, 615. float32 of more than 64
+// columns, whose long second derivatives are attention_f64.cu's, one after the other forward, backward and that: 64 structures
+// of 20-50 atoms x 1 x 128 154 / 190, of 9-40 150 / 183, 64 of 30-60 x 4 x 128 533 / 597, 300 of 30-60 x 1 x 72 465 / 529.
 constexpr int LONG_AVERAGE = 40, TC_SECOND_WIDTH = 64, TC_ROWS = 128, TC_TILE = 64;
 
 struct Plan { bool long_ones, short_ones; };
