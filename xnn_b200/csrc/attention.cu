@@ -380,8 +380,8 @@ cudaError_t launch(const Params<T>& p, int heads, int row_tiles, int key_tiles, 
 }
 
 // The square tiles of 32 rows. float: a 2 x 4 corner of the scores a thread (one molecule of 21 atoms at 64 columns: 5 us with
-// 128 threads, 9 with 64 and 4 x 4 corners; 4000 x 4 heads: 253 and 279 us, of 97 to move the data: what is read from shared
-// memory bounds it). double: 2 x 2, since the accumulators of 4 x 4 alone would take 128 registers at 128 columns.
+// 128 threads, 9 with 64 and 4 x 4 corners; 4000 of 8-31 x 4 heads: 253 and 279 us, of 49 to move the data: reads of shared
+// memory bound it). double: 2 x 2, since the accumulators of 4 x 4 alone would take 128 registers at 128 columns.
 template <typename T, int DP> struct Small;
 template <int DP> struct Small<float, DP> { using C = Cfg<float, 32, 32, DP, 2, 8>; };
 template <int DP> struct Small<double, DP> { using C = Cfg<double, 32, 32, DP, 2, 16>; };

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(uint32_t items, uint32_t pe
 }
 
 // Rows that are no whole number of 16 bytes (or not on such boundaries): a thread writes 16 bytes of the output, whatever rows
-// they are of. 400000 rows of 127 floats: 61 us (97 with single
+// they are of. 400000 rows of 127 floats: 58 us (97 with single
 // elements, each with its own division).
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) lookup_odd_kernel(uint32_t items, uint32_t C, int64_t V, const T* __restrict__ table,
@@ -298,7 +298,7 @@ __device__ __forceinline__ void run_part(const T* part, int c0, int j0, int j1, 
 // A warp per table row and 32 W columns: zeros where no id came, the partials of a run over several chunks added up. Rows of
 // more than MANY partials (the few elements that most atoms are) are left to the whole block. A block's rows lie gridDim.x
 // apart, so that the popular ids, which are neighbours, meet in different blocks; a table of at most a row an SM has a block
-// of 32 warps a row (gradient of 400000 ids of 5 elements, 512 columns: 163 us, 747 with eight rows in one block).
+// of 32 warps a row (gradient of 400000 ids of 5 elements, 512 columns: 171 us, 747 with eight rows in one block).
 constexpr int MANY = 32;
 
 template <typename T, int W, int WARPS, int ROWS>
@@ -433,10 +433,10 @@ int run_chunk(int64_t N) {
   return (int)(r < 32 ? 32 : (r + 7) / 8 * 8);
 }
 // Collecting costs N V id reads in all, a block a table row, and sums a row's entries, in the worst case all of them, in one
-// block; the sort costs four to ten launches, 15-25 us on the device and as much of the host. Collecting, device: 4868 ids of
-// 1777 rows, 11 columns 16 us, 8192 ids of 4000 rows 48, 8192 ids of 4 rows x 128 columns 80, x 512 306; 8192 of 1000, 64
-// columns 18, 611 of 87 x 64 4. The blocks alone: 16 ids x 64 columns, collected and sorted, of 8192 rows 18 and 17 us on the
-// device (the call 53 and 71), of 16384 34 and 18 (53 and 71), of 32768 66 and 22 (72 and 72), of 2^20 2058 and 223.
+// block; the sort costs four to ten launches, 15-25 us on the device and as much of the host. Device, collected and sorted, in us:
+// 4868 ids of 1777 rows x 11 columns 16 and 22, 8192 of 2000 x 16 27 and 23, of 4000 x 16 49 and 25, of 4 x 16 18 and 15, of
+// 4 x 128 53 and 15, of 4 x 512 202 and 15, 611 of 87 x 64 3 and 14; the blocks alone, 16 ids x 64 columns: of 8192 rows 18 and
+// 18 (the call 53 and 71), of 16384 35 and 20 (53 and 71), of 32768 68 and 25 (72 and 72), of 2^20 2058 and 223.
 constexpr int64_t COLLECTED_ROWS = 16384;
 bool collects(int64_t N, int64_t V, int64_t C) {
   return N <= SMALL_ROWS && V <= COLLECTED_ROWS && N * V <= (int64_t)1 << 24 && N * C <= (int64_t)1 << 17;
